@@ -132,6 +132,40 @@ int    l3m_k_rmsnorm(float *y, const float *x, const float *w, int n, float eps,
 int    l3m_k_rope(float *v, int n_heads, int hd, int pos, const float *table, void *stream);      // ops.c:29
 int    l3m_k_silu_mul(float *h, const float *g, int n, void *stream);                            // ops.c:49
 int    l3m_k_argmax(const float *x, int n, int32_t *out, void *stream);                          // engine.c:290-301
+// A K/V cache of 4-bit blocks (no counterpart in the reference, whose cache is bf16): a row's 32-value blocks as q4_0
+// (f16 scale) or mxfp4 (power-of-two scale), 0.56 and 0.53 bytes a value. A cache holds one layer's kv heads; its planes lie in one
+// allocation of l3m_kv4_bytes (0 for a shape that is refused: dtype L3M_HIP_Q4_0 or L3M_HIP_MXFP4, hd a multiple of 8 up to 256,
+// cap up to 2^30 positions), 16-byte aligned, which need not be cleared. Codes are stored in the order the attention reads
+// them: rows go in and out through these calls.
+// Every call refuses (-1, l3m_dev_error) what its arguments cannot mean, before it launches anything. Calls are
+// asynchronous on `stream` (NULL: the library's) of device 0, allocate nothing, and may be captured into a graph.
+typedef struct {
+    uint8_t *kq, *ks, *vq, *vs;  // K codes and scales, V codes and scales
+    int nkv, hd, cap, dtype;
+} l3m_kv4;
+size_t l3m_kv4_bytes(int dtype, int nkv, int hd, int cap);
+int    l3m_kv4_init(l3m_kv4 *c, int dtype, int nkv, int hd, int cap, void *mem);   // host only: fills *c
+// RMSNorm of every query and key head (l3m_k_rmsnorm over the head's hd values; weights wq, wk [hd] shared by the heads, NULL for no
+// norm) and the rotation (NULL table for none; l3m_rope_table's, row pos + t for token t), in one pass and one rounding: pairs
+// (2i, 2i + 1), as l3m_k_rope, or with halves (i, i + hd / 2). rows: n tokens, `stride` floats apart, each [q heads | k heads | ..] as
+// a q/k/v product leaves them; q [n][nq][hd], k [n][nkv][hd]. q and k lie apart from rows, or, for one token, may be its heads.
+// hd even, at most 256; nq or nkv may be 0.
+int l3m_k_qk_norm_rope(float *q, float *k, const float *rows, int stride, int n, int nq, int nkv, int hd, const float *wq, const float *wk,
+                       float eps, int halves, int pos, const float *table, void *stream);
+// The same on rows [q heads | k heads | v heads]: q as above; K (normed, rotated) and V rows into the cache at
+// positions pos .. pos + n - 1, rounded as l3m_quantize_row rounds (the nearest code; mxfp4 scales from 2^-126 up; q4_0 scales saturate). A block with a value
+// that is not finite reads back as NaN. nq 0 (q unused): the cache alone, with wk and table NULL plain rows. Other
+// positions of the cache stay as they are. Two calls that write positions of the same eight (pos / 8) must not overlap in time.
+int l3m_k_kv4_append(const l3m_kv4 *c, float *q, const float *rows, int stride, int n, int nq, const float *wq, const float *wk, float eps,
+                     int halves, int pos, const float *table, void *stream);
+// Positions pos .. pos + n - 1 as values: k and v [n][nkv][hd] (either may be NULL).
+int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *stream);
+// Attention of n tokens at positions pos .. pos + n - 1, token t over positions 0 .. pos + t (whose rows, its own among them, are in
+// the cache), scores q.k / sqrt(hd): q and out [n][nq][hd] float32, out may be q; query head h reads kv head h / (nq / nkv). What the
+// cache holds past a token's position does not reach it. work: l3m_kv4_work_bytes(c, n, nq) bytes, 16-byte aligned, of any
+// contents, used by one call at a time (a captured call uses it at every replay); a larger n's serves a smaller one.
+size_t l3m_kv4_work_bytes(const l3m_kv4 *c, int n, int nq);
+int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq, int pos, void *work, size_t work_bytes, void *stream);
 // The decode step's own pieces, alone (parity hooks):
 // rows [row0, row0 + n) of m dequantized by the step's embedding lookup (l3m_dequant_row, pack.c:55-62)
 // into out[n][32 * m->nb];

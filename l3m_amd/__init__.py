@@ -37,6 +37,7 @@ Opts = _struct("Opts", [("cpus", C.POINTER(C.c_int))] + [(n, C.c_int) for n in "
 PERF_FIELDS = "tokens ns_token ns_compute ns_wait bytes_token l2_bytes l3_miss dram_bytes energy_j llc_occupancy".split()
 Perf = _struct("Perf", [(n, C.c_double) for n in PERF_FIELDS])
 DMat = _struct("DMat", [("q", C.c_void_p), ("s", C.c_void_p)] + [(n, C.c_int) for n in "rows tiles nb dtype".split()])
+KV4 = _struct("KV4", [(n, C.c_void_p) for n in "kq ks vq vs".split()] + [(n, C.c_int) for n in "nkv hd cap dtype".split()])
 GenSpec = _struct("GenSpec", [("arch", C.c_char_p)] + [(n, C.c_int) for n in "dim n_layers n_heads n_kv_heads ffn_dim vocab ctx".split()]
                   + [("rope_theta", C.c_float), ("norm_eps", C.c_float)] + [(n, C.c_int) for n in "dtype head_dtype tied".split()]
                   + [("seed", C.c_uint64), ("std", C.c_float), ("norm_jitter", C.c_float), ("bos", C.c_int), ("eos", C.c_int)])
@@ -46,7 +47,7 @@ _CODES = {"v": None, "i": C.c_int, "I": C.c_int32, "w": C.c_uint16, "q": C.c_uin
           "d": C.c_double, "p": C.c_void_p, "s": C.c_char_p, "*i": C.POINTER(C.c_int), "*I": _i32, "*f": _f,
           "*d": C.POINTER(C.c_double),
           "**": C.POINTER(C.c_void_p), "O": C.POINTER(Opts), "P": C.POINTER(Perf), "M": C.POINTER(DMat),
-          "G": C.POINTER(GenSpec), "cb": TOKEN_CALLBACK}
+          "G": C.POINTER(GenSpec), "K": C.POINTER(KV4), "cb": TOKEN_CALLBACK}
 _SIGNATURES = """
 l3m_load p s O                  | l3m_free v p                   | l3m_logits *f p
 l3m_generate i p *I i i f q cb p | l3m_vocab i p                 | l3m_ctx i p
@@ -76,6 +77,9 @@ l3m_decode_window i p
 l3m_k_step_mv i i i M p i p i p  | l3m_step_matvec i p i i i *f *f | l3m_step_layout v p *i
 l3m_widen_rows i i i i ** p | l3m_decode_spin_limit v p l | l3m_time_launch_interval d i
 l3m_tokenize i s s i *I i | l3m_head_dim i p | l3m_gemv_matrix_cores i i
+l3m_kv4_bytes z i i i i | l3m_kv4_init i K i i i i p | l3m_kv4_work_bytes z K i i
+l3m_k_qk_norm_rope i p p p i i i i i p p f i i p p | l3m_k_kv4_append i K p p i i i p p f i i p p
+l3m_k_kv4_rows i K p p i i p | l3m_k_kv4_attend i p p K i i i p z p
 l3m_time_read d ** i z i         | l3m_hip_attend_noalloc i p p p p i i i | l3m_phase_stamps i i i i p
 """
 _SIG = {}
@@ -446,3 +450,56 @@ class Device:
         do = self.alloc(4)
         self._check(self.lib.l3m_k_argmax(self.put(np.float32(x)), len(x), do, None), "argmax")
         return int(self.get(do, 1, np.int32)[0])
+
+    def rope_table(self, ctx, hd, theta):
+        """The rotation's table on the device: [ctx][hd / 2] (cos, sin)."""
+        table = np.zeros(ctx * hd, np.float32)
+        self.lib.l3m_rope_table(_p(table, _f), ctx, hd, theta)
+        return self.put(table)
+
+    def _opt(self, w):
+        return None if w is None else self.put(np.float32(w))
+
+    def qk_norm_rope(self, rows, nq, nkv, hd, wq=None, wk=None, eps=1e-5, halves=False, pos=0, table=None):
+        """Norm and rotation of the query and key heads of rows [n, width]: q [n, nq, hd], k [n, nkv, hd] (l3m_k_qk_norm_rope)."""
+        rows = np.ascontiguousarray(rows, np.float32)
+        n, width = rows.shape
+        dq, dk = self.alloc(max(4 * n * nq * hd, 4)), self.alloc(max(4 * n * nkv * hd, 4))
+        self._check(self.lib.l3m_k_qk_norm_rope(dq, dk, self.put(rows), width, n, nq, nkv, hd, self._opt(wq), self._opt(wk), eps, int(halves), pos,
+                                                table, None), "qk_norm_rope")
+        return self.get(dq, (n, nq, hd), np.float32), self.get(dk, (n, nkv, hd), np.float32)
+
+    def kv4(self, dtype, nkv, hd, cap):
+        """An empty 4-bit K/V cache (Q4_0 or MXFP4) of cap positions."""
+        c = KV4()
+        size = self.lib.l3m_kv4_bytes(dtype, nkv, hd, cap)
+        if not size:
+            raise ValueError(f"no 4-bit cache of dtype {dtype}, {nkv} heads of {hd}, {cap} positions")
+        self._check(self.lib.l3m_kv4_init(C.byref(c), dtype, nkv, hd, cap, self.alloc(size)), "kv4")
+        return c
+
+    def kv4_append(self, c, rows, nq, pos, wq=None, wk=None, eps=1e-5, halves=False, table=None):
+        """rows [n, width] of [q | k | v] heads: K and V into the cache at pos.., the queries returned [n, nq, hd] (l3m_k_kv4_append)."""
+        rows = np.ascontiguousarray(rows, np.float32)
+        n, width = rows.shape
+        dq = self.alloc(4 * n * nq * c.hd) if nq else None
+        self._check(self.lib.l3m_k_kv4_append(C.byref(c), dq, self.put(rows), width, n, nq, self._opt(wq), self._opt(wk), eps, int(halves), pos,
+                                              table, None), "kv4_append")
+        return self.get(dq, (n, nq, c.hd), np.float32) if nq else None
+
+    def kv4_rows(self, c, pos, n):
+        """Positions pos.. of the cache as values: k, v [n, nkv, hd]."""
+        dk, dv = (self.alloc(4 * max(n, 1) * c.nkv * c.hd) for _ in range(2))
+        self._check(self.lib.l3m_k_kv4_rows(C.byref(c), dk, dv, pos, n, None), "kv4_rows")
+        return tuple(self.get(p, (n, c.nkv, c.hd), np.float32) for p in (dk, dv))
+
+    def kv4_attend(self, c, q, pos):
+        """Attention of q [n, nq, hd] at positions pos.. over the cache: [n, nq, hd] (l3m_k_kv4_attend)."""
+        q = np.ascontiguousarray(q, np.float32)
+        n, nq, hd = q.shape
+        if hd != c.hd:
+            raise ValueError(f"heads of {hd}, the cache holds heads of {c.hd}")
+        size = self.lib.l3m_kv4_work_bytes(C.byref(c), n, nq)
+        do = self.alloc(q.nbytes)
+        self._check(self.lib.l3m_k_kv4_attend(do, self.put(q), C.byref(c), n, nq, pos, self.alloc(size), size, None), "kv4_attend")
+        return self.get(do, q.shape, np.float32)

@@ -117,6 +117,8 @@ int         l3m_dev_upload(void *dst, const void *src, size_t bytes);
 int         l3m_dev_download(void *dst, const void *src, size_t bytes);
 int         l3m_dev_sync(void);
 void       *l3m_dev_stream(void);
+int         l3m_dev_fail(const char *msg);          // records msg as the sticky error when it is the first; -1
+int         l3m_dev_launched(const char *what);     // 0, or the last launch's error recorded and -1
 
 // ------------------------------------------------------------------ single kernels
 size_t l3m_act_bytes(int dtype, int k);         // prepared activation: per 32-block values (q8_0 32 B, q4_0 nibble planes 32 B, mxfp4 f16 pairs 64 B) + scale[nb] + sum[nb] (mxfp4: + fp8 parts h, l 64 B per block), bf16[kp] or f32[kp]

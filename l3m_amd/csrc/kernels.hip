@@ -4498,6 +4498,11 @@ void l3m_dev_clear_error(void) { (void)hipGetLastError(); g_has_err = 0; g_err[0
 const char *l3m_dev_name(void) { return g_name; }
 unsigned l3m_dev_lds_max(void) { return l3m_dev_init() ? 65536u : g_lds_max; }
 void *l3m_dev_stream(void) { return (void *)g_stream; }
+int l3m_dev_fail(const char *msg) { return fail_msg(msg); }
+int l3m_dev_launched(const char *what) {
+    CKL(what);
+    return 0;
+}
 
 void *l3m_dev_alloc(size_t bytes) {
     void *p = NULL;
