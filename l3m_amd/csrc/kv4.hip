@@ -6,7 +6,8 @@
 //   K codes  [nkv][tile][half 2][lane 64][NB words]   lane 16 c + m, half f: position 8 (m / 4) + 4 f + m % 4, word b its dimensions
 //                                                     32 b + 8 c .. + 7
 //   V codes  [nkv][tile][lane 64][2 NB words]         lane 16 g + j: word t holds dimension 16 t + j of positions 8 g .. 8 g + 7
-//   scales   [nkv][tile][NB][32 positions]            of K and of V: f16 d (q4_0), a biased exponent byte (mxfp4)
+//   scales   [nkv][tile][NB][32 positions]            f16 d (q4_0), a biased exponent byte (mxfp4); mxfp4's of K [nkv][tile][m 16][f 2][NB],
+//                                                     as the lanes that hold the codes
 // Both codes of a tile and head take 512 NB bytes. Element i of a word's eight (a dimension of K, a position of V) is the nibble at
 // bit nib(dt, i): q4_0's masked bytes are then elements 0..3 and 4..7, mxfp4's byte pairs come in order.
 #include <hip/hip_runtime.h>
@@ -42,7 +43,12 @@ __device__ __forceinline__ size_t k_word(int nb, int p, int d) {
 __device__ __forceinline__ size_t v_word(int nb, int p, int d) {
     return ((size_t)(p >> 5) * 64 + ((p & 31) >> 3) * 16 + (d & 15)) * 2 * nb + (d >> 4);
 }
-__device__ __forceinline__ size_t scale_at(int nb, int p, int b) { return ((size_t)(p >> 5) * nb + b) * TILE + (p & 31); }
+__device__ __forceinline__ size_t v_scale(int nb, int p, int b) { return ((size_t)(p >> 5) * nb + b) * TILE + (p & 31); }
+template <int DT> __device__ __forceinline__ size_t k_scale(int nb, int p, int b) {
+    if constexpr (DT == L3M_Q4_0) return v_scale(nb, p, b);
+    const int w = p & 31;
+    return (((size_t)(p >> 5) * 16 + (w >> 3) * 4 + (w & 3)) * 2 + ((w >> 2) & 1)) * nb + b;
+}
 
 template <int DT> __device__ __forceinline__ float scale_value(const uint8_t *s, size_t i) {
     if constexpr (DT == L3M_Q4_0) return (float)((const _Float16 *)s)[i];
@@ -170,7 +176,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_rows_in(RowsIn a, l3m
                 for (int m = 1; m < 8; m <<= 1) code |= (uint32_t)__shfl_xor((int)code, m);
                 if (b < nb) {
                     if ((d & 7) == 0) H.kq[k_word(nb, p, d)] = code;
-                    if ((d & 31) == 0) put_scale<DT>(H.ks, scale_at(nb, p, b), stored);
+                    if ((d & 31) == 0) put_scale<DT>(H.ks, k_scale<DT>(nb, p, b), stored);
                 }
             }
         }
@@ -199,7 +205,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_rows_in(RowsIn a, l3m
                 uint32_t stored;
                 word |= quantize<DT>(x[i], stored) << nib(DT, i);
                 mine |= 15u << nib(DT, i);
-                if ((d & 31) == 0 && b < nb) put_scale<DT>(H.vs, scale_at(nb, p, b), stored);
+                if ((d & 31) == 0 && b < nb) put_scale<DT>(H.vs, v_scale(nb, p, b), stored);
             }
             if (b < nb) {
                 uint32_t *to = H.vq + v_word(nb, 8 * o, d);
@@ -216,55 +222,324 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
     if (row >= (size_t)n * c.nkv) return;
     const int d = (int)(i % c.hd), h = (int)(row % c.nkv), p = pos + (int)(row / c.nkv), b = d >> 5;
     const Head H = head_of(c, nb, sbytes(DT), h);
-    if (k) k[i] = code_value<DT>(H.kq[k_word(nb, p, d & ~7)] >> nib(DT, d & 7) & 15) * scale_value<DT>(H.ks, scale_at(nb, p, b));
-    if (v) v[i] = code_value<DT>(H.vq[v_word(nb, p, d)] >> nib(DT, p & 7) & 15) * scale_value<DT>(H.vs, scale_at(nb, p, b));
+    if (k) k[i] = code_value<DT>(H.kq[k_word(nb, p, d & ~7)] >> nib(DT, d & 7) & 15) * scale_value<DT>(H.ks, k_scale<DT>(nb, p, b));
+    if (v) v[i] = code_value<DT>(H.vq[v_word(nb, p, d)] >> nib(DT, p & 7) & 15) * scale_value<DT>(H.vs, v_scale(nb, p, b));
 }
 
 // ---------------------------------------------------------------- attention
-// One wavefront a (token, query head): 64 positions at a time, a lane scores one, then holds dimensions lane, lane + 64, .. of the
-// output; running maximum and sum.
-template <int DT> __global__ void __launch_bounds__(64) k_kv4_attend(float *out, const float *q, l3m_kv4 c, int nq, int pos) {
-    __shared__ float q_s[HD_MAX], p_s[64];
-    const int lane = threadIdx.x, hd = c.hd, nb = (hd + 31) >> 5, t = (int)(blockIdx.x / nq), hq = (int)(blockIdx.x % nq), seen = pos + t + 1;
-    const Head H = head_of(c, nb, sbytes(DT), hq / (nq / c.nkv));
-    for (int d = lane; d < HD_MAX; d += 64) q_s[d] = d < hd ? q[(size_t)blockIdx.x * hd + d] / sqrtf((float)hd) : 0.f;
-    float m = -INFINITY, l = 0.f, o[HD_MAX / 64] = {};
-    __syncthreads();
-    for (int p0 = 0; p0 < seen; p0 += 64) {
-        const int p = p0 + lane;
-        float s = -INFINITY;
-        if (p < seen) {
-            s = 0.f;
-            for (int b = 0; b < nb; b++) {
-                float dot = 0.f;
-                for (int ch = 0; ch < 4; ch++) {
-                    const uint32_t w = H.kq[k_word(nb, p, 32 * b + 8 * ch)];
-                    for (int i = 0; i < 8; i++) dot = fmaf(q_s[32 * b + 8 * ch + i], code_value<DT>(w >> nib(DT, i) & 15), dot);
-                }
-                s = fmaf(dot, scale_value<DT>(H.ks, scale_at(nb, p, b)), s);
+// Rows: the n g (token, query head) pairs of a kv head, a token's heads side by side (g = nq / nkv); 16 are a product's columns. Per tile of
+// 32 positions and wavefront, with the keys as the left operand so that lane 16 g4 + r holds the scores of row r for positions
+// 8 g4 .. 8 g4 + 7, which is where the second product wants the weights:
+//   S = K Q^T   16 positions x 16 rows x 32 dimensions (v_mfma_f32_16x16x32_bf16), twice a block; q scaled by log2(e) / sqrt(hd), in three
+//               bf16 parts (8 + 8 + 8 bits: exact). mxfp4: a lane's word is one position's, so its scale goes into the conversion of the
+//               codes, exactly, and the blocks add up in one accumulator; q4_0: codes 0 .. 15, begun at -8 sum q, a block's sum times d.
+//   P = 2^(S - m), m the rows' running maximum, moved only when a score passes it by 8 (weights then stay below 2^8)
+//   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions. A position's scale differs from block to block and multiplies P, in
+//               32 bits; the product is then held in two bf16 parts, off by 2^-18 at most. q4_0's -8 is a product of its own with the same
+//               parts, so what they lose is lost in proportion to the value, not to the code.
+// All sums in 32 bits. A workgroup's four wavefronts share 16 CT rows and split the tiles; they meet in LDS, and the workgroups of a
+// long cache (splits > 1) in the workspace, added in order by k_kv4_join.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int WAVES = 4;
+constexpr float M0 = -3e38f;                                         // below every score
+
+// A word's eight codes (q4_0: 0 .. 15; mxfp4: times scale, a power of two) in bf16, exactly. q4_0: a nibble alone in a byte is the e4m3
+// number 2^-9 times it.
+template <int DT> __device__ __forceinline__ bf16x8 widen(uint32_t w, float scale) {
+    bf16x2 p[4];
+    if constexpr (DT == L3M_Q4_0) {
+        const int lo = (int)(w & 0x0F0F0F0Fu), hi = (int)(w >> 4 & 0x0F0F0F0Fu);
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+    }
+    return bf16x8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+}
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// Byte i of w as the power of two that it is the exponent of.
+__device__ __forceinline__ float pow2_byte(uint32_t w, int i) {
+    return __uint_as_float((i < 3 ? w << (23 - 8 * i) : w >> 1) & 0x7F800000u);
+}
+
+// What a lane reads of a tile's keys: its words of the two halves, and the scales of its positions 8 g4 .. (q4_0) or of the position its
+// words belong to (mxfp4).
+template <int DT, int NB> struct KeysIn {
+    uint32_t q[2][NB], e[(2 * NB + 3) / 4];
+    f16x8    d[DT == L3M_Q4_0 ? NB : 1];
+    __device__ __forceinline__ void load(const Head &H, int tile, int lane) {
+        const size_t T = (size_t)tile;
+        __builtin_memcpy(q[0], __builtin_assume_aligned(H.kq + (T * 128 + lane) * NB, 4), 4 * NB);
+        __builtin_memcpy(q[1], __builtin_assume_aligned(H.kq + (T * 128 + 64 + lane) * NB, 4), 4 * NB);
+        if constexpr (DT == L3M_Q4_0) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) d[b] = *(const f16x8 *)(H.ks + 2 * ((T * NB + b) * TILE + 8 * (lane >> 4)));
+        } else __builtin_memcpy(e, __builtin_assume_aligned(H.ks + (T * 16 + (lane & 15)) * 2 * NB, 2), 2 * NB);
+    }
+};
+// Of its values: its dimensions' words, and the scales of its positions.
+template <int DT, int NB> struct ValuesIn {
+    uint32_t q[2 * NB], e[NB][2];
+    f16x8    d[DT == L3M_Q4_0 ? NB : 1];
+    __device__ __forceinline__ void load(const Head &H, int tile, int lane) {
+        const size_t T = (size_t)tile;
+        __builtin_memcpy(q, __builtin_assume_aligned(H.vq + (T * 64 + lane) * 2 * NB, 4), 8 * NB);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if constexpr (DT == L3M_Q4_0) d[b] = *(const f16x8 *)(H.vs + 2 * ((T * NB + b) * TILE + 8 * (lane >> 4)));
+            else __builtin_memcpy(e[b], __builtin_assume_aligned(H.vs + (T * NB + b) * TILE + 8 * (lane >> 4), 8), 8);
+        }
+    }
+};
+
+struct AttendIn {
+    float       *out, *parts;
+    const float *q;
+    l3m_kv4      c;
+    int          n, nq, pos, groups, splits;
+};
+// Floats of the workspace's part of `rows` rows: the rows' outputs, then their maxima and sums.
+__host__ __device__ constexpr size_t part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
+
+template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) k_kv4_attend(AttendIn a) {
+    constexpr int ROWS = 16 * CT, OS = 32 * NB + 4;                  // a row's stride in LDS
+    __shared__ float o_s[WAVES / 2][ROWS][OS], m_s[WAVES][ROWS], l_s[WAVES][ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4, hd = a.c.hd, nkv = a.c.nkv, g = a.nq / nkv;
+    // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each. The longest rows first.
+    const int h = (int)(blockIdx.x % nkv), rest = (int)(blockIdx.x / nkv), split = rest % a.splits, group = a.groups - 1 - rest / a.splits;
+    const long long R = (long long)a.n * g, row0 = (long long)group * ROWS;
+    const int first = (int)(row0 / g), last = (int)(min(row0 + ROWS, R) - 1) / g;                   // tokens of the first and last row
+    const int tiles = (a.pos + last + TILE) / TILE, whole = (a.pos + first + 1) / TILE;              // tiles seen; those with nothing masked
+    const int part = split * WAVES + wave, of = a.splits * WAVES;
+    const int t0 = (int)((long long)tiles * part / of), t1 = (int)((long long)tiles * (part + 1) / of);
+    const Head H = head_of(a.c, NB, sbytes(DT), h);
+
+    bf16x8 qp[CT][NB][3];
+    float  q8[CT][NB];                                               // -8 sum of a block's q
+    int    seen[CT];                                                 // positions a row sees
+    const float scale = 1.44269504f / sqrtf((float)hd);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const long long r = row0 + 16 * ct + r16;
+        const int t = (int)(min(r, R - 1) / g), hq = h * g + (int)(min(r, R - 1) % g);
+        seen[ct] = a.pos + t + 1;
+        const float *q = a.q + ((size_t)t * a.nq + hq) * hd;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const int d = 32 * b + 8 * g4;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float x = d < hd ? q[d + i] * scale : 0.f;
+                const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), rem = x - hi, mid = __uint_as_float(__float_as_uint(rem) & 0xFFFF0000u);
+                qp[ct][b][0][i] = (__bf16)hi;
+                qp[ct][b][1][i] = (__bf16)mid;
+                qp[ct][b][2][i] = (__bf16)(rem - mid);
+                sum += x;
+            }
+            if constexpr (DT == L3M_Q4_0) {
+                sum += __shfl_xor(sum, 16);
+                sum += __shfl_xor(sum, 32);
+                q8[ct][b] = -8.f * sum;
             }
         }
-        float top = s;
-        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-        const float nm = fmaxf(m, top), base = nm == -INFINITY ? 0.f : nm, f = expf(m - base), e = p < seen ? expf(s - base) : 0.f;
-        float sum = e;
-        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-        l = l * f + sum;
-        m = nm;
-        p_s[lane] = e;
-        __syncthreads();
-        const int cnt = min(64, seen - p0);
-        for (int i = 0; i < HD_MAX / 64; i++) {
-            const int d = lane + 64 * i;
-            if (d >= hd) break;
-            o[i] *= f;
-            for (int j = 0; j < cnt; j++)
-                o[i] = fmaf(p_s[j], code_value<DT>(H.vq[v_word(nb, p0 + j, d)] >> nib(DT, (p0 + j) & 7) & 15) * scale_value<DT>(H.vs, scale_at(nb, p0 + j, d >> 5)), o[i]);
+    }
+
+    f32x4 acc[CT][2 * NB], off[CT][NB];
+    float m[CT], l[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        m[ct] = M0;
+        l[ct] = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2 * NB; t++) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NB; b++) off[ct][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const __bf16 m8 = (__bf16)-8.f;
+    const bf16x8 minus8 = {m8, m8, m8, m8, m8, m8, m8, m8};
+
+    KeysIn<DT, NB> keys;
+    ValuesIn<DT, NB> vals;
+    if (t0 < t1) keys.load(H, t0, lane);
+    for (int tile = t0; tile < t1; tile++) {
+        vals.load(H, tile, lane);
+        float s[CT][8];
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            f32x4 c[CT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) c[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const int e = f * NB + b;
+                const bf16x8 k = widen<DT>(keys.q[f][b], DT == L3M_Q4_0 ? 1.f : pow2_byte(keys.e[e / 4], e & 3));
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    if constexpr (DT == L3M_Q4_0) {
+                        f32x4 x = {q8[ct][b], q8[ct][b], q8[ct][b], q8[ct][b]};
+#pragma unroll
+                        for (int i = 0; i < 3; i++) x = mfma(k, qp[ct][b][i], x);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) c[ct][r] = fmaf(x[r], (float)keys.d[b][4 * f + r], c[ct][r]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 3; i++) c[ct] = mfma(k, qp[ct][b][i], c[ct]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[ct][4 * f + r] = c[ct][r];
         }
+        keys.load(H, min(tile + 1, t1 - 1), lane);
+        const bool masked = tile >= whole;
+        const int p0 = tile * TILE + 8 * g4;
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            if (masked)
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[ct][i] = p0 + i < seen[ct] ? s[ct][i] : -INFINITY;
+            float top = fmaxf(fmaxf(fmaxf(s[ct][0], s[ct][1]), fmaxf(s[ct][2], s[ct][3])), fmaxf(fmaxf(s[ct][4], s[ct][5]), fmaxf(s[ct][6], s[ct][7])));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const bool move = top > m[ct] + 8.f;
+            if (__ballot(move)) {
+                const float nm = move ? top : m[ct], f = __builtin_amdgcn_exp2f(m[ct] - nm);
+                m[ct] = nm;
+                l[ct] *= f;
+#pragma unroll
+                for (int t = 0; t < 2 * NB; t++) acc[ct][t] *= f;
+                if constexpr (DT == L3M_Q4_0)
+#pragma unroll
+                    for (int b = 0; b < NB; b++) off[ct][b] *= f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                s[ct][i] = __builtin_amdgcn_exp2f(s[ct][i] - m[ct]);
+                l[ct] += s[ct][i];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float d[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if constexpr (DT == L3M_Q4_0) d[i] = (float)vals.d[b][i];
+                else d[i] = pow2_byte(vals.e[b][i >> 2], i & 3);
+            }
+            const bf16x8 v0 = widen<DT>(vals.q[2 * b], 1.f), v1 = widen<DT>(vals.q[2 * b + 1], 1.f);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                bf16x8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    f32x2 w = {s[ct][i] * d[i], s[ct][i + 1] * d[i + 1]};
+                    if (masked) {                                    // what a masked position's scale is does not matter
+                        w.x = p0 + i < seen[ct] ? w.x : 0.f;
+                        w.y = p0 + i + 1 < seen[ct] ? w.y : 0.f;
+                    }
+                    const bf16x2 hh = __builtin_convertvector(w, bf16x2);
+                    const uint32_t u = __builtin_bit_cast(uint32_t, hh);
+                    const f32x2 rem = {w.x - __uint_as_float(u << 16), w.y - __uint_as_float(u & 0xFFFF0000u)};
+                    const bf16x2 ll = __builtin_convertvector(rem, bf16x2);
+                    hi[i] = hh.x; hi[i + 1] = hh.y;
+                    lo[i] = ll.x; lo[i + 1] = ll.y;
+                }
+                acc[ct][2 * b] = mfma(v0, lo, mfma(v0, hi, acc[ct][2 * b]));
+                acc[ct][2 * b + 1] = mfma(v1, lo, mfma(v1, hi, acc[ct][2 * b + 1]));
+                if constexpr (DT == L3M_Q4_0) off[ct][b] = mfma(minus8, lo, mfma(minus8, hi, off[ct][b]));
+            }
+        }
+    }
+
+    // the wavefronts' parts at their common maximum
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        l[ct] += __shfl_xor(l[ct], 16);
+        l[ct] += __shfl_xor(l[ct], 32);
+        if (g4 == 0) {
+            m_s[wave][16 * ct + r16] = m[ct];
+            l_s[wave][16 * ct + r16] = l[ct];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int half = 1; half >= 0; half--) {                          // wavefronts 2 and 3, then 0 and 1 onto them
+        if (wave >> 1 == half)
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const int r = 16 * ct + r16;
+                float top = m_s[0][r];
+#pragma unroll
+                for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][r]);
+                const float f = __builtin_amdgcn_exp2f(m[ct] - top);
+#pragma unroll
+                for (int t = 0; t < 2 * NB; t++) {
+                    f32x4 x = acc[ct][t];
+                    if constexpr (DT == L3M_Q4_0) x += off[ct][t >> 1];
+                    f32x4 &to = *(f32x4 *)&o_s[wave & 1][r][16 * t + 4 * g4];
+                    to = half ? x * f : to + x * f;
+                }
+            }
         __syncthreads();
     }
+    const int rows = (int)min(R - row0, (long long)ROWS), quads = hd >> 2;
+    float *po = a.parts + (((size_t)group * nkv + h) * a.splits + split) * part_floats(min(R, (long long)ROWS), hd), *pml = po + (size_t)rows * hd;
+    for (int i = threadIdx.x; i < rows * quads; i += 64 * WAVES) {
+        const int r = i / quads, d = 4 * (i - r * quads);
+        float top = m_s[0][r], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][r]);
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) sum = fmaf(l_s[w][r], __builtin_amdgcn_exp2f(m_s[w][r] - top), sum);
+        const f32x4 x = *(const f32x4 *)&o_s[0][r][d] + *(const f32x4 *)&o_s[1][r][d];
+        if (a.splits == 1) {
+            const long long row = row0 + r;
+            float *to = a.out + ((size_t)(row / g) * a.nq + h * g + (int)(row % g)) * hd + d;
+#pragma unroll
+            for (int j = 0; j < 4; j++) to[j] = x[j] / sum;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) po[(size_t)r * hd + d + j] = x[j];
+            if (d == 0) { pml[2 * r] = top; pml[2 * r + 1] = sum; }
+        }
+    }
+}
+
+// The splits' parts of a row, one wavefront a (token, query head), added in the splits' order.
+__global__ void __launch_bounds__(64) k_kv4_join(AttendIn a, int per) {
+    const int lane = threadIdx.x, hd = a.c.hd, nkv = a.c.nkv, g = a.nq / nkv, hq = (int)(blockIdx.x % a.nq), h = hq / g;
+    const long long row = (long long)(blockIdx.x / a.nq) * g + hq % g, R = (long long)a.n * g;
+    const int group = (int)(row / per), r = (int)(row - (long long)group * per), rows = (int)min(R - (long long)group * per, (long long)per);
+    const size_t size = part_floats((int)min(R, (long long)per), hd);
+    const float *part = a.parts + ((size_t)group * nkv + h) * a.splits * size;
+    float top = M0;
+    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, part[s * size + (size_t)rows * hd + 2 * r]);
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    float sum = 0.f, o[HD_MAX / 64] = {};
+    for (int s = 0; s < a.splits; s++) {
+        const float *p = part + s * size, f = __builtin_amdgcn_exp2f(p[(size_t)rows * hd + 2 * r] - top);
+        sum = fmaf(p[(size_t)rows * hd + 2 * r + 1], f, sum);
+#pragma unroll
+        for (int i = 0; i < HD_MAX / 64; i++)
+            if (lane + 64 * i < hd) o[i] = fmaf(p[(size_t)r * hd + lane + 64 * i], f, o[i]);
+    }
+#pragma unroll
     for (int i = 0; i < HD_MAX / 64; i++)
-        if (lane + 64 * i < hd) out[(size_t)blockIdx.x * hd + lane + 64 * i] = o[i] / l;
+        if (lane + 64 * i < hd) a.out[(size_t)blockIdx.x * hd + lane + 64 * i] = o[i] / sum;
 }
 
 // ---------------------------------------------------------------- argument checks
@@ -307,6 +582,24 @@ template <int DT> void launch_rows_in(const RowsIn &a, const l3m_kv4 &c, hipStre
     long long items = (long long)a.n * (a.nq + a.nkv);
     if (DT >= 0) items += (long long)(((a.pos + a.n - 1) >> 3) - (a.pos >> 3) + 1) * a.nkv;
     hipLaunchKernelGGL(k_rows_in<DT>, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, a, c);
+}
+// Columns of 16 rows a workgroup takes of a kv head's `rows`.
+int tile_columns(int hd, long long rows) { return rows > 16 && hd <= 128 ? 2 : 1; }
+constexpr int SPLIT_WGS = 512;                                       // workgroups up to which a cache is split
+template <int DT> void launch_attend(const AttendIn &a, int ct, hipStream_t st) {
+    const dim3 grid((unsigned)((long long)a.c.nkv * a.groups * a.splits)), wg(64 * WAVES);
+#define ATTEND(NB, CT) hipLaunchKernelGGL((k_kv4_attend<DT, NB, CT>), grid, wg, 0, st, a)
+    switch ((a.c.hd + 31) / 32) {
+    case 1: if (ct == 1) ATTEND(1, 1); else ATTEND(1, 2); break;
+    case 2: if (ct == 1) ATTEND(2, 1); else ATTEND(2, 2); break;
+    case 3: if (ct == 1) ATTEND(3, 1); else ATTEND(3, 2); break;
+    case 4: if (ct == 1) ATTEND(4, 1); else ATTEND(4, 2); break;
+    case 5: ATTEND(5, 1); break;
+    case 6: ATTEND(6, 1); break;
+    case 7: ATTEND(7, 1); break;
+    default: ATTEND(8, 1); break;
+    }
+#undef ATTEND
 }
 constexpr long long MAX_ITEMS = (1ll << 26) - 4;                     // wavefronts of a launch (its threads are counted in 32 bits)
 
@@ -363,8 +656,9 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
 }
 
 size_t l3m_kv4_work_bytes(const l3m_kv4 *c, int n, int nq) {
-    if (kv4_bad(c) || n < 1 || n > c->cap || nq < 1 || nq % c->nkv) return 0;
-    return 256;
+    if (kv4_bad(c) || n < 1 || n > c->cap || nq < 1 || nq > 65536 || nq % c->nkv) return 0;
+    const size_t rows = (size_t)n * (nq / c->nkv), most = 16 * tile_columns(c->hd, 17);
+    return 4 * (size_t)SPLIT_WGS * part_floats((int)(rows < most ? rows : most), c->hd);
 }
 
 int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq, int pos, void *work, size_t work_bytes, void *stream) {
@@ -376,8 +670,15 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
         return l3m_dev_fail("kv4_attend: q and out must be floats, the same or apart");
     if (!work || (uintptr_t)work % 16 || work_bytes < l3m_kv4_work_bytes(c, n, nq)) return l3m_dev_fail("kv4_attend: the workspace is too small (l3m_kv4_work_bytes)");
     if (rows > (size_t)MAX_ITEMS) return l3m_dev_fail("kv4_attend: too many rows for one call");
-    if (c->dtype == L3M_Q4_0) hipLaunchKernelGGL(k_kv4_attend<L3M_Q4_0>, dim3((unsigned)rows), dim3(64), 0, as_stream(stream), out, q, *c, nq, pos);
-    else hipLaunchKernelGGL(k_kv4_attend<L3M_MXFP4>, dim3((unsigned)rows), dim3(64), 0, as_stream(stream), out, q, *c, nq, pos);
+    const long long R = (long long)n * (nq / c->nkv);
+    const int per = 16 * tile_columns(c->hd, R), groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;
+    const long long alone = (long long)c->nkv * groups;
+    const int most = (tiles + WAVES - 1) / WAVES, splits = alone >= SPLIT_WGS ? 1 : (int)(SPLIT_WGS / alone < most ? SPLIT_WGS / alone : most);
+    const AttendIn a = {out, (float *)work, q, *c, n, nq, pos, groups, splits};
+    hipStream_t st = as_stream(stream);
+    if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, per / 16, st);
+    else launch_attend<L3M_MXFP4>(a, per / 16, st);
+    if (splits > 1) hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)rows), dim3(64), 0, st, a, per);
     return l3m_dev_launched("k_kv4_attend");
 }
 

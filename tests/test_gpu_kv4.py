@@ -54,26 +54,37 @@ def table_of(ctx, hd):
     return t.reshape(ctx, hd // 2, 2)
 
 
-def attended(q, k, v, pos):
+def summed(dtype, x):
+    """The magnitude of the terms a sum over x's codes is made of. mxfp4: |x|. q4_0: x = (u - 8) d is summed as u d, u in 0..15, and -8 d; the
+    block's largest value has u = 0, so |8 d| is its magnitude, and a partial sum's terms are at most |u d| + |8 d| <= |x| + 2 |8 d|."""
+    if dtype == MXFP4:
+        return np.abs(x)
+    wide = np.abs(x)
+    for b in range(0, x.shape[-1], 32):
+        wide[..., b:b + 32] += 2 * wide[..., b:b + 32].max(-1, keepdims=True)
+    return wide
+
+
+def attended(dtype, q, k, v, pos):
     """out and the bound of its error: q [n][nq][hd], k, v [pos + n][nkv][hd] in 64 bits.
 
-    A score is a sum of hd products in float32: off by (hd + 16) 2^-24 of the sum of their magnitudes A at most; a weight by twice that
-    (itself and the sum's). An output adds 2^-17 for the two 8-bit parts a weight is held in with its scale, and a float32 rounding
-    for each of the sums' steps: 32 positions each, and those that join partial results."""
+    A score is a sum of hd products in float32: off by (hd + 16) 2^-24 of the sum of its terms' magnitudes at most; a weight by twice that
+    (itself and the sum's). An output adds 2^-17 of its values for the two 8-bit parts a weight is held in with its scale, and a float32
+    rounding of its terms for each of the sums' steps: 32 positions each, and those that join partial results."""
     n, nq, hd = q.shape
     nkv, g = k.shape[1], q.shape[1] // k.shape[1]
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
     for h in range(nq):
         kh, vh, qh = k[:, h // g], v[:, h // g], q[:, h].astype(np.float64)
         s = qh @ kh.T / np.sqrt(hd)
-        mag = np.abs(qh) @ np.abs(kh).T / np.sqrt(hd)
+        mag = np.abs(qh) @ summed(dtype, kh).T / np.sqrt(hd)
         late = np.arange(len(k))[None] > pos + np.arange(n)[:, None]
         s[late], mag[late] = -np.inf, 0
         p = np.exp(s - s.max(1, keepdims=True))
         p /= p.sum(1, keepdims=True)
         out[:, h] = p @ vh
-        off = 2 * (hd + 16) * 2.0 ** -24 * mag.max(1) + 2.0 ** -17 + (len(k) / 32 + 64) * 2.0 ** -24
-        tol[:, h] = off[:, None] * (p @ np.abs(vh)) + 1e-30
+        off = 2 * (hd + 16) * 2.0 ** -24 * mag.max(1) + 2.0 ** -17
+        tol[:, h] = off[:, None] * (p @ np.abs(vh)) + (len(k) / 32 + 64) * 2.0 ** -24 * (p @ summed(dtype, vh)) + 1e-30
     return out, tol
 
 
@@ -197,7 +208,7 @@ def test_attend_one_token(dev, dtype, hd, nq, nkv):
     for seen in (1, 2, 31, 32, 33, 64, 127, 300, 1025):
         c, k, v, rng = filled(dev, dtype, nkv, hd, seen, hd + seen)
         q = rng.standard_normal((1, nq, hd)).astype(np.float32) * 2
-        near(dev.kv4_attend(c, q, seen - 1), *attended(q, k, v, seen - 1))
+        near(dev.kv4_attend(c, q, seen - 1), *attended(dtype, q, k, v, seen - 1))
         dev.free_all()
 
 
@@ -208,7 +219,7 @@ def test_attend_tokens(dev, dtype, hd, nq, nkv, pos, n):
     c, k, v, rng = filled(dev, dtype, nkv, hd, pos + n, pos + n)
     q = rng.standard_normal((n, nq, hd)).astype(np.float32) * 2
     got = dev.kv4_attend(c, q, pos)
-    near(got, *attended(q, k, v, pos))
+    near(got, *attended(dtype, q, k, v, pos))
     assert np.array_equal(got, dev.kv4_attend(c, q, pos))            # the same sums in the same order
 
 
@@ -218,9 +229,9 @@ def test_attend_long(dev, dtype, seen):
     nq, nkv, hd = 8, 2, 128
     c, k, v, rng = filled(dev, dtype, nkv, hd, seen, seen)
     q = rng.standard_normal((1, nq, hd)).astype(np.float32) * 2
-    near(dev.kv4_attend(c, q, seen - 1), *attended(q, k, v, seen - 1))
+    near(dev.kv4_attend(c, q, seen - 1), *attended(dtype, q, k, v, seen - 1))
     q = rng.standard_normal((3, nq, hd)).astype(np.float32)
-    near(dev.kv4_attend(c, q, seen - 3), *attended(q, k, v, seen - 3))
+    near(dev.kv4_attend(c, q, seen - 3), *attended(dtype, q, k, v, seen - 3))
 
 
 @DTYPES
@@ -235,7 +246,7 @@ def test_attend_leaves_out_what_follows(dev, dtype, hd):
         c0, k, v, _ = filled(dev, dtype, nkv, hd, seen, 5, cap=seen + 90)
         c1 = filled(dev, dtype, nkv, hd, seen, 5, cap=seen + 90, dirty=True)[0]
         want = dev.kv4_attend(c0, q, pos)
-        near(want, *attended(q, k, v, pos))
+        near(want, *attended(dtype, q, k, v, pos))
         assert np.array_equal(dev.kv4_attend(c1, q, pos), want)
         at = pos + n // 2                                             # a key of NaN in the middle, for kv head 1
         bad = np.zeros((1, 2 * nkv * hd), np.float32)
@@ -272,7 +283,7 @@ def test_attend_large_scores(dev, dtype):
         dev.kv4_append(c, rows, 0, 0)
         k, v = (x.astype(np.float64) for x in dev.kv4_rows(c, 0, seen))
         q = np.stack([k[at, 0], -k[at, 0]])[None].astype(np.float32)
-        near(dev.kv4_attend(c, q, seen - 1), *attended(q, k, v, seen - 1))
+        near(dev.kv4_attend(c, q, seen - 1), *attended(dtype, q, k, v, seen - 1))
 
 
 @DTYPES
@@ -287,7 +298,7 @@ def test_attend_mixed_scales(dev, dtype):
     dev.kv4_append(c, rows.reshape(seen, -1), 0, 0)
     k, v = (x.astype(np.float64) for x in dev.kv4_rows(c, 0, seen))
     q = rng.standard_normal((1, nq, hd)).astype(np.float32)
-    near(dev.kv4_attend(c, q, seen - 1), *attended(q, k, v, seen - 1))
+    near(dev.kv4_attend(c, q, seen - 1), *attended(dtype, q, k, v, seen - 1))
 
 
 def test_out_may_be_q(dev):
@@ -331,7 +342,7 @@ def test_planes_past_32_bits(dev, dtype):
             assert np.array_equal(k, stored(dtype, x[:, 0]).astype(np.float32)) and np.array_equal(v, stored(dtype, x[:, 1]).astype(np.float32))
             if pos == 0:
                 q = rng.standard_normal((3, nkv, hd)).astype(np.float32)
-                near(dev.kv4_attend(c, q, 37), *attended(q, k.astype(np.float64), v.astype(np.float64), 37))
+                near(dev.kv4_attend(c, q, 37), *attended(dtype, q, k.astype(np.float64), v.astype(np.float64), 37))
         dev.free_all()
 
 
@@ -404,12 +415,12 @@ def test_prompt_then_steps(dev, dtype):
         q64 = turned(x[:, :nq], w[0], 1e-6, False, table[pos:pos + n])
         assert np.all(np.abs(q - q64) <= np.abs(q64) * 2.0 ** -24 * (1 + 1e-6) + 1e-13)
         got = dev.kv4_attend(c, q, pos)
-        near(got, *attended(q, k, v, pos))
+        near(got, *attended(dtype, q, k, v, pos))
         prompt = (rows, got) if prompt is None else prompt
     c2, at = dev.kv4(dtype, nkv, hd, cap), 0
     for n in (1, 13, 32, 24):
         q = dev.kv4_append(c2, prompt[0][at:at + n], nq, at, *w, 1e-6, False, dt)
-        want, tol = attended(q, k[:at + n], v[:at + n], at)
+        want, tol = attended(dtype, q, k[:at + n], v[:at + n], at)
         got = dev.kv4_attend(c2, q, at)
         near(got, want, tol)
         assert np.all(np.abs(got - prompt[1][at:at + n]) <= 2 * tol)
