@@ -247,6 +247,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
+constexpr int SPLIT_WGS = 512;                                       // workgroups up to which a cache is split
 constexpr float M0 = -3e38f;                                         // below every score
 
 // A word's eight codes (q4_0: 0 .. 15; mxfp4: times scale, a power of two) in bf16, exactly. q4_0: a nibble alone in a byte is the e4m3
@@ -309,21 +310,27 @@ struct AttendIn {
     l3m_kv4      c;
     int          n, nq, pos, groups, splits;
 };
-// Floats of the workspace's part of `rows` rows: the rows' outputs, then their maxima and sums.
-__host__ __device__ constexpr size_t part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
+// Floats of the workspace's part of `rows` rows: the rows' outputs, then their maxima and sums; a multiple of 4.
+__host__ __device__ constexpr size_t part_floats(int rows, int hd) { return (size_t)rows * hd + (2 * rows + 3) / 4 * 4; }
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));                  // q and out need no alignment beyond a float's
 
 template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) k_kv4_attend(AttendIn a) {
     constexpr int ROWS = 16 * CT, OS = 32 * NB + 4;                  // a row's stride in LDS
     __shared__ float o_s[WAVES / 2][ROWS][OS], m_s[WAVES][ROWS], l_s[WAVES][ROWS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4, hd = a.c.hd, nkv = a.c.nkv, g = a.nq / nkv;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each. The longest rows first.
-    const int h = (int)(blockIdx.x % nkv), rest = (int)(blockIdx.x / nkv), split = rest % a.splits, group = a.groups - 1 - rest / a.splits;
-    const long long R = (long long)a.n * g, row0 = (long long)group * ROWS;
-    const int first = (int)(row0 / g), last = (int)(min(row0 + ROWS, R) - 1) / g;                   // tokens of the first and last row
-    const int tiles = (a.pos + last + TILE) / TILE, whole = (a.pos + first + 1) / TILE;              // tiles seen; those with nothing masked
-    const int part = split * WAVES + wave, of = a.splits * WAVES;
-    const int t0 = (int)((long long)tiles * part / of), t1 = (int)((long long)tiles * (part + 1) / of);
+    const int h = (int)(blockIdx.x % (unsigned)nkv), rest = (int)(blockIdx.x / (unsigned)nkv);
+    const int split = (int)((unsigned)rest % (unsigned)a.splits), group = a.groups - 1 - (int)((unsigned)rest / (unsigned)a.splits);
+    const int R = a.n * g, row0 = group * ROWS, rows = min(R - row0, ROWS);
+    const int first = (int)((unsigned)row0 / (unsigned)g), last = (int)((unsigned)(row0 + rows - 1) / (unsigned)g);   // the rows' tokens
+    const unsigned tiles = (unsigned)(a.pos + last + TILE) / TILE, whole = (unsigned)(a.pos + first + 1) / TILE;   // tiles seen; those with nothing masked
+    const unsigned part = (unsigned)(split * WAVES + wave), of = (unsigned)a.splits * WAVES, share = tiles / of, more = tiles % of;
+    const int t0 = (int)(part * share + min(part, more)), t1 = t0 + (int)(share + (part < more));
     const Head H = head_of(a.c, NB, sbytes(DT), h);
+    KeysIn<DT, NB> keys;
+    ValuesIn<DT, NB> vals;
+    keys.load(H, min(t0, (int)tiles - 1), lane);
+    vals.load(H, min(t0, (int)tiles - 1), lane);
 
     bf16x8 qp[CT][NB][3];
     float  q8[CT][NB];                                               // -8 sum of a block's q
@@ -331,17 +338,18 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     const float scale = 1.44269504f / sqrtf((float)hd);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const long long r = row0 + 16 * ct + r16;
-        const int t = (int)(min(r, R - 1) / g), hq = h * g + (int)(min(r, R - 1) % g);
-        seen[ct] = a.pos + t + 1;
-        const float *q = a.q + ((size_t)t * a.nq + hq) * hd;
+        const unsigned r = (unsigned)min(row0 + 16 * ct + r16, R - 1), t = r / (unsigned)g;   // columns past the last row repeat it
+        seen[ct] = a.pos + (int)t + 1;
+        const float *q = a.q + ((size_t)t * a.nq + h * g + (r - t * (unsigned)g)) * hd;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             const int d = 32 * b + 8 * g4;
+            const bool in = d < hd;
+            const f32x4 x0 = *(const f32x4_a4 *)(q + (in ? d : 0)), x1 = *(const f32x4_a4 *)(q + (in ? d + 4 : 4));
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float x = d < hd ? q[d + i] * scale : 0.f;
+                const float x = in ? (i < 4 ? x0[i & 3] : x1[i & 3]) * scale : 0.f;
                 const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), rem = x - hi, mid = __uint_as_float(__float_as_uint(rem) & 0xFFFF0000u);
                 qp[ct][b][0][i] = (__bf16)hi;
                 qp[ct][b][1][i] = (__bf16)mid;
@@ -370,11 +378,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     const __bf16 m8 = (__bf16)-8.f;
     const bf16x8 minus8 = {m8, m8, m8, m8, m8, m8, m8, m8};
 
-    KeysIn<DT, NB> keys;
-    ValuesIn<DT, NB> vals;
-    if (t0 < t1) keys.load(H, t0, lane);
     for (int tile = t0; tile < t1; tile++) {
-        vals.load(H, tile, lane);
         float s[CT][8];
 #pragma unroll
         for (int f = 0; f < 2; f++) {
@@ -405,7 +409,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
                 for (int r = 0; r < 4; r++) s[ct][4 * f + r] = c[ct][r];
         }
         keys.load(H, min(tile + 1, t1 - 1), lane);
-        const bool masked = tile >= whole;
+        const bool masked = tile >= (int)whole;
         const int p0 = tile * TILE + 8 * g4;
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
@@ -463,6 +467,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
                 if constexpr (DT == L3M_Q4_0) off[ct][b] = mfma(minus8, lo, mfma(minus8, hi, off[ct][b]));
             }
         }
+        vals.load(H, min(tile + 1, t1 - 1), lane);
     }
 
     // the wavefronts' parts at their common maximum
@@ -496,10 +501,10 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             }
         __syncthreads();
     }
-    const int rows = (int)min(R - row0, (long long)ROWS), quads = hd >> 2;
-    float *po = a.parts + (((size_t)group * nkv + h) * a.splits + split) * part_floats(min(R, (long long)ROWS), hd), *pml = po + (size_t)rows * hd;
-    for (int i = threadIdx.x; i < rows * quads; i += 64 * WAVES) {
-        const int r = i / quads, d = 4 * (i - r * quads);
+    const unsigned quads = (unsigned)hd >> 2;
+    float *po = a.parts + (((size_t)group * nkv + h) * a.splits + split) * part_floats(min(R, ROWS), hd), *pml = po + rows * hd;
+    for (unsigned i = threadIdx.x; i < rows * quads; i += 64 * WAVES) {
+        const unsigned r = i / quads, d = 4 * (i - r * quads);
         float top = m_s[0][r], sum = 0.f;
 #pragma unroll
         for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][r]);
@@ -507,39 +512,61 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         for (int w = 0; w < WAVES; w++) sum = fmaf(l_s[w][r], __builtin_amdgcn_exp2f(m_s[w][r] - top), sum);
         const f32x4 x = *(const f32x4 *)&o_s[0][r][d] + *(const f32x4 *)&o_s[1][r][d];
         if (a.splits == 1) {
-            const long long row = row0 + r;
-            float *to = a.out + ((size_t)(row / g) * a.nq + h * g + (int)(row % g)) * hd + d;
-#pragma unroll
-            for (int j = 0; j < 4; j++) to[j] = x[j] / sum;
+            const unsigned row = row0 + r, t = row / (unsigned)g;
+            *(f32x4_a4 *)(a.out + ((size_t)t * a.nq + h * g + (row - t * (unsigned)g)) * hd + d) = x / sum;
         } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) po[(size_t)r * hd + d + j] = x[j];
+            *(f32x4 *)(po + r * hd + d) = x;
             if (d == 0) { pml[2 * r] = top; pml[2 * r + 1] = sum; }
         }
     }
 }
 
-// The splits' parts of a row, one wavefront a (token, query head), added in the splits' order.
-__global__ void __launch_bounds__(64) k_kv4_join(AttendIn a, int per) {
-    const int lane = threadIdx.x, hd = a.c.hd, nkv = a.c.nkv, g = a.nq / nkv, hq = (int)(blockIdx.x % a.nq), h = hq / g;
-    const long long row = (long long)(blockIdx.x / a.nq) * g + hq % g, R = (long long)a.n * g;
-    const int group = (int)(row / per), r = (int)(row - (long long)group * per), rows = (int)min(R - (long long)group * per, (long long)per);
-    const size_t size = part_floats((int)min(R, (long long)per), hd);
-    const float *part = a.parts + ((size_t)group * nkv + h) * a.splits * size;
+// The splits' parts of a row, one workgroup a (token, query head): groups of hd / 4 lanes take every so many splits, 16 bytes a lane and
+// eight loads in flight, and meet in LDS in a fixed order.
+__global__ void __launch_bounds__(256) k_kv4_join(AttendIn a, int per) {
+    __shared__ float f_s[SPLIT_WGS], w_s[4][2];
+    __shared__ f32x4 o_s[256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, nkv = a.c.nkv, S = a.splits;
+    const unsigned g = (unsigned)(a.nq / nkv), t = blockIdx.x / (unsigned)a.nq, hq = blockIdx.x % (unsigned)a.nq, h = hq / g;
+    const int R = a.n * (int)g, row = (int)(t * g + hq % g), group = row / per, r = row - group * per, rows = min(R - group * per, per);
+    const size_t size = part_floats(min(R, per), hd);
+    const float *part = a.parts + ((size_t)group * nkv + h) * S * size, *ml = part + rows * hd + 2 * r;
+    const unsigned quads = (unsigned)hd >> 2, groups = 256 / quads, mine = tid / quads, d = 4 * (tid - mine * quads);
+    f32x4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(part + min(mine + i * groups, (unsigned)S - 1) * size + r * hd + d);
     float top = M0;
-    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, part[s * size + (size_t)rows * hd + 2 * r]);
-    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-    float sum = 0.f, o[HD_MAX / 64] = {};
-    for (int s = 0; s < a.splits; s++) {
-        const float *p = part + s * size, f = __builtin_amdgcn_exp2f(p[(size_t)rows * hd + 2 * r] - top);
-        sum = fmaf(p[(size_t)rows * hd + 2 * r + 1], f, sum);
-#pragma unroll
-        for (int i = 0; i < HD_MAX / 64; i++)
-            if (lane + 64 * i < hd) o[i] = fmaf(p[(size_t)r * hd + lane + 64 * i], f, o[i]);
+    for (int s = tid; s < S; s += 256) top = fmaxf(top, f_s[s] = ml[s * size]);
+    for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
+    if (lane == 0) w_s[wave][0] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(w_s[0][0], w_s[1][0]), fmaxf(w_s[2][0], w_s[3][0]));
+    float sum = 0.f;
+    for (int s = tid; s < S; s += 256) {
+        const float f = __builtin_amdgcn_exp2f(f_s[s] - top);
+        sum = fmaf(ml[s * size + 1], f, sum);
+        f_s[s] = f;
     }
+    for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
+    if (lane == 0) w_s[wave][1] = sum;
+    __syncthreads();
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (mine < groups) {
+        for (unsigned s = mine; s < (unsigned)S; s += 8 * groups) {
 #pragma unroll
-    for (int i = 0; i < HD_MAX / 64; i++)
-        if (lane + 64 * i < hd) a.out[(size_t)blockIdx.x * hd + lane + 64 * i] = o[i] / sum;
+            for (int i = 0; i < 8; i++) {
+                const unsigned at = s + i * groups;
+                if (at < (unsigned)S) o += x[i] * f_s[at];
+                x[i] = *(const f32x4 *)(part + min(at + 8 * groups, (unsigned)S - 1) * size + r * hd + d);
+            }
+        }
+        o_s[tid] = o;
+    }
+    __syncthreads();
+    if (tid < (int)quads) {
+        for (unsigned i = 1; i < groups; i++) o += o_s[i * quads + tid];
+        *(f32x4_a4 *)(a.out + (size_t)blockIdx.x * hd + d) = o / ((w_s[0][1] + w_s[1][1]) + (w_s[2][1] + w_s[3][1]));
+    }
 }
 
 // ---------------------------------------------------------------- argument checks
@@ -585,7 +612,6 @@ template <int DT> void launch_rows_in(const RowsIn &a, const l3m_kv4 &c, hipStre
 }
 // Columns of 16 rows a workgroup takes of a kv head's `rows`.
 int tile_columns(int hd, long long rows) { return rows > 16 && hd <= 128 ? 2 : 1; }
-constexpr int SPLIT_WGS = 512;                                       // workgroups up to which a cache is split
 template <int DT> void launch_attend(const AttendIn &a, int ct, hipStream_t st) {
     const dim3 grid((unsigned)((long long)a.c.nkv * a.groups * a.splits)), wg(64 * WAVES);
 #define ATTEND(NB, CT) hipLaunchKernelGGL((k_kv4_attend<DT, NB, CT>), grid, wg, 0, st, a)
@@ -678,7 +704,7 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     hipStream_t st = as_stream(stream);
     if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, per / 16, st);
     else launch_attend<L3M_MXFP4>(a, per / 16, st);
-    if (splits > 1) hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)rows), dim3(64), 0, st, a, per);
+    if (splits > 1) hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)rows), dim3(256), 0, st, a, per);
     return l3m_dev_launched("k_kv4_attend");
 }
 
