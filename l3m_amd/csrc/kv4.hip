@@ -5,14 +5,17 @@
 // with zeros. A tile is laid out as the matrix cores' operands, so a lane's words are one contiguous load and no value crosses lanes:
 //   K codes  [nkv][tile][half 2][lane 64][NB words]   lane 16 c + m, half f: position 8 (m / 4) + 4 f + m % 4, word b its dimensions
 //                                                     32 b + 8 c .. + 7
-//   V codes  [nkv][tile][lane 64][2 NB words]         lane 16 g + j: word t holds dimension 16 t + j of positions 8 g .. 8 g + 7
+//   V codes  [nkv][tile][lane 64][2 NB words]         lane 16 g + j, q4_0: word t holds dimension 16 t + j of positions 8 g .. 8 g + 7;
+//                                                     mxfp4: word 2 b + u dimensions 32 b + j (low) and 32 b + 16 + j of positions
+//                                                     8 g + 4 u .. + 3, a position's two in a byte, which its scale converts
 //   scales   [nkv][tile][NB][32 positions]            f16 d (q4_0), a biased exponent byte (mxfp4); mxfp4's of K [nkv][tile][m 16][f 2][NB],
 //                                                     as the lanes that hold the codes
-// Both codes of a tile and head take 512 NB bytes. Element i of a word's eight (a dimension of K, a position of V) is the nibble at
+// Both codes of a tile and head take 512 NB bytes. Element i of a word's eight (a dimension of K, a position of q4_0's V) is the nibble at
 // bit nib(dt, i): q4_0's masked bytes are then elements 0..3 and 4..7, mxfp4's byte pairs come in order.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 #include "dev.h"
 #include "format.h"
 
@@ -34,15 +37,16 @@ __device__ __forceinline__ Head head_of(const l3m_kv4 &c, int nb, int sb, int h)
     const size_t tiles = ((size_t)c.cap + TILE - 1) / TILE, words = tiles * 128 * nb, scales = tiles * TILE * nb * sb;
     return {(uint32_t *)c.kq + h * words, (uint32_t *)c.vq + h * words, c.ks + h * scales, c.vs + h * scales};
 }
-// The word of K that holds dimensions d .. d + 7 (d a multiple of 8) of position p, of V that holds dimension d of p's eight positions,
-// and the element of the scale of position p's block b.
+// The word of K that holds dimensions d .. d + 7 (d a multiple of 8) of position p; the word of V that holds dimension d of position p, and
+// its bit; the element of the scale of position p's block b.
 __device__ __forceinline__ size_t k_word(int nb, int p, int d) {
     const int w = p & 31, lane = ((d & 31) >> 3) * 16 + (w >> 3) * 4 + (w & 3);
     return ((size_t)(p >> 5) * 128 + ((w >> 2) & 1) * 64 + lane) * nb + (d >> 5);
 }
-__device__ __forceinline__ size_t v_word(int nb, int p, int d) {
-    return ((size_t)(p >> 5) * 64 + ((p & 31) >> 3) * 16 + (d & 15)) * 2 * nb + (d >> 4);
+template <int DT> __device__ __forceinline__ size_t v_word(int nb, int p, int d) {
+    return ((size_t)(p >> 5) * 64 + ((p & 31) >> 3) * 16 + (d & 15)) * 2 * nb + (DT == L3M_Q4_0 ? d >> 4 : 2 * (d >> 5) + ((p >> 2) & 1));
 }
+template <int DT> __device__ __forceinline__ int v_bit(int p, int d) { return DT == L3M_Q4_0 ? nib(DT, p & 7) : 8 * (p & 3) + ((d >> 2) & 4); }
 __device__ __forceinline__ size_t v_scale(int nb, int p, int b) { return ((size_t)(p >> 5) * nb + b) * TILE + (p & 31); }
 template <int DT> __device__ __forceinline__ size_t k_scale(int nb, int p, int b) {
     if constexpr (DT == L3M_Q4_0) return v_scale(nb, p, b);
@@ -197,19 +201,26 @@ template <int DT> __global__ void __launch_bounds__(256) k_rows_in(RowsIn a, l3m
                 const int p = 8 * o + i;
                 x[i] = p >= first && p < end && d < a.hd ? v[(p - a.pos) * a.stride + d] : 0.f;
             }
-            uint32_t word = 0, mine = 0;
+            uint32_t word[2] = {0, 0}, mine[2] = {0, 0};             // mxfp4: the positions' first and second four
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int p = 8 * o + i;
+                const int p = 8 * o + i, u = DT == L3M_Q4_0 ? 0 : i >> 2;
                 if (p < first || p >= end) continue;                 // the same in every lane
                 uint32_t stored;
-                word |= quantize<DT>(x[i], stored) << nib(DT, i);
-                mine |= 15u << nib(DT, i);
+                word[u] |= quantize<DT>(x[i], stored) << v_bit<DT>(i, d);
+                mine[u] |= (DT == L3M_Q4_0 ? 15u : 255u) << (v_bit<DT>(i, 0));
                 if ((d & 31) == 0 && b < nb) put_scale<DT>(H.vs, v_scale(nb, p, b), stored);
             }
-            if (b < nb) {
-                uint32_t *to = H.vq + v_word(nb, 8 * o, d);
-                *to = mine == ~0u ? word : (*to & ~mine) | word;     // the word's other positions stay
+            int u = 0;
+            if constexpr (DT != L3M_Q4_0) {                          // dimensions d and d ^ 16 share words: each lane stores one
+                u = (d >> 4) & 1;
+                word[0] |= (uint32_t)__shfl_xor((int)word[0], 16);
+                word[1] |= (uint32_t)__shfl_xor((int)word[1], 16);
+            }
+            const uint32_t in = u ? word[1] : word[0], bits = u ? mine[1] : mine[0];
+            if (b < nb && bits) {
+                uint32_t *to = H.vq + v_word<DT>(nb, 8 * o + 4 * u, d);
+                *to = bits == ~0u ? in : (*to & ~bits) | in;         // the word's other positions stay
             }
         }
     }
@@ -223,7 +234,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
     const int d = (int)(i % c.hd), h = (int)(row % c.nkv), p = pos + (int)(row / c.nkv), b = d >> 5;
     const Head H = head_of(c, nb, sbytes(DT), h);
     if (k) k[i] = code_value<DT>(H.kq[k_word(nb, p, d & ~7)] >> nib(DT, d & 7) & 15) * scale_value<DT>(H.ks, k_scale<DT>(nb, p, b));
-    if (v) v[i] = code_value<DT>(H.vq[v_word(nb, p, d)] >> nib(DT, p & 7) & 15) * scale_value<DT>(H.vs, v_scale(nb, p, b));
+    if (v) v[i] = code_value<DT>(H.vq[v_word<DT>(nb, p, d)] >> v_bit<DT>(p, d) & 15) * scale_value<DT>(H.vs, v_scale(nb, p, b));
 }
 
 // ---------------------------------------------------------------- attention
@@ -233,10 +244,13 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 //   S = K Q^T   16 positions x 16 rows x 32 dimensions (v_mfma_f32_16x16x32_bf16), twice a block; q scaled by log2(e) / sqrt(hd), in three
 //               bf16 parts (8 + 8 + 8 bits: exact). mxfp4: a lane's word is one position's, so its scale goes into the conversion of the
 //               codes, exactly, and the blocks add up in one accumulator; q4_0: codes 0 .. 15, begun at -8 sum q, a block's sum times d.
-//   P = 2^(S - m), m the rows' running maximum, moved only when a score passes it by 8 (weights then stay below 2^8)
-//   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions. A position's scale differs from block to block and multiplies P, in
-//               32 bits; the product is then held in two bf16 parts, off by 2^-18 at most. q4_0's -8 is a product of its own with the same
-//               parts, so what they lose is lost in proportion to the value, not to the code.
+//   P = 2^(S - m), m near the rows' running maximum: it moves only when a score passes it by 8 (weights then stay below 2^8), and -m is what the
+//               scores' accumulators begin at
+//   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions, P in two bf16 parts, off by 2^-18 at most. A position's scale differs from
+//               block to block: mxfp4's goes into the conversion of its codes, exactly (a layout of its own); q4_0's multiplies P,
+//               in 32 bits, before it is split, and its -8 is a product of its own with the same parts, so what they lose is lost in
+//               proportion to the value, not to the code. Where rows mask positions, mxfp4's scales go into P too: a value that is not
+//               finite meets no row that does not see it.
 // All sums in 32 bits. A workgroup's four wavefronts share 16 CT rows and split the tiles; they meet in LDS, and the workgroups of a
 // long cache (splits > 1) in the workspace, added in order by k_kv4_join.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -248,7 +262,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
 constexpr int SPLIT_WGS = 512;                                       // workgroups up to which a cache is split
-constexpr float M0 = -3e38f;                                         // below every score
+constexpr float M0 = -3e38f;                                         // the maximum of no score: below every one
 
 // A word's eight codes (q4_0: 0 .. 15; mxfp4: times scale, a power of two) in bf16, exactly. q4_0: a nibble alone in a byte is the e4m3
 // number 2^-9 times it.
@@ -270,8 +284,35 @@ template <int DT> __device__ __forceinline__ bf16x8 widen(uint32_t w, float scal
 }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 // Byte i of w as the power of two that it is the exponent of.
-__device__ __forceinline__ float pow2_byte(uint32_t w, int i) {
-    return __uint_as_float((i < 3 ? w << (23 - 8 * i) : w >> 1) & 0x7F800000u);
+__device__ __forceinline__ float pow2_byte(uint32_t w, int i) { return __uint_as_float((w >> 8 * i & 255u) << 23); }
+// Eight float32 values as the sum of two bf16 ones, rounded each.
+__device__ __forceinline__ void two_parts(const float w[8], bf16x8 &hi, bf16x8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const bf16x2 h = __builtin_convertvector((f32x2{w[i], w[i + 1]}), bf16x2);
+        const uint32_t u = __builtin_bit_cast(uint32_t, h);
+        const bf16x2 l = __builtin_convertvector((f32x2{w[i] - __uint_as_float(u << 16), w[i + 1] - __uint_as_float(u & 0xFFFF0000u)}), bf16x2);
+        hi[i] = h.x; hi[i + 1] = h.y;
+        lo[i] = l.x; lo[i + 1] = l.y;
+    }
+}
+// mxfp4 V words of a block, eight positions of dimensions j and 16 + j, a position's scale each, as the two operands.
+__device__ __forceinline__ void widen_v(const uint32_t w[2], const float d[8], bf16x8 &v0, bf16x8 &v1) {
+    uint32_t r[8], a[4], b[4];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        r[4 * u] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u], 0));
+        r[4 * u + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u + 1], 1));
+        r[4 * u + 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u + 2], 2));
+        r[4 * u + 3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u + 3], 3));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        a[i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x05040100u);
+        b[i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x07060302u);
+    }
+    v0 = __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], a[2], a[3]});
+    v1 = __builtin_bit_cast(bf16x8, u32x4{b[0], b[1], b[2], b[3]});
 }
 
 // What a lane reads of a tile's keys: its words of the two halves, and the scales of its positions 8 g4 .. (q4_0) or of the position its
@@ -365,10 +406,11 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     }
 
     f32x4 acc[CT][2 * NB], off[CT][NB];
-    float m[CT], l[CT];
+    float m[CT], lim[CT], l[CT];                                     // what scores are less by; the score that moves it; sum of weights
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        m[ct] = M0;
+        m[ct] = 0.f;
+        lim[ct] = -INFINITY;                                         // a row's first score always does
         l[ct] = 0.f;
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -378,13 +420,15 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     const __bf16 m8 = (__bf16)-8.f;
     const bf16x8 minus8 = {m8, m8, m8, m8, m8, m8, m8, m8};
 
-    for (int tile = t0; tile < t1; tile++) {
+    auto step = [&](const int tile, auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        const int p0 = tile * TILE + 8 * g4;
         float s[CT][8];
 #pragma unroll
         for (int f = 0; f < 2; f++) {
             f32x4 c[CT];
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) c[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int ct = 0; ct < CT; ct++) c[ct] = f32x4{-m[ct], -m[ct], -m[ct], -m[ct]};
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const int e = f * NB + b;
@@ -406,24 +450,22 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) s[ct][4 * f + r] = c[ct][r];
+                for (int r = 0; r < 4; r++) s[ct][4 * f + r] = !MASK || p0 + 4 * f + r < seen[ct] ? c[ct][r] : -INFINITY;
         }
         keys.load(H, min(tile + 1, t1 - 1), lane);
-        const bool masked = tile >= (int)whole;
-        const int p0 = tile * TILE + 8 * g4;
+        bf16x8 hi[CT], lo[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            if (masked)
-#pragma unroll
-                for (int i = 0; i < 8; i++) s[ct][i] = p0 + i < seen[ct] ? s[ct][i] : -INFINITY;
             float top = fmaxf(fmaxf(fmaxf(s[ct][0], s[ct][1]), fmaxf(s[ct][2], s[ct][3])), fmaxf(fmaxf(s[ct][4], s[ct][5]), fmaxf(s[ct][6], s[ct][7])));
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const bool move = top > m[ct] + 8.f;
-            if (__ballot(move)) {
-                const float nm = move ? top : m[ct], f = __builtin_amdgcn_exp2f(m[ct] - nm);
-                m[ct] = nm;
+            if (__ballot(top > lim[ct])) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float up = top > lim[ct] ? top : 0.f, f = __builtin_amdgcn_exp2f(-up);
+                if (top > lim[ct]) lim[ct] = 8.f;
+                m[ct] += up;
                 l[ct] *= f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[ct][i] -= up;
 #pragma unroll
                 for (int t = 0; t < 2 * NB; t++) acc[ct][t] *= f;
                 if constexpr (DT == L3M_Q4_0)
@@ -432,49 +474,55 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                s[ct][i] = __builtin_amdgcn_exp2f(s[ct][i] - m[ct]);
+                s[ct][i] = __builtin_amdgcn_exp2f(s[ct][i]);
                 l[ct] += s[ct][i];
             }
+            if constexpr (DT != L3M_Q4_0 && !MASK) two_parts(s[ct], hi[ct], lo[ct]);
         }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
+            bf16x8 v0, v1;
             float d[8];
+            if constexpr (DT == L3M_Q4_0) {
+                v0 = widen<DT>(vals.q[2 * b], 1.f);
+                v1 = widen<DT>(vals.q[2 * b + 1], 1.f);
+            } else {
+                float one[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if constexpr (DT == L3M_Q4_0) d[i] = (float)vals.d[b][i];
-                else d[i] = pow2_byte(vals.e[b][i >> 2], i & 3);
+                for (int i = 0; i < 8; i++) {
+                    d[i] = pow2_byte(vals.e[b][i >> 2], i & 3);
+                    one[i] = 1.f;
+                }
+                widen_v(&vals.q[2 * b], MASK ? one : d, v0, v1);
             }
-            const bf16x8 v0 = widen<DT>(vals.q[2 * b], 1.f), v1 = widen<DT>(vals.q[2 * b + 1], 1.f);
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                bf16x8 hi, lo;
+                if constexpr (DT == L3M_Q4_0 || MASK) {
+                    float w[8];
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    f32x2 w = {s[ct][i] * d[i], s[ct][i + 1] * d[i + 1]};
-                    if (masked) {                                    // what a masked position's scale is does not matter
-                        w.x = p0 + i < seen[ct] ? w.x : 0.f;
-                        w.y = p0 + i + 1 < seen[ct] ? w.y : 0.f;
+                    for (int i = 0; i < 8; i++) {
+                        w[i] = fmaf(s[ct][i], DT == L3M_Q4_0 ? (float)vals.d[b][i] : d[i], 0.f);
+                        if constexpr (MASK) w[i] = p0 + i < seen[ct] ? w[i] : 0.f;   // whatever a masked position's scale is
                     }
-                    const bf16x2 hh = __builtin_convertvector(w, bf16x2);
-                    const uint32_t u = __builtin_bit_cast(uint32_t, hh);
-                    const f32x2 rem = {w.x - __uint_as_float(u << 16), w.y - __uint_as_float(u & 0xFFFF0000u)};
-                    const bf16x2 ll = __builtin_convertvector(rem, bf16x2);
-                    hi[i] = hh.x; hi[i + 1] = hh.y;
-                    lo[i] = ll.x; lo[i + 1] = ll.y;
+                    two_parts(w, hi[ct], lo[ct]);
                 }
-                acc[ct][2 * b] = mfma(v0, lo, mfma(v0, hi, acc[ct][2 * b]));
-                acc[ct][2 * b + 1] = mfma(v1, lo, mfma(v1, hi, acc[ct][2 * b + 1]));
-                if constexpr (DT == L3M_Q4_0) off[ct][b] = mfma(minus8, lo, mfma(minus8, hi, off[ct][b]));
+                acc[ct][2 * b] = mfma(v0, lo[ct], mfma(v0, hi[ct], acc[ct][2 * b]));
+                acc[ct][2 * b + 1] = mfma(v1, lo[ct], mfma(v1, hi[ct], acc[ct][2 * b + 1]));
+                if constexpr (DT == L3M_Q4_0) off[ct][b] = mfma(minus8, lo[ct], mfma(minus8, hi[ct], off[ct][b]));
             }
         }
         vals.load(H, min(tile + 1, t1 - 1), lane);
-    }
+    };
+    int tile = t0;
+    for (; tile < min(t1, (int)whole); tile++) step(tile, std::false_type{});
+    for (; tile < t1; tile++) step(tile, std::true_type{});
 
     // the wavefronts' parts at their common maximum
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         l[ct] += __shfl_xor(l[ct], 16);
         l[ct] += __shfl_xor(l[ct], 32);
+        if (lim[ct] == -INFINITY) m[ct] = M0;                        // nothing seen
         if (g4 == 0) {
             m_s[wave][16 * ct + r16] = m[ct];
             l_s[wave][16 * ct + r16] = l[ct];
