@@ -3,15 +3,16 @@
 //
 // Layout. Per kv head, tiles of 32 positions; NB = ceil(hd / 32) blocks of 32 dimensions, a last block short of dimensions filled
 // with zeros. A tile is laid out as the matrix cores' operands, so a lane's words are one contiguous load and no value crosses lanes:
-//   K codes  [nkv][tile][half 2][lane 64][NB words]   lane 16 c + m, half f: position 8 (m / 4) + 4 f + m % 4, word b its dimensions
-//                                                     32 b + 8 c .. + 7
-//   V codes  [nkv][tile][lane 64][2 NB words]         lane 16 g + j, q4_0: word t holds dimension 16 t + j of positions 8 g .. 8 g + 7;
-//                                                     mxfp4: word 2 b + u dimensions 32 b + j (low) and 32 b + 16 + j of positions
-//                                                     8 g + 4 u .. + 3, a position's two in a byte, which its scale converts
-//   scales   [nkv][tile][NB][32 positions]            f16 d (q4_0), a biased exponent byte (mxfp4); mxfp4's of K [nkv][tile][m 16][f 2][NB],
-//                                                     as the lanes that hold the codes
-// Both codes of a tile and head take 512 NB bytes. Element i of a word's eight (a dimension of K, a position of q4_0's V) is the nibble at
-// bit nib(dt, i): q4_0's masked bytes are then elements 0..3 and 4..7, mxfp4's byte pairs come in order.
+// Half f of a tile is its positions 8 (m / 4) + 4 f + m % 4, m = 0 .. 15.
+//   K codes   q4_0   [nkv][tile][half 2][lane 64][NB words]    lane 16 c + m: word b holds dimensions 32 b + 8 c .. + 7
+//             mxfp4  [nkv][tile][half 2][NB][m 16][4 words]    a block as it is
+//   V codes   q4_0   [nkv][tile][lane 64][2 NB words]          lane 16 g + j: word t holds dimension 16 t + j of positions 8 g .. 8 g + 7
+//             mxfp4  the same shape                            word 2 b + u: dimensions 32 b + j (low nibbles) and 32 b + 16 + j of
+//                                                              positions 8 g + 4 u .. + 3, a position's two in a byte
+//   scales    q4_0   [nkv][tile][NB][32 positions]             f16 d, of K and of V
+//             mxfp4  [nkv][tile][NB][m 16][half 2] of K, [nkv][tile][NB][32 positions] of V: a biased exponent byte
+// Both codes of a tile and head take 512 NB bytes. Element i of eight dimensions of K, or positions of q4_0's V, is the nibble at bit
+// nib(dt, i): q4_0's masked bytes are then elements 0..3 and 4..7, mxfp4's come in order.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -39,9 +40,12 @@ __device__ __forceinline__ Head head_of(const l3m_kv4 &c, int nb, int sb, int h)
 }
 // The word of K that holds dimensions d .. d + 7 (d a multiple of 8) of position p; the word of V that holds dimension d of position p, and
 // its bit; the element of the scale of position p's block b.
-__device__ __forceinline__ size_t k_word(int nb, int p, int d) {
-    const int w = p & 31, lane = ((d & 31) >> 3) * 16 + (w >> 3) * 4 + (w & 3);
-    return ((size_t)(p >> 5) * 128 + ((w >> 2) & 1) * 64 + lane) * nb + (d >> 5);
+__device__ __forceinline__ int half_of(int p) { return (p >> 2) & 1; }
+__device__ __forceinline__ int row_of(int p) { return ((p & 31) >> 3) * 4 + (p & 3); }
+template <int DT> __device__ __forceinline__ size_t k_word(int nb, int p, int d) {
+    const int b = d >> 5, c = (d & 31) >> 3;
+    if constexpr (DT == L3M_Q4_0) return ((size_t)(p >> 5) * 128 + half_of(p) * 64 + c * 16 + row_of(p)) * nb + b;
+    return ((((size_t)(p >> 5) * 2 + half_of(p)) * nb + b) * 16 + row_of(p)) * 4 + c;
 }
 template <int DT> __device__ __forceinline__ size_t v_word(int nb, int p, int d) {
     return ((size_t)(p >> 5) * 64 + ((p & 31) >> 3) * 16 + (d & 15)) * 2 * nb + (DT == L3M_Q4_0 ? d >> 4 : 2 * (d >> 5) + ((p >> 2) & 1));
@@ -50,8 +54,7 @@ template <int DT> __device__ __forceinline__ int v_bit(int p, int d) { return DT
 __device__ __forceinline__ size_t v_scale(int nb, int p, int b) { return ((size_t)(p >> 5) * nb + b) * TILE + (p & 31); }
 template <int DT> __device__ __forceinline__ size_t k_scale(int nb, int p, int b) {
     if constexpr (DT == L3M_Q4_0) return v_scale(nb, p, b);
-    const int w = p & 31;
-    return (((size_t)(p >> 5) * 16 + (w >> 3) * 4 + (w & 3)) * 2 + ((w >> 2) & 1)) * nb + b;
+    return (((size_t)(p >> 5) * nb + b) * 16 + row_of(p)) * 2 + half_of(p);
 }
 
 template <int DT> __device__ __forceinline__ float scale_value(const uint8_t *s, size_t i) {
@@ -179,7 +182,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_rows_in(RowsIn a, l3m
 #pragma unroll
                 for (int m = 1; m < 8; m <<= 1) code |= (uint32_t)__shfl_xor((int)code, m);
                 if (b < nb) {
-                    if ((d & 7) == 0) H.kq[k_word(nb, p, d)] = code;
+                    if ((d & 7) == 0) H.kq[k_word<DT>(nb, p, d)] = code;
                     if ((d & 31) == 0) put_scale<DT>(H.ks, k_scale<DT>(nb, p, b), stored);
                 }
             }
@@ -233,7 +236,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
     if (row >= (size_t)n * c.nkv) return;
     const int d = (int)(i % c.hd), h = (int)(row % c.nkv), p = pos + (int)(row / c.nkv), b = d >> 5;
     const Head H = head_of(c, nb, sbytes(DT), h);
-    if (k) k[i] = code_value<DT>(H.kq[k_word(nb, p, d & ~7)] >> nib(DT, d & 7) & 15) * scale_value<DT>(H.ks, k_scale<DT>(nb, p, b));
+    if (k) k[i] = code_value<DT>(H.kq[k_word<DT>(nb, p, d & ~7)] >> nib(DT, d & 7) & 15) * scale_value<DT>(H.ks, k_scale<DT>(nb, p, b));
     if (v) v[i] = code_value<DT>(H.vq[v_word<DT>(nb, p, d)] >> v_bit<DT>(p, d) & 15) * scale_value<DT>(H.vs, v_scale(nb, p, b));
 }
 
@@ -241,9 +244,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // Rows: the n g (token, query head) pairs of a kv head, a token's heads side by side (g = nq / nkv); 16 are a product's columns. Per tile of
 // 32 positions and wavefront, with the keys as the left operand so that lane 16 g4 + r holds the scores of row r for positions
 // 8 g4 .. 8 g4 + 7, which is where the second product wants the weights:
-//   S = K Q^T   16 positions x 16 rows x 32 dimensions (v_mfma_f32_16x16x32_bf16), twice a block; q scaled by log2(e) / sqrt(hd), in three
-//               bf16 parts (8 + 8 + 8 bits: exact). mxfp4: a lane's word is one position's, so its scale goes into the conversion of the
-//               codes, exactly, and the blocks add up in one accumulator; q4_0: codes 0 .. 15, begun at -8 sum q, a block's sum times d.
+//   S = K Q^T   16 positions x 16 rows, twice; q scaled by log2(e) / sqrt(hd) and held in parts (below)
 //   P = 2^(S - m), m near the rows' running maximum: it moves only when a score passes it by 8 (weights then stay below 2^8), and -m is what the
 //               scores' accumulators begin at
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions, P in two bf16 parts, off by 2^-18 at most. A position's scale differs from
@@ -259,28 +260,22 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));   // q and out need no alignment beyond a float's
 
 constexpr int WAVES = 4;
 constexpr int SPLIT_WGS = 512;                                       // workgroups up to which a cache is split
 constexpr float M0 = -3e38f;                                         // the maximum of no score: below every one
 
-// A word's eight codes (q4_0: 0 .. 15; mxfp4: times scale, a power of two) in bf16, exactly. q4_0: a nibble alone in a byte is the e4m3
-// number 2^-9 times it.
-template <int DT> __device__ __forceinline__ bf16x8 widen(uint32_t w, float scale) {
-    bf16x2 p[4];
-    if constexpr (DT == L3M_Q4_0) {
-        const int lo = (int)(w & 0x0F0F0F0Fu), hi = (int)(w >> 4 & 0x0F0F0F0Fu);
-        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false);
-        p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true);
-        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false);
-        p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true);
-    } else {
-        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
-        p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
-        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
-        p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
-    }
-    return bf16x8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+// A q4_0 word's eight codes, 0 .. 15, in bf16: a nibble alone in a byte is the e4m3 number 2^-9 times it.
+__device__ __forceinline__ bf16x8 widen(uint32_t w) {
+    const int lo = (int)(w & 0x0F0F0F0Fu), hi = (int)(w >> 4 & 0x0F0F0F0Fu);
+    const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true);
+    const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true);
+    return bf16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
 }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 // Byte i of w as the power of two that it is the exponent of.
@@ -315,21 +310,162 @@ __device__ __forceinline__ void widen_v(const uint32_t w[2], const float d[8], b
     v1 = __builtin_bit_cast(bf16x8, u32x4{b[0], b[1], b[2], b[3]});
 }
 
-// What a lane reads of a tile's keys: its words of the two halves, and the scales of its positions 8 g4 .. (q4_0) or of the position its
-// words belong to (mxfp4).
-template <int DT, int NB> struct KeysIn {
-    uint32_t q[2][NB], e[(2 * NB + 3) / 4];
-    f16x8    d[DT == L3M_Q4_0 ? NB : 1];
+// The scores of one half of a tile, 16 positions x 16 rows, from the queries of a row held in parts (Queries) and what a lane reads of the
+// keys (KeysIn).
+//
+// q4_0: 16x16x32 bf16 products of a block's codes 0 .. 15 with q in three bf16 parts (8 + 8 + 8 bits: exact), begun at -8 sum q; a block's
+// sum times d, which belongs to a position, in 32 bits.
+//
+// mxfp4: 16x16x128 products of the codes as they lie with their scales (v_mfma_scale_f32_16x16x128_f8f6f4, fp4 operand): lane 16 c + m gives
+// block c of position m, and q is the fp6 (e2m3) operand, a block in five parts with scales of their own. A part takes five bits of
+// the block's largest magnitude: with a in [2, 4) units, rounded to 1/4 at most, 1/8 unit is left, which is 4 of the next part's, 32
+// times smaller. Five leave 2^-24 of the largest magnitude. Where a head has one or two blocks, the lane groups past them take
+// other parts of the same blocks.
+template <int DT, int NB> struct KeysIn;
+template <int DT, int NB> struct Queries;
+
+template <int NB> struct KeysIn<L3M_Q4_0, NB> {
+    uint32_t q[2][NB];
+    f16x8    d[NB];                                                  // of positions 8 g4 .. + 7
     __device__ __forceinline__ void load(const Head &H, int tile, int lane) {
         const size_t T = (size_t)tile;
         __builtin_memcpy(q[0], __builtin_assume_aligned(H.kq + (T * 128 + lane) * NB, 4), 4 * NB);
         __builtin_memcpy(q[1], __builtin_assume_aligned(H.kq + (T * 128 + 64 + lane) * NB, 4), 4 * NB);
-        if constexpr (DT == L3M_Q4_0) {
 #pragma unroll
-            for (int b = 0; b < NB; b++) d[b] = *(const f16x8 *)(H.ks + 2 * ((T * NB + b) * TILE + 8 * (lane >> 4)));
-        } else __builtin_memcpy(e, __builtin_assume_aligned(H.ks + (T * 16 + (lane & 15)) * 2 * NB, 2), 2 * NB);
+        for (int b = 0; b < NB; b++) d[b] = *(const f16x8 *)(H.ks + 2 * ((T * NB + b) * TILE + 8 * (lane >> 4)));
     }
 };
+template <int NB> struct Queries<L3M_Q4_0, NB> {
+    bf16x8 part[NB][3];
+    float  off[NB];                                                  // -8 sum of a block's q
+    __device__ __forceinline__ void load(const float *q, int hd, float scale, int lane) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const int d = 32 * b + 8 * (lane >> 4);
+            const bool in = d < hd;
+            const f32x4 x0 = *(const f32x4_a4 *)(q + (in ? d : 0)), x1 = *(const f32x4_a4 *)(q + (in ? d + 4 : 4));
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float x = in ? (i < 4 ? x0[i & 3] : x1[i & 3]) * scale : 0.f;
+                const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), rem = x - hi, mid = __uint_as_float(__float_as_uint(rem) & 0xFFFF0000u);
+                part[b][0][i] = (__bf16)hi;
+                part[b][1][i] = (__bf16)mid;
+                part[b][2][i] = (__bf16)(rem - mid);
+                sum += x;
+            }
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            off[b] = -8.f * sum;
+        }
+    }
+};
+template <int NB, int CT> __device__ __forceinline__ void scores(const KeysIn<L3M_Q4_0, NB> &k, const Queries<L3M_Q4_0, NB> (&q)[CT], int f, f32x4 (&c)[CT]) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const bf16x8 w = widen(k.q[f][b]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            f32x4 x = {q[ct].off[b], q[ct].off[b], q[ct].off[b], q[ct].off[b]};
+#pragma unroll
+            for (int i = 0; i < 3; i++) x = mfma(w, q[ct].part[b][i], x);
+#pragma unroll
+            for (int r = 0; r < 4; r++) c[ct][r] = fmaf(x[r], (float)k.d[b][4 * f + r], c[ct][r]);
+        }
+    }
+}
+
+constexpr int Q_PARTS = 5;
+// Blocks by fours (a product's lane groups); parts that one product takes; products a four.
+template <int NB> struct Mx {
+    static constexpr int fours = (NB + 3) / 4, at_once = NB == 1 ? 4 : NB == 2 ? 2 : 1, times = (Q_PARTS + at_once - 1) / at_once;
+    static __device__ __forceinline__ int block(int four, int group) { return NB <= 2 ? group % NB : min(4 * four + group, NB - 1); }
+};
+template <int NB> struct KeysIn<L3M_MXFP4, NB> {
+    u32x4    q[2][Mx<NB>::fours];
+    uint32_t e[Mx<NB>::fours];                                       // the two halves' exponents
+    __device__ __forceinline__ void load(const Head &H, int tile, int lane) {
+        const size_t T = (size_t)tile;
+#pragma unroll
+        for (int i = 0; i < Mx<NB>::fours; i++) {
+            const int b = Mx<NB>::block(i, lane >> 4), m = lane & 15;
+            q[0][i] = ((const u32x4 *)H.kq)[(T * 2 * NB + b) * 16 + m];
+            q[1][i] = ((const u32x4 *)H.kq)[((T * 2 + 1) * NB + b) * 16 + m];
+            e[i] = ((const uint16_t *)H.ks)[(T * NB + b) * 16 + m];
+        }
+    }
+};
+template <int NB> struct Queries<L3M_MXFP4, NB> {
+    u32x6 part[Mx<NB>::fours][Mx<NB>::times];
+    int   e[Mx<NB>::fours][Mx<NB>::times];
+    __device__ __forceinline__ void load(const float *q, int hd, float scale, int lane) {
+        const int c = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < Mx<NB>::fours; i++) {
+            const int b = Mx<NB>::block(i, c), first = NB == 1 ? c : NB == 2 ? c >> 1 : 0;       // this lane's part of the first product
+            const bool used = NB <= 2 || 4 * i + c < NB;
+            float x[32];
+            uint32_t peak = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int d = 32 * b + 4 * j;
+                const bool in = d < hd;
+                const f32x4 v = *(const f32x4_a4 *)(q + (in ? d : 0));
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    x[4 * j + r] = in ? v[r] * scale : 0.f;
+                    peak = max(peak, __float_as_uint(x[4 * j + r]) & 0x7FFFFFFFu);
+                }
+            }
+            const bool bad = peak >= 0x7F800000u;                    // a scale of NaN for a row that is not finite
+            // The conversions of 32 values take several cycles and may not write over what they read, which the compiler does not see to:
+            // the empty asm statements keep their operands in registers of their own (without them, now and then wrong last parts).
+#pragma unroll
+            for (int t = 0; t < Mx<NB>::times; t++) {
+                part[i][t] = u32x6{0, 0, 0, 0, 0, 0};
+                e[i][t] = 127;
+            }
+#pragma unroll
+            for (int p = 0; p < Q_PARTS; p++) {
+                const int ex = max((int)(peak >> 23) - 1 - 5 * p, 1);
+                const float unit = __uint_as_float((uint32_t)ex << 23);
+                f32x16 even, odd;
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    even[j] = x[2 * j];
+                    odd[j] = x[2 * j + 1];
+                }
+                u32x6 w = __builtin_bit_cast(u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, unit));
+                asm volatile("" : "+v"(w) : "v"(even), "v"(odd), "v"(unit));
+                f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, unit);
+                asm volatile("" : "+v"(back) : "v"(w), "v"(unit));
+#pragma unroll
+                for (int j = 0; j < 32; j++) x[j] -= back[j];
+                const int t = p / Mx<NB>::at_once, at = p - t * Mx<NB>::at_once;
+                if (used && (Mx<NB>::at_once == 1 || first == at)) {
+                    part[i][t] = w;
+                    e[i][t] = bad ? E8M0_NAN : ex;
+                }
+            }
+        }
+    }
+};
+template <int NB, int CT> __device__ __forceinline__ void scores(const KeysIn<L3M_MXFP4, NB> &k, const Queries<L3M_MXFP4, NB> (&q)[CT], int f, f32x4 (&c)[CT]) {
+#pragma unroll
+    for (int i = 0; i < Mx<NB>::fours; i++) {
+        const i32x8 a = {(int)k.q[f][i].x, (int)k.q[f][i].y, (int)k.q[f][i].z, (int)k.q[f][i].w, 0, 0, 0, 0};
+        const int   e = (int)(k.e[i] >> 8 * f);
+#pragma unroll
+        for (int t = 0; t < Mx<NB>::times; t++)
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const u32x6 &w = q[ct].part[i][t];
+                const i32x8 b = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], (int)w[4], (int)w[5], 0, 0};
+                c[ct] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c[ct], 4, 2, 0, e, 0, q[ct].e[i][t]);
+            }
+    }
+}
+
 // Of its values: its dimensions' words, and the scales of its positions.
 template <int DT, int NB> struct ValuesIn {
     uint32_t q[2 * NB], e[NB][2];
@@ -353,7 +489,6 @@ struct AttendIn {
 };
 // Floats of the workspace's part of `rows` rows: the rows' outputs, then their maxima and sums; a multiple of 4.
 __host__ __device__ constexpr size_t part_floats(int rows, int hd) { return (size_t)rows * hd + (2 * rows + 3) / 4 * 4; }
-typedef f32x4 f32x4_a4 __attribute__((aligned(4)));                  // q and out need no alignment beyond a float's
 
 template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) k_kv4_attend(AttendIn a) {
     constexpr int ROWS = 16 * CT, OS = 32 * NB + 4;                  // a row's stride in LDS
@@ -373,36 +508,14 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     keys.load(H, min(t0, (int)tiles - 1), lane);
     vals.load(H, min(t0, (int)tiles - 1), lane);
 
-    bf16x8 qp[CT][NB][3];
-    float  q8[CT][NB];                                               // -8 sum of a block's q
-    int    seen[CT];                                                 // positions a row sees
+    Queries<DT, NB> qs[CT];
+    int seen[CT];                                                    // positions a row sees
     const float scale = 1.44269504f / sqrtf((float)hd);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         const unsigned r = (unsigned)min(row0 + 16 * ct + r16, R - 1), t = r / (unsigned)g;   // columns past the last row repeat it
         seen[ct] = a.pos + (int)t + 1;
-        const float *q = a.q + ((size_t)t * a.nq + h * g + (r - t * (unsigned)g)) * hd;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const int d = 32 * b + 8 * g4;
-            const bool in = d < hd;
-            const f32x4 x0 = *(const f32x4_a4 *)(q + (in ? d : 0)), x1 = *(const f32x4_a4 *)(q + (in ? d + 4 : 4));
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float x = in ? (i < 4 ? x0[i & 3] : x1[i & 3]) * scale : 0.f;
-                const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), rem = x - hi, mid = __uint_as_float(__float_as_uint(rem) & 0xFFFF0000u);
-                qp[ct][b][0][i] = (__bf16)hi;
-                qp[ct][b][1][i] = (__bf16)mid;
-                qp[ct][b][2][i] = (__bf16)(rem - mid);
-                sum += x;
-            }
-            if constexpr (DT == L3M_Q4_0) {
-                sum += __shfl_xor(sum, 16);
-                sum += __shfl_xor(sum, 32);
-                q8[ct][b] = -8.f * sum;
-            }
-        }
+        qs[ct].load(a.q + ((size_t)t * a.nq + h * g + (r - t * (unsigned)g)) * hd, hd, scale, lane);
     }
 
     f32x4 acc[CT][2 * NB], off[CT][NB];
@@ -429,24 +542,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             f32x4 c[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) c[ct] = f32x4{-m[ct], -m[ct], -m[ct], -m[ct]};
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const int e = f * NB + b;
-                const bf16x8 k = widen<DT>(keys.q[f][b], DT == L3M_Q4_0 ? 1.f : pow2_byte(keys.e[e / 4], e & 3));
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++) {
-                    if constexpr (DT == L3M_Q4_0) {
-                        f32x4 x = {q8[ct][b], q8[ct][b], q8[ct][b], q8[ct][b]};
-#pragma unroll
-                        for (int i = 0; i < 3; i++) x = mfma(k, qp[ct][b][i], x);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) c[ct][r] = fmaf(x[r], (float)keys.d[b][4 * f + r], c[ct][r]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 3; i++) c[ct] = mfma(k, qp[ct][b][i], c[ct]);
-                    }
-                }
-            }
+            scores<NB, CT>(keys, qs, f, c);
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
@@ -484,8 +580,8 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             bf16x8 v0, v1;
             float d[8];
             if constexpr (DT == L3M_Q4_0) {
-                v0 = widen<DT>(vals.q[2 * b], 1.f);
-                v1 = widen<DT>(vals.q[2 * b + 1], 1.f);
+                v0 = widen(vals.q[2 * b]);
+                v1 = widen(vals.q[2 * b + 1]);
             } else {
                 float one[8];
 #pragma unroll
@@ -675,6 +771,12 @@ template <int DT> void launch_attend(const AttendIn &a, int ct, hipStream_t st) 
     }
 #undef ATTEND
 }
+// Workgroups that share a kv head's positions, `alone` of them without a split. A split costs the join, about 5 us, a tile about 0.2 us a block
+// and wavefront: up to 96 blocks one workgroup goes alone.
+int split_count(long long alone, int tiles, int nb, bool few_rows) {
+    const long long room = (few_rows ? SPLIT_WGS : SPLIT_WGS / 2) / alone, most = (tiles + WAVES - 1) / WAVES;
+    return (long long)tiles * nb <= 96 || room < 2 ? 1 : (int)(room < most ? room : most);
+}
 constexpr long long MAX_ITEMS = (1ll << 26) - 4;                     // wavefronts of a launch (its threads are counted in 32 bits)
 
 }  // namespace
@@ -747,7 +849,7 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     const long long R = (long long)n * (nq / c->nkv);
     const int per = 16 * tile_columns(c->hd, R), groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;
     const long long alone = (long long)c->nkv * groups;
-    const int most = (tiles + WAVES - 1) / WAVES, splits = alone >= SPLIT_WGS ? 1 : (int)(SPLIT_WGS / alone < most ? SPLIT_WGS / alone : most);
+    const int splits = split_count(alone, tiles, (c->hd + 31) / 32 * (per / 16), R <= 16);
     const AttendIn a = {out, (float *)work, q, *c, n, nq, pos, groups, splits};
     hipStream_t st = as_stream(stream);
     if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, per / 16, st);
