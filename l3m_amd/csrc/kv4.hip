@@ -70,30 +70,86 @@ template <int DT> __device__ __forceinline__ float code_value(uint32_t c) {
 }
 
 // ---------------------------------------------------------------- writer
-// Blocks of 32 values, one a lane of half a wavefront: this lane's code, and the block's scale as it is stored (the same in every
-// lane). The file formats' rounding to the nearest (l3m_quantize_row), in the same float32 steps, so the stored bytes do not depend on
+template <int M> __device__ __forceinline__ uint32_t quad_xor(uint32_t x) {                 // lane ^ M's, M 1 or 2
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, M == 1 ? 0xB1 : 0x4E, 0xF, 0xF, true);
+}
+__device__ __forceinline__ void wave_sync() {                        // LDS values pass between a wavefront's lanes
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// x of another lane of the row of 16 (DPP), added.
+template <int CTRL> __device__ __forceinline__ double dpp_add(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+    return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// The sum over each 1 << lg lanes, in all of them.
+__device__ __forceinline__ double lanes_sum(double x, int lg) {
+    if (lg > 0) x = dpp_add<0xB1>(x);                                // lane ^ 1
+    if (lg > 1) x = dpp_add<0x4E>(x);                                // lane ^ 2
+    if (lg > 2) x = dpp_add<0x141>(x);                               // the row's half mirrored: the other quad
+    if (lg > 3) x = dpp_add<0x140>(x);                               // the row mirrored: the other half
+    if (lg > 4) x += __shfl_xor(x, 16);
+    return x;
+}
+// 1 / sqrt(x) by the hardware's estimate and two Newton steps, each of which squares the relative error: some 2^-52.
+__device__ __forceinline__ double rsqrt64(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+    if (!(x > 0 && x < 1e300)) return 1.0 / sqrt(x);
+#pragma unroll
+    for (int i = 0; i < 2; i++) y += 0.5 * y * (1.0 - x * y * y);
+    return y;
+}
+// Codes in order, value i in bits 4 i .., as a word of K holds them.
+template <int DT> __device__ __forceinline__ uint32_t in_order(uint32_t w) {
+    if constexpr (DT != L3M_Q4_0) return w;
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) r |= (w >> 4 * i & 15u) << nib(DT, i);
+    return r;
+}
+// Eight values of a block of 32 in each lane of a quad: their codes, value i in bits 4 i .., and the block's scale as it is stored (the
+// same in the four). The file formats' rounding to the nearest (l3m_quantize_row), in the same float32 steps, so the stored bytes do not depend on
 // where a row is quantized; a block holding a value that is not finite reads as NaN, a scale past f16 saturates, mxfp4 exponents end at
 // 2^-126.
-template <int DT> __device__ __forceinline__ uint32_t quantize(float x, uint32_t &stored) {
+template <int DT> __device__ __forceinline__ uint32_t quantize(const float (&x)[8], uint32_t &stored) {
 #pragma clang fp contract(off)
-    const uint32_t mag = __float_as_uint(x) & 0x7FFFFFFFu;
-    uint32_t peak = mag;
+    float    top = x[0];
+    uint32_t mag = __float_as_uint(x[0]) & 0x7FFFFFFFu;
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) peak = max(peak, (uint32_t)__shfl_xor((int)peak, m));
-    const bool bad = peak >= 0x7F800000u;
-    if constexpr (DT == L3M_Q4_0) {
-        const uint64_t held = __ballot(mag == peak) >> (threadIdx.x & 32) & 0xFFFFFFFFu;     // the first of equal ones gives the sign
-        const float top = __shfl(x, (int)(threadIdx.x & 32) + __builtin_ctzll(held | 1ull << 32), 64);
-        const float d = top * -0.125f, r = d != 0.f ? 1.0f / d : 0.f, scaled = x * r, v = floorf(scaled + 8.5f);
-        stored = bad ? 0x7E00u : __builtin_bit_cast(uint16_t, (_Float16)fminf(fmaxf(d, -65504.f), 65504.f));
-        return bad ? 8u : v <= 0.f ? 0u : v >= 15.f ? 15u : (uint32_t)(int)v & 15u;
-    } else {
-        const int e = max((int)(peak >> 23) - 2, 1);
-        const float y = fabsf(x) * __uint_as_float((uint32_t)(254 - e) << 23);               // exact
-        const uint32_t c = (y > 0.25f) + (y > 0.75f) + (y > 1.25f) + (y > 1.75f) + (y > 2.5f) + (y > 3.5f) + (y > 5.f);
-        stored = bad ? (uint32_t)E8M0_NAN : (uint32_t)e;
-        return bad || !c ? 0u : c | (x < 0.f ? 8u : 0u);
+    for (int i = 1; i < 8; i++) {
+        const uint32_t m = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+        top = m > mag ? x[i] : top;                                  // the first of equal ones
+        mag = max(mag, m);
     }
+    uint32_t peak = max(mag, quad_xor<1>(mag));
+    peak = max(peak, quad_xor<2>(peak));
+    const bool bad = peak >= 0x7F800000u;
+    uint32_t word = 0;
+    if constexpr (DT == L3M_Q4_0) {
+        const uint32_t first = (threadIdx.x & 60) + __builtin_ctz((uint32_t)(__ballot(mag == peak) >> (threadIdx.x & 60)) & 15u);
+        const float d = __shfl(top, (int)first) * -0.125f, r = d != 0.f ? 1.0f / d : 0.f;
+        stored = bad ? 0x7E00u : __builtin_bit_cast(uint16_t, (_Float16)fminf(fmaxf(d, -65504.f), 65504.f));
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float scaled = x[i] * r, v = floorf(scaled + 8.5f);
+            word |= (uint32_t)(int)fminf(fmaxf(v, 0.f), 15.f) << 4 * i;
+        }
+    } else {
+        const int   e = max((int)(peak >> 23) - 2, 1);
+        const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+        stored = bad ? (uint32_t)E8M0_NAN : (uint32_t)e;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float    y = fabsf(x[i]) * inv;                    // exact
+            const uint32_t c = (y > 0.25f) + (y > 0.75f) + (y > 1.25f) + (y > 1.75f) + (y > 2.5f) + (y > 3.5f) + (y > 5.f);
+            word |= (c | (c && x[i] < 0.f ? 8u : 0u)) << 4 * i;
+        }
+        if (bad) word = 0;
+    }
+    return word;
 }
 template <int DT> __device__ __forceinline__ void put_scale(uint8_t *s, size_t i, uint32_t stored) {
     if constexpr (DT == L3M_Q4_0) ((uint16_t *)s)[i] = (uint16_t)stored;
@@ -104,140 +160,190 @@ struct RowsIn {
     const float *x, *wq, *wk, *table;
     float       *q, *k;
     long long    stride;
-    int          n, nq, nkv, hd, halves, pos;
+    int          n, nq, nkv, hd, halves, pos, lg;                    // 1 << lg lanes hold a head
+    unsigned     qk_waves;
     float        eps;
 };
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));   // floats need no alignment beyond their own
 
-// Norm and rotation of one head row by one wavefront: pair i of the rotation in lane i % 64, x s w with s = 1 / sqrt(mean x^2 + eps),
-// then the pair turned by the table's angle. In 64 bits up to the one rounding of each result, because a key's 4-bit code hangs on which
-// side of a border it lies: the row is the float32 nearest to the formula's, whatever the order of the sum.
-constexpr int PAIRS = HD_MAX / 2 / 64;
-__device__ __forceinline__ void norm_rope(const RowsIn &a, const float *x, const float *w, const float *cs, float out[PAIRS][2]) {
-    const int lane = threadIdx.x & 63, np = a.hd >> 1, second = a.halves ? np : 1, step = a.halves ? 1 : 2;
-    double v[PAIRS][2], ss = 0;
+// A lane's four rotation pairs, pairs 4 i .. of a head row at x: first and second values. VEC: np a multiple of 4. Lanes past the head zeros.
+template <bool VEC> __device__ __forceinline__ void load_pairs(const float *x, int i, int np, bool halves, float v0[4], float v1[4]) {
+    if constexpr (VEC) {
+        const bool in = 4 * i < np;
+        const f32x4 a = *(const f32x4_a4 *)(x + (in ? (halves ? 4 * i : 8 * i) : 0)), b = *(const f32x4_a4 *)(x + (in ? (halves ? np + 4 * i : 8 * i + 4) : 0));
 #pragma unroll
-    for (int i = 0; i < PAIRS; i++) {
-        const int p = lane + 64 * i;
-        v[i][0] = p < np ? (double)x[step * p] : 0;
-        v[i][1] = p < np ? (double)x[step * p + second] : 0;
-        ss += v[i][0] * v[i][0] + v[i][1] * v[i][1];
-    }
-    double s = 1;
-    if (w) {
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) ss += __shfl_xor(ss, m);
-        s = 1.0 / sqrt(ss / a.hd + (double)a.eps);
-    }
-#pragma unroll
-    for (int i = 0; i < PAIRS; i++) {
-        const int p = lane + 64 * i;
-        if (p >= np) continue;
-        double y0 = v[i][0], y1 = v[i][1];
-        if (w) {
-            y0 *= s * (double)w[step * p];
-            y1 *= s * (double)w[step * p + second];
+        for (int j = 0; j < 4; j++) {
+            v0[j] = !in ? 0.f : halves ? a[j] : j < 2 ? a[2 * j] : b[2 * j - 4];
+            v1[j] = !in ? 0.f : halves ? b[j] : j < 2 ? a[2 * j + 1] : b[2 * j - 3];
         }
-        if (cs) {
-            const double c = (double)cs[2 * p], t = (double)cs[2 * p + 1], z = y0 * c - y1 * t;
-            y1 = y0 * t + y1 * c;
-            y0 = z;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int p = 4 * i + j;
+            v0[j] = p < np ? x[halves ? p : 2 * p] : 0.f;
+            v1[j] = p < np ? x[halves ? np + p : 2 * p + 1] : 0.f;
         }
-        out[i][0] = (float)y0;
-        out[i][1] = (float)y1;
+    }
+}
+template <bool VEC> __device__ __forceinline__ void store_pairs(float *x, int i, int np, bool halves, const float v0[4], const float v1[4]) {
+    if constexpr (VEC) {
+        if (4 * i >= np) return;
+        *(f32x4_a4 *)(x + (halves ? 4 * i : 8 * i)) = halves ? f32x4{v0[0], v0[1], v0[2], v0[3]} : f32x4{v0[0], v1[0], v0[1], v1[1]};
+        *(f32x4_a4 *)(x + (halves ? np + 4 * i : 8 * i + 4)) = halves ? f32x4{v1[0], v1[1], v1[2], v1[3]} : f32x4{v0[2], v1[2], v0[3], v1[3]};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int p = 4 * i + j;
+            if (p < np) {
+                x[halves ? p : 2 * p] = v0[j];
+                x[halves ? np + p : 2 * p + 1] = v1[j];
+            }
+        }
     }
 }
 
-// One wavefront a (token, query or key head), then one a (eight positions, kv head) of V. DT < 0: keys go to a.k as floats and V is
-// left alone.
-template <int DT> __global__ void __launch_bounds__(256) k_rows_in(RowsIn a, l3m_kv4 c) {
-    __shared__ float row_s[4][HD_MAX];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, heads = a.nq + a.nkv, nb = (a.hd + 31) >> 5;
-    const long long item = (long long)blockIdx.x * 4 + wave, qk = (long long)a.n * heads;
-    if (item < qk) {
-        const int t = (int)(item / heads), h = (int)(item % heads), np = a.hd >> 1, second = a.halves ? np : 1, step = a.halves ? 1 : 2;
-        const bool key = h >= a.nq;
-        float y[PAIRS][2];
-        norm_rope(a, a.x + t * a.stride + (size_t)h * a.hd, key ? a.wk : a.wq, a.table ? a.table + (size_t)(a.pos + t) * a.hd : nullptr, y);
-        float *to = row_s[wave];
-        if (!key) to = a.q + ((size_t)t * a.nq + h) * a.hd;
-        else if (DT < 0) to = a.k + ((size_t)t * a.nkv + h - a.nq) * a.hd;
+// Norm and rotation of query and key heads, eight values a lane and 64 >> lg heads a wavefront: x s w with s = 1 / sqrt(mean x^2 + eps), then
+// the pairs turned by the table's angles. In 64 bits up to the one rounding of each result, because a key's 4-bit code hangs on which
+// side of a border it lies: the row is the float32 nearest to the formula's, whatever the order of the sum. Then, DT < 0, keys
+// go to a.k; else they are quantized, eight consecutive dimensions a lane (through LDS where the lane's own are two fours a half head
+// apart). Wavefronts behind a.qk_waves take eight positions of 64 dimensions of V each: a lane quantizes eight dimensions of one
+// position, and the words, which run along positions, are put together through LDS.
+//
+// Bound by the bytes for many tokens.
+template <int DT, bool VEC> __global__ void __launch_bounds__(256) k_rows_in(RowsIn a, l3m_kv4 c) {
+    __shared__ __align__(16) float row_s[4][512];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, heads = a.nq + a.nkv, nb = (a.hd + 31) >> 5, np = a.hd >> 1;
+    const unsigned w = blockIdx.x * 4 + wave;
+    if (w < a.qk_waves) {
+        const int sub = lane >> a.lg, i = lane & ((1 << a.lg) - 1);
+        const unsigned item = w * (64u >> a.lg) + sub, items = (unsigned)a.n * heads, at = min(item, items - 1), t = at / (unsigned)heads;
+        const int h = (int)(at - t * heads);
+        const bool key = h >= a.nq, halves = a.halves;
+        const float *x = a.x + (long long)t * a.stride + (size_t)h * a.hd, *wt = key ? a.wk : a.wq;
+        float v0[4], v1[4], g0[4], g1[4], cs0[4], cs1[4];
+        load_pairs<VEC>(x, i, np, halves, v0, v1);
+        const bool any_norm = a.wq || a.wk;
+        if (any_norm) load_pairs<VEC>(wt ? wt : x, i, np, halves, g0, g1);
+        if (a.table) load_pairs<VEC>(a.table + (size_t)(a.pos + (int)t) * a.hd, i, np, false, cs0, cs1);
+        double s = 1;
+        if (any_norm) {
+            double ss = 0;
 #pragma unroll
-        for (int i = 0; i < PAIRS; i++) {
-            const int p = lane + 64 * i;
-            if (p < np) {
-                to[step * p] = y[i][0];
-                to[step * p + second] = y[i][1];
-            }
+            for (int j = 0; j < 4; j++) ss += (double)v0[j] * v0[j] + (double)v1[j] * v1[j];
+            s = rsqrt64(lanes_sum(ss, a.lg) / a.hd + (double)a.eps);
         }
-        if constexpr (DT >= 0) {
-            if (!key) return;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            const Head H = head_of(c, nb, sbytes(DT), h - a.nq);
-            const int p = a.pos + t;
-            for (int d = lane; d < 32 * ((nb + 1) & ~1); d += 64) {  // both halves run as long as one has a block
-                const int b = d >> 5;
-                uint32_t stored, code = quantize<DT>(d < a.hd ? row_s[wave][d] : 0.f, stored) << nib(DT, d & 7);
 #pragma unroll
-                for (int m = 1; m < 8; m <<= 1) code |= (uint32_t)__shfl_xor((int)code, m);
-                if (b < nb) {
-                    if ((d & 7) == 0) H.kq[k_word<DT>(nb, p, d)] = code;
-                    if ((d & 31) == 0) put_scale<DT>(H.ks, k_scale<DT>(nb, p, b), stored);
+        for (int j = 0; j < 4; j++) {
+            double y0 = v0[j], y1 = v1[j];
+            if (any_norm && wt) {
+                y0 *= s * (double)g0[j];
+                y1 *= s * (double)g1[j];
+            }
+            if (a.table) {
+                const double co = cs0[j], si = cs1[j], z = y0 * co - y1 * si;
+                y1 = y0 * si + y1 * co;
+                y0 = z;
+            }
+            v0[j] = (float)y0;
+            v1[j] = (float)y1;
+        }
+        if (item < items && (DT < 0 || !key))
+            store_pairs<VEC>(key ? a.k + ((size_t)t * a.nkv + h - a.nq) * a.hd : a.q + ((size_t)t * a.nq + h) * a.hd, i, np, halves, v0, v1);
+        if constexpr (DT >= 0) {
+            if (!__ballot(key)) return;                              // queries alone
+            float k[8];
+            if (halves) {
+                float *row = row_s[wave] + (sub << a.lg) * 8;
+                store_pairs<VEC>(row, i, np, true, v0, v1);
+                wave_sync();
+#pragma unroll
+                for (int j = 0; j < 8; j++) k[j] = 8 * i < a.hd ? row[8 * i + j] : 0.f;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    k[2 * j] = v0[j];
+                    k[2 * j + 1] = v1[j];
                 }
+            }
+            uint32_t stored;
+            const uint32_t codes = quantize<DT>(k, stored);
+            if (key && item < items && 8 * i < 32 * nb) {
+                const Head H = head_of(c, nb, sbytes(DT), h - a.nq);
+                const int p = a.pos + (int)t;
+                H.kq[k_word<DT>(nb, p, 8 * i)] = in_order<DT>(codes);
+                if ((i & 3) == 0) put_scale<DT>(H.ks, k_scale<DT>(nb, p, i >> 2), stored);
             }
         }
         return;
     }
     if constexpr (DT >= 0) {
-        const long long vi = item - qk;
-        const int o0 = a.pos >> 3, octets = ((a.pos + a.n - 1) >> 3) - o0 + 1;
-        if (vi >= (long long)octets * a.nkv) return;
-        const int o = o0 + (int)(vi / a.nkv), h = (int)(vi % a.nkv), first = max(8 * o, a.pos), end = min(8 * o + 8, a.pos + a.n);
+        const unsigned vw = w - a.qk_waves, chunks = (unsigned)(nb + 1) >> 1, per = chunks * a.nkv;
+        const unsigned o0 = (unsigned)a.pos >> 3, octets = ((unsigned)(a.pos + a.n - 1) >> 3) - o0 + 1, oi = vw / per;
+        if (oi >= octets) return;
+        const int h = (int)((vw - oi * per) / chunks), chunk = (int)((vw - oi * per) % chunks), p0 = (int)(o0 + oi) * 8;
+        const int first = max(p0, a.pos), end = min(p0 + 8, a.pos + a.n);
         const Head H = head_of(c, nb, sbytes(DT), h);
-        const float *v = a.x + (size_t)(heads + h) * a.hd;
-        for (int d = lane; d < 32 * ((nb + 1) & ~1); d += 64) {
-            const int b = d >> 5;
-            float x[8];
+        const int p = p0 + (lane >> 3), d = 64 * chunk + 8 * (lane & 7);
+        const bool in = p >= first && p < end && d < a.hd;
+        const float *v = a.x + (size_t)(heads + h) * a.hd + (in ? (p - a.pos) * a.stride + d : 0);
+        const f32x4 v0 = *(const f32x4_a4 *)v, v1 = *(const f32x4_a4 *)(v + 4);
+        float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int p = 8 * o + i;
-                x[i] = p >= first && p < end && d < a.hd ? v[(p - a.pos) * a.stride + d] : 0.f;
-            }
-            uint32_t word[2] = {0, 0}, mine[2] = {0, 0};             // mxfp4: the positions' first and second four
+        for (int j = 0; j < 8; j++) x[j] = in ? j < 4 ? v0[j & 3] : v1[j & 3] : 0.f;
+        uint32_t stored, *word_s = (uint32_t *)row_s[wave];
+        word_s[lane] = quantize<DT>(x, stored);                      // [position][eight dimensions]
+        if ((lane & 3) == 0 && p >= first && p < end && d < 32 * nb) put_scale<DT>(H.vs, v_scale(nb, p, d >> 5), stored);
+        wave_sync();
+        // lane's word: q4_0 dimension 64 chunk + lane of the eight positions; mxfp4 dimensions 64 chunk + 32 (lane / 32) + lane % 16 and 16 more
+        // of four
+        const int u = DT == L3M_Q4_0 ? 0 : lane >> 4 & 1, e = DT == L3M_Q4_0 ? lane : (lane & 32) + (lane & 15);
+        uint32_t word = 0, mine = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int p = 8 * o + i, u = DT == L3M_Q4_0 ? 0 : i >> 2;
-                if (p < first || p >= end) continue;                 // the same in every lane
-                uint32_t stored;
-                word[u] |= quantize<DT>(x[i], stored) << v_bit<DT>(i, d);
-                mine[u] |= (DT == L3M_Q4_0 ? 15u : 255u) << (v_bit<DT>(i, 0));
-                if ((d & 31) == 0 && b < nb) put_scale<DT>(H.vs, v_scale(nb, p, b), stored);
-            }
-            int u = 0;
-            if constexpr (DT != L3M_Q4_0) {                          // dimensions d and d ^ 16 share words: each lane stores one
-                u = (d >> 4) & 1;
-                word[0] |= (uint32_t)__shfl_xor((int)word[0], 16);
-                word[1] |= (uint32_t)__shfl_xor((int)word[1], 16);
-            }
-            const uint32_t in = u ? word[1] : word[0], bits = u ? mine[1] : mine[0];
-            if (b < nb && bits) {
-                uint32_t *to = H.vq + v_word<DT>(nb, 8 * o + 4 * u, d);
-                *to = bits == ~0u ? in : (*to & ~bits) | in;         // the word's other positions stay
-            }
+        for (int j = 0; j < (DT == L3M_Q4_0 ? 8 : 4); j++) {
+            const int q = 4 * u + j;
+            const bool has = p0 + q >= first && p0 + q < end;
+            word |= (word_s[8 * q + (e >> 3)] >> 4 * (e & 7) & 15u) << v_bit<DT>(q, 0);
+            if constexpr (DT != L3M_Q4_0) word |= (word_s[8 * q + (e >> 3) + 2] >> 4 * (e & 7) & 15u) << v_bit<DT>(q, 16);
+            if (has) mine |= (DT == L3M_Q4_0 ? 15u : 255u) << v_bit<DT>(q, 0);
+        }
+        if (64 * chunk + e < 32 * nb && mine) {
+            uint32_t *to = H.vq + v_word<DT>(nb, p0 + 4 * u, 64 * chunk + e);
+            *to = mine == ~0u ? word : (*to & ~mine) | (word & mine);   // the word's other positions stay
         }
     }
 }
 
 // ---------------------------------------------------------------- read-back
-template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, float *k, float *v, int pos, int n) {
+// A thread a word of K (eight dimensions of a position), then one a dimension of V (its eight positions).
+template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, float *k, float *v, int pos, int n, unsigned k_threads) {
     const int nb = (c.hd + 31) >> 5;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / c.hd;
-    if (row >= (size_t)n * c.nkv) return;
-    const int d = (int)(i % c.hd), h = (int)(row % c.nkv), p = pos + (int)(row / c.nkv), b = d >> 5;
-    const Head H = head_of(c, nb, sbytes(DT), h);
-    if (k) k[i] = code_value<DT>(H.kq[k_word<DT>(nb, p, d & ~7)] >> nib(DT, d & 7) & 15) * scale_value<DT>(H.ks, k_scale<DT>(nb, p, b));
-    if (v) v[i] = code_value<DT>(H.vq[v_word<DT>(nb, p, d)] >> v_bit<DT>(p, d) & 15) * scale_value<DT>(H.vs, v_scale(nb, p, b));
+    const unsigned id = blockIdx.x * 256 + threadIdx.x, nkv = c.nkv, hd = c.hd;
+    if (id < k_threads) {
+        const unsigned per = hd >> 3, row = id / per, d = 8 * (id - row * per), t = row / nkv, h = row - t * nkv;
+        if (t >= (unsigned)n) return;
+        const Head H = head_of(c, nb, sbytes(DT), (int)h);
+        const int p = pos + (int)t;
+        const uint32_t w = H.kq[k_word<DT>(nb, p, (int)d)];
+        const float s = scale_value<DT>(H.ks, k_scale<DT>(nb, p, (int)d >> 5));
+        f32x4 x[2];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = code_value<DT>(w >> nib(DT, i) & 15) * s;
+        float *to = k + (size_t)row * hd + d;
+        *(f32x4_a4 *)to = x[0];
+        *(f32x4_a4 *)(to + 4) = x[1];
+        return;
+    }
+    const unsigned vi = id - k_threads, oh = vi / hd, d = vi - oh * hd, o = oh / nkv, h = oh - o * nkv, p0 = 8 * (((unsigned)pos >> 3) + o);
+    if (!v || p0 >= (unsigned)(pos + n)) return;
+    const Head H = head_of(c, nb, sbytes(DT), (int)h);
+    const uint32_t w[2] = {H.vq[v_word<DT>(nb, (int)p0, (int)d)], H.vq[v_word<DT>(nb, (int)p0 + 4, (int)d)]};   // q4_0: the same
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int p = (int)p0 + i;
+        if (p < pos || p >= pos + n) continue;
+        v[((size_t)(p - pos) * nkv + h) * hd + d] = code_value<DT>(w[i >> 2] >> v_bit<DT>(i, (int)d) & 15) * scale_value<DT>(H.vs, v_scale(nb, p, (int)d >> 5));
+    }
 }
 
 // ---------------------------------------------------------------- attention
@@ -256,7 +362,6 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // long cache (splits > 1) in the workspace, added in order by k_kv4_join.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -264,7 +369,6 @@ typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x32 __attribute__((ext_vector_type(32)));
-typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));   // q and out need no alignment beyond a float's
 
 constexpr int WAVES = 4;
 constexpr int SPLIT_WGS = 512;                                       // workgroups up to which a cache is split
@@ -749,10 +853,16 @@ const char *rows_bad(const RowsIn &a, bool floats) {
     if (nqb && nkb && overlap(a.q, nqb, a.k, nkb)) return "rows: q overlaps k";
     return nullptr;
 }
-template <int DT> void launch_rows_in(const RowsIn &a, const l3m_kv4 &c, hipStream_t st) {
-    long long items = (long long)a.n * (a.nq + a.nkv);
-    if (DT >= 0) items += (long long)(((a.pos + a.n - 1) >> 3) - (a.pos >> 3) + 1) * a.nkv;
-    hipLaunchKernelGGL(k_rows_in<DT>, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, a, c);
+template <int DT> void launch_rows_in(RowsIn a, const l3m_kv4 &c, hipStream_t st) {
+    a.lg = DT >= 0 ? 2 : 0;                                          // a block's four lanes at least
+    while (8 << a.lg < a.hd) a.lg++;
+    const unsigned per = 64u >> a.lg, items = (unsigned)((long long)a.n * (a.nq + a.nkv));
+    a.qk_waves = (items + per - 1) / per;
+    unsigned waves = a.qk_waves;
+    if (DT >= 0) waves += (unsigned)(((a.pos + a.n - 1) >> 3) - (a.pos >> 3) + 1) * a.nkv * (((a.hd + 31) / 32 + 1) / 2);
+    const dim3 grid((waves + 3) / 4);
+    if (a.hd % 8 == 0) hipLaunchKernelGGL((k_rows_in<DT, true>), grid, dim3(256), 0, st, a, c);
+    else if constexpr (DT < 0) hipLaunchKernelGGL((k_rows_in<DT, false>), grid, dim3(256), 0, st, a, c);
 }
 // Columns of 16 rows a workgroup takes of a kv head's `rows`.
 int tile_columns(int hd, long long rows) { return rows > 16 && hd <= 128 ? 2 : 1; }
@@ -800,7 +910,7 @@ int l3m_kv4_init(l3m_kv4 *c, int dtype, int nkv, int hd, int cap, void *mem) {
 int l3m_k_qk_norm_rope(float *q, float *k, const float *rows, int stride, int n, int nq, int nkv, int hd, const float *wq, const float *wk,
                        float eps, int halves, int pos, const float *table, void *stream) {
     if (hd < 2 || hd > HD_MAX || hd % 2) return l3m_dev_fail("qk_norm_rope: hd must be even and at most 256");
-    const RowsIn a = {rows, wq, wk, table, q, k, stride, n, nq, nkv, hd, halves, pos, eps};
+    const RowsIn a = {rows, wq, wk, table, q, k, stride, n, nq, nkv, hd, halves != 0, pos, 0, 0, eps};
     if (const char *why = rows_bad(a, true)) return l3m_dev_fail(why);
     if ((long long)n * (nq + nkv) > MAX_ITEMS) return l3m_dev_fail("qk_norm_rope: too many rows for one call");
     launch_rows_in<-1>(a, l3m_kv4{}, as_stream(stream));
@@ -811,7 +921,7 @@ int l3m_k_kv4_append(const l3m_kv4 *c, float *q, const float *rows, int stride, 
                      int halves, int pos, const float *table, void *stream) {
     if (const char *why = kv4_bad(c)) return l3m_dev_fail(why);
     if (!span_ok(c, pos, n)) return l3m_dev_fail("kv4_append: positions past the cache's end");
-    const RowsIn a = {rows, wq, wk, table, q, nullptr, stride, n, nq, c->nkv, c->hd, halves, pos, eps};
+    const RowsIn a = {rows, wq, wk, table, q, nullptr, stride, n, nq, c->nkv, c->hd, halves != 0, pos, 0, 0, eps};
     if (const char *why = rows_bad(a, false)) return l3m_dev_fail(why);
     if ((long long)n * (nq + 2 * c->nkv) > MAX_ITEMS) return l3m_dev_fail("kv4_append: too many rows for one call");
     if (c->dtype == L3M_Q4_0) launch_rows_in<L3M_Q4_0>(a, *c, as_stream(stream));
@@ -825,9 +935,11 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
     if ((!k && !v) || ((uintptr_t)k | (uintptr_t)v) % 4) return l3m_dev_fail("kv4_rows: no output, or one that is not 4-byte aligned");
     const size_t vals = (size_t)n * c->nkv * c->hd;
     if (vals > (size_t)MAX_ITEMS * 64) return l3m_dev_fail("kv4_rows: too many rows for one call");
-    const dim3 grid((unsigned)((vals + 255) / 256));
-    if (c->dtype == L3M_Q4_0) hipLaunchKernelGGL(k_kv4_rows<L3M_Q4_0>, grid, dim3(256), 0, as_stream(stream), *c, k, v, pos, n);
-    else hipLaunchKernelGGL(k_kv4_rows<L3M_MXFP4>, grid, dim3(256), 0, as_stream(stream), *c, k, v, pos, n);
+    const unsigned k_threads = k ? (unsigned)((vals / 8 + 255) / 256 * 256) : 0;
+    const size_t v_threads = v ? (size_t)(((pos + n - 1) >> 3) - (pos >> 3) + 1) * c->nkv * c->hd : 0;
+    const dim3 grid((unsigned)((k_threads + v_threads + 255) / 256));
+    if (c->dtype == L3M_Q4_0) hipLaunchKernelGGL(k_kv4_rows<L3M_Q4_0>, grid, dim3(256), 0, as_stream(stream), *c, k, v, pos, n, k_threads);
+    else hipLaunchKernelGGL(k_kv4_rows<L3M_MXFP4>, grid, dim3(256), 0, as_stream(stream), *c, k, v, pos, n, k_threads);
     return l3m_dev_launched("k_kv4_rows");
 }
 
