@@ -371,7 +371,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x32 __attribute__((ext_vector_type(32)));
 
 constexpr int WAVES = 4;
-constexpr int SPLIT_WGS = 512;                                       // workgroups up to which a cache is split
+constexpr int SPLIT_WGS = 512, SPLITS = 256;                         // workgroups up to which a cache is split; most parts of it
 constexpr float M0 = -3e38f;                                         // the maximum of no score: below every one
 
 // A q4_0 word's eight codes, 0 .. 15, in bf16: a nibble alone in a byte is the e4m3 number 2^-9 times it.
@@ -586,25 +586,59 @@ template <int DT, int NB> struct ValuesIn {
 };
 
 struct AttendIn {
-    float       *out, *parts;
+    float       *out, *ml, *parts;                                   // ml, parts: [row of out][split] maximum and sum, output
     const float *q;
     l3m_kv4      c;
-    int          n, nq, pos, groups, splits;
+    int          n, nq, g, pos, groups, group0, splits;              // splits: a power of two
+    uint32_t     g_mul, quad_mul;                                    // of g and hd / 4 (divide)
 };
-// Floats of the workspace's part of `rows` rows: the rows' outputs, then their maxima and sums; a multiple of 4.
-__host__ __device__ constexpr size_t part_floats(int rows, int hd) { return (size_t)rows * hd + (2 * rows + 3) / 4 * 4; }
+// x / d by d's multiplier, exact while x d < 2^32; 0: d is 1, or too large for it.
+__host__ inline uint32_t multiplier(uint32_t d, uint32_t most) {
+    return d > 1 && (uint64_t)most * d < 1ull << 32 ? (uint32_t)((1ull << 32) / d) + 1 : 0;
+}
+__device__ __forceinline__ uint32_t divide(uint32_t x, uint32_t d, uint32_t mul) { return mul ? __umulhi(x, mul) : d == 1 ? x : x / d; }
+// The maximum and the sum of a row of 16 lanes' (DPP), over lane ^ 16 and lane ^ 32.
+__device__ __forceinline__ float other16(float x, float &y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    y = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float other32(float x, float &y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    y = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float max_g4(float x) {
+    float y;
+    x = other16(x, y); x = fmaxf(x, y);
+    x = other32(x, y); return fmaxf(x, y);
+}
+__device__ __forceinline__ float sum_g4(float x) {
+    float y;
+    x = other16(x, y); x += y;
+    x = other32(x, y); return x + y;
+}
+template <int CTRL> __device__ __forceinline__ float dpp(float x) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true)); }
+__device__ __forceinline__ float max_wave(float x) {
+    x = fmaxf(x, dpp<0xB1>(x)); x = fmaxf(x, dpp<0x4E>(x)); x = fmaxf(x, dpp<0x141>(x)); x = fmaxf(x, dpp<0x140>(x));
+    return max_g4(x);
+}
+__device__ __forceinline__ float sum_wave(float x) {
+    x += dpp<0xB1>(x); x += dpp<0x4E>(x); x += dpp<0x141>(x); x += dpp<0x140>(x);
+    return sum_g4(x);
+}
 
 template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) k_kv4_attend(AttendIn a) {
-    constexpr int ROWS = 16 * CT, OS = 32 * NB + 4;                  // a row's stride in LDS
-    __shared__ float o_s[WAVES / 2][ROWS][OS], m_s[WAVES][ROWS], l_s[WAVES][ROWS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4, hd = a.c.hd, nkv = a.c.nkv, g = a.nq / nkv;
+    constexpr int ROWS = 16 * CT, OS = 32 * NB + 4;                  // OS: a row's stride in LDS
+    constexpr int O_WAVES = WAVES * ROWS * OS * 4 <= 60000 ? WAVES : WAVES / 2;   // wavefronts whose outputs LDS holds at once
+    __shared__ float o_s[O_WAVES][ROWS][OS], m_s[WAVES][ROWS], l_s[WAVES][ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4, hd = a.c.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each. The longest rows first.
-    const int h = (int)(blockIdx.x % (unsigned)nkv), rest = (int)(blockIdx.x / (unsigned)nkv);
-    const int split = (int)((unsigned)rest % (unsigned)a.splits), group = a.groups - 1 - (int)((unsigned)rest / (unsigned)a.splits);
+    const int h = (int)blockIdx.x, split = (int)blockIdx.y, group = a.groups - 1 - a.group0 - (int)blockIdx.z;
     const int R = a.n * g, row0 = group * ROWS, rows = min(R - row0, ROWS);
-    const int first = (int)((unsigned)row0 / (unsigned)g), last = (int)((unsigned)(row0 + rows - 1) / (unsigned)g);   // the rows' tokens
+    const int first = (int)divide(row0, g, a.g_mul), last = (int)divide(row0 + rows - 1, g, a.g_mul);   // the rows' tokens
     const unsigned tiles = (unsigned)(a.pos + last + TILE) / TILE, whole = (unsigned)(a.pos + first + 1) / TILE;   // tiles seen; those with nothing masked
-    const unsigned part = (unsigned)(split * WAVES + wave), of = (unsigned)a.splits * WAVES, share = tiles / of, more = tiles % of;
+    const unsigned part = (unsigned)(split * WAVES + wave), of = (unsigned)a.splits * WAVES, share = tiles >> (31 - __clz(of)), more = tiles & (of - 1);
     const int t0 = (int)(part * share + min(part, more)), t1 = t0 + (int)(share + (part < more));
     const Head H = head_of(a.c, NB, sbytes(DT), h);
     KeysIn<DT, NB> keys;
@@ -617,7 +651,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     const float scale = 1.44269504f / sqrtf((float)hd);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const unsigned r = (unsigned)min(row0 + 16 * ct + r16, R - 1), t = r / (unsigned)g;   // columns past the last row repeat it
+        const unsigned r = (unsigned)min(row0 + 16 * ct + r16, R - 1), t = divide(r, g, a.g_mul);   // columns past the last row repeat it
         seen[ct] = a.pos + (int)t + 1;
         qs[ct].load(a.q + ((size_t)t * a.nq + h * g + (r - t * (unsigned)g)) * hd, hd, scale, lane);
     }
@@ -658,8 +692,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         for (int ct = 0; ct < CT; ct++) {
             float top = fmaxf(fmaxf(fmaxf(s[ct][0], s[ct][1]), fmaxf(s[ct][2], s[ct][3])), fmaxf(fmaxf(s[ct][4], s[ct][5]), fmaxf(s[ct][6], s[ct][7])));
             if (__ballot(top > lim[ct])) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
+                top = max_g4(top);
                 const float up = top > lim[ct] ? top : 0.f, f = __builtin_amdgcn_exp2f(-up);
                 if (top > lim[ct]) lim[ct] = 8.f;
                 m[ct] += up;
@@ -717,103 +750,116 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     for (; tile < min(t1, (int)whole); tile++) step(tile, std::false_type{});
     for (; tile < t1; tile++) step(tile, std::true_type{});
 
-    // the wavefronts' parts at their common maximum
+    // the wavefronts' parts at their common maximum; where LDS has no room for all, the second half first and the first half onto them
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        l[ct] += __shfl_xor(l[ct], 16);
-        l[ct] += __shfl_xor(l[ct], 32);
+        l[ct] = sum_g4(l[ct]);
         if (lim[ct] == -INFINITY) m[ct] = M0;                        // nothing seen
         if (g4 == 0) {
             m_s[wave][16 * ct + r16] = m[ct];
             l_s[wave][16 * ct + r16] = l[ct];
         }
     }
-    __syncthreads();
+    auto put_acc = [&](int at, auto add, const float (&f)[CT]) {
 #pragma unroll
-    for (int half = 1; half >= 0; half--) {                          // wavefronts 2 and 3, then 0 and 1 onto them
-        if (wave >> 1 == half)
+        for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-                const int r = 16 * ct + r16;
-                float top = m_s[0][r];
-#pragma unroll
-                for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][r]);
-                const float f = __builtin_amdgcn_exp2f(m[ct] - top);
-#pragma unroll
-                for (int t = 0; t < 2 * NB; t++) {
-                    f32x4 x = acc[ct][t];
-                    if constexpr (DT == L3M_Q4_0) x += off[ct][t >> 1];
-                    f32x4 &to = *(f32x4 *)&o_s[wave & 1][r][16 * t + 4 * g4];
-                    to = half ? x * f : to + x * f;
-                }
+            for (int t = 0; t < 2 * NB; t++) {
+                f32x4 x = acc[ct][t];
+                if constexpr (DT == L3M_Q4_0) x += off[ct][t >> 1];
+                f32x4 &to = *(f32x4 *)&o_s[at][16 * ct + r16][16 * t + 4 * g4];
+                if constexpr (decltype(add)::value) to += x * f[ct];
+                else to = x * f[ct];
             }
+    };
+    float f[CT];
+    if constexpr (O_WAVES == WAVES) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) f[ct] = 1.f;
+        put_acc(wave, std::false_type{}, f);
+        __syncthreads();
+    } else {
+        __syncthreads();
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            float top = m_s[0][16 * ct + r16];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][16 * ct + r16]);
+            f[ct] = __builtin_amdgcn_exp2f(m[ct] - top);
+        }
+        if (wave >= O_WAVES) put_acc(wave - O_WAVES, std::false_type{}, f);
+        __syncthreads();
+        if (wave < O_WAVES) put_acc(wave, std::true_type{}, f);
         __syncthreads();
     }
     const unsigned quads = (unsigned)hd >> 2;
-    float *po = a.parts + (((size_t)group * nkv + h) * a.splits + split) * part_floats(min(R, ROWS), hd), *pml = po + rows * hd;
     for (unsigned i = threadIdx.x; i < rows * quads; i += 64 * WAVES) {
-        const unsigned r = i / quads, d = 4 * (i - r * quads);
+        const unsigned r = __umulhi(i, a.quad_mul), d = 4 * (i - r * quads);
         float top = m_s[0][r], sum = 0.f;
 #pragma unroll
         for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][r]);
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) sum = fmaf(l_s[w][r], __builtin_amdgcn_exp2f(m_s[w][r] - top), sum);
-        const f32x4 x = *(const f32x4 *)&o_s[0][r][d] + *(const f32x4 *)&o_s[1][r][d];
-        if (a.splits == 1) {
-            const unsigned row = row0 + r, t = row / (unsigned)g;
-            *(f32x4_a4 *)(a.out + ((size_t)t * a.nq + h * g + (row - t * (unsigned)g)) * hd + d) = x / sum;
-        } else {
-            *(f32x4 *)(po + r * hd + d) = x;
-            if (d == 0) { pml[2 * r] = top; pml[2 * r + 1] = sum; }
+        for (int w = 0; w < WAVES; w++) {
+            const float e = __builtin_amdgcn_exp2f(m_s[w][r] - top);
+            sum = fmaf(l_s[w][r], e, sum);
+            if constexpr (O_WAVES == WAVES) x += *(const f32x4 *)&o_s[w][r][d] * e;
+            else if (w < O_WAVES) x += *(const f32x4 *)&o_s[w][r][d];
+        }
+        const unsigned row = row0 + r, t = divide(row, g, a.g_mul);
+        const size_t at = (size_t)t * a.nq + h * g + (row - t * (unsigned)g);
+        if (a.splits == 1) *(f32x4_a4 *)(a.out + at * hd + d) = x / sum;
+        else {
+            const size_t to = at * a.splits + split;
+            *(f32x4 *)(a.parts + to * hd + d) = x;
+            if (d == 0) *(f32x2 *)(a.ml + 2 * to) = f32x2{top, sum};
         }
     }
 }
 
 // The splits' parts of a row, one workgroup a (token, query head): groups of hd / 4 lanes take every so many splits, 16 bytes a lane and
-// eight loads in flight, and meet in LDS in a fixed order.
-__global__ void __launch_bounds__(256) k_kv4_join(AttendIn a, int per) {
-    __shared__ float f_s[SPLIT_WGS], w_s[4][2];
+// eight loads in flight while every wavefront makes the splits' factors for itself; they meet in LDS in a fixed order.
+__global__ void __launch_bounds__(256) k_kv4_join(AttendIn a) {
+    __shared__ float f_s[4][SPLITS];
     __shared__ f32x4 o_s[256];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, nkv = a.c.nkv, S = a.splits;
-    const unsigned g = (unsigned)(a.nq / nkv), t = blockIdx.x / (unsigned)a.nq, hq = blockIdx.x % (unsigned)a.nq, h = hq / g;
-    const int R = a.n * (int)g, row = (int)(t * g + hq % g), group = row / per, r = row - group * per, rows = min(R - group * per, per);
-    const size_t size = part_floats(min(R, per), hd);
-    const float *part = a.parts + ((size_t)group * nkv + h) * S * size, *ml = part + rows * hd + 2 * r;
-    const unsigned quads = (unsigned)hd >> 2, groups = 256 / quads, mine = tid / quads, d = 4 * (tid - mine * quads);
+    const unsigned tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, S = a.splits, quads = hd >> 2;
+    const unsigned mine = __umulhi(tid, a.quad_mul), groups = __umulhi(256, a.quad_mul), d = 4 * (tid - mine * quads);
+    const float *part = a.parts + (size_t)blockIdx.x * S * hd + d, *ml = a.ml + (size_t)blockIdx.x * S * 2;
+    f32x2 v[SPLITS / 64];
+#pragma unroll
+    for (int i = 0; i < SPLITS / 64; i++) v[i] = i == 0 || 64u * i < S ? *(const f32x2 *)(ml + 2 * min(lane + 64 * i, S - 1)) : f32x2{M0, 0.f};
     f32x4 x[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(part + min(mine + i * groups, (unsigned)S - 1) * size + r * hd + d);
-    float top = M0;
-    for (int s = tid; s < S; s += 256) top = fmaxf(top, f_s[s] = ml[s * size]);
-    for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
-    if (lane == 0) w_s[wave][0] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(w_s[0][0], w_s[1][0]), fmaxf(w_s[2][0], w_s[3][0]));
-    float sum = 0.f;
-    for (int s = tid; s < S; s += 256) {
-        const float f = __builtin_amdgcn_exp2f(f_s[s] - top);
-        sum = fmaf(ml[s * size + 1], f, sum);
-        f_s[s] = f;
-    }
-    for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
-    if (lane == 0) w_s[wave][1] = sum;
-    __syncthreads();
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (mine < groups) {
-        for (unsigned s = mine; s < (unsigned)S; s += 8 * groups) {
+    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(part + (size_t)min(mine + i * groups, S - 1) * hd);
+    float top = v[0].x, sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const unsigned at = s + i * groups;
-                if (at < (unsigned)S) o += x[i] * f_s[at];
-                x[i] = *(const f32x4 *)(part + min(at + 8 * groups, (unsigned)S - 1) * size + r * hd + d);
-            }
+    for (int i = 1; i < SPLITS / 64; i++) top = fmaxf(top, v[i].x);
+    top = max_wave(top);
+#pragma unroll
+    for (int i = 0; i < SPLITS / 64; i++) {
+        const float f = __builtin_amdgcn_exp2f(v[i].x - top);
+        if (lane + 64 * i < S) {
+            sum = fmaf(v[i].y, f, sum);
+            f_s[wave][lane + 64 * i] = f;
         }
-        o_s[tid] = o;
     }
+    sum = sum_wave(sum);
+    wave_sync();
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (mine < groups)
+        for (unsigned s = mine; s < S; s += 8 * groups) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (s + i * groups < S) o += x[i] * f_s[wave][s + i * groups];
+            if (s + 8 * groups < S)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(part + (size_t)min(s + (8 + i) * groups, S - 1) * hd);
+        }
+    o_s[tid] = o;
     __syncthreads();
-    if (tid < (int)quads) {
+    if (tid < quads) {
         for (unsigned i = 1; i < groups; i++) o += o_s[i * quads + tid];
-        *(f32x4_a4 *)(a.out + (size_t)blockIdx.x * hd + d) = o / ((w_s[0][1] + w_s[1][1]) + (w_s[2][1] + w_s[3][1]));
+        *(f32x4_a4 *)(a.out + (size_t)blockIdx.x * hd + d) = o / sum;
     }
 }
 
@@ -866,26 +912,31 @@ template <int DT> void launch_rows_in(RowsIn a, const l3m_kv4 &c, hipStream_t st
 }
 // Columns of 16 rows a workgroup takes of a kv head's `rows`.
 int tile_columns(int hd, long long rows) { return rows > 16 && hd <= 128 ? 2 : 1; }
-template <int DT> void launch_attend(const AttendIn &a, int ct, hipStream_t st) {
-    const dim3 grid((unsigned)((long long)a.c.nkv * a.groups * a.splits)), wg(64 * WAVES);
+template <int DT> void launch_attend(AttendIn a, int ct, hipStream_t st) {
+    for (; a.group0 < a.groups; a.group0 += 65535) {                 // a grid's last dimension
+        const dim3 grid(a.c.nkv, a.splits, a.groups - a.group0 < 65535 ? a.groups - a.group0 : 65535), wg(64 * WAVES);
 #define ATTEND(NB, CT) hipLaunchKernelGGL((k_kv4_attend<DT, NB, CT>), grid, wg, 0, st, a)
-    switch ((a.c.hd + 31) / 32) {
-    case 1: if (ct == 1) ATTEND(1, 1); else ATTEND(1, 2); break;
-    case 2: if (ct == 1) ATTEND(2, 1); else ATTEND(2, 2); break;
-    case 3: if (ct == 1) ATTEND(3, 1); else ATTEND(3, 2); break;
-    case 4: if (ct == 1) ATTEND(4, 1); else ATTEND(4, 2); break;
-    case 5: ATTEND(5, 1); break;
-    case 6: ATTEND(6, 1); break;
-    case 7: ATTEND(7, 1); break;
-    default: ATTEND(8, 1); break;
-    }
+        switch ((a.c.hd + 31) / 32) {
+        case 1: if (ct == 1) ATTEND(1, 1); else ATTEND(1, 2); break;
+        case 2: if (ct == 1) ATTEND(2, 1); else ATTEND(2, 2); break;
+        case 3: if (ct == 1) ATTEND(3, 1); else ATTEND(3, 2); break;
+        case 4: if (ct == 1) ATTEND(4, 1); else ATTEND(4, 2); break;
+        case 5: ATTEND(5, 1); break;
+        case 6: ATTEND(6, 1); break;
+        case 7: ATTEND(7, 1); break;
+        default: ATTEND(8, 1); break;
+        }
 #undef ATTEND
+    }
 }
 // Workgroups that share a kv head's positions, `alone` of them without a split. A split costs the join, about 5 us, a tile about 0.2 us a block
 // and wavefront: up to 96 blocks one workgroup goes alone.
 int split_count(long long alone, int tiles, int nb, bool few_rows) {
     const long long room = (few_rows ? SPLIT_WGS : SPLIT_WGS / 2) / alone, most = (tiles + WAVES - 1) / WAVES;
-    return (long long)tiles * nb <= 96 || room < 2 ? 1 : (int)(room < most ? room : most);
+    int splits = 1;
+    if ((long long)tiles * nb > 96)
+        while (2 * splits <= room && 2 * splits <= most && 2 * splits <= SPLITS) splits *= 2;
+    return splits;
 }
 constexpr long long MAX_ITEMS = (1ll << 26) - 4;                     // wavefronts of a launch (its threads are counted in 32 bits)
 
@@ -946,7 +997,7 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
 size_t l3m_kv4_work_bytes(const l3m_kv4 *c, int n, int nq) {
     if (kv4_bad(c) || n < 1 || n > c->cap || nq < 1 || nq > 65536 || nq % c->nkv) return 0;
     const size_t rows = (size_t)n * (nq / c->nkv), most = 16 * tile_columns(c->hd, 17);
-    return 4 * (size_t)SPLIT_WGS * part_floats((int)(rows < most ? rows : most), c->hd);
+    return 4 * (size_t)SPLIT_WGS * (rows < most ? rows : most) * (c->hd + 2);
 }
 
 int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq, int pos, void *work, size_t work_bytes, void *stream) {
@@ -962,11 +1013,13 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     const int per = 16 * tile_columns(c->hd, R), groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;
     const long long alone = (long long)c->nkv * groups;
     const int splits = split_count(alone, tiles, (c->hd + 31) / 32 * (per / 16), R <= 16);
-    const AttendIn a = {out, (float *)work, q, *c, n, nq, pos, groups, splits};
+    const int g = nq / c->nkv;
+    float *ml = (float *)work;
+    const AttendIn a = {out, ml, ml + 2 * rows * splits, q, *c, n, nq, g, pos, groups, 0, splits, multiplier(g, (uint32_t)R), multiplier(c->hd / 4, 4096)};
     hipStream_t st = as_stream(stream);
     if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, per / 16, st);
     else launch_attend<L3M_MXFP4>(a, per / 16, st);
-    if (splits > 1) hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)rows), dim3(256), 0, st, a, per);
+    if (splits > 1) hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)rows), dim3(256), 0, st, a);
     return l3m_dev_launched("k_kv4_attend");
 }
 
