@@ -351,8 +351,8 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // 32 positions and wavefront, with the keys as the left operand so that lane 16 g4 + r holds the scores of row r for positions
 // 8 g4 .. 8 g4 + 7, which is where the second product wants the weights:
 //   S = K Q^T   16 positions x 16 rows, twice; q scaled by log2(e) / sqrt(hd) and held in parts (below)
-//   P = 2^(S - m), m near the rows' running maximum: it moves only when a score passes it by 8 (weights then stay below 2^8), and -m is what the
-//               scores' accumulators begin at
+//   P = 2^(S - m), m near the rows' running maximum: it moves only when a weight passes 2^8, and -m is what the scores' accumulators begin
+//               at
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions, P in two bf16 parts, off by 2^-18 at most. A position's scale differs from
 //               block to block: mxfp4's goes into the conversion of its codes, exactly (a layout of its own); q4_0's multiplies P,
 //               in 32 bits, before it is split, and its -8 is a product of its own with the same parts, so what they lose is lost in
@@ -383,7 +383,19 @@ __device__ __forceinline__ bf16x8 widen(uint32_t w) {
 }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 // Byte i of w as the power of two that it is the exponent of.
-__device__ __forceinline__ float pow2_byte(uint32_t w, int i) { return __uint_as_float((w >> 8 * i & 255u) << 23); }
+__device__ __forceinline__ float pow2_byte(uint32_t w, int i) {     // one instruction, where the compiler takes a shift and a mask
+    float r;
+#define BYTE_OF(N) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_" #N : "=v"(r) : "v"(23), "v"(w))
+    if (i == 0) BYTE_OF(0);
+    else if (i == 1) BYTE_OF(1);
+    else if (i == 2) BYTE_OF(2);
+    else BYTE_OF(3);
+#undef BYTE_OF
+    return r;
+}
+__device__ __forceinline__ float max8(const float (&s)[8]) {
+    return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+}
 // Eight float32 values as the sum of two bf16 ones, rounded each.
 __device__ __forceinline__ void two_parts(const float w[8], bf16x8 &hi, bf16x8 &lo) {
 #pragma unroll
@@ -657,11 +669,11 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     }
 
     f32x4 acc[CT][2 * NB], off[CT][NB];
-    float m[CT], lim[CT], l[CT];                                     // what scores are less by; the score that moves it; sum of weights
+    float m[CT], lim[CT], l[CT];                                     // what scores are less by; the weight that moves it; sum of weights
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         m[ct] = 0.f;
-        lim[ct] = -INFINITY;                                         // a row's first score always does
+        lim[ct] = -1.f;                                              // a row's first score always does
         l[ct] = 0.f;
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -690,15 +702,18 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         bf16x8 hi[CT], lo[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            float top = fmaxf(fmaxf(fmaxf(s[ct][0], s[ct][1]), fmaxf(s[ct][2], s[ct][3])), fmaxf(fmaxf(s[ct][4], s[ct][5]), fmaxf(s[ct][6], s[ct][7])));
-            if (__ballot(top > lim[ct])) {
-                top = max_g4(top);
-                const float up = top > lim[ct] ? top : 0.f, f = __builtin_amdgcn_exp2f(-up);
-                if (top > lim[ct]) lim[ct] = 8.f;
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(s[ct][i]);
+            if (__ballot(max8(p) > lim[ct])) {
+                const float top = max_g4(max8(s[ct]));
+                const bool move = top > (lim[ct] < 0.f ? -INFINITY : 8.f);
+                const float up = move ? top : 0.f, f = __builtin_amdgcn_exp2f(-up);
+                if (move) lim[ct] = 256.f;
                 m[ct] += up;
                 l[ct] *= f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) s[ct][i] -= up;
+                for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(s[ct][i] - up);
 #pragma unroll
                 for (int t = 0; t < 2 * NB; t++) acc[ct][t] *= f;
                 if constexpr (DT == L3M_Q4_0)
@@ -707,8 +722,8 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                s[ct][i] = __builtin_amdgcn_exp2f(s[ct][i]);
-                l[ct] += s[ct][i];
+                s[ct][i] = p[i];
+                l[ct] += p[i];
             }
             if constexpr (DT != L3M_Q4_0 && !MASK) two_parts(s[ct], hi[ct], lo[ct]);
         }
@@ -754,7 +769,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         l[ct] = sum_g4(l[ct]);
-        if (lim[ct] == -INFINITY) m[ct] = M0;                        // nothing seen
+        if (lim[ct] < 0.f) m[ct] = M0;                               // nothing seen
         if (g4 == 0) {
             m_s[wave][16 * ct + r16] = m[ct];
             l_s[wave][16 * ct + r16] = l[ct];
@@ -910,17 +925,26 @@ template <int DT> void launch_rows_in(RowsIn a, const l3m_kv4 &c, hipStream_t st
     if (a.hd % 8 == 0) hipLaunchKernelGGL((k_rows_in<DT, true>), grid, dim3(256), 0, st, a, c);
     else if constexpr (DT < 0) hipLaunchKernelGGL((k_rows_in<DT, false>), grid, dim3(256), 0, st, a, c);
 }
-// Columns of 16 rows a workgroup takes of a kv head's `rows`.
-int tile_columns(int hd, long long rows) { return rows > 16 && hd <= 128 ? 2 : 1; }
+// Columns of 16 rows a workgroup takes of each kv head's `rows`. Two share a tile's conversions, which pays for mxfp4 heads of 65 to 128
+// once every CU has two workgroups all the same: 1024 tokens behind 2999, 32 heads over 8, hd 128: 98 us, one column 113; 128
+// tokens behind 2000: 23 us, one column 13. q4_0 has no registers for it (183 us with one, 235 with two), shorter heads little to share (hd 64,
+// 2048 tokens behind 2000, 9 heads over 3: 43 and 40 us).
+int tile_columns(int dt, int nb, int nkv, long long rows) { return dt == L3M_MXFP4 && (nb == 3 || nb == 4) && nkv * ((rows + 31) / 32) >= 512 ? 2 : 1; }
 template <int DT> void launch_attend(AttendIn a, int ct, hipStream_t st) {
     for (; a.group0 < a.groups; a.group0 += 65535) {                 // a grid's last dimension
         const dim3 grid(a.c.nkv, a.splits, a.groups - a.group0 < 65535 ? a.groups - a.group0 : 65535), wg(64 * WAVES);
 #define ATTEND(NB, CT) hipLaunchKernelGGL((k_kv4_attend<DT, NB, CT>), grid, wg, 0, st, a)
+        if constexpr (DT == L3M_MXFP4)
+            if (ct == 2) {
+                if (a.c.hd <= 96) ATTEND(3, 2);
+                else ATTEND(4, 2);
+                continue;
+            }
         switch ((a.c.hd + 31) / 32) {
-        case 1: if (ct == 1) ATTEND(1, 1); else ATTEND(1, 2); break;
-        case 2: if (ct == 1) ATTEND(2, 1); else ATTEND(2, 2); break;
-        case 3: if (ct == 1) ATTEND(3, 1); else ATTEND(3, 2); break;
-        case 4: if (ct == 1) ATTEND(4, 1); else ATTEND(4, 2); break;
+        case 1: ATTEND(1, 1); break;
+        case 2: ATTEND(2, 1); break;
+        case 3: ATTEND(3, 1); break;
+        case 4: ATTEND(4, 1); break;
         case 5: ATTEND(5, 1); break;
         case 6: ATTEND(6, 1); break;
         case 7: ATTEND(7, 1); break;
@@ -929,13 +953,16 @@ template <int DT> void launch_attend(AttendIn a, int ct, hipStream_t st) {
 #undef ATTEND
     }
 }
-// Workgroups that share a kv head's positions, `alone` of them without a split. A split costs the join, about 5 us, a tile about 0.2 us a block
-// and wavefront: up to 96 blocks one workgroup goes alone.
-int split_count(long long alone, int tiles, int nb, bool few_rows) {
-    const long long room = (few_rows ? SPLIT_WGS : SPLIT_WGS / 2) / alone, most = (tiles + WAVES - 1) / WAVES;
+// Workgroups that share the positions of 16 rows, a power of two, with `alone` workgroups unsplit. A split costs the join, some 3.5 us and what
+// the rows' parts take; a tile costs a wavefront about 0.21 us a block (q4_0), 0.13 (mxfp4). Unsplit against split: q4_0, 32 heads over 8
+// of 128, one token over 256 positions 5.4 and 7.2 us, 512: 7.1 and 7.1, 1024: 10.6 and 7.2; mxfp4 over 512: 5.7 and 6.8; 64 tokens behind 2000 (mxfp4)
+// 12.7 and 14.1, behind 4000 (q4_0) 32.7 and 25.3. Past one workgroup a CU many rows' parts cost more than they save (16 tokens behind
+// 2000, 256 workgroups 9.3 us, 512 11.3); one token takes two.
+int split_count(int dt, long long alone, int tiles, int nb, long long rows, bool one_group) {
+    if ((long long)tiles * nb <= (dt == L3M_Q4_0 ? 56 : 90) + rows / 8) return 1;
+    const long long room = (one_group ? SPLIT_WGS : SPLIT_WGS / 2) / alone, most = (tiles + WAVES - 1) / WAVES;
     int splits = 1;
-    if ((long long)tiles * nb > 96)
-        while (2 * splits <= room && 2 * splits <= most && 2 * splits <= SPLITS) splits *= 2;
+    while (2 * splits <= room && 2 * splits <= most && 2 * splits <= SPLITS) splits *= 2;
     return splits;
 }
 constexpr long long MAX_ITEMS = (1ll << 26) - 4;                     // wavefronts of a launch (its threads are counted in 32 bits)
@@ -996,8 +1023,8 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
 
 size_t l3m_kv4_work_bytes(const l3m_kv4 *c, int n, int nq) {
     if (kv4_bad(c) || n < 1 || n > c->cap || nq < 1 || nq > 65536 || nq % c->nkv) return 0;
-    const size_t rows = (size_t)n * (nq / c->nkv), most = 16 * tile_columns(c->hd, 17);
-    return 4 * (size_t)SPLIT_WGS * (rows < most ? rows : most) * (c->hd + 2);
+    const size_t rows = (size_t)n * (nq / c->nkv);                   // a workgroup's of a split: 16 at most
+    return 4 * (size_t)SPLIT_WGS * (rows < 16 ? rows : 16) * (c->hd + 2);
 }
 
 int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq, int pos, void *work, size_t work_bytes, void *stream) {
@@ -1010,15 +1037,15 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     if (!work || (uintptr_t)work % 16 || work_bytes < l3m_kv4_work_bytes(c, n, nq)) return l3m_dev_fail("kv4_attend: the workspace is too small (l3m_kv4_work_bytes)");
     if (rows > (size_t)MAX_ITEMS) return l3m_dev_fail("kv4_attend: too many rows for one call");
     const long long R = (long long)n * (nq / c->nkv);
-    const int per = 16 * tile_columns(c->hd, R), groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;
+    const int ct = tile_columns(c->dtype, (c->hd + 31) / 32, c->nkv, R), per = 16 * ct, groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;
     const long long alone = (long long)c->nkv * groups;
-    const int splits = split_count(alone, tiles, (c->hd + 31) / 32 * (per / 16), R <= 16);
+    const int splits = split_count(c->dtype, alone, tiles, (c->hd + 31) / 32, (long long)rows, R <= 16);
     const int g = nq / c->nkv;
     float *ml = (float *)work;
     const AttendIn a = {out, ml, ml + 2 * rows * splits, q, *c, n, nq, g, pos, groups, 0, splits, multiplier(g, (uint32_t)R), multiplier(c->hd / 4, 4096)};
     hipStream_t st = as_stream(stream);
-    if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, per / 16, st);
-    else launch_attend<L3M_MXFP4>(a, per / 16, st);
+    if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, ct, st);
+    else launch_attend<L3M_MXFP4>(a, ct, st);
     if (splits > 1) hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)rows), dim3(256), 0, st, a);
     return l3m_dev_launched("k_kv4_attend");
 }
