@@ -1013,6 +1013,7 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
     if ((!k && !v) || ((uintptr_t)k | (uintptr_t)v) % 4) return l3m_dev_fail("kv4_rows: no output, or one that is not 4-byte aligned");
     const size_t vals = (size_t)n * c->nkv * c->hd;
     if (vals > (size_t)MAX_ITEMS * 64) return l3m_dev_fail("kv4_rows: too many rows for one call");
+    if (k && v && overlap(k, 4 * vals, v, 4 * vals)) return l3m_dev_fail("kv4_rows: k overlaps v");
     const unsigned k_threads = k ? (unsigned)((vals / 8 + 255) / 256 * 256) : 0;
     const size_t v_threads = v ? (size_t)(((pos + n - 1) >> 3) - (pos >> 3) + 1) * c->nkv * c->hd : 0;
     const dim3 grid((unsigned)((k_threads + v_threads + 255) / 256));
@@ -1034,7 +1035,9 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     const size_t rows = (size_t)n * nq, bytes = 4 * rows * c->hd;
     if (!out || !q || ((uintptr_t)out | (uintptr_t)q) % 4 || (out != q && overlap(out, bytes, q, bytes)))
         return l3m_dev_fail("kv4_attend: q and out must be floats, the same or apart");
-    if (!work || (uintptr_t)work % 16 || work_bytes < l3m_kv4_work_bytes(c, n, nq)) return l3m_dev_fail("kv4_attend: the workspace is too small (l3m_kv4_work_bytes)");
+    const size_t need = l3m_kv4_work_bytes(c, n, nq);
+    if (!work || (uintptr_t)work % 16 || work_bytes < need) return l3m_dev_fail("kv4_attend: the workspace is too small (l3m_kv4_work_bytes) or not 16-byte aligned");
+    if (overlap(work, need, q, bytes) || overlap(work, need, out, bytes)) return l3m_dev_fail("kv4_attend: the workspace overlaps q or out");
     if (rows > (size_t)MAX_ITEMS) return l3m_dev_fail("kv4_attend: too many rows for one call");
     const long long R = (long long)n * (nq / c->nkv);
     const int ct = tile_columns(c->dtype, (c->hd + 31) / 32, c->nkv, R), per = 16 * ct, groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;

@@ -7,7 +7,7 @@ import l3m_amd as A
 from weights import BF16, MXFP4, Q4_0, Q8_0
 
 lib = A.lib()
-P = 1 << 20                                       # stands for device memory: nothing reads it
+P = 1 << 24                                       # stands for device memory: nothing reads it
 BIG = 1 << 30
 
 
@@ -100,7 +100,7 @@ def test_append_refused(change):
 
 
 @pytest.mark.parametrize("change", [{"nq": 0}, {"nq": 3}, {"nq": -2}, {"out": None}, {"q": None}, {"out": P + 2}, {"q": 9 * P + 1}, {"out": 9 * P + 4}, {"work": None},
-                                    {"work": P + 4}, {"size": 0}], ids=str)
+                                    {"work": P + 4}, {"size": 0}, {"work": P + 4096 - 16}, {"work": 9 * P + 16}], ids=str)
 def test_attend_refused(change):
     a = {"out": P, "q": 9 * P, "n": 4, "nq": 4, "pos": 3, "work": P, "size": BIG, **change}
     assert refused(lib.l3m_k_kv4_attend(a["out"], a["q"], C.byref(cache()), a["n"], a["nq"], a["pos"], a["work"], a["size"], None))
@@ -119,3 +119,5 @@ def test_read_back_refused():
     assert refused(lib.l3m_k_kv4_rows(c, None, None, 0, 1, None))
     assert refused(lib.l3m_k_kv4_rows(c, P + 2, P, 0, 1, None))
     assert refused(lib.l3m_k_kv4_rows(None, P, P, 0, 1, None))
+    assert refused(lib.l3m_k_kv4_rows(c, P, P, 0, 1, None))
+    assert refused(lib.l3m_k_kv4_rows(c, P + 4 * 2 * 64 - 4, P, 0, 1, None))

@@ -272,6 +272,36 @@ def test_attend_value_not_finite(dev):
 
 
 @DTYPES
+@pytest.mark.parametrize("hd", [32, 64, 128, 200])
+def test_attend_query_not_finite(dev, dtype, hd):
+    """A query that holds a NaN or an infinity gives NaN, its neighbours' outputs stay as they are."""
+    nq, nkv, n = 6, 2, 40
+    for bad in (np.nan, np.inf, -np.inf):
+        c, k, v, rng = filled(dev, dtype, nkv, hd, n, 3)
+        q = rng.standard_normal((n, nq, hd)).astype(np.float32)
+        want = dev.kv4_attend(c, q, 0)
+        q[17, 4, hd - 3] = bad
+        got = dev.kv4_attend(c, q, 0)
+        assert np.isnan(got[17, 4]).all()
+        got[17, 4] = want[17, 4]
+        assert np.array_equal(got, want)
+        dev.free_all()
+
+
+@DTYPES
+def test_attend_query_sizes(dev, dtype):
+    """Queries of very different sizes, in a row and between rows, down to subnormal ones and zeros."""
+    nq, nkv, hd, seen = 8, 1, 128, 100
+    c, k, v, rng = filled(dev, dtype, nkv, hd, seen, 6)
+    q = rng.standard_normal((1, nq, hd)).astype(np.float32) * np.exp2(rng.integers(-20, 1, (1, nq, hd))).astype(np.float32)
+    q[0, 1] *= 2.0 ** -110
+    q[0, 2] *= 2.0 ** -130
+    q[0, 3] = 0
+    q[0, 4] *= 2.0 ** 6
+    near(dev.kv4_attend(c, q, seen - 1), *attended(dtype, q, k, v, seen - 1))
+
+
+@DTYPES
 def test_attend_large_scores(dev, dtype):
     """Scores of hundreds, the largest in any part of the cache: the others' weights vanish."""
     nq, nkv, hd, seen = 2, 1, 64, 3000
