@@ -6,13 +6,14 @@
 // Half f of a tile is its positions 8 (m / 4) + 4 f + m % 4, m = 0 .. 15.
 //   K codes   q4_0   [nkv][tile][half 2][lane 64][NB words]    lane 16 c + m: word b holds dimensions 32 b + 8 c .. + 7
 //             mxfp4  [nkv][tile][half 2][NB][m 16][4 words]    a block as it is
-//   V codes   q4_0   [nkv][tile][lane 64][2 NB words]          lane 16 g + j: word t holds dimension 16 t + j of positions 8 g .. 8 g + 7
+//   V codes   q4_0   [nkv][tile][lane 64][2 NB words]          lane 16 g + j: word t holds dimension 16 t + j of positions 8 g .. 8 g + 7,
+//                                                              position i at bit 4 (i / 2) + 16 (i % 2): pairs of f16 halves
 //             mxfp4  the same shape                            word 2 b + u: dimensions 32 b + j (low nibbles) and 32 b + 16 + j of
 //                                                              positions 8 g + 4 u .. + 3, a position's two in a byte
 //   scales    q4_0   [nkv][tile][NB][32 positions]             f16 d, of K and of V
 //             mxfp4  [nkv][tile][NB][m 16][half 2] of K, [nkv][tile][NB][32 positions] of V: a biased exponent byte
-// Both codes of a tile and head take 512 NB bytes. Element i of eight dimensions of K, or positions of q4_0's V, is the nibble at bit
-// nib(dt, i): q4_0's masked bytes are then elements 0..3 and 4..7, mxfp4's come in order.
+// Both codes of a tile and head take 512 NB bytes. Dimension i of a word of K is the nibble at bit nib(dt, i): q4_0's masked bytes are then
+// dimensions 0..3 and 4..7, mxfp4's come in order.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -50,7 +51,7 @@ template <int DT> __device__ __forceinline__ size_t k_word(int nb, int p, int d)
 template <int DT> __device__ __forceinline__ size_t v_word(int nb, int p, int d) {
     return ((size_t)(p >> 5) * 64 + ((p & 31) >> 3) * 16 + (d & 15)) * 2 * nb + (DT == L3M_Q4_0 ? d >> 4 : 2 * (d >> 5) + ((p >> 2) & 1));
 }
-template <int DT> __device__ __forceinline__ int v_bit(int p, int d) { return DT == L3M_Q4_0 ? nib(DT, p & 7) : 8 * (p & 3) + ((d >> 2) & 4); }
+template <int DT> __device__ __forceinline__ int v_bit(int p, int d) { return DT == L3M_Q4_0 ? 4 * ((p >> 1) & 3) + 16 * (p & 1) : 8 * (p & 3) + ((d >> 2) & 4); }
 __device__ __forceinline__ size_t v_scale(int nb, int p, int b) { return ((size_t)(p >> 5) * nb + b) * TILE + (p & 31); }
 template <int DT> __device__ __forceinline__ size_t k_scale(int nb, int p, int b) {
     if constexpr (DT == L3M_Q4_0) return v_scale(nb, p, b);
@@ -138,7 +139,7 @@ template <int DT> __device__ __forceinline__ uint32_t quantize(const float (&x)[
             word |= (uint32_t)(int)fminf(fmaxf(v, 0.f), 15.f) << 4 * i;
         }
     } else {
-        const int   e = max((int)(peak >> 23) - 2, 1);
+        const int   e = peak ? max((int)(peak >> 23) - 2, 1) : 127;  // a block of zeros: an ordinary scale
         const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
         stored = bad ? (uint32_t)E8M0_NAN : (uint32_t)e;
 #pragma unroll
@@ -351,18 +352,19 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // 32 positions and wavefront, with the keys as the left operand so that lane 16 g4 + r holds the scores of row r for positions
 // 8 g4 .. 8 g4 + 7, which is where the second product wants the weights:
 //   S = K Q^T   16 positions x 16 rows, twice; q scaled by log2(e) / sqrt(hd) and held in parts (below)
-//   P = 2^(S - m), m near the rows' running maximum: it moves only when a weight passes 2^8, and -m is what the scores' accumulators begin
-//               at
-//   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions, P in two bf16 parts, off by 2^-18 at most. A position's scale differs from
-//               block to block: mxfp4's goes into the conversion of its codes, exactly (a layout of its own); q4_0's multiplies P,
-//               in 32 bits, before it is split, and its -8 is a product of its own with the same parts, so what they lose is lost in
-//               proportion to the value, not to the code. Where rows mask positions, mxfp4's scales go into P too: a value that is not
-//               finite meets no row that does not see it.
+//   P = 2^(S - m), m such that the largest weight lies between 2^7 and 2^15: it moves only when one passes that, and -m is what the scores'
+//               accumulators begin at
+//   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions (v_mfma_f32_16x16x32_f16), P in two f16 parts: 22 bits, and 2^-32 of the largest at the
+//               least. A position's scale differs from block to block. q4_0's multiplies P, in 32 bits, before it is split (the range of
+//               the weights then goes by the products). mxfp4's goes into the conversion of its codes (a layout of its own), exactly where
+//               it lies between 2^-23 and 2^13; for others the accumulators take another unit. A value that is not finite meets no row
+//               that does not see it.
 // All sums in 32 bits. A workgroup's four wavefronts share 16 CT rows and split the tiles; they meet in LDS, and the workgroups of a
 // long cache (splits > 1) in the workspace, added in order by k_kv4_join.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
@@ -394,36 +396,56 @@ __device__ __forceinline__ float pow2_byte(uint32_t w, int i) {     // one instr
     return r;
 }
 __device__ __forceinline__ float max8(const float (&s)[8]) {
-    return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    return fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(s[0], s[1]), s[2]), s[3]), s[4]), s[5]), s[6]), s[7]);
 }
-// Eight float32 values as the sum of two bf16 ones, rounded each.
-__device__ __forceinline__ void two_parts(const float w[8], bf16x8 &hi, bf16x8 &lo) {
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// Eight float32 values as the sum of two f16 ones each: 22 bits, 2^-25 at the least; below 65520. The rests by the instruction that takes a
+// half as it lies in its pair (the compiler converts it first).
+__device__ __forceinline__ void two_parts(const float (&w)[8], f16x8 &hi, f16x8 &lo) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-        const bf16x2 h = __builtin_convertvector((f32x2{w[i], w[i + 1]}), bf16x2);
-        const uint32_t u = __builtin_bit_cast(uint32_t, h);
-        const bf16x2 l = __builtin_convertvector((f32x2{w[i] - __uint_as_float(u << 16), w[i + 1] - __uint_as_float(u & 0xFFFF0000u)}), bf16x2);
+        const f16x2 h = __builtin_convertvector((f32x2{w[i], w[i + 1]}), f16x2);
+        float r0, r1;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(w[i]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(w[i + 1]));
+        const f16x2 l = __builtin_convertvector((f32x2{r0, r1}), f16x2);
         hi[i] = h.x; hi[i + 1] = h.y;
         lo[i] = l.x; lo[i + 1] = l.y;
     }
 }
+// A q4_0 V word's values -8 .. 7 in f16: 1024 + code is the half 0x6400 | code, 1032 less is exact.
+__device__ __forceinline__ f16x8 widen_f16(uint32_t w) {
+    uint32_t r[4], codes = 0x000F000Fu;
+    asm("" : "+v"(codes));                                           // in a vector register: the and and the or are one instruction
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const _Float16 c = (_Float16)-1032.f;
+        r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (w >> 4 * i & codes) | 0x64006400u) + f16x2{c, c});
+    }
+    return __builtin_bit_cast(f16x8, u32x4{r[0], r[1], r[2], r[3]});
+}
 // mxfp4 V words of a block, eight positions of dimensions j and 16 + j, a position's scale each, as the two operands.
-__device__ __forceinline__ void widen_v(const uint32_t w[2], const float d[8], bf16x8 &v0, bf16x8 &v1) {
+__device__ __forceinline__ void widen_v(const uint32_t w[2], const float d[8], f16x8 &v0, f16x8 &v1) {
     uint32_t r[8], a[4], b[4];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        r[4 * u] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u], 0));
-        r[4 * u + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u + 1], 1));
-        r[4 * u + 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u + 2], 2));
-        r[4 * u + 3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[u], d[4 * u + 3], 3));
+        r[4 * u] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[u], d[4 * u], 0));
+        r[4 * u + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[u], d[4 * u + 1], 1));
+        r[4 * u + 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[u], d[4 * u + 2], 2));
+        r[4 * u + 3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[u], d[4 * u + 3], 3));
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         a[i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x05040100u);
         b[i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x07060302u);
     }
-    v0 = __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], a[2], a[3]});
-    v1 = __builtin_bit_cast(bf16x8, u32x4{b[0], b[1], b[2], b[3]});
+    v0 = __builtin_bit_cast(f16x8, u32x4{a[0], a[1], a[2], a[3]});
+    v1 = __builtin_bit_cast(f16x8, u32x4{b[0], b[1], b[2], b[3]});
+}
+// Whether the four exponents of w lie in 104 .. 140, where e2m1 codes with them are f16 numbers (k 2^-24 .. 6 2^13).
+__device__ __forceinline__ bool f16_range(uint32_t w) {
+    const uint32_t a = w & 0x7F7F7F7Fu, from104 = a + 0x18181818u, from141 = a + 0x73737373u;   // bit 7: of 104 .. 127, of 141 ..
+    return ((from104 ^ w) & ~(from141 & w) & 0x80808080u) == 0x80808080u;
 }
 
 // The scores of one half of a tile, 16 positions x 16 rows, from the queries of a row held in parts (Queries) and what a lane reads of the
@@ -500,8 +522,10 @@ template <int NB> struct Mx {
 template <int NB> struct KeysIn<L3M_MXFP4, NB> {
     u32x4    q[2][Mx<NB>::fours];
     uint32_t e[Mx<NB>::fours];                                       // the two halves' exponents
+    uint32_t four;                                                   // of the tile's 32 NB values' exponents, which are looked over first: 4 lane ..
     __device__ __forceinline__ void load(const Head &H, int tile, int lane) {
         const size_t T = (size_t)tile;
+        four = ((const uint32_t *)(H.vs + T * NB * TILE))[min(lane, 8 * NB - 1)];
 #pragma unroll
         for (int i = 0; i < Mx<NB>::fours; i++) {
             const int b = Mx<NB>::block(i, lane >> 4), m = lane & 15;
@@ -668,8 +692,11 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         qs[ct].load(a.q + ((size_t)t * a.nq + h * g + (r - t * (unsigned)g)) * hd, hd, scale, lane);
     }
 
-    f32x4 acc[CT][2 * NB], off[CT][NB];
+    f32x4 acc[CT][2 * NB];
     float m[CT], lim[CT], l[CT];                                     // what scores are less by; the weight that moves it; sum of weights
+    float base = 7.f;                                                // log2 of the weight a new maximum gets
+    int   unit = 0;                                                  // mxfp4: acc counts 2^unit
+    bool  based = DT != L3M_Q4_0;                                    // q4_0: of its product with the first tile's largest scale
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         m[ct] = 0.f;
@@ -677,16 +704,42 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         l[ct] = 0.f;
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int b = 0; b < NB; b++) off[ct][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const __bf16 m8 = (__bf16)-8.f;
-    const bf16x8 minus8 = {m8, m8, m8, m8, m8, m8, m8, m8};
+    auto scale_acc = [&](int ct, float f) {
+#pragma unroll
+        for (int t = 0; t < 2 * NB; t++) acc[ct][t] *= f;
+    };
+    // mxfp4, a tile whose exponents are not all f16's: another unit where its largest needs one (the first tile's own, later a larger one;
+    // values below 2^-33 of the largest are then rounded), and its exponents in that unit. What the accumulators are to be multiplied by.
+    auto fit_unit = [&](uint32_t four, bool fresh) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t e = four >> 8 * i & 255u;
+            top = e == E8M0_NAN ? top : max(top, e);
+        }
+        const int most = __builtin_amdgcn_readfirstlane((int)max_wave((float)top)), was = unit;
+        if (fresh) unit = most ? most - 137 : 0;
+        else if (most - unit > 140) unit = most - 137;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                uint32_t to = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = (int)(vals.e[b][j] >> 8 * i & 255u);
+                    to |= (uint32_t)(e == E8M0_NAN ? e : min(max(e - unit, 0), 254)) << 8 * i;
+                }
+                vals.e[b][j] = to;
+            }
+        return fresh ? 1.f : ldexpf(1.f, was - unit);
+    };
 
     auto step = [&](const int tile, auto masked) {
         constexpr bool MASK = decltype(masked)::value;
         const int p0 = tile * TILE + 8 * g4;
-        float s[CT][8];
+        float p[CT][8];
 #pragma unroll
         for (int f = 0; f < 2; f++) {
             f32x4 c[CT];
@@ -696,74 +749,148 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) s[ct][4 * f + r] = !MASK || p0 + 4 * f + r < seen[ct] ? c[ct][r] : -INFINITY;
+                for (int r = 0; r < 4; r++) p[ct][4 * f + r] = !MASK || p0 + 4 * f + r < seen[ct] ? c[ct][r] : -INFINITY;
         }
+        uint32_t four = 0;
+        if constexpr (DT != L3M_Q4_0) four = keys.four;
         keys.load(H, min(tile + 1, t1 - 1), lane);
-        bf16x8 hi[CT], lo[CT];
+        float to_unit = 1.f;
+        uint32_t nan[CT];                                            // blocks whose value is NaN at a position the row sees
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) nan[ct] = 0;
+        if constexpr (DT != L3M_Q4_0) {
+            uint32_t none = 0;                                       // exponents of positions that no row sees do not count
+            if constexpr (MASK) {
+                const int left = a.pos + last + 1 - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
+                none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left;
+            }
+            if (unit || __ballot(!f16_range((four & ~none) | (0x7F7F7F7Fu & none)))) {
+                to_unit = fit_unit(four | none, tile == t0);
+                if constexpr (MASK)                                  // NaN for the rows that see it, and for no other: 0 here, put in below
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if ((vals.e[b][i >> 2] >> 8 * (i & 3) & 255u) == E8M0_NAN) {
+                                vals.e[b][i >> 2] ^= 128u << 8 * (i & 3);   // 127; a NaN block's codes are 0
+#pragma unroll
+                                for (int ct = 0; ct < CT; ct++) nan[ct] |= p0 + i < seen[ct] ? 1u << b : 0u;
+                            }
+            }
+        }
+        f16x8 hi[CT], lo[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            float p[8];
+            float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(s[ct][i]);
-            if (__ballot(max8(p) > lim[ct])) {
-                const float top = max_g4(max8(s[ct]));
-                const bool move = top > (lim[ct] < 0.f ? -INFINITY : 8.f);
-                const float up = move ? top : 0.f, f = __builtin_amdgcn_exp2f(-up);
-                if (move) lim[ct] = 256.f;
+            for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(p[ct][i]);
+            if (__ballot(max8(e) > lim[ct]) || to_unit != 1.f) {
+                if (!based) {
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int b = 0; b < (DT == L3M_Q4_0 ? NB : 0); b++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const uint32_t u = __builtin_bit_cast(uint16_t, vals.d[b][i]) & 0x7FFFu;
+                            most = max(most, u < 0x7C00u ? u : 0u);
+                        }
+                    base -= (float)max((int)max_wave((float)most) >> 10, 1) - 15.f;
+                    based = true;
+                }
+                const float top = max_g4(max8(p[ct]));
+                const bool move = top > (lim[ct] < 0.f ? -INFINITY : base + 8.f);
+                const float up = move ? top - base : 0.f, f = __builtin_amdgcn_exp2f(-up);
+                if (move) lim[ct] = __builtin_amdgcn_exp2f(base + 8.f);
                 m[ct] += up;
                 l[ct] *= f;
+                scale_acc(ct, f * to_unit);
 #pragma unroll
-                for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(s[ct][i] - up);
-#pragma unroll
-                for (int t = 0; t < 2 * NB; t++) acc[ct][t] *= f;
-                if constexpr (DT == L3M_Q4_0)
-#pragma unroll
-                    for (int b = 0; b < NB; b++) off[ct][b] *= f;
+                for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(p[ct][i] - up);
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                s[ct][i] = p[i];
-                l[ct] += p[i];
+                p[ct][i] = e[i];
+                l[ct] += e[i];
             }
-            if constexpr (DT != L3M_Q4_0 && !MASK) two_parts(s[ct], hi[ct], lo[ct]);
+            if constexpr (DT != L3M_Q4_0) two_parts(p[ct], hi[ct], lo[ct]);
         }
+        if constexpr (DT == L3M_Q4_0) {
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            bf16x8 v0, v1;
-            float d[8];
-            if constexpr (DT == L3M_Q4_0) {
-                v0 = widen(vals.q[2 * b]);
-                v1 = widen(vals.q[2 * b + 1]);
-            } else {
-                float one[8];
+            for (int ct = 0; ct < CT; ct++) {
+                constexpr int KEPT = NB <= 4 ? NB : 1;               // long heads have no registers for every block's products
+                float w[KEPT][8], most = 0.f;
+                auto products = [&](int b) {
+                    float (&x)[8] = w[b % KEPT];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        x[i] = fmaf(p[ct][i], (float)vals.d[b][i], 0.f);
+                        if constexpr (MASK) x[i] = p0 + i < seen[ct] ? x[i] : 0.f;         // a masked position's scale may be anything
+                    }
+                };
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    products(b);
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) most = fmaxf(fmaxf(most, fabsf(w[b % KEPT][i])), fabsf(w[b % KEPT][i + 1]));
+                }
+                // past f16 soon: every weight of the rows 2^-16 of what it was (a scale of another size than the first tile's)
+                while (__ballot(most > 32768.f)) {
+                    scale_acc(ct, 0x1p-16f);
+                    l[ct] *= 0x1p-16f;
+                    m[ct] += 16.f;
+                    lim[ct] *= lim[ct] < 0.f ? 1.f : 0x1p-16f;
+                    base -= 16.f;
+                    most *= 0x1p-16f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) p[ct][i] *= 0x1p-16f;
+#pragma unroll
+                    for (int b = 0; b < KEPT; b++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) w[b][i] *= 0x1p-16f;
+                }
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    if constexpr (KEPT < NB) products(b);
+                    const f16x8 v0 = widen_f16(vals.q[2 * b]), v1 = widen_f16(vals.q[2 * b + 1]);
+                    two_parts(w[b % KEPT], hi[ct], lo[ct]);
+                    acc[ct][2 * b] = mfma(v0, lo[ct], mfma(v0, hi[ct], acc[ct][2 * b]));
+                    acc[ct][2 * b + 1] = mfma(v1, lo[ct], mfma(v1, hi[ct], acc[ct][2 * b + 1]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float d[8];
+                f16x8 v0, v1;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     d[i] = pow2_byte(vals.e[b][i >> 2], i & 3);
-                    one[i] = 1.f;
+                    if constexpr (MASK) d[i] = p0 + i <= a.pos + last ? d[i] : 1.f;
                 }
-                widen_v(&vals.q[2 * b], MASK ? one : d, v0, v1);
-            }
+                widen_v(&vals.q[2 * b], d, v0, v1);
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-                if constexpr (DT == L3M_Q4_0 || MASK) {
-                    float w[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        w[i] = fmaf(s[ct][i], DT == L3M_Q4_0 ? (float)vals.d[b][i] : d[i], 0.f);
-                        if constexpr (MASK) w[i] = p0 + i < seen[ct] ? w[i] : 0.f;   // whatever a masked position's scale is
-                    }
-                    two_parts(w, hi[ct], lo[ct]);
+                for (int ct = 0; ct < CT; ct++) {
+                    acc[ct][2 * b] = mfma(v0, lo[ct], mfma(v0, hi[ct], acc[ct][2 * b]));
+                    acc[ct][2 * b + 1] = mfma(v1, lo[ct], mfma(v1, hi[ct], acc[ct][2 * b + 1]));
                 }
-                acc[ct][2 * b] = mfma(v0, lo[ct], mfma(v0, hi[ct], acc[ct][2 * b]));
-                acc[ct][2 * b + 1] = mfma(v1, lo[ct], mfma(v1, hi[ct], acc[ct][2 * b + 1]));
-                if constexpr (DT == L3M_Q4_0) off[ct][b] = mfma(minus8, lo[ct], mfma(minus8, hi[ct], off[ct][b]));
             }
+            if constexpr (MASK)
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+                    if (__ballot(nan[ct] != 0))
+#pragma unroll
+                        for (int b = 0; b < NB; b++)
+                            if (max_g4((float)(nan[ct] >> b & 1u)) != 0.f) acc[ct][2 * b] = acc[ct][2 * b + 1] = f32x4{NAN, NAN, NAN, NAN};
         }
         vals.load(H, min(tile + 1, t1 - 1), lane);
     };
     int tile = t0;
     for (; tile < min(t1, (int)whole); tile++) step(tile, std::false_type{});
     for (; tile < t1; tile++) step(tile, std::true_type{});
+    if constexpr (DT != L3M_Q4_0)
+        if (unit)
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) scale_acc(ct, ldexpf(1.f, unit));
 
     // the wavefronts' parts at their common maximum; where LDS has no room for all, the second half first and the first half onto them
 #pragma unroll
@@ -780,11 +907,9 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         for (int ct = 0; ct < CT; ct++)
 #pragma unroll
             for (int t = 0; t < 2 * NB; t++) {
-                f32x4 x = acc[ct][t];
-                if constexpr (DT == L3M_Q4_0) x += off[ct][t >> 1];
                 f32x4 &to = *(f32x4 *)&o_s[at][16 * ct + r16][16 * t + 4 * g4];
-                if constexpr (decltype(add)::value) to += x * f[ct];
-                else to = x * f[ct];
+                if constexpr (decltype(add)::value) to += acc[ct][t] * f[ct];
+                else to = acc[ct][t] * f[ct];
             }
     };
     float f[CT];

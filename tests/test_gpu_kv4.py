@@ -69,8 +69,10 @@ def attended(dtype, q, k, v, pos):
     """out and the bound of its error: q [n][nq][hd], k, v [pos + n][nkv][hd] in 64 bits.
 
     A score is a sum of hd products in float32: off by (hd + 16) 2^-24 of the sum of its terms' magnitudes at most; a weight by twice that
-    (itself and the sum's). An output adds 2^-17 of its values for the two 8-bit parts a weight is held in with its scale, and a float32
-    rounding of its terms for each of the sums' steps: 32 positions each, and those that join partial results."""
+    (itself and the sum's). A weight (q4_0: with its scale) is held in two parts of 11 bits, half a step of the second being 2^-22, and no
+    less than 2^-25 where the largest is 2^7 at least: 2^-32 of the largest weight times the largest value for each position; mxfp4's values
+    are exact down to 2^-33 of the largest. And a float32 rounding of its terms for each of the sums' steps: 32 positions each, and those
+    that join partial results."""
     n, nq, hd = q.shape
     nkv, g = k.shape[1], q.shape[1] // k.shape[1]
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
@@ -83,8 +85,9 @@ def attended(dtype, q, k, v, pos):
         p = np.exp(s - s.max(1, keepdims=True))
         p /= p.sum(1, keepdims=True)
         out[:, h] = p @ vh
-        off = 2 * (hd + 16) * 2.0 ** -24 * mag.max(1) + 2.0 ** -17
-        tol[:, h] = off[:, None] * (p @ np.abs(vh)) + (len(k) / 32 + 64) * 2.0 ** -24 * (p @ summed(dtype, vh)) + 1e-30
+        off = 2 * (hd + 16) * 2.0 ** -24 * mag.max(1) + 2.0 ** -21
+        least = (len(k) * p.max(1) + 1) * 2.0 ** -32 * np.abs(vh).max()
+        tol[:, h] = off[:, None] * (p @ np.abs(vh)) + (len(k) / 32 + 64) * 2.0 ** -24 * (p @ summed(dtype, vh)) + least[:, None] + 1e-42
     return out, tol
 
 
@@ -329,6 +332,27 @@ def test_attend_mixed_scales(dev, dtype):
     k, v = (x.astype(np.float64) for x in dev.kv4_rows(c, 0, seen))
     q = rng.standard_normal((1, nq, hd)).astype(np.float32)
     near(dev.kv4_attend(c, q, seen - 1), *attended(dtype, q, k, v, seen - 1))
+
+
+@DTYPES
+@pytest.mark.parametrize("sizes", [(-100, -100, -100), (-15, -15, -15), (100, 100, 100), (14, 14, 14), (-100, 0, 90), (-15, 0, 14), (90, 0, -100), (14, -3, -15), (0, 14, 0)],
+                         ids=str)
+def test_attend_value_sizes(dev, dtype, sizes):
+    """V rows of 2^sizes in the first, middle and last third, past what f16 holds (mxfp4) and at the ends of f16 scales (q4_0, whose sizes end
+    there): one token, and a prompt, whose rows see more and more of them."""
+    if dtype == Q4_0 and max(map(abs, sizes)) > 15:
+        pytest.skip("past q4_0's f16 scales")
+    nq, nkv, hd = 3, 1, 64
+    for seen, n in ((1500, 1), (200, 200)):
+        rng = np.random.default_rng(seen)
+        rows = rng.standard_normal((seen, 2, hd)).astype(np.float32)
+        rows[:, 1] *= np.exp2(np.repeat(np.float32(sizes), -(-seen // 3))[:seen])[:, None]
+        c = dev.kv4(dtype, nkv, hd, seen)
+        dev.kv4_append(c, rows.reshape(seen, -1), 0, 0)
+        k, v = (x.astype(np.float64) for x in dev.kv4_rows(c, 0, seen))
+        q = rng.standard_normal((n, nq, hd)).astype(np.float32)
+        near(dev.kv4_attend(c, q, seen - n), *attended(dtype, q, k, v, seen - n))
+        dev.free_all()
 
 
 def test_out_may_be_q(dev):
