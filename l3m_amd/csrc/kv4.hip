@@ -833,8 +833,9 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) most = fmaxf(fmaxf(most, fabsf(w[b % KEPT][i])), fabsf(w[b % KEPT][i + 1]));
                 }
-                // past f16 soon: every weight of the rows 2^-16 of what it was (a scale of another size than the first tile's)
-                while (__ballot(most > 32768.f)) {
+                // past f16 soon: every weight of the rows 2^-16 of what it was (a scale of another size than the first tile's). A scale that
+                // is infinite, which only memory that was never written holds, stays infinite and is not waited for
+                while (__ballot(most > 32768.f && most < INFINITY)) {
                     scale_acc(ct, 0x1p-16f);
                     l[ct] *= 0x1p-16f;
                     m[ct] += 16.f;

@@ -275,6 +275,25 @@ def test_attend_value_not_finite(dev):
 
 
 @DTYPES
+@pytest.mark.parametrize("hd", [40, 128, 200])
+def test_attend_position_never_written(dev, dtype, hd):
+    """A position in the middle that was never written, its memory holding infinite f16 scales: the call ends, and the tokens before it are
+    what they are over the whole cache."""
+    nq, nkv, n = 4, 2, 40
+    size, rng = dev.lib.l3m_kv4_bytes(dtype, nkv, hd, n), np.random.default_rng(4)
+    rows, q = rng.standard_normal((n, 2 * nkv * hd)).astype(np.float32), rng.standard_normal((n, nq, hd)).astype(np.float32)
+    whole, c = dev.kv4(dtype, nkv, hd, n), dev.kv4(dtype, nkv, hd, n)
+    assert dev.lib.l3m_dev_upload(c.kq, np.full(size // 2, 0x7C00, np.uint16).ctypes.data, size) == 0
+    dev.kv4_append(whole, rows, 0, 0)
+    dev.kv4_append(c, rows[:20], 0, 0)
+    dev.kv4_append(c, rows[21:], 0, 21)
+    got, want = dev.kv4_attend(c, q, 0), dev.kv4_attend(whole, q, 0)
+    assert np.array_equal(got[:20], want[:20])
+    if dtype == Q4_0:
+        assert not np.isfinite(got[20:]).any()
+
+
+@DTYPES
 @pytest.mark.parametrize("hd", [32, 64, 128, 200])
 def test_attend_query_not_finite(dev, dtype, hd):
     """A query that holds a NaN or an infinity gives NaN, its neighbours' outputs stay as they are."""
