@@ -15,6 +15,7 @@
 // Both codes of a tile and head take 512 NB bytes. Dimension i of a word of K is the nibble at bit nib(dt, i): q4_0's masked bytes are then
 // dimensions 0..3 and 4..7, mxfp4's come in order.
 #include <hip/hip_runtime.h>
+#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 #include <type_traits>
@@ -357,8 +358,8 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions (v_mfma_f32_16x16x32_f16), P in two f16 parts: 22 bits, and 2^-32 of the largest at the
 //               least. A position's scale differs from block to block. q4_0's multiplies P, in 32 bits, before it is split (the range of
 //               the weights then goes by the products). mxfp4's goes into the conversion of its codes (a layout of its own), exactly where
-//               it lies between 2^-23 and 2^13; for others the accumulators take another unit. A value that is not finite meets no row
-//               that does not see it.
+//               it lies between 2^-23 and 2^13; for others the accumulators take another unit. A row's range, and NaN, come from
+//               positions that it sees, never from one behind it.
 // All sums in 32 bits. A workgroup's four wavefronts share 16 CT rows and split the tiles; they meet in LDS, and the workgroups of a
 // long cache (splits > 1) in the workspace, added in order by k_kv4_join.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -668,7 +669,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     constexpr int ROWS = 16 * CT, OS = 32 * NB + 4;                  // OS: a row's stride in LDS
     constexpr int O_WAVES = WAVES * ROWS * OS * 4 <= 60000 ? WAVES : WAVES / 2;   // wavefronts whose outputs LDS holds at once
     __shared__ float o_s[O_WAVES][ROWS][OS], m_s[WAVES][ROWS], l_s[WAVES][ROWS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4, hd = a.c.hd, g = a.g;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g4 = lane >> 4, hd = a.c.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each. The longest rows first.
     const int h = (int)blockIdx.x, split = (int)blockIdx.y, group = a.groups - 1 - a.group0 - (int)blockIdx.z;
     const int R = a.n * g, row0 = group * ROWS, rows = min(R - row0, ROWS);
@@ -694,11 +695,12 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 
     f32x4 acc[CT][2 * NB];
     float m[CT], lim[CT], l[CT];                                     // what scores are less by; the weight that moves it; sum of weights
-    float base = 7.f;                                                // log2 of the weight a new maximum gets
+    float base[CT];                                                  // log2 of the weight a new maximum gets
     int   unit = 0;                                                  // mxfp4: acc counts 2^unit
-    bool  based = DT != L3M_Q4_0;                                    // q4_0: of its product with the first tile's largest scale
+    bool  based = DT != L3M_Q4_0;                                    // q4_0: of its product with the largest scale the row sees in the first tile
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
+        base[ct] = 7.f;
         m[ct] = 0.f;
         lim[ct] = -1.f;                                              // a row's first score always does
         l[ct] = 0.f;
@@ -736,9 +738,22 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         return fresh ? 1.f : ldexpf(1.f, was - unit);
     };
 
-    auto step = [&](const int tile, auto masked) {
+    // mxfp4: whether a tile's exponents, those of positions before `end`, are all f16's.
+    auto narrow = [&](int tile, int end) {
+        if constexpr (DT == L3M_Q4_0) return true;
+        else {
+            const int left = end - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
+            const uint32_t none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left;
+            return !__ballot(!f16_range((keys.four & ~none) | (0x7F7F7F7Fu & none)));
+        }
+    };
+    // A tile (masked: the positions before `end`; each: for the rows that see just those, alone). Then the words of tile `next`.
+    auto step = [&](const int tile, const int next, const int end, const bool each, auto masked) {
         constexpr bool MASK = decltype(masked)::value;
         const int p0 = tile * TILE + 8 * g4;
+        int upto[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) upto[ct] = each && seen[ct] != end ? 0 : seen[ct];
         float p[CT][8];
 #pragma unroll
         for (int f = 0; f < 2; f++) {
@@ -749,11 +764,12 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) p[ct][4 * f + r] = !MASK || p0 + 4 * f + r < seen[ct] ? c[ct][r] : -INFINITY;
+                for (int r = 0; r < 4; r++) p[ct][4 * f + r] = !MASK || p0 + 4 * f + r < upto[ct] ? c[ct][r] : -INFINITY;
         }
         uint32_t four = 0;
         if constexpr (DT != L3M_Q4_0) four = keys.four;
-        keys.load(H, min(tile + 1, t1 - 1), lane);
+        const bool fits = narrow(tile, MASK ? end : INT_MAX);
+        keys.load(H, next, lane);
         float to_unit = 1.f;
         uint32_t nan[CT];                                            // blocks whose value is NaN at a position the row sees
 #pragma unroll
@@ -761,10 +777,10 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         if constexpr (DT != L3M_Q4_0) {
             uint32_t none = 0;                                       // exponents of positions that no row sees do not count
             if constexpr (MASK) {
-                const int left = a.pos + last + 1 - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
+                const int left = end - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
                 none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left;
             }
-            if (unit || __ballot(!f16_range((four & ~none) | (0x7F7F7F7Fu & none)))) {
+            if (unit || !fits) {
                 to_unit = fit_unit(four | none, tile == t0);
                 if constexpr (MASK)                                  // NaN for the rows that see it, and for no other: 0 here, put in below
 #pragma unroll
@@ -774,7 +790,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
                             if ((vals.e[b][i >> 2] >> 8 * (i & 3) & 255u) == E8M0_NAN) {
                                 vals.e[b][i >> 2] ^= 128u << 8 * (i & 3);   // 127; a NaN block's codes are 0
 #pragma unroll
-                                for (int ct = 0; ct < CT; ct++) nan[ct] |= p0 + i < seen[ct] ? 1u << b : 0u;
+                                for (int ct = 0; ct < CT; ct++) nan[ct] |= p0 + i < upto[ct] ? 1u << b : 0u;
                             }
             }
         }
@@ -792,18 +808,18 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const uint32_t u = __builtin_bit_cast(uint16_t, vals.d[b][i]) & 0x7FFFu;
-                            most = max(most, u < 0x7C00u ? u : 0u);
+                            most = max(most, u < 0x7C00u && (!MASK || p0 + i < upto[ct]) ? u : 0u);
                         }
-                    base -= (float)max((int)max_wave((float)most) >> 10, 1) - 15.f;
+                    base[ct] -= (float)max((int)max_g4((float)most) >> 10, 1) - 15.f;
                     based = true;
                 }
                 const float top = max_g4(max8(p[ct]));
-                const bool move = top > (lim[ct] < 0.f ? -INFINITY : base + 8.f);
-                const float up = move ? top - base : 0.f, f = __builtin_amdgcn_exp2f(-up);
-                if (move) lim[ct] = __builtin_amdgcn_exp2f(base + 8.f);
+                const bool move = top > (lim[ct] < 0.f ? -INFINITY : base[ct] + 8.f);
+                const float up = move ? top - base[ct] : 0.f, f = __builtin_amdgcn_exp2f(-up);
+                if (move) lim[ct] = __builtin_amdgcn_exp2f(base[ct] + 8.f);
                 m[ct] += up;
                 l[ct] *= f;
-                scale_acc(ct, f * to_unit);
+                scale_acc(ct, f * (each && seen[ct] != end ? 1.f : to_unit));
 #pragma unroll
                 for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(p[ct][i] - up);
             }
@@ -824,7 +840,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         x[i] = fmaf(p[ct][i], (float)vals.d[b][i], 0.f);
-                        if constexpr (MASK) x[i] = p0 + i < seen[ct] ? x[i] : 0.f;         // a masked position's scale may be anything
+                        if constexpr (MASK) x[i] = p0 + i < upto[ct] ? x[i] : 0.f;         // a masked position's scale may be anything
                     }
                 };
 #pragma unroll
@@ -833,21 +849,24 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) most = fmaxf(fmaxf(most, fabsf(w[b % KEPT][i])), fabsf(w[b % KEPT][i + 1]));
                 }
-                // past f16 soon: every weight of the rows 2^-16 of what it was (a scale of another size than the first tile's). A scale that
+                // past f16 soon: every weight of the row 2^-16 of what it was (a scale of another size than the first tile's). A scale that
                 // is infinite, which only memory that was never written holds, stays infinite and is not waited for
-                while (__ballot(most > 32768.f && most < INFINITY)) {
-                    scale_acc(ct, 0x1p-16f);
-                    l[ct] *= 0x1p-16f;
-                    m[ct] += 16.f;
-                    lim[ct] *= lim[ct] < 0.f ? 1.f : 0x1p-16f;
-                    base -= 16.f;
-                    most *= 0x1p-16f;
+                most = most < INFINITY ? most : 0.f;
+                while (__ballot(most > 32768.f)) {
+                    const bool  down = max_g4(most) > 32768.f;
+                    const float f = down ? 0x1p-16f : 1.f;
+                    scale_acc(ct, f);
+                    l[ct] *= f;
+                    m[ct] += down ? 16.f : 0.f;
+                    lim[ct] *= lim[ct] < 0.f ? 1.f : f;
+                    base[ct] -= down ? 16.f : 0.f;
+                    most *= f;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) p[ct][i] *= 0x1p-16f;
+                    for (int i = 0; i < 8; i++) p[ct][i] *= f;
 #pragma unroll
                     for (int b = 0; b < KEPT; b++)
 #pragma unroll
-                        for (int i = 0; i < 8; i++) w[b][i] *= 0x1p-16f;
+                        for (int i = 0; i < 8; i++) w[b][i] *= f;
                 }
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
@@ -866,7 +885,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     d[i] = pow2_byte(vals.e[b][i >> 2], i & 3);
-                    if constexpr (MASK) d[i] = p0 + i <= a.pos + last ? d[i] : 1.f;
+                    if constexpr (MASK) d[i] = p0 + i < end ? d[i] : 1.f;
                 }
                 widen_v(&vals.q[2 * b], d, v0, v1);
 #pragma unroll
@@ -883,15 +902,45 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
                         for (int b = 0; b < NB; b++)
                             if (max_g4((float)(nan[ct] >> b & 1u)) != 0.f) acc[ct][2 * b] = acc[ct][2 * b + 1] = f32x4{NAN, NAN, NAN, NAN};
         }
-        vals.load(H, min(tile + 1, t1 - 1), lane);
+        vals.load(H, next, lane);
     };
     int tile = t0;
-    for (; tile < min(t1, (int)whole); tile++) step(tile, std::false_type{});
-    for (; tile < t1; tile++) step(tile, std::true_type{});
-    if constexpr (DT != L3M_Q4_0)
-        if (unit)
+    for (; tile < min(t1, (int)whole); tile++) step(tile, min(tile + 1, t1 - 1), INT_MAX, false, std::false_type{});
+    // mxfp4 exponents of a masked tile that are not all f16's: a token at a time, in a unit of its own, so that no token's output hangs on
+    // positions behind it
+    int units[CT];
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) scale_acc(ct, ldexpf(1.f, unit));
+    for (int ct = 0; ct < CT; ct++) units[ct] = unit;
+    for (; tile < t1; tile++) {
+        const int end = a.pos + last + 1;
+        bool each = false;
+        if constexpr (DT != L3M_Q4_0) {
+            each = !narrow(tile, end);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) each = each || __ballot(units[ct] != 0);
+        }
+        for (int to = each ? a.pos + first + 1 : end; to <= end; to++) {
+            if (each) {
+                float u = -1000.f;
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) u = seen[ct] == to ? fmaxf(u, (float)units[ct]) : u;
+                unit = __builtin_amdgcn_readfirstlane((int)max_wave(u));
+            }
+            step(tile, to < end ? tile : min(tile + 1, t1 - 1), to, each, std::true_type{});
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) units[ct] = each && seen[ct] != to ? units[ct] : unit;
+        }
+    }
+    if constexpr (DT != L3M_Q4_0) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+            if (__ballot(units[ct] != 0)) {
+                const bool far = units[ct] > 60;                     // sums of values near float32's end: weights 2^-48 of what they were
+                scale_acc(ct, ldexpf(1.f, far ? units[ct] - 48 : units[ct]));
+                l[ct] *= far ? 0x1p-48f : 1.f;
+                m[ct] += far ? 48.f : 0.f;
+            }
+    }
 
     // the wavefronts' parts at their common maximum; where LDS has no room for all, the second half first and the first half onto them
 #pragma unroll

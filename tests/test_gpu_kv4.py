@@ -374,6 +374,38 @@ def test_attend_value_sizes(dev, dtype, sizes):
         dev.free_all()
 
 
+def each_near(dtype, got, q, k, v, pos):
+    """Every token against what it sees alone: the bound of its error knows nothing of the positions behind it."""
+    for t in range(len(q)):
+        near(got[t:t + 1], *attended(dtype, q[t:t + 1], k[:pos + t + 1], v[:pos + t + 1], pos + t))
+
+
+@DTYPES
+@pytest.mark.parametrize("sizes", ["high", "low", "rising", "top"])
+@pytest.mark.parametrize("nq, nkv, hd, n", [(6, 2, 64, 50), (2, 1, 200, 70), (64, 64, 96, 250)], ids=str)
+def test_attend_sizes_behind(dev, dtype, nq, nkv, hd, n, sizes):
+    """V rows whose size changes from one position of a tile to the next, up to the ends of what the scales hold: a token is as near its formula as
+    if the positions behind it were not there, whether the call's own tokens wrote them or an earlier, longer sequence did. (64, 64, 96, 250: two
+    columns of rows a workgroup.)"""
+    top, bottom = (14, -14) if dtype == Q4_0 else (123, -110)
+    rng, at = np.random.default_rng(n), np.arange(n)
+    e = {"high": np.where(at < 20, 0, top), "low": np.where(at < 20, 0, bottom), "rising": bottom + (top - bottom) * at // n, "top": np.full(n, top)}[sizes]
+    rows = rng.standard_normal((n, 2, nkv, hd)).astype(np.float32)
+    rows[:, 1] *= np.exp2(e.astype(np.float64)).astype(np.float32)[:, None, None]
+    assert np.isfinite(rows).all()
+    c = dev.kv4(dtype, nkv, hd, n)
+    dev.kv4_append(c, rows.reshape(n, -1), 0, 0)
+    k, v = (x.astype(np.float64) for x in dev.kv4_rows(c, 0, n))
+    q = rng.standard_normal((n, nq, hd)).astype(np.float32)
+    g = nq // nkv
+    all_heads = dev.kv4_attend(c, q, 0)
+    few = dev.kv4_attend(c, q[10:15], 10)
+    for h in sorted({0, nkv // 2, nkv - 1}):
+        heads = slice(h * g, (h + 1) * g)
+        each_near(dtype, all_heads[:, heads], q[:, heads], k[:, h:h + 1], v[:, h:h + 1], 0)
+        each_near(dtype, few[:, heads], q[10:15, heads], k[:15, h:h + 1], v[:15, h:h + 1], 10)
+
+
 def test_out_may_be_q(dev):
     nq, nkv, hd = 8, 2, 128
     for n, seen in ((1, 5000), (70, 100)):
