@@ -451,6 +451,30 @@ def test_planes_past_32_bits(dev, dtype):
         dev.free_all()
 
 
+@DTYPES
+def test_attend_past_32_bits(dev, dtype):
+    """One head's positions past 4 GiB of codes: rows of zeros but for 90, whose scores stand out. Weights add up over the whole length, outputs over
+    the 90."""
+    hd, nq, cap, step = 256, 2, (1 << 25) + 100, 1 << 18
+    c, rng = dev.kv4(dtype, 1, hd, cap), np.random.default_rng(1)
+    zeros = dev.alloc(8 * hd * step)
+    assert dev.lib.l3m_dev_upload(zeros, np.zeros(2 * hd * step, np.float32).ctypes.data, 8 * hd * step) == 0
+    for pos in range(0, cap, step):
+        assert dev.lib.l3m_k_kv4_append(C.byref(c), None, zeros, 2 * hd, min(step, cap - pos), 0, None, None, 0.0, 0, pos, None, None) == 0
+    ks, vs = [], []
+    for pos in (5, (1 << 24) + 17, cap - 30):
+        dev.kv4_append(c, (rng.standard_normal((30, 2, hd)) * [[[4], [1]]]).astype(np.float32).reshape(30, -1), 0, pos)
+        k, v = dev.kv4_rows(c, pos, 30)
+        ks.append(k[:, 0].astype(np.float64)), vs.append(v[:, 0].astype(np.float64))
+    k, v, q = np.concatenate(ks), np.concatenate(vs), (rng.standard_normal((1, nq, hd)) * 1.5).astype(np.float32)
+    got = dev.kv4_attend(c, q, cap - 1)
+    s = q[0].astype(np.float64) @ k.T / 16
+    p = np.exp(s)
+    p /= p.sum(1, keepdims=True) + cap - 90
+    off = 2 * (hd + 16) * 2.0 ** -24 * (np.abs(q[0].astype(np.float64)) @ summed(dtype, k).T / 16).max(1) + 2.0 ** -21 + (cap / 32 + 64) * 2.0 ** -24
+    near(got[0], p @ v, off[:, None] * (p @ summed(dtype, v)) + 91 * 2.0 ** -32 * np.abs(v).max())
+
+
 # ---------------------------------------------------------------- streams, graphs, and all of them together
 
 def test_streams_and_capture(dev):
