@@ -626,8 +626,8 @@ struct AttendIn {
     float       *out, *ml, *parts;                                   // ml, parts: [row of out][split] maximum and sum, output
     const float *q;
     l3m_kv4      c;
-    int          n, nq, g, pos, groups, group0, splits;              // splits: a power of two
-    uint32_t     g_mul, quad_mul;                                    // of g and hd / 4 (divide)
+    int          n, nq, g, pos, groups, group0, splits;
+    uint32_t     g_mul, quad_mul, of_mul;                            // of g, hd / 4 and splits WAVES (divide)
 };
 // x / d by d's multiplier, exact while x d < 2^32; 0: d is 1, or too large for it.
 __host__ inline uint32_t multiplier(uint32_t d, uint32_t most) {
@@ -675,7 +675,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     const int R = a.n * g, row0 = group * ROWS, rows = min(R - row0, ROWS);
     const int first = (int)divide(row0, g, a.g_mul), last = (int)divide(row0 + rows - 1, g, a.g_mul);   // the rows' tokens
     const unsigned tiles = (unsigned)(a.pos + last + TILE) / TILE, whole = (unsigned)(a.pos + first + 1) / TILE;   // tiles seen; those with nothing masked
-    const unsigned part = (unsigned)(split * WAVES + wave), of = (unsigned)a.splits * WAVES, share = tiles >> (31 - __clz(of)), more = tiles & (of - 1);
+    const unsigned part = (unsigned)(split * WAVES + wave), of = (unsigned)a.splits * WAVES, share = divide(tiles, of, a.of_mul), more = tiles - share * of;
     const int t0 = (int)(part * share + min(part, more)), t1 = t0 + (int)(share + (part < more));
     const Head H = head_of(a.c, NB, sbytes(DT), h);
     KeysIn<DT, NB> keys;
@@ -1101,9 +1101,9 @@ template <int DT> void launch_rows_in(RowsIn a, const l3m_kv4 &c, hipStream_t st
     else if constexpr (DT < 0) hipLaunchKernelGGL((k_rows_in<DT, false>), grid, dim3(256), 0, st, a, c);
 }
 // Columns of 16 rows a workgroup takes of each kv head's `rows`. Two share a tile's conversions, which pays for mxfp4 heads of 65 to 128
-// once every CU has two workgroups all the same: 1024 tokens behind 2999, 32 heads over 8, hd 128: 98 us, one column 113; 128
-// tokens behind 2000: 23 us, one column 13. q4_0 has no registers for it (183 us with one, 235 with two), shorter heads little to share (hd 64,
-// 2048 tokens behind 2000, 9 heads over 3: 43 and 40 us).
+// once every CU has two workgroups all the same: 1024 tokens behind 2999, 32 heads over 8, hd 128: 99 us, one column 117 (hd 96: 86 and 100);
+// 128 tokens behind 2000: 22 us, one column 15. q4_0 has no registers for it (198 us with one, 286 with two), shorter heads little to
+// share (hd 64, 2048 tokens behind 2000, 9 heads over 3: 42 us both).
 int tile_columns(int dt, int nb, int nkv, long long rows) { return dt == L3M_MXFP4 && (nb == 3 || nb == 4) && nkv * ((rows + 31) / 32) >= 512 ? 2 : 1; }
 template <int DT> void launch_attend(AttendIn a, int ct, hipStream_t st) {
     for (; a.group0 < a.groups; a.group0 += 65535) {                 // a grid's last dimension
@@ -1128,17 +1128,17 @@ template <int DT> void launch_attend(AttendIn a, int ct, hipStream_t st) {
 #undef ATTEND
     }
 }
-// Workgroups that share the positions of 16 rows, a power of two, with `alone` workgroups unsplit. A split costs the join, some 3.5 us and what
-// the rows' parts take; a tile costs a wavefront about 0.21 us a block (q4_0), 0.13 (mxfp4). Unsplit against split: q4_0, 32 heads over 8
-// of 128, one token over 256 positions 5.4 and 7.2 us, 512: 7.1 and 7.1, 1024: 10.6 and 7.2; mxfp4 over 512: 5.7 and 6.8; 64 tokens behind 2000 (mxfp4)
-// 12.7 and 14.1, behind 4000 (q4_0) 32.7 and 25.3. Past one workgroup a CU many rows' parts cost more than they save (16 tokens behind
-// 2000, 256 workgroups 9.3 us, 512 11.3); one token takes two.
-int split_count(int dt, long long alone, int tiles, int nb, long long rows, bool one_group) {
+// Workgroups that share the positions of 16 rows, with `alone` workgroups unsplit. A split costs the join, some 3.5 us and what the rows'
+// parts take; a tile costs a wavefront about 0.21 us a block (q4_0), 0.13 (mxfp4). Unsplit against split: q4_0, 32 heads over 8 of 128, one
+// token over 256 positions 5.6 and 7.2 us, 512: 7.7 and 7.2, 1024: 11.7 and 7.3; mxfp4 over 512: 6.0 and 6.9, 1024: 8.2 and 6.9; 64 tokens
+// behind 2000 (mxfp4) 14.8 and 15.3, behind 4000 (q4_0) 37 and 26. Down to a tile a wavefront: against two tiles, one token over 1024 (q4_0) 7.3
+// and 8.3 us. Up to one workgroup a CU, two where a wavefront has six tiles all the same (then they
+// hide each other's loads; between the two some CUs are left with half): one token over 32768 (mxfp4, 32 heads over 8 of 128; caches past
+// the Infinity Cache in turn) 15.0 us with one, 16.1 with two; 131071: 38.4 and 34.6, q4_0 49.4 and 46.9; 16 tokens behind 2000 9.6 and 11.9.
+int split_count(int dt, long long alone, int tiles, int nb, long long rows) {
     if ((long long)tiles * nb <= (dt == L3M_Q4_0 ? 56 : 90) + rows / 8) return 1;
-    const long long room = (one_group ? SPLIT_WGS : SPLIT_WGS / 2) / alone, most = (tiles + WAVES - 1) / WAVES;
-    int splits = 1;
-    while (2 * splits <= room && 2 * splits <= most && 2 * splits <= SPLITS) splits *= 2;
-    return splits;
+    const long long two = SPLIT_WGS / alone, most = (tiles + WAVES - 1) / WAVES, room = most >= 6 * two ? two : two / 2, splits = room < most ? room : most;
+    return splits < 2 ? 1 : splits < SPLITS ? (int)splits : SPLITS;
 }
 constexpr long long MAX_ITEMS = (1ll << 26) - 4;                     // wavefronts of a launch (its threads are counted in 32 bits)
 
@@ -1200,7 +1200,7 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
 size_t l3m_kv4_work_bytes(const l3m_kv4 *c, int n, int nq) {
     if (kv4_bad(c) || n < 1 || n > c->cap || nq < 1 || nq > 65536 || nq % c->nkv) return 0;
     const size_t rows = (size_t)n * (nq / c->nkv);                   // a workgroup's of a split: 16 at most
-    return 4 * (size_t)SPLIT_WGS * (rows < 16 ? rows : 16) * (c->hd + 2);
+    return 4 * (size_t)SPLIT_WGS * (rows < 16 ? rows : 16) * (c->hd + 2) + 16;
 }
 
 int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq, int pos, void *work, size_t work_bytes, void *stream) {
@@ -1217,10 +1217,11 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     const long long R = (long long)n * (nq / c->nkv);
     const int ct = tile_columns(c->dtype, (c->hd + 31) / 32, c->nkv, R), per = 16 * ct, groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;
     const long long alone = (long long)c->nkv * groups;
-    const int splits = split_count(c->dtype, alone, tiles, (c->hd + 31) / 32, (long long)rows, R <= 16);
+    const int splits = split_count(c->dtype, alone, tiles, (c->hd + 31) / 32, (long long)rows);
     const int g = nq / c->nkv;
     float *ml = (float *)work;
-    const AttendIn a = {out, ml, ml + 2 * rows * splits, q, *c, n, nq, g, pos, groups, 0, splits, multiplier(g, (uint32_t)R), multiplier(c->hd / 4, 4096)};
+    const AttendIn a = {out, ml, ml + (2 * rows * splits + 3) / 4 * 4, q, *c, n, nq, g, pos, groups, 0, splits, multiplier(g, (uint32_t)R), multiplier(c->hd / 4, 4096),
+                        multiplier(splits * WAVES, (uint32_t)tiles)};
     hipStream_t st = as_stream(stream);
     if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, ct, st);
     else launch_attend<L3M_MXFP4>(a, ct, st);
