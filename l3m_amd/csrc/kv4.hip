@@ -1128,15 +1128,17 @@ template <int DT> void launch_attend(AttendIn a, int ct, hipStream_t st) {
 #undef ATTEND
     }
 }
-// Workgroups that share the positions of 16 rows, with `alone` workgroups unsplit. A split costs the join, some 3.5 us and what the rows'
-// parts take; a tile costs a wavefront about 0.21 us a block (q4_0), 0.13 (mxfp4). Unsplit against split: q4_0, 32 heads over 8 of 128, one
-// token over 256 positions 5.6 and 7.2 us, 512: 7.7 and 7.2, 1024: 11.7 and 7.3; mxfp4 over 512: 6.0 and 6.9, 1024: 8.2 and 6.9; 64 tokens
-// behind 2000 (mxfp4) 14.8 and 15.3, behind 4000 (q4_0) 37 and 26. Down to a tile a wavefront: against two tiles, one token over 1024 (q4_0) 7.3
-// and 8.3 us. Up to one workgroup a CU, two where a wavefront has six tiles all the same (then they
-// hide each other's loads; between the two some CUs are left with half): one token over 32768 (mxfp4, 32 heads over 8 of 128; caches past
-// the Infinity Cache in turn) 15.0 us with one, 16.1 with two; 131071: 38.4 and 34.6, q4_0 49.4 and 46.9; 16 tokens behind 2000 9.6 and 11.9.
+// Workgroups that share the positions of 16 rows, with `alone` workgroups unsplit. A split costs the join, 2.5 us and more with the rows'
+// parts; a tile costs a wavefront 0.2 us and 0.2 (q4_0) or 0.1 (mxfp4) a block. Unsplit against split over 78 shapes of 1 to 64 tokens and 128
+// to 2048 positions, heads of 32 to 256 (the rule is at most 5% off the better one, 0.15% on average), one token of 32 heads over 8 of 128:
+// q4_0 over 256 positions 5.5 and 7.2 us, 512: 7.6 and 7.3, 1024: 11.5 and 7.4; mxfp4 over 512: 6.0 and 6.9, 1024: 8.3 and 6.9; 64 tokens of
+// 2048: mxfp4 14.7 and 15.1, q4_0 21 and 19. Down to a tile a wavefront: against two tiles, one token over 1024 (q4_0) 7.3 and 8.3 us. Up to
+// one workgroup a CU, two where a wavefront has six tiles all the same (then they hide each other's loads; between the two some CUs
+// are left with half): one token over 32768 (mxfp4, 32 heads over 8 of 128; caches past the Infinity Cache in turn) 15.0 us with one, 16.1 with
+// two; 131071: 38.4 and 34.6, q4_0 49.4 and 46.9; 16 tokens behind 2000 9.6 and 11.9.
 int split_count(int dt, long long alone, int tiles, int nb, long long rows) {
-    if ((long long)tiles * nb <= (dt == L3M_Q4_0 ? 56 : 90) + rows / 8) return 1;
+    const bool q4 = dt == L3M_Q4_0;
+    if ((long long)tiles * (nb + (q4 ? 1 : 2)) <= (q4 ? 66 : 120) + rows / 10) return 1;
     const long long two = SPLIT_WGS / alone, most = (tiles + WAVES - 1) / WAVES, room = most >= 6 * two ? two : two / 2, splits = room < most ? room : most;
     return splits < 2 ? 1 : splits < SPLITS ? (int)splits : SPLITS;
 }
