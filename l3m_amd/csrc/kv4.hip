@@ -373,8 +373,6 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // by instruction issue: 1024 tokens behind 2999, the same heads, mxfp4, 99 us, 590 TFLOP/s; a SIMD issues VALU work for 158k of 212k cycles, 309
 // instructions a tile of 32 rows, and its matrix unit is busy for 92k. Tried without gain: eight wavefronts a workgroup, a tile
 // requested ahead, values a tile ahead, raised wave priority around the products.
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -388,14 +386,13 @@ constexpr int WAVES = 4;
 constexpr int SPLIT_WGS = 512, SPLITS = 256;                         // workgroups up to which a cache is split; most parts of it
 constexpr float M0 = -3e38f;                                         // the maximum of no score: below every one
 
-// A q4_0 word's eight codes, 0 .. 15, in bf16: a nibble alone in a byte is the e4m3 number 2^-9 times it.
-__device__ __forceinline__ bf16x8 widen(uint32_t w) {
+// A q4_0 K word's eight codes, 0 .. 15, in f16: a nibble alone in a byte is the e4m3 number 2^-9 times it.
+__device__ __forceinline__ f16x8 widen(uint32_t w) {
     const int lo = (int)(w & 0x0F0F0F0Fu), hi = (int)(w >> 4 & 0x0F0F0F0Fu);
-    const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true);
-    const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true);
-    return bf16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+    const f16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, true);
+    const f16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, true);
+    return f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
 }
-__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 // Byte i of w as the power of two that it is the exponent of.
 __device__ __forceinline__ float pow2_byte(uint32_t w, int i) {     // one instruction, where the compiler takes a shift and a mask
     float r;
@@ -460,11 +457,34 @@ __device__ __forceinline__ bool f16_range(uint32_t w) {
     return ((from104 ^ w) & ~(from141 & w) & 0x80808080u) == 0x80808080u;
 }
 
+// The maximum and the sum of a row of 16 lanes' (DPP), over lane ^ 16 and lane ^ 32.
+__device__ __forceinline__ float other16(float x, float &y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    y = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float other32(float x, float &y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    y = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float max_g4(float x) {
+    float y;
+    x = other16(x, y); x = fmaxf(x, y);
+    x = other32(x, y); return fmaxf(x, y);
+}
+__device__ __forceinline__ float sum_g4(float x) {
+    float y;
+    x = other16(x, y); x += y;
+    x = other32(x, y); return x + y;
+}
+
 // The scores of one half of a tile, 16 positions x 16 rows, from the queries of a row held in parts (Queries) and what a lane reads of the
 // keys (KeysIn).
 //
-// q4_0: 16x16x32 bf16 products of a block's codes 0 .. 15 with q in three bf16 parts (8 + 8 + 8 bits: exact), begun at -8 sum q; a block's
-// sum times d, which belongs to a position, in 32 bits.
+// q4_0: 16x16x32 f16 products of a block's codes 0 .. 15 with q in two f16 parts, begun at -8 sum q; a block's sum times d, which belongs to
+// a position, in 32 bits. A row of q is scaled by a power of two to a largest value of 2^13 .. 2^14: 22 bits of each value, and 2^-38 of
+// the largest at the least.
 //
 // mxfp4: 16x16x128 products of the codes as they lie with their scales (v_mfma_scale_f32_16x16x128_f8f6f4, fp4 operand): lane 16 c + m gives
 // block c of position m, and q is the fp6 (e2m3) operand, a block in five parts with scales of their own. A part takes five bits of
@@ -486,39 +506,49 @@ template <int NB> struct KeysIn<L3M_Q4_0, NB> {
     }
 };
 template <int NB> struct Queries<L3M_Q4_0, NB> {
-    bf16x8 part[NB][3];
-    float  off[NB];                                                  // -8 sum of a block's q
+    f16x8 part[NB][2];
+    f32x4 off[NB];                                                   // -8 sum of a block's q
+    float unit;                                                      // of the scores
     __device__ __forceinline__ void load(const float *q, int hd, float scale, int lane) {
+        float x[NB][8];
+        uint32_t peak = 0;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             const int d = 32 * b + 8 * (lane >> 4);
             const bool in = d < hd;
             const f32x4 x0 = *(const f32x4_a4 *)(q + (in ? d : 0)), x1 = *(const f32x4_a4 *)(q + (in ? d + 4 : 4));
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[b][i] = in ? (i < 4 ? x0[i & 3] : x1[i & 3]) * scale : 0.f;
+                peak = max(peak, __float_as_uint(x[b][i]) & 0x7FFFFFFFu);
+            }
+        }
+        peak = __float_as_uint(max_g4(__uint_as_float(min(peak, 0x7F7FFFFFu))));
+        const int e = 140 - (int)(peak >> 23);
+        unit = ldexpf(1.f, -e);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float x = in ? (i < 4 ? x0[i & 3] : x1[i & 3]) * scale : 0.f;
-                const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), rem = x - hi, mid = __uint_as_float(__float_as_uint(rem) & 0xFFFF0000u);
-                part[b][0][i] = (__bf16)hi;
-                part[b][1][i] = (__bf16)mid;
-                part[b][2][i] = (__bf16)(rem - mid);
-                sum += x;
+                const float y = ldexpf(x[b][i], e);
+                const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
+                part[b][0][i] = hi;
+                part[b][1][i] = lo;
+                sum += y;
             }
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            off[b] = -8.f * sum;
+            sum = -8.f * sum_g4(sum);
+            off[b] = f32x4{sum, sum, sum, sum};
         }
     }
 };
 template <int NB, int CT> __device__ __forceinline__ void scores(const KeysIn<L3M_Q4_0, NB> &k, const Queries<L3M_Q4_0, NB> (&q)[CT], int f, f32x4 (&c)[CT]) {
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        const bf16x8 w = widen(k.q[f][b]);
+        const f16x8 w = widen(k.q[f][b]);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            f32x4 x = {q[ct].off[b], q[ct].off[b], q[ct].off[b], q[ct].off[b]};
-#pragma unroll
-            for (int i = 0; i < 3; i++) x = mfma(w, q[ct].part[b][i], x);
+            const f32x4 x = mfma(w, q[ct].part[b][1], mfma(w, q[ct].part[b][0], q[ct].off[b]));
 #pragma unroll
             for (int r = 0; r < 4; r++) c[ct][r] = fmaf(x[r], (float)k.d[b][4 * f + r], c[ct][r]);
         }
@@ -645,27 +675,6 @@ __host__ inline uint32_t multiplier(uint32_t d, uint32_t most) {
     return d > 1 && (uint64_t)most * d < 1ull << 32 ? (uint32_t)((1ull << 32) / d) + 1 : 0;
 }
 __device__ __forceinline__ uint32_t divide(uint32_t x, uint32_t d, uint32_t mul) { return mul ? __umulhi(x, mul) : d == 1 ? x : x / d; }
-// The maximum and the sum of a row of 16 lanes' (DPP), over lane ^ 16 and lane ^ 32.
-__device__ __forceinline__ float other16(float x, float &y) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    y = __uint_as_float(r[1]);
-    return __uint_as_float(r[0]);
-}
-__device__ __forceinline__ float other32(float x, float &y) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    y = __uint_as_float(r[1]);
-    return __uint_as_float(r[0]);
-}
-__device__ __forceinline__ float max_g4(float x) {
-    float y;
-    x = other16(x, y); x = fmaxf(x, y);
-    x = other32(x, y); return fmaxf(x, y);
-}
-__device__ __forceinline__ float sum_g4(float x) {
-    float y;
-    x = other16(x, y); x += y;
-    x = other32(x, y); return x + y;
-}
 template <int CTRL> __device__ __forceinline__ float dpp(float x) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true)); }
 __device__ __forceinline__ float max_wave(float x) {
     x = fmaxf(x, dpp<0xB1>(x)); x = fmaxf(x, dpp<0x4E>(x)); x = fmaxf(x, dpp<0x141>(x)); x = fmaxf(x, dpp<0x140>(x));
@@ -770,8 +779,16 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         for (int f = 0; f < 2; f++) {
             f32x4 c[CT];
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) c[ct] = f32x4{-m[ct], -m[ct], -m[ct], -m[ct]};
+            for (int ct = 0; ct < CT; ct++) {
+                const float from = DT == L3M_Q4_0 ? 0.f : -m[ct];
+                c[ct] = f32x4{from, from, from, from};
+            }
             scores<NB, CT>(keys, qs, f, c);
+            if constexpr (DT == L3M_Q4_0)
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) c[ct][r] = fmaf(c[ct][r], qs[ct].unit, -m[ct]);
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
@@ -844,46 +861,36 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         if constexpr (DT == L3M_Q4_0) {
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                constexpr int KEPT = NB <= 4 ? NB : 1;               // long heads have no registers for every block's products
-                float w[KEPT][8], most = 0.f;
-                auto products = [&](int b) {
-                    float (&x)[8] = w[b % KEPT];
+                float w[NB][8], most = 0.f;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        x[i] = fmaf(p[ct][i], (float)vals.d[b][i], 0.f);
-                        if constexpr (MASK) x[i] = p0 + i < upto[ct] ? x[i] : 0.f;         // a masked position's scale may be anything
+                        w[b][i] = fmaf(p[ct][i], (float)vals.d[b][i], 0.f);
+                        if constexpr (MASK) w[b][i] = p0 + i < upto[ct] ? w[b][i] : 0.f;   // a masked position's scale may be anything
+                        if (i & 1) most = fmaxf(fmaxf(most, fabsf(w[b][i - 1])), fabsf(w[b][i]));
                     }
-                };
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    products(b);
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) most = fmaxf(fmaxf(most, fabsf(w[b % KEPT][i])), fabsf(w[b % KEPT][i + 1]));
-                }
-                // past f16 soon: every weight of the row 2^-16 of what it was (a scale of another size than the first tile's). A scale that
-                // is infinite, which only memory that was never written holds, stays infinite and is not waited for
+                // past f16 soon: the row's weights such that its largest product here lies between 2^7 and 2^8 (a scale of another size than the
+                // first tile's). An infinite scale, which only memory that was never written holds, has no part in that
                 most = most < INFINITY ? most : 0.f;
-                while (__ballot(most > 32768.f)) {
-                    const bool  down = max_g4(most) > 32768.f;
-                    const float f = down ? 0x1p-16f : 1.f;
+                if (__ballot(most > 32768.f)) {
+                    const float top = max_g4(most);
+                    const int   k = top > 32768.f ? (int)(__float_as_uint(top) >> 23) - 134 : 0;
+                    const float f = __uint_as_float((uint32_t)(127 - k) << 23);
                     scale_acc(ct, f);
                     l[ct] *= f;
-                    m[ct] += down ? 16.f : 0.f;
+                    m[ct] += (float)k;
                     lim[ct] *= lim[ct] < 0.f ? 1.f : f;
-                    base[ct] -= down ? 16.f : 0.f;
-                    most *= f;
+                    base[ct] -= (float)k;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) p[ct][i] *= f;
-#pragma unroll
-                    for (int b = 0; b < KEPT; b++)
+                    for (int b = 0; b < NB; b++)
 #pragma unroll
                         for (int i = 0; i < 8; i++) w[b][i] *= f;
                 }
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    if constexpr (KEPT < NB) products(b);
                     const f16x8 v0 = widen_f16(vals.q[2 * b]), v1 = widen_f16(vals.q[2 * b + 1]);
-                    two_parts(w[b % KEPT], hi[ct], lo[ct]);
+                    two_parts(w[b], hi[ct], lo[ct]);
                     acc[ct][2 * b] = mfma(v0, lo[ct], mfma(v0, hi[ct], acc[ct][2 * b]));
                     acc[ct][2 * b + 1] = mfma(v1, lo[ct], mfma(v1, hi[ct], acc[ct][2 * b + 1]));
                 }
