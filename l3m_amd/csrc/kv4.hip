@@ -715,9 +715,8 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 
     f32x4 acc[CT][2 * NB];
     float m[CT], lim[CT], l[CT];                                     // what scores are less by; the weight that moves it; sum of weights
-    float base[CT];                                                  // log2 of the weight a new maximum gets
+    float base[CT];                                                  // log2 of the weight a new maximum gets; q4_0: with the first tile's largest scale
     int   unit = 0;                                                  // mxfp4: acc counts 2^unit
-    bool  based = DT != L3M_Q4_0;                                    // q4_0: of its product with the largest scale the row sees in the first tile
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         base[ct] = 7.f;
@@ -727,6 +726,19 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    if constexpr (DT == L3M_Q4_0)                                    // of those that the row sees
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t u = __builtin_bit_cast(uint16_t, vals.d[b][i]) & 0x7FFFu;
+                    most = max(most, u < 0x7C00u && t0 * TILE + 8 * g4 + i < seen[ct] ? u : 0u);
+                }
+            base[ct] -= (float)max((int)max_g4((float)most) >> 10, 1) - 15.f;
+        }
     auto scale_acc = [&](int ct, float f) {
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] *= f;
@@ -829,18 +841,6 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
             for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(p[ct][i]);
             if (__ballot(max8(e) > lim[ct]) || to_unit != 1.f) {
-                if (!based) {
-                    uint32_t most = 0;
-#pragma unroll
-                    for (int b = 0; b < (DT == L3M_Q4_0 ? NB : 0); b++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const uint32_t u = __builtin_bit_cast(uint16_t, vals.d[b][i]) & 0x7FFFu;
-                            most = max(most, u < 0x7C00u && (!MASK || p0 + i < upto[ct]) ? u : 0u);
-                        }
-                    base[ct] -= (float)max((int)max_g4((float)most) >> 10, 1) - 15.f;
-                    based = true;
-                }
                 const float top = max_g4(max8(p[ct]));
                 const bool move = top > (lim[ct] < 0.f ? -INFINITY : base[ct] + 8.f);
                 const float up = move ? top - base[ct] : 0.f, f = __builtin_amdgcn_exp2f(-up);
@@ -1119,18 +1119,23 @@ template <int DT> void launch_rows_in(RowsIn a, const l3m_kv4 &c, hipStream_t st
     if (a.hd % 8 == 0) hipLaunchKernelGGL((k_rows_in<DT, true>), grid, dim3(256), 0, st, a, c);
     else if constexpr (DT < 0) hipLaunchKernelGGL((k_rows_in<DT, false>), grid, dim3(256), 0, st, a, c);
 }
-// Columns of 16 rows a workgroup takes of each kv head's `rows`. Two share a tile's conversions, which pays for mxfp4 heads of 65 to 128
-// once every CU has two workgroups all the same: 1024 tokens behind 2999, 32 heads over 8, hd 128: 99 us, one column 117 (hd 96: 86 and 100);
-// 128 tokens behind 2000: 22 us, one column 15. q4_0 has no registers for it (198 us with one, 286 with two), shorter heads little to
-// share (hd 64, 2048 tokens behind 2000, 9 heads over 3: 42 us both).
-int tile_columns(int dt, int nb, int nkv, long long rows) { return dt == L3M_MXFP4 && (nb == 3 || nb == 4) && nkv * ((rows + 31) / 32) >= 512 ? 2 : 1; }
+// Columns of 16 rows a workgroup takes of each kv head's `rows`. Two share a tile's conversions, which pays for mxfp4 heads of 33 to 128
+// where every CU has two workgroups all the same and a last turn of them is not nearly empty: 1024 tokens behind 2999, 32 heads over 8,
+// hd 128: 98 us, one column 115 (96: 86 and 100, 64: 67 and 77); 128 tokens behind 2000: 22 us, one column 15; 564 workgroups (1500
+// tokens, 12 heads of 128) 28.8 and 25.4, 640 (1024 behind 2000, 20 heads over 5) 55.4 and 56. q4_0's do not pay: hd 128 has no registers
+// (228 us with two, 177 with one), hd 64 96 and 95.
+int tile_columns(int dt, int nb, int nkv, long long rows) {
+    const long long two = nkv * ((rows + 31) / 32), turns = (two + 511) / 512;
+    return dt == L3M_MXFP4 && nb >= 2 && nb <= 4 && two >= 512 && 5 * two >= 3 * 512 * turns ? 2 : 1;
+}
 template <int DT> void launch_attend(AttendIn a, int ct, hipStream_t st) {
     for (; a.group0 < a.groups; a.group0 += 65535) {                 // a grid's last dimension
         const dim3 grid(a.c.nkv, a.splits, a.groups - a.group0 < 65535 ? a.groups - a.group0 : 65535), wg(64 * WAVES);
 #define ATTEND(NB, CT) hipLaunchKernelGGL((k_kv4_attend<DT, NB, CT>), grid, wg, 0, st, a)
         if constexpr (DT == L3M_MXFP4)
             if (ct == 2) {
-                if (a.c.hd <= 96) ATTEND(3, 2);
+                if (a.c.hd <= 64) ATTEND(2, 2);
+                else if (a.c.hd <= 96) ATTEND(3, 2);
                 else ATTEND(4, 2);
                 continue;
             }

@@ -406,6 +406,27 @@ def test_attend_sizes_behind(dev, dtype, nq, nkv, hd, n, sizes):
         each_near(dtype, few[:, heads], q[10:15, heads], k[:15, h:h + 1], v[:15, h:h + 1], 10)
 
 
+@DTYPES
+@pytest.mark.parametrize("hd", [40, 64, 96, 128])
+def test_attend_many_rows(dev, dtype, hd):
+    """As many rows as take two columns a workgroup (mxfp4): heads of their own formula, a K and a V row that are not finite for the tokens
+    from theirs on alone."""
+    nq, nkv, n = 128, 64, 150
+    c, k, v, rng = filled(dev, dtype, nkv, hd, n, hd)
+    q = rng.standard_normal((n, nq, hd)).astype(np.float32)
+    got = dev.kv4_attend(c, q, 0)
+    for h in (0, 31, 63):
+        near(got[:, 2 * h:2 * h + 2], *attended(dtype, q[:, 2 * h:2 * h + 2], k[:, h:h + 1], v[:, h:h + 1], 0))
+    rows = np.concatenate([k[50], v[50]]).reshape(1, -1).astype(np.float32)
+    rows[0, 3 * hd], rows[0, (nkv + 5) * hd] = np.nan, np.inf
+    dev.kv4_append(c, rows, 0, 50)
+    bad = dev.kv4_attend(c, q, 0)
+    assert np.array_equal(bad[:50], got[:50])
+    assert np.isnan(bad[50:, 6:8]).all() and np.isnan(bad[50:, 10:12, :32]).all()
+    others = [h for h in range(nq) if h // 2 not in (3, 5)]
+    assert np.isfinite(bad[:, others]).all() and np.isfinite(bad[:, 10:12, 32:]).all()
+
+
 def test_out_may_be_q(dev):
     nq, nkv, hd = 8, 2, 128
     for n, seen in ((1, 5000), (70, 100)):
