@@ -579,7 +579,7 @@ template <int NB> struct KeysIn<L3M_MXFP4, NB> {
 };
 template <int NB> struct Queries<L3M_MXFP4, NB> {
     u32x6 part[Mx<NB>::fours][Mx<NB>::times];
-    int   e[Mx<NB>::fours][Mx<NB>::times];
+    int   e[Mx<NB>::fours][(Mx<NB>::times + 3) / 4];                 // the parts' exponents, a byte each
     __device__ __forceinline__ void load(const float *q, int hd, float scale, int lane) {
         const int c = lane >> 4;
 #pragma unroll
@@ -605,7 +605,7 @@ template <int NB> struct Queries<L3M_MXFP4, NB> {
 #pragma unroll
             for (int t = 0; t < Mx<NB>::times; t++) {
                 part[i][t] = u32x6{0, 0, 0, 0, 0, 0};
-                e[i][t] = 127;
+                e[i][t / 4] = 0x7F7F7F7F;
             }
 #pragma unroll
             for (int p = 0; p < Q_PARTS; p++) {
@@ -626,7 +626,7 @@ template <int NB> struct Queries<L3M_MXFP4, NB> {
                 const int t = p / Mx<NB>::at_once, at = p - t * Mx<NB>::at_once;
                 if (used && (Mx<NB>::at_once == 1 || first == at)) {
                     part[i][t] = w;
-                    e[i][t] = bad ? E8M0_NAN : ex;
+                    e[i][t / 4] ^= ((bad ? E8M0_NAN : ex) ^ 127) << 8 * (t % 4);
                 }
             }
         }
@@ -636,15 +636,24 @@ template <int NB, int CT> __device__ __forceinline__ void scores(const KeysIn<L3
 #pragma unroll
     for (int i = 0; i < Mx<NB>::fours; i++) {
         const i32x8 a = {(int)k.q[f][i].x, (int)k.q[f][i].y, (int)k.q[f][i].z, (int)k.q[f][i].w, 0, 0, 0, 0};
-        const int   e = (int)(k.e[i] >> 8 * f);
-#pragma unroll
-        for (int t = 0; t < Mx<NB>::times; t++)
+        auto part = [&](auto which, auto half) {
+            constexpr int t = decltype(which)::value, F = decltype(half)::value;
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 const u32x6 &w = q[ct].part[i][t];
                 const i32x8 b = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], (int)w[4], (int)w[5], 0, 0};
-                c[ct] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c[ct], 4, 2, 0, e, 0, q[ct].e[i][t]);
+                c[ct] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c[ct], 4, 2, F, (int)k.e[i], t % 4, q[ct].e[i][t / 4]);
             }
+        };
+        auto parts = [&](auto half) {
+            part(std::integral_constant<int, 0>{}, half);
+            if constexpr (Mx<NB>::times > 1) part(std::integral_constant<int, 1>{}, half);
+            if constexpr (Mx<NB>::times > 2) part(std::integral_constant<int, 2>{}, half);
+            if constexpr (Mx<NB>::times > 3) part(std::integral_constant<int, 3>{}, half);
+            if constexpr (Mx<NB>::times > 4) part(std::integral_constant<int, 4>{}, half);
+        };
+        if (f == 0) parts(std::integral_constant<int, 0>{});
+        else parts(std::integral_constant<int, 1>{});
     }
 }
 
