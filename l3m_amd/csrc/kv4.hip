@@ -357,8 +357,8 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // 32 positions and wavefront, with the keys as the left operand so that lane 16 g4 + r holds the scores of row r for positions
 // 8 g4 .. 8 g4 + 7, which is where the second product wants the weights:
 //   S = K Q^T   16 positions x 16 rows, twice; q scaled by log2(e) / sqrt(hd) and held in parts (below)
-//   P = 2^(S - m), m such that the largest weight lies between 2^7 and 2^15: it moves only when one passes that, and -m is what the scores'
-//               accumulators begin at
+//   P = 2^(S - m), m such that the largest weight lies between 2^7 and 2^15: it moves only when one passes that, and -m is what mxfp4's
+//               accumulators begin at (q4_0's scores get it with their unit, in one operation)
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions (v_mfma_f32_16x16x32_f16), P in two f16 parts: 22 bits, and 2^-32 of the largest at the
 //               least. A position's scale differs from block to block. q4_0's multiplies P, in 32 bits, before it is split (the range of
 //               the weights then goes by the products). mxfp4's goes into the conversion of its codes (a layout of its own), exactly where
@@ -369,10 +369,11 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 //
 // A few tokens are bound by latency (one token over 40 positions 3.7 us, 256: 4.3, 480 tokens of 9 heads over 3 of 64 6.2 us: one
 // workgroup's tiles one after the other), long caches by the cache's bytes and the conversions together: one token over 131071 positions, 32
-// heads over 8 of 128, q4_0 (151 MB) 41 us, 3.7 TB/s with the SIMDs issuing three quarters of the time; mxfp4 over 32768 (36 MB) 10.4 us. Prompts
-// by instruction issue: 1024 tokens behind 2999, the same heads, mxfp4, 99 us, 590 TFLOP/s; a SIMD issues VALU work for 158k of 212k cycles, 309
-// instructions a tile of 32 rows, and its matrix unit is busy for 92k. Tried without gain: eight wavefronts a workgroup, a tile
-// requested ahead, values a tile ahead, raised wave priority around the products.
+// heads over 8 of 128, q4_0 (151 MB) 37.5 us, 4.0 TB/s with the SIMDs issuing three quarters of the time; mxfp4 over 32768 (36 MB) 10 us.
+// Prompts by instruction issue: 1024 tokens behind 2999, the same heads, mxfp4, 98 us, 600 TFLOP/s: VALU and matrix instructions, some 256 and 52
+// a tile of 32 rows, are issued for 158k of 211k cycles, the matrix unit is busy for 92k. q4_0, with every scale on the weights,
+// 177 us. Tried without gain: eight wavefronts a workgroup, a tile requested ahead, values a tile ahead, raised wave priority around the
+// products; a tile's scores beside the products of the one before has no registers.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -1035,8 +1036,8 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 }
 
 // The splits' parts of a row, one workgroup a (token, query head): groups of hd / 4 lanes take every so many splits, 16 bytes a lane and
-// eight loads in flight while every wavefront makes the splits' factors for itself; they meet in LDS in a fixed order. Bound by latency: 2.3 us
-// for 32 rows of 32 parts, 3.2 of 64. As the last workgroup's work in the launch before (tickets in memory) it took as long.
+// eight loads in flight while every wavefront makes the splits' factors for itself; they meet in LDS in a fixed order. Bound by latency: 2.4 us
+// for 32 rows of 32 parts, 3.8 of 64. As the last workgroup's work in the launch before (tickets in memory) it took as long.
 __global__ void __launch_bounds__(256) k_kv4_join(AttendIn a) {
     __shared__ float f_s[4][SPLITS];
     __shared__ f32x4 o_s[256];
