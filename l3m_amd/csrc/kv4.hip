@@ -736,17 +736,16 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if constexpr (DT == L3M_Q4_0)                                    // of those that the row sees
+    if constexpr (DT == L3M_Q4_0)                                    // of those that the row sees, of every eighth position: larger ones lower the weights
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             uint32_t most = 0;
 #pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t u = __builtin_bit_cast(uint16_t, vals.d[b][i]) & 0x7FFFu;
-                    most = max(most, u < 0x7C00u && t0 * TILE + 8 * g4 + i < seen[ct] ? u : 0u);
-                }
+            for (int b = 0; b < NB; b++) {
+                const _Float16 d = vals.d[b][0];
+                const uint32_t u = __builtin_bit_cast(uint16_t, d) & 0x7FFFu;
+                most = max(most, u < 0x7C00u && t0 * TILE + 8 * g4 < seen[ct] ? u : 0u);
+            }
             base[ct] -= (float)max((int)max_g4((float)most) >> 10, 1) - 15.f;
         }
     auto scale_acc = [&](int ct, float f) {
