@@ -852,7 +852,8 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             if (__ballot(max8(e) > lim[ct]) || to_unit != 1.f) {
                 const float top = max_g4(max8(p[ct]));
                 const bool move = top > (lim[ct] < 0.f ? -INFINITY : base[ct] + 8.f);
-                const float up = move ? top - base[ct] : 0.f, f = __builtin_amdgcn_exp2f(-up);
+                // a row's first maximum scales nothing: 2^-up of one below -121 is infinite, and the sums are zeros
+                const float up = move ? top - base[ct] : 0.f, f = lim[ct] < 0.f ? 1.f : __builtin_amdgcn_exp2f(-up);
                 if (move) lim[ct] = __builtin_amdgcn_exp2f(base[ct] + 8.f);
                 m[ct] += up;
                 l[ct] *= f;
