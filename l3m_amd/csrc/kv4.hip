@@ -357,11 +357,11 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // 32 positions and wavefront, with the keys as the left operand so that lane 16 g4 + r holds the scores of row r for positions
 // 8 g4 .. 8 g4 + 7, which is where the second product wants the weights:
 //   S = K Q^T   16 positions x 16 rows, twice; q scaled by log2(e) / sqrt(hd) and held in parts (below)
-//   P = 2^(S - m), m such that the largest weight lies between 2^7 and 2^15: it moves only when one passes that, and -m is what mxfp4's
-//               accumulators begin at (q4_0's scores get it with their unit, in one operation)
+//   P = 2^(S - m), m such that the largest weight lies between 2^7 and 2^15 (q4_0: times the largest scale): it moves only when one passes
+//               that, and -m is what mxfp4's accumulators begin at (q4_0's scores get it with their unit, in one operation)
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions (v_mfma_f32_16x16x32_f16), P in two f16 parts: 22 bits, and 2^-32 of the largest at the
 //               least. A position's scale differs from block to block. q4_0's multiplies P, in 32 bits, before it is split (the range of
-//               the weights then goes by the products). mxfp4's goes into the conversion of its codes (a layout of its own), exactly where
+//               the weights then goes by the scales). mxfp4's goes into the conversion of its codes (a layout of its own), exactly where
 //               it lies between 2^-23 and 2^13; for others the accumulators take another unit. A row's range, and NaN, come from
 //               positions that it sees, never from one behind it.
 // All sums in 32 bits. A workgroup's four wavefronts share 16 CT rows and split the tiles; they meet in LDS, and the workgroups of a
@@ -725,7 +725,8 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 
     f32x4 acc[CT][2 * NB];
     float m[CT], lim[CT], l[CT];                                     // what scores are less by; the weight that moves it; sum of weights
-    float base[CT];                                                  // log2 of the weight a new maximum gets; q4_0: with the first tile's largest scale
+    float base[CT];                                                  // log2 of the weight a new maximum gets; q4_0: of its product with the largest scale 7
+    constexpr float RISE = DT == L3M_Q4_0 ? 7.98f : 8.f;             // how far weights pass 2^base before it moves (q4_0: 2^16 less f16's room for products)
     int   unit = 0;                                                  // mxfp4: acc counts 2^unit
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
@@ -736,7 +737,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if constexpr (DT == L3M_Q4_0)                                    // of those that the row sees, of every eighth position: larger ones lower the weights
+    if constexpr (DT == L3M_Q4_0)                                    // the first tile's, of those that the row sees, of every eighth position: larger ones lower base
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             uint32_t most = 0;
@@ -851,10 +852,10 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(p[ct][i]);
             if (__ballot(max8(e) > lim[ct]) || to_unit != 1.f) {
                 const float top = max_g4(max8(p[ct]));
-                const bool move = top > (lim[ct] < 0.f ? -INFINITY : base[ct] + 8.f);
+                const bool move = top > (lim[ct] < 0.f ? -INFINITY : base[ct] + RISE);
                 // a row's first maximum scales nothing: 2^-up of one below -121 is infinite, and the sums are zeros
                 const float up = move ? top - base[ct] : 0.f, f = lim[ct] < 0.f ? 1.f : __builtin_amdgcn_exp2f(-up);
-                if (move) lim[ct] = __builtin_amdgcn_exp2f(base[ct] + 8.f);
+                if (move) lim[ct] = __builtin_amdgcn_exp2f(base[ct] + RISE);
                 m[ct] += up;
                 l[ct] *= f;
                 scale_acc(ct, f * (each && seen[ct] != end ? 1.f : to_unit));
@@ -880,12 +881,24 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
                         if constexpr (MASK) w[b][i] = p0 + i < upto[ct] ? w[b][i] : 0.f;   // a masked position's scale may be anything
                         if (i & 1) most = fmaxf(fmaxf(most, fabsf(w[b][i - 1])), fabsf(w[b][i]));
                     }
-                // past f16 soon: the row's weights such that its largest product here lies between 2^7 and 2^8 (a scale of another size than the
-                // first tile's). An infinite scale, which only memory that was never written holds, has no part in that
+                // past f16 soon, so a scale of more than 2^(8 - base): base goes by the largest one here, and 2^(base + RISE) times it is below
+                // 2^16 again. It goes by the scale, not by the product, whose weight may lie anywhere above 2^base: the next maximum's weight is 2^base,
+                // and times the largest scale still 2^7. An infinite scale, which only memory that was never written holds, has no part in that
                 most = most < INFINITY ? most : 0.f;
-                if (__ballot(most > 32768.f)) {
+                if (__ballot(most > 65000.f)) {
                     const float top = max_g4(most);
-                    const int   k = top > 32768.f ? (int)(__float_as_uint(top) >> 23) - 134 : 0;
+                    uint32_t u = 0;
+                    for (int b = 0; b < NB; b++) {                   // read again: the registers are the weights' by now
+                        const f16x8 at = *(const f16x8 *)(H.vs + 2 * (((size_t)tile * NB + b) * TILE + 8 * g4));
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const _Float16 d = at[i];
+                            const uint32_t x = __builtin_bit_cast(uint16_t, d) & 0x7FFFu;
+                            u = max(u, x < 0x7C00u && (!MASK || p0 + i < upto[ct]) ? x : 0u);
+                        }
+                    }
+                    const float d = max_g4((float)__builtin_bit_cast(_Float16, (uint16_t)u));
+                    const int   k = top > 65000.f ? (int)base[ct] - 134 + (int)(__float_as_uint(d) >> 23) : 0;
                     const float f = __uint_as_float((uint32_t)(127 - k) << 23);
                     scale_acc(ct, f);
                     l[ct] *= f;

@@ -1,8 +1,10 @@
-"""The attention over the 4-bit K/V cache where ranges end: scores far below zero."""
+"""The attention over the 4-bit K/V cache where ranges end: scores far below zero, values whose sizes change along
+the cache."""
 import numpy as np
 import pytest
 
 from test_gpu_kv4 import DTYPES, attended, clean, near  # noqa: F401 (clean: a fixture)
+from weights import Q4_0
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +47,39 @@ def test_attend_a_low_tile(dev, dtype, seen, n, at):
     c, k, v = cache_of(dev, dtype, k, rng.standard_normal((seen, nkv, hd)))
     q = (rng.standard_normal((n, nq, hd)) * 0.3 + side * 150 / np.sqrt(hd)).astype(np.float32)
     near(dev.kv4_attend(c, q, seen - n), *attended(dtype, q, k, v, seen - n))
+
+
+# ---------------------------------------------------------------- values' sizes
+
+def shares(q, k, v):
+    """One token's output over keys whose scores are exact (their codes have one dimension other than zero), and its error's bound: a weight is off
+    by the roundings of its own score, of the maxima it was taken against (three moves of them) and of its parts, and a share ends at 2^-32 of the largest weight
+    times the largest value."""
+    s = (q.astype(np.float64) @ k.T) / np.sqrt(len(q))
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    off = (4 * np.abs(s) + 3 * 1.45 * np.abs(s).max() + 32) * 2.0 ** -24
+    out = p @ v
+    sums = (len(k) / 32 + 64) * 2.0 ** -24 * (p @ np.abs(v))
+    return out, (p * off) @ np.abs(v) + (p @ off) * np.abs(out) + sums + (len(k) * p.max() + 1) * 2.0 ** -32 * np.abs(v).max()
+
+
+@pytest.mark.parametrize("up", [3.0, 5.4, 7.5, 7.9])
+@pytest.mark.parametrize("below", [0.3, 0.55, 0.8])
+def test_attend_range_after_lowering(dev, up, below):
+    """q4_0, three tiles of one wavefront: small values; then a weight near the end of its range on values 2^13 times larger, which lowers the row's
+    range; then the largest weights, on small values again. Those keep their 2^-32."""
+    hd, seen = 64, 384                                                # twelve tiles, three for a wavefront
+    tile = np.arange(seen) // 32
+    level = np.where(tile % 3 == 1, -40.0 + up, -40.0)                # log2 of the weights
+    level[-32:] = -below
+    level[-32] = 0
+    d = np.where(tile % 3 == 1, 2.0 ** 7, 2.0 ** -6)
+    k, v = np.zeros((seen, 1, hd)), np.full((seen, 1, hd), 7.0)
+    k[:, 0, 0] = level
+    v[:, :, ::32] = -8
+    c, k, v = cache_of(dev, Q4_0, k, v * d[:, None, None])
+    q = np.zeros((1, 1, hd), np.float32)
+    q[..., 0] = np.sqrt(hd) * np.log(2)
+    want, tol = shares(q[0, 0], k[:, 0], v[:, 0])
+    near(dev.kv4_attend(c, q, seen - 1)[0, 0], want, tol)
