@@ -740,14 +740,15 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     if constexpr (DT == L3M_Q4_0)                                    // the first tile's, of those that the row sees, of every eighth position: larger ones lower base
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            uint32_t most = 0;
+            uint32_t most = 1;                                       // 2^-24, the smallest scale there is
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const _Float16 d = vals.d[b][0];
                 const uint32_t u = __builtin_bit_cast(uint16_t, d) & 0x7FFFu;
                 most = max(most, u < 0x7C00u && t0 * TILE + 8 * g4 < seen[ct] ? u : 0u);
             }
-            base[ct] -= (float)max((int)max_g4((float)most) >> 10, 1) - 15.f;
+            const float d = max_g4((float)__builtin_bit_cast(_Float16, (uint16_t)most));
+            base[ct] -= (float)((int)(__float_as_uint(d) >> 23) - 127);
         }
     auto scale_acc = [&](int ct, float f) {
 #pragma unroll

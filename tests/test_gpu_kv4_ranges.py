@@ -83,3 +83,21 @@ def test_attend_range_after_lowering(dev, up, below):
     q[..., 0] = np.sqrt(hd) * np.log(2)
     want, tol = shares(q[0, 0], k[:, 0], v[:, 0])
     near(dev.kv4_attend(c, q, seen - 1)[0, 0], want, tol)
+
+
+@pytest.mark.parametrize("e", [-24, -23, -22, -20, -18, -14, -10, 0])
+def test_attend_small_scales_shares(dev, e):
+    """q4_0 values down to f16's subnormal scales: many small weights count beside a large one."""
+    hd, seen = 64, 1500
+    rng = np.random.default_rng(-e)
+    v = rng.integers(-7, 8, (1, hd)) * 2.0 ** e
+    v[:, ::32] = -8 * 2.0 ** e
+    v = np.tile(v, (seen, 1))
+    v[0] = 0
+    k = np.zeros((seen, 1, hd))
+    k[1:, 0, 0] = -18.45
+    c, k, v = cache_of(dev, Q4_0, k, v[:, None])
+    q = np.zeros((1, 1, hd), np.float32)
+    q[..., 0] = np.sqrt(hd) * np.log(2)
+    want, tol = shares(q[0, 0], k[:, 0], v[:, 0])
+    near(dev.kv4_attend(c, q, seen - 1)[0, 0], want, tol)
