@@ -362,8 +362,8 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions (v_mfma_f32_16x16x32_f16), P in two f16 parts: 22 bits, and 2^-32 of the largest at the
 //               least. A position's scale differs from block to block. q4_0's multiplies P, in 32 bits, before it is split (the range of
 //               the weights then goes by the scales). mxfp4's goes into the conversion of its codes (a layout of its own), exactly where
-//               it lies between 2^-23 and 2^13; for others the accumulators take another unit. A row's range, and NaN, come from
-//               positions that it sees, never from one behind it.
+//               it lies between 2^-23 and 2^13; other tiles' values and the accumulators take another unit. A row's range, and NaN, come
+//               from positions that it sees, never from one behind it.
 // All sums in 32 bits. A workgroup's four wavefronts share 16 CT rows and split the tiles; they meet in LDS, and the workgroups of a
 // long cache (splits > 1) in the workspace, added in order by k_kv4_join.
 //
@@ -385,6 +385,7 @@ typedef float f32x32 __attribute__((ext_vector_type(32)));
 
 constexpr int WAVES = 4;
 constexpr int SPLIT_WGS = 512, SPLITS = 256;                         // workgroups up to which a cache is split; most parts of it
+constexpr int NONE = -1000;
 constexpr float M0 = -3e38f;                                         // the maximum of no score: below every one
 
 // A q4_0 K word's eight codes, 0 .. 15, in f16: a nibble alone in a byte is the e4m3 number 2^-9 times it.
@@ -727,7 +728,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     float m[CT], lim[CT], l[CT];                                     // what scores are less by; the weight that moves it; sum of weights
     float base[CT];                                                  // log2 of the weight a new maximum gets; q4_0: of its product with the largest scale 7
     constexpr float RISE = DT == L3M_Q4_0 ? 7.98f : 8.f;             // how far weights pass 2^base before it moves (q4_0: 2^16 less f16's room for products)
-    int   unit = 0;                                                  // mxfp4: acc counts 2^unit
+    int   unit = 0, high = NONE;                                     // mxfp4: acc counts 2^unit; the largest unit that fit_unit chose or found
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         base[ct] = 7.f;
@@ -754,9 +755,11 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
 #pragma unroll
         for (int t = 0; t < 2 * NB; t++) acc[ct][t] *= f;
     };
-    // mxfp4, a tile whose exponents are not all f16's: another unit where its largest needs one (the first tile's own, later a larger one;
-    // values below 2^-33 of the largest are then rounded), and its exponents in that unit. What the accumulators are to be multiplied by.
-    auto fit_unit = [&](uint32_t four, bool fresh) {
+    // mxfp4, a tile whose exponents are not all f16's (or one behind it): its values in a unit of their own, the largest 2^10 to 2^13 and values of
+    // 2^-33 of it exact, and its exponents in that unit. What the accumulators are to be multiplied by, exactly: they hold less than 2^61 times
+    // the largest unit so far, and the unit never lies 60 below that (values that much smaller have no part in the sums). Tiles that were
+    // not brought here counted as unit 0; where the first has no value, the next is brought here too.
+    auto fit_unit = [&](int tile, uint32_t four) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -764,8 +767,12 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
             top = e == E8M0_NAN ? top : max(top, e);
         }
         const int most = __builtin_amdgcn_readfirstlane((int)max_wave((float)top)), was = unit;
-        if (fresh) unit = most ? most - 137 : 0;
-        else if (most - unit > 140) unit = most - 137;
+        if (tile != t0 && unit == 0 && high == NONE) high = 0;
+        const bool first = high == NONE;
+        if (most) {
+            unit = max(most - 137, high - 60);
+            high = max(high, unit);
+        } else if (first) unit = -1;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -778,7 +785,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
                 }
                 vals.e[b][j] = to;
             }
-        return fresh ? 1.f : ldexpf(1.f, was - unit);
+        return first ? 1.f : ldexpf(1.f, was - unit);
     };
 
     // mxfp4: whether a tile's exponents, those of positions before `end`, are all f16's.
@@ -832,7 +839,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
                 none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left;
             }
             if (unit || !fits) {
-                to_unit = fit_unit(four | none, tile == t0);
+                to_unit = fit_unit(tile, four | none);
                 if constexpr (MASK)                                  // NaN for the rows that see it, and for no other: 0 here, put in below
 #pragma unroll
                     for (int b = 0; b < NB; b++)
@@ -950,38 +957,43 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
     for (; tile < min(t1, (int)whole); tile++) step(tile, min(tile + 1, t1 - 1), INT_MAX, false, std::false_type{});
     // mxfp4 exponents of a masked tile that are not all f16's: a token at a time, in a unit of its own, so that no token's output hangs on
     // positions behind it
-    int units[CT];
+    int range[CT];                                                   // of a row's token: high, unit (16 bits each)
+    auto pack = [&] { return high * 65536 | (unit & 0xFFFF); };
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) units[ct] = unit;
+    for (int ct = 0; ct < CT; ct++) range[ct] = pack();
     for (; tile < t1; tile++) {
         const int end = a.pos + last + 1;
         bool each = false;
         if constexpr (DT != L3M_Q4_0) {
             each = !narrow(tile, end);
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) each = each || __ballot(units[ct] != 0);
+            for (int ct = 0; ct < CT; ct++) each = each || __ballot((range[ct] & 0xFFFF) != 0);
         }
         for (int to = each ? a.pos + first + 1 : end; to <= end; to++) {
-            if (each) {
-                float u = -1000.f;
+            if (each)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) u = seen[ct] == to ? fmaxf(u, (float)units[ct]) : u;
-                unit = __builtin_amdgcn_readfirstlane((int)max_wave(u));
-            }
+                for (int ct = 0; ct < CT; ct++)
+                    if (const uint64_t rows_of = __ballot(seen[ct] == to)) {
+                        const int r = __builtin_amdgcn_readlane(range[ct], __builtin_ctzll(rows_of));
+                        unit = (int16_t)r;
+                        high = r >> 16;
+                    }
             step(tile, to < end ? tile : min(tile + 1, t1 - 1), to, each, std::true_type{});
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) units[ct] = each && seen[ct] != to ? units[ct] : unit;
+            for (int ct = 0; ct < CT; ct++) range[ct] = each && seen[ct] == to ? pack() : range[ct];
         }
     }
     if constexpr (DT != L3M_Q4_0) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++)
-            if (__ballot(units[ct] != 0)) {
-                const bool far = units[ct] > 60;                     // sums of values near float32's end: weights 2^-48 of what they were
-                scale_acc(ct, ldexpf(1.f, far ? units[ct] - 48 : units[ct]));
+        for (int ct = 0; ct < CT; ct++) {
+            const int u = (int16_t)range[ct];
+            const bool far = range[ct] >> 16 > 60;                   // sums of values near float32's end: weights 2^-48 of what they were
+            if (__ballot(u != 0 || far)) {
+                scale_acc(ct, ldexpf(1.f, far ? u - 48 : u));
                 l[ct] *= far ? 0x1p-48f : 1.f;
                 m[ct] += far ? 48.f : 0.f;
             }
+        }
     }
 
     // the wavefronts' parts at their common maximum; where LDS has no room for all, the second half first and the first half onto them

@@ -3,8 +3,8 @@ the cache."""
 import numpy as np
 import pytest
 
-from test_gpu_kv4 import DTYPES, attended, clean, near  # noqa: F401 (clean: a fixture)
-from weights import Q4_0
+from test_gpu_kv4 import DTYPES, attended, clean, each_near, near  # noqa: F401 (clean: a fixture)
+from weights import MXFP4, Q4_0
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,21 @@ def test_attend_small_scales_shares(dev, e):
     q[..., 0] = np.sqrt(hd) * np.log(2)
     want, tol = shares(q[0, 0], k[:, 0], v[:, 0])
     near(dev.kv4_attend(c, q, seen - 1)[0, 0], want, tol)
+
+
+SIZES = [(-20, -30, -30), (-22, -40, -26), (-20, 0, -30), (-100, -40, -110), (100, 30, -100), (-22, -110, -22), (-110, 120, -20), (120, 60, 0)]
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=str)
+@pytest.mark.parametrize("hd, n, seen", [(64, 1, 900), (128, 1, 20000), (96, 70, 90), (40, 5, 200), (64, 40, 930)])
+def test_attend_value_sizes_down(dev, hd, n, seen, sizes):
+    """mxfp4 V rows of 2^sizes in the first, middle and last third, smaller ones behind larger ones: a value counts
+    down to 2^-32 of the largest that its token sees."""
+    nq, nkv = 3, 1
+    rng = np.random.default_rng(seen)
+    third = -(-seen // 3)
+    scale = np.repeat([2.0 ** s for s in sizes], third)[:seen]
+    v = np.abs(rng.standard_normal((seen, nkv, hd))) * scale[:, None, None]
+    c, k, v = cache_of(dev, MXFP4, rng.standard_normal((seen, nkv, hd)), v)
+    q = (rng.standard_normal((n, nq, hd)) * np.array([2.0 ** -12, 2.0 ** -5, 1])[:, None]).astype(np.float32)   # weights alike, and not
+    each_near(MXFP4, dev.kv4_attend(c, q, seen - n), q, k, v, seen - n)
