@@ -11,7 +11,7 @@
 //             mxfp4  the same shape                            word 2 b + u: dimensions 32 b + j (low nibbles) and 32 b + 16 + j of
 //                                                              positions 8 g + 4 u .. + 3, a position's two in a byte
 //   scales    q4_0   [nkv][tile][NB][32 positions]             f16 d, of K and of V
-//             mxfp4  [nkv][tile][NB][m 16][half 2] of K, [nkv][tile][NB][32 positions] of V: a biased exponent byte
+//             mxfp4  [nkv][tile][NB][m 16][half 2] of K, [nkv][tile][NB][32 positions] of V: a biased exponent byte, 0 of a block of zeros
 // Both codes of a tile and head take 512 NB bytes. Dimension i of a word of K is the nibble at bit nib(dt, i): q4_0's masked bytes are then
 // dimensions 0..3 and 4..7, mxfp4's come in order.
 #include <hip/hip_runtime.h>
@@ -140,8 +140,8 @@ template <int DT> __device__ __forceinline__ uint32_t quantize(const float (&x)[
             word |= (uint32_t)(int)fminf(fmaxf(v, 0.f), 15.f) << 4 * i;
         }
     } else {
-        const int   e = peak ? max((int)(peak >> 23) - 2, 1) : 127;  // a block of zeros: an ordinary scale
-        const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+        const int   e = peak ? max((int)(peak >> 23) - 2, 1) : 0;    // a block of zeros: no value's exponent, so none is measured by it
+        const float inv = __uint_as_float((uint32_t)(peak ? 254 - e : 127) << 23);
         stored = bad ? (uint32_t)E8M0_NAN : (uint32_t)e;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -788,13 +788,15 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         return first ? 1.f : ldexpf(1.f, was - unit);
     };
 
-    // mxfp4: whether a tile's exponents, those of positions before `end`, are all f16's.
+    // mxfp4: whether a tile's exponents, those of positions before `end`, are all f16's, or zeros' beside those.
     auto narrow = [&](int tile, int end) {
         if constexpr (DT == L3M_Q4_0) return true;
         else {
             const int left = end - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
-            const uint32_t none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left;
-            return !__ballot(!f16_range((keys.four & ~none) | (0x7F7F7F7Fu & none)));
+            const uint32_t none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left, w = (keys.four & ~none) | (0x7F7F7F7Fu & none);
+            if (!__ballot(!f16_range(w))) return true;
+            const uint32_t some = (((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | w) & 0x80808080u, zeros = (some ^ 0x80808080u) >> 7;   // bytes that are not 0, that are
+            return !__ballot(!f16_range(w | zeros * 0x7Fu)) && __ballot((keys.four & ~none) != 0) != 0;
         }
     };
     // A tile (masked: the positions before `end`; each: for the rows that see just those, alone). Then the words of tile `next`.

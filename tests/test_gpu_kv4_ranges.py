@@ -119,3 +119,33 @@ def test_attend_value_sizes_down(dev, hd, n, seen, sizes):
     c, k, v = cache_of(dev, MXFP4, rng.standard_normal((seen, nkv, hd)), v)
     q = (rng.standard_normal((n, nq, hd)) * np.array([2.0 ** -12, 2.0 ** -5, 1])[:, None]).astype(np.float32)   # weights alike, and not
     each_near(MXFP4, dev.kv4_attend(c, q, seen - n), q, k, v, seen - n)
+
+
+@pytest.mark.parametrize("e", [0, -20, -40, -120])
+@pytest.mark.parametrize("hd, n, seen", [(64, 1, 40), (128, 1, 3000), (128, 40, 60)])
+def test_attend_blocks_of_zeros(dev, hd, n, seen, e):
+    """mxfp4 values of 2^e among blocks and rows of zeros, in every tile: zeros have no size."""
+    nq, nkv = 2, 1
+    rng = np.random.default_rng(seen)
+    v = rng.standard_normal((seen, nkv, hd)) * 2.0 ** e
+    v[::5] = 0
+    v[::3, :, 32:] = 0
+    c, k, v = cache_of(dev, MXFP4, rng.standard_normal((seen, nkv, hd)), v)
+    assert not v[::5].any() and v[1::5].any(-1).all()
+    q = rng.standard_normal((n, nq, hd)).astype(np.float32)
+    each_near(MXFP4, dev.kv4_attend(c, q, seen - n), q, k, v, seen - n)
+
+
+@pytest.mark.parametrize("sizes", [(None, -40, -40), (None, -100, -60), (-110, None, -120), (0, None, -20), (-20, None, -30), (None, None, -120), (None, 20, -30), (None, None, None)],
+                         ids=str)
+@pytest.mark.parametrize("hd, n, seen", [(64, 1, 900), (128, 1, 20000), (96, 70, 90), (40, 5, 200), (64, 40, 930), (32, 64, 64)])
+def test_attend_value_sizes_and_zeros(dev, hd, n, seen, sizes):
+    """As above, None for rows of zeros: what lies beside or behind them counts as if they were not there."""
+    nq, nkv = 3, 1
+    rng = np.random.default_rng(seen)
+    third = -(-seen // 3)
+    scale = np.repeat([0.0 if s is None else 2.0 ** s for s in sizes], third)[:seen]
+    v = np.abs(rng.standard_normal((seen, nkv, hd))) * scale[:, None, None]
+    c, k, v = cache_of(dev, MXFP4, rng.standard_normal((seen, nkv, hd)), v)
+    q = (rng.standard_normal((n, nq, hd)) * np.array([2.0 ** -12, 2.0 ** -5, 1])[:, None]).astype(np.float32)
+    each_near(MXFP4, dev.kv4_attend(c, q, seen - n), q, k, v, seen - n)
