@@ -49,6 +49,23 @@ def test_attend_a_low_tile(dev, dtype, seen, n, at):
     near(dev.kv4_attend(c, q, seen - n), *attended(dtype, q, k, v, seen - n))
 
 
+@DTYPES
+def test_attend_lowest_scores(dev, dtype):
+    """A score at the end of what float32 holds, in base 2, alone: the answer is the position's value. The other wavefronts have seen nothing, which is
+    less. mxfp4's stops at 3.1e38: a partial sum leaves float32 above 3.2e38, since the first part of q is q rounded to 1/4 of [2, 4), up to
+    1/16 more, and 17/16 of 3.2e38 is 3.4e38."""
+    hd = 8
+    k = -8 * 65504.0 if dtype == Q4_0 else -6 * 2.0 ** 60
+    for score in (3.2e38, 3.39e38) if dtype == Q4_0 else (3.05e38, 3.1e38):
+        x, y = np.zeros((1, 1, hd)), np.arange(1.0, hd + 1)[None, None]
+        x[..., 0] = k
+        c, kk, v = cache_of(dev, dtype, x, y)
+        q = np.zeros((1, 1, hd), np.float32)
+        q[..., 0] = score / -kk[0, 0, 0] * np.sqrt(hd) / 1.44269504
+        got = dev.kv4_attend(c, q, 0)
+        assert np.all(np.abs(got - v) <= np.abs(v) * 2.0 ** -21), got
+
+
 # ---------------------------------------------------------------- values' sizes
 
 def shares(q, k, v):
