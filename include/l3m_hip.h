@@ -137,7 +137,8 @@ int    l3m_k_argmax(const float *x, int n, int32_t *out, void *stream);         
 // allocation of l3m_kv4_bytes (0 for a shape that is refused: dtype L3M_HIP_Q4_0 or L3M_HIP_MXFP4, hd a multiple of 8 up to 256,
 // cap up to 2^30 positions), 16-byte aligned, which need not be cleared. Codes are stored in the order the attention reads
 // them: rows go in and out through these calls.
-// Every call refuses (-1, l3m_dev_error) what its arguments cannot mean, before it launches anything. Calls are
+// Every call refuses (-1, l3m_dev_error) what its arguments cannot mean, before it launches anything: outputs and
+// workspaces that lie on what it reads (but where it says so) or on the cache among it. Calls are
 // asynchronous on `stream` (NULL: the library's) of device 0, allocate nothing, and may be captured into a graph.
 typedef struct {
     uint8_t *kq, *ks, *vq, *vs;  // K codes and scales, V codes and scales

@@ -1119,18 +1119,29 @@ bool kv4_shape(int dt, int nkv, int hd, int cap) {
 }
 size_t codes_bytes(int nkv, int hd, int cap) { return (size_t)nkv * ((cap + TILE - 1) / TILE) * 512 * ((hd + 31) / 32); }
 size_t scales_bytes(int dt, int nkv, int hd, int cap) { return (size_t)nkv * ((cap + TILE - 1) / TILE) * TILE * ((hd + 31) / 32) * sbytes(dt); }
+bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+    return na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+// Whether n bytes at p (NULL: none) lie on the cache's memory.
+bool on_cache(const l3m_kv4 *c, const void *p, size_t n) {
+    const size_t q = codes_bytes(c->nkv, c->hd, c->cap), s = scales_bytes(c->dtype, c->nkv, c->hd, c->cap);
+    return p && (overlap(p, n, c->kq, q) || overlap(p, n, c->ks, s) || overlap(p, n, c->vq, q) || overlap(p, n, c->vs, s));
+}
 const char *kv4_bad(const l3m_kv4 *c) {
     if (!c || !kv4_shape(c->dtype, c->nkv, c->hd, c->cap)) return "kv4: not a cache of q4_0 or mxfp4 blocks, hd a multiple of 8 up to 256";
     if (!c->kq || !c->ks || !c->vq || !c->vs) return "kv4: a cache without memory";
     if (((uintptr_t)c->kq | (uintptr_t)c->vq | (uintptr_t)c->ks | (uintptr_t)c->vs) % 16) return "kv4: planes must be 16-byte aligned";
+    const size_t q = codes_bytes(c->nkv, c->hd, c->cap), s = scales_bytes(c->dtype, c->nkv, c->hd, c->cap);
+    if (overlap(c->kq, q, c->vq, q) || overlap(c->ks, s, c->vs, s) || overlap(c->kq, q, c->ks, s) || overlap(c->kq, q, c->vs, s) ||
+        overlap(c->vq, q, c->ks, s) || overlap(c->vq, q, c->vs, s))
+        return "kv4: planes overlap";
     return nullptr;
 }
 bool span_ok(const l3m_kv4 *c, int pos, int n) { return pos >= 0 && n >= 1 && pos <= c->cap && n <= c->cap - pos; }
-bool overlap(const void *a, size_t na, const void *b, size_t nb) {
-    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
-}
 hipStream_t as_stream(void *s) { return (hipStream_t)(s ? s : l3m_dev_stream()); }
 
+// The rows of the table that a call reads, n of hd floats.
+const float *table_rows(const RowsIn &a) { return a.table ? a.table + (size_t)a.pos * a.hd : nullptr; }
 // What is wrong with a call's rows and outputs, or NULL. An output may be the rows' own heads only where a token's are dense: one token.
 const char *rows_bad(const RowsIn &a, bool floats) {
     const long long width = (long long)(a.nq + (floats ? 1 : 2) * (long long)a.nkv) * a.hd;
@@ -1141,9 +1152,15 @@ const char *rows_bad(const RowsIn &a, bool floats) {
     if (((uintptr_t)a.x | (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.wq | (uintptr_t)a.wk | (uintptr_t)a.table) % 4) return "rows: floats must be 4-byte aligned";
     const size_t in = 4 * ((size_t)(a.n - 1) * a.stride + width), nqb = 4 * (size_t)a.n * a.nq * a.hd, nkb = floats ? 4 * (size_t)a.n * a.nkv * a.hd : 0;
     const bool one = a.n == 1;
-    if (nqb && overlap(a.q, nqb, a.x, in) && !(one && a.q == a.x)) return "rows: q overlaps the rows";
-    if (nkb && overlap(a.k, nkb, a.x, in) && !(one && a.k == a.x + (size_t)a.nq * a.hd)) return "rows: k overlaps the rows";
-    if (nqb && nkb && overlap(a.q, nqb, a.k, nkb)) return "rows: q overlaps k";
+    if (overlap(a.q, nqb, a.x, in) && !(one && a.q == a.x)) return "rows: q overlaps the rows";
+    if (overlap(a.k, nkb, a.x, in) && !(one && a.k == a.x + (size_t)a.nq * a.hd)) return "rows: k overlaps the rows";
+    if (overlap(a.q, nqb, a.k, nkb)) return "rows: q overlaps k";
+    const size_t w = 4 * (size_t)a.hd;
+    const float *turn = table_rows(a);
+    auto read = [&](const float *to, size_t n) {
+        return (a.wq && overlap(to, n, a.wq, w)) || (a.wk && overlap(to, n, a.wk, w)) || (turn && overlap(to, n, turn, w * a.n));
+    };
+    if (read(a.q, nqb) || read(a.k, nkb)) return "rows: q or k overlaps the weights or the table";
     return nullptr;
 }
 template <int DT> void launch_rows_in(RowsIn a, const l3m_kv4 &c, hipStream_t st) {
@@ -1240,6 +1257,10 @@ int l3m_k_kv4_append(const l3m_kv4 *c, float *q, const float *rows, int stride, 
     if (!span_ok(c, pos, n)) return l3m_dev_fail("kv4_append: positions past the cache's end");
     const RowsIn a = {rows, wq, wk, table, q, nullptr, stride, n, nq, c->nkv, c->hd, halves != 0, pos, 0, 0, eps};
     if (const char *why = rows_bad(a, false)) return l3m_dev_fail(why);
+    const size_t w = 4 * (size_t)c->hd;
+    if (on_cache(c, q, w * n * nq) || on_cache(c, rows, 4 * ((size_t)(n - 1) * stride + (size_t)(nq + 2 * c->nkv) * c->hd)) || on_cache(c, wq, w) ||
+        on_cache(c, wk, w) || on_cache(c, table_rows(a), w * n))
+        return l3m_dev_fail("kv4_append: rows, queries, weights or table overlap the cache");
     if ((long long)n * (nq + 2 * c->nkv) > MAX_ITEMS) return l3m_dev_fail("kv4_append: too many rows for one call");
     if (c->dtype == L3M_Q4_0) launch_rows_in<L3M_Q4_0>(a, *c, as_stream(stream));
     else launch_rows_in<L3M_MXFP4>(a, *c, as_stream(stream));
@@ -1253,6 +1274,7 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
     const size_t vals = (size_t)n * c->nkv * c->hd;
     if (vals > (size_t)MAX_ITEMS * 64) return l3m_dev_fail("kv4_rows: too many rows for one call");
     if (k && v && overlap(k, 4 * vals, v, 4 * vals)) return l3m_dev_fail("kv4_rows: k overlaps v");
+    if (on_cache(c, k, 4 * vals) || on_cache(c, v, 4 * vals)) return l3m_dev_fail("kv4_rows: k or v overlaps the cache");
     const unsigned k_threads = k ? (unsigned)((vals / 8 + 255) / 256 * 256) : 0;
     const size_t v_threads = v ? (size_t)(((pos + n - 1) >> 3) - (pos >> 3) + 1) * c->nkv * c->hd : 0;
     const dim3 grid((unsigned)((k_threads + v_threads + 255) / 256));
@@ -1277,6 +1299,7 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     const size_t need = l3m_kv4_work_bytes(c, n, nq);
     if (!work || (uintptr_t)work % 16 || work_bytes < need) return l3m_dev_fail("kv4_attend: the workspace is too small (l3m_kv4_work_bytes) or not 16-byte aligned");
     if (overlap(work, need, q, bytes) || overlap(work, need, out, bytes)) return l3m_dev_fail("kv4_attend: the workspace overlaps q or out");
+    if (on_cache(c, out, bytes) || on_cache(c, work, need)) return l3m_dev_fail("kv4_attend: out or the workspace overlaps the cache");
     if (rows > (size_t)MAX_ITEMS) return l3m_dev_fail("kv4_attend: too many rows for one call");
     const long long R = (long long)n * (nq / c->nkv);
     const int ct = tile_columns(c->dtype, (c->hd + 31) / 32, c->nkv, R), per = 16 * ct, groups = (int)((R + per - 1) / per), tiles = (pos + n + TILE - 1) / TILE;
