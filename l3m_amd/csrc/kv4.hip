@@ -1138,7 +1138,15 @@ const char *kv4_bad(const l3m_kv4 *c) {
     return nullptr;
 }
 bool span_ok(const l3m_kv4 *c, int pos, int n) { return pos >= 0 && n >= 1 && pos <= c->cap && n <= c->cap - pos; }
-hipStream_t as_stream(void *s) { return (hipStream_t)(s ? s : l3m_dev_stream()); }
+// The stream of a call that names none: the library's, made now if this is its first call. False: there is no device, or it was shut down.
+bool stream_of(void *s, hipStream_t &st) {
+    if (!s && l3m_dev_init()) {
+        l3m_dev_fail("no usable device, or the library was shut down");
+        return false;
+    }
+    st = (hipStream_t)(s ? s : l3m_dev_stream());
+    return true;
+}
 
 // The rows of the table that a call reads, n of hd floats.
 const float *table_rows(const RowsIn &a) { return a.table ? a.table + (size_t)a.pos * a.hd : nullptr; }
@@ -1247,7 +1255,9 @@ int l3m_k_qk_norm_rope(float *q, float *k, const float *rows, int stride, int n,
     const RowsIn a = {rows, wq, wk, table, q, k, stride, n, nq, nkv, hd, halves != 0, pos, 0, 0, eps};
     if (const char *why = rows_bad(a, true)) return l3m_dev_fail(why);
     if ((long long)n * (nq + nkv) > MAX_ITEMS) return l3m_dev_fail("qk_norm_rope: too many rows for one call");
-    launch_rows_in<-1>(a, l3m_kv4{}, as_stream(stream));
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
+    launch_rows_in<-1>(a, l3m_kv4{}, st);
     return l3m_dev_launched("k_qk_norm_rope");
 }
 
@@ -1262,8 +1272,10 @@ int l3m_k_kv4_append(const l3m_kv4 *c, float *q, const float *rows, int stride, 
         on_cache(c, wk, w) || on_cache(c, table_rows(a), w * n))
         return l3m_dev_fail("kv4_append: rows, queries, weights or table overlap the cache");
     if ((long long)n * (nq + 2 * c->nkv) > MAX_ITEMS) return l3m_dev_fail("kv4_append: too many rows for one call");
-    if (c->dtype == L3M_Q4_0) launch_rows_in<L3M_Q4_0>(a, *c, as_stream(stream));
-    else launch_rows_in<L3M_MXFP4>(a, *c, as_stream(stream));
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
+    if (c->dtype == L3M_Q4_0) launch_rows_in<L3M_Q4_0>(a, *c, st);
+    else launch_rows_in<L3M_MXFP4>(a, *c, st);
     return l3m_dev_launched("k_kv4_append");
 }
 
@@ -1278,8 +1290,10 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
     const unsigned k_threads = k ? (unsigned)((vals / 8 + 255) / 256 * 256) : 0;
     const size_t v_threads = v ? (size_t)(((pos + n - 1) >> 3) - (pos >> 3) + 1) * c->nkv * c->hd : 0;
     const dim3 grid((unsigned)((k_threads + v_threads + 255) / 256));
-    if (c->dtype == L3M_Q4_0) hipLaunchKernelGGL(k_kv4_rows<L3M_Q4_0>, grid, dim3(256), 0, as_stream(stream), *c, k, v, pos, n, k_threads);
-    else hipLaunchKernelGGL(k_kv4_rows<L3M_MXFP4>, grid, dim3(256), 0, as_stream(stream), *c, k, v, pos, n, k_threads);
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
+    if (c->dtype == L3M_Q4_0) hipLaunchKernelGGL(k_kv4_rows<L3M_Q4_0>, grid, dim3(256), 0, st, *c, k, v, pos, n, k_threads);
+    else hipLaunchKernelGGL(k_kv4_rows<L3M_MXFP4>, grid, dim3(256), 0, st, *c, k, v, pos, n, k_threads);
     return l3m_dev_launched("k_kv4_rows");
 }
 
@@ -1309,7 +1323,8 @@ int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq
     float *ml = (float *)work;
     const AttendIn a = {out, ml, ml + (2 * rows * splits + 3) / 4 * 4, q, *c, n, nq, g, pos, groups, 0, splits, multiplier(g, (uint32_t)R), multiplier(c->hd / 4, 4096),
                         multiplier(splits * WAVES, (uint32_t)tiles)};
-    hipStream_t st = as_stream(stream);
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
     if (c->dtype == L3M_Q4_0) launch_attend<L3M_Q4_0>(a, ct, st);
     else launch_attend<L3M_MXFP4>(a, ct, st);
     if (splits > 1) hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)rows), dim3(256), 0, st, a);
