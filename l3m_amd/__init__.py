@@ -345,7 +345,7 @@ class Device:
         if self.lib.l3m_dev_init():
             err = self.lib.l3m_dev_error()
             raise RuntimeError(f"no usable HIP device: {err.decode() if err else '?'}")
-        self._live = []
+        self._live = {}                       # pointer: bytes
 
     def _check(self, rc, what):
         if rc:
@@ -356,7 +356,7 @@ class Device:
         p = self.lib.l3m_dev_alloc(nbytes)
         if not p:
             raise MemoryError(f"device alloc of {nbytes} bytes")
-        self._live.append(p)
+        self._live[p] = nbytes
         return p
 
     def put(self, a):
@@ -374,7 +374,7 @@ class Device:
         self.lib.l3m_dev_sync()
         for p in self._live:
             self.lib.l3m_dev_free(p)
-        self._live = []
+        self._live = {}
 
     def pack_rows(self, dtype, rows, k):
         """File rows (uint8 [n, row_bytes] or a list with None for zero rows) -> host lane-tile planes."""
@@ -457,16 +457,24 @@ class Device:
         self.lib.l3m_rope_table(_p(table, _f), ctx, hd, theta)
         return self.put(table)
 
-    def _opt(self, w):
-        return None if w is None else self.put(np.float32(w))
+    def _norm_rope_args(self, hd, end, wq, wk, table):
+        """The norms' weights, refused unless they hold hd values, and nothing for None; a table of this Device's is refused if it ends before row `end`."""
+        wq, wk = (None if w is None else np.ascontiguousarray(w, np.float32) for w in (wq, wk))
+        if any(w is not None and w.shape != (hd,) for w in (wq, wk)):
+            raise ValueError(f"weights of the norms must hold {hd} values")
+        if table is not None and self._live.get(table, 4 * end * hd) < 4 * end * hd:
+            raise ValueError(f"the table ends before position {end - 1}")
+        return (None if w is None else self.put(w) for w in (wq, wk))
 
     def qk_norm_rope(self, rows, nq, nkv, hd, wq=None, wk=None, eps=1e-5, halves=False, pos=0, table=None):
-        """Norm and rotation of the query and key heads of rows [n, width]: q [n, nq, hd], k [n, nkv, hd] (l3m_k_qk_norm_rope)."""
+        """Norm and rotation of the query and key heads of rows [n, width]: q [n, nq, hd], k [n, nkv, hd] (l3m_k_qk_norm_rope). table:
+        rope_table's, or a device pointer to as many rows as pos + n."""
         rows = np.ascontiguousarray(rows, np.float32)
         n, width = rows.shape
+        dwq, dwk = self._norm_rope_args(hd, pos + n, wq, wk, table)
         dq, dk = self.alloc(max(4 * n * nq * hd, 4)), self.alloc(max(4 * n * nkv * hd, 4))
-        self._check(self.lib.l3m_k_qk_norm_rope(dq, dk, self.put(rows), width, n, nq, nkv, hd, self._opt(wq), self._opt(wk), eps, int(halves), pos,
-                                                table, None), "qk_norm_rope")
+        self._check(self.lib.l3m_k_qk_norm_rope(dq, dk, self.put(rows), width, n, nq, nkv, hd, dwq, dwk, eps, int(halves), pos, table, None),
+                    "qk_norm_rope")
         return self.get(dq, (n, nq, hd), np.float32), self.get(dk, (n, nkv, hd), np.float32)
 
     def kv4(self, dtype, nkv, hd, cap):
@@ -482,9 +490,9 @@ class Device:
         """rows [n, width] of [q | k | v] heads: K and V into the cache at pos.., the queries returned [n, nq, hd] (l3m_k_kv4_append)."""
         rows = np.ascontiguousarray(rows, np.float32)
         n, width = rows.shape
+        dwq, dwk = self._norm_rope_args(c.hd, pos + n, wq, wk, table)
         dq = self.alloc(4 * n * nq * c.hd) if nq else None
-        self._check(self.lib.l3m_k_kv4_append(C.byref(c), dq, self.put(rows), width, n, nq, self._opt(wq), self._opt(wk), eps, int(halves), pos,
-                                              table, None), "kv4_append")
+        self._check(self.lib.l3m_k_kv4_append(C.byref(c), dq, self.put(rows), width, n, nq, dwq, dwk, eps, int(halves), pos, table, None), "kv4_append")
         return self.get(dq, (n, nq, c.hd), np.float32) if nq else None
 
     def kv4_rows(self, c, pos, n):

@@ -1,6 +1,8 @@
-"""Calls around the 4-bit K/V cache whose outputs lie on what the call reads or on the cache: refused on the host, before a launch, with the reason."""
+"""Calls around the 4-bit K/V cache whose outputs lie on what the call reads or on the cache: refused on the host, before a launch, with the reason. And
+the Python calls' weights and tables, which have to be as long as the call reads them."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 import l3m_amd as A
@@ -102,3 +104,15 @@ def test_neighbours_are_not_overlaps():
                  lambda: append(c, q=WK, wk=None, wq=None), lambda: attend(c, q=PLANES["kq"])):
         assert call() == -1 and b"overlap" not in lib.l3m_dev_error()
         lib.l3m_dev_clear_error()
+
+
+@pytest.mark.parametrize("wq, wk, rows", [(HD - 1, None, 14), (None, HD // 2, 14), (HD + 1, HD, 14), (HD, HD, 13), (None, None, 0), ((1, HD), None, 14)], ids=str)
+def test_python_lengths(dev_free, wq, wk, rows):
+    """Weights of another length than a head's, a table that ends before the last token's row: refused before anything is uploaded."""
+    dev_free._live = {TABLE: 4 * HD * rows}
+    x = np.zeros((4, 8 * HD), np.float32)
+    wq, wk = (None if n is None else np.ones(n, np.float32) for n in (wq, wk))
+    with pytest.raises(ValueError):
+        dev_free.qk_norm_rope(x, 4, 2, HD, wq, wk, pos=10, table=TABLE)
+    with pytest.raises(ValueError):
+        dev_free.kv4_append(A.KV4(**PLANES, nkv=NKV, hd=HD, cap=CAP, dtype=Q4_0), x, 4, 10, wq, wk, table=TABLE)
