@@ -602,8 +602,9 @@ template <int NB> struct Queries<L3M_MXFP4, NB> {
                 }
             }
             const bool bad = peak >= 0x7F800000u;                    // a scale of NaN for a row that is not finite
-            // The conversions of 32 values take several cycles and may not write over what they read, which the compiler does not see to:
-            // the empty asm statements keep their operands in registers of their own (without them, now and then wrong last parts).
+            // The conversions of 32 values take several cycles and may not write over what they read (with results on their sources, now and then
+            // wrong last parts). The compiler does not know it of its builtins, so they are written out with results that it keeps apart (=&);
+            // the wait behind each is for a product that reads its result next. No product is under way here that they could meet.
 #pragma unroll
             for (int t = 0; t < Mx<NB>::times; t++) {
                 part[i][t] = u32x6{0, 0, 0, 0, 0, 0};
@@ -619,10 +620,10 @@ template <int NB> struct Queries<L3M_MXFP4, NB> {
                     even[j] = x[2 * j];
                     odd[j] = x[2 * j + 1];
                 }
-                u32x6 w = __builtin_bit_cast(u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, unit));
-                asm volatile("" : "+v"(w) : "v"(even), "v"(odd), "v"(unit));
-                f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, unit);
-                asm volatile("" : "+v"(back) : "v"(w), "v"(unit));
+                u32x6 w;
+                f32x32 back;
+                asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 1" : "=&v"(w) : "v"(even), "v"(odd), "v"(unit));
+                asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2\n\ts_nop 1" : "=&v"(back) : "v"(w), "v"(unit));
 #pragma unroll
                 for (int j = 0; j < 32; j++) x[j] -= back[j];
                 const int t = p / Mx<NB>::at_once, at = p - t * Mx<NB>::at_once;
