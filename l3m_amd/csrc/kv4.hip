@@ -395,30 +395,26 @@ __device__ __forceinline__ f16x8 widen(uint32_t w) {
     const f16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, true);
     return f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
 }
-// Byte i of w as the power of two that it is the exponent of.
-__device__ __forceinline__ float pow2_byte(uint32_t w, int i) {     // one instruction, where the compiler takes a shift and a mask
-    float r;
-#define BYTE_OF(N) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_" #N : "=v"(r) : "v"(23), "v"(w))
-    if (i == 0) BYTE_OF(0);
-    else if (i == 1) BYTE_OF(1);
-    else if (i == 2) BYTE_OF(2);
-    else BYTE_OF(3);
-#undef BYTE_OF
-    return r;
+// Byte i of w as the power of two that it is the exponent of: one instruction, a product with 2^23 that takes the byte where it lies; as a shift,
+// or a product that the compiler sees to be one, it is a shift and a mask.
+__device__ __forceinline__ float pow2_byte(uint32_t w, int i) {
+    uint32_t unit = 1u << 23;
+    asm("" : "+s"(unit));
+    return __uint_as_float(__umul24(w >> 8 * i & 255u, unit));
 }
 __device__ __forceinline__ float max8(const float (&s)[8]) {
     return fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(s[0], s[1]), s[2]), s[3]), s[4]), s[5]), s[6]), s[7]);
 }
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // Eight float32 values as the sum of two f16 ones each: 22 bits, 2^-25 at the least; below 65520. The rests by the instruction that takes a
-// half as it lies in its pair (the compiler converts it first).
+// half as it lies in its pair (v_fma_mix_f32; a difference is a conversion first, so the compiler does not see the factor).
 __device__ __forceinline__ void two_parts(const float (&w)[8], f16x8 &hi, f16x8 &lo) {
+    float minus1 = -1.f;
+    asm("" : "+s"(minus1));
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const f16x2 h = __builtin_convertvector((f32x2{w[i], w[i + 1]}), f16x2);
-        float r0, r1;
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(w[i]));
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(w[i + 1]));
+        const float r0 = fmaf((float)h.x, minus1, w[i]), r1 = fmaf((float)h.y, minus1, w[i + 1]);
         const f16x2 l = __builtin_convertvector((f32x2{r0, r1}), f16x2);
         hi[i] = h.x; hi[i + 1] = h.y;
         lo[i] = l.x; lo[i + 1] = l.y;
