@@ -1,8 +1,9 @@
 """The attention over the 4-bit K/V cache where ranges end: scores far below zero, values whose sizes change along
-the cache."""
+the cache; and its precision at ordinary sizes."""
 import numpy as np
 import pytest
 
+from test_cpu_kv4_precision import LIMIT, apart, ordinary
 from test_gpu_kv4 import DTYPES, attended, clean, each_near, near  # noqa: F401 (clean: a fixture)
 from weights import MXFP4, Q4_0
 
@@ -166,3 +167,21 @@ def test_attend_value_sizes_and_zeros(dev, hd, n, seen, sizes):
     c, k, v = cache_of(dev, MXFP4, rng.standard_normal((seen, nkv, hd)), v)
     q = (rng.standard_normal((n, nq, hd)) * np.array([2.0 ** -12, 2.0 ** -5, 1])[:, None]).astype(np.float32)
     each_near(MXFP4, dev.kv4_attend(c, q, seen - n), q, k, v, seen - n)
+
+
+# ---------------------------------------------------------------- precision
+
+@DTYPES
+@pytest.mark.parametrize("hd", [8, 32, 48, 64, 80, 96, 128, 160, 200, 224, 256])
+@pytest.mark.parametrize("pos, n, nq, nkv", [(39, 1, 8, 2), (999, 1, 8, 2), (20000, 1, 8, 2), (0, 150, 4, 2), (600, 40, 6, 3), (0, 300, 64, 64)])
+def test_attend_precision(dev, dtype, hd, pos, n, nq, nkv):
+    """Inputs of ordinary size: as near the formula as float32 sums are (LIMIT), which a lost part of the weights or the queries is not."""
+    q, k, v = ordinary(hd, pos, n, nq, nkv)
+    c, k, v = cache_of(dev, dtype, k, v)
+    got = dev.kv4_attend(c, q, pos)
+    heads = sorted({0, nkv // 2, nkv - 1})
+    g = nq // nkv
+    for h in heads:
+        part = slice(h * g, (h + 1) * g)
+        want = attended(dtype, q[:, part], k[:, h:h + 1], v[:, h:h + 1], pos)[0]
+        assert apart(got[:, part], want) <= LIMIT, (h, apart(got[:, part], want))
