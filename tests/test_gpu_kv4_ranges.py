@@ -1,10 +1,10 @@
 """The attention over the 4-bit K/V cache where ranges end: scores far below zero, values whose sizes change along
-the cache; and its precision at ordinary sizes."""
+the cache; its precision at ordinary sizes; and heads beside one that is not finite."""
 import numpy as np
 import pytest
 
 from test_cpu_kv4_precision import LIMIT, apart, ordinary
-from test_gpu_kv4 import DTYPES, attended, clean, each_near, near  # noqa: F401 (clean: a fixture)
+from test_gpu_kv4 import DTYPES, attended, clean, each_near, filled, near  # noqa: F401 (clean: a fixture)
 from weights import MXFP4, Q4_0
 
 pytestmark = pytest.mark.gpu
@@ -185,3 +185,25 @@ def test_attend_precision(dev, dtype, hd, pos, n, nq, nkv):
         part = slice(h * g, (h + 1) * g)
         want = attended(dtype, q[:, part], k[:, h:h + 1], v[:, h:h + 1], pos)[0]
         assert apart(got[:, part], want) <= LIMIT, (h, apart(got[:, part], want))
+
+
+@DTYPES
+@pytest.mark.parametrize("pos, n", [(0, 1), (37, 1), (20, 40), (0, 70), (3000, 2)])
+def test_attend_head_beside_nan(dev, dtype, pos, n):
+    """A key or value row of NaN in kv head 1, head 0's row there as it was: head 0's outputs stay bit for bit."""
+    nq, nkv, hd = 6, 2, 128
+    c, k, v, rng = filled(dev, dtype, nkv, hd, pos + n, 5)
+    q = rng.standard_normal((n, nq, hd)).astype(np.float32)
+    want = dev.kv4_attend(c, q, pos)
+    at = pos + n // 2
+    for plane in (0, 1):
+        rows = np.stack([k[at], v[at]]).astype(np.float32)
+        rows[plane, 1, 7] = np.nan
+        dev.kv4_append(c, rows.reshape(1, -1), 0, at)
+        back = dev.kv4_rows(c, at, 1)
+        assert np.array_equal(back[0][0, 0], k[at, 0].astype(np.float32)) and np.array_equal(back[1][0, 0], v[at, 0].astype(np.float32))
+        got = dev.kv4_attend(c, q, pos)
+        assert np.array_equal(got[:, :nq // 2], want[:, :nq // 2])
+        assert np.array_equal(got[:at - pos], want[:at - pos])
+        bad = got[at - pos:, nq // 2:] if plane == 0 else got[at - pos:, nq // 2:, :32]
+        assert np.isnan(bad).all()
