@@ -785,16 +785,16 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         return first ? 1.f : ldexpf(1.f, was - unit);
     };
 
-    // mxfp4: whether a tile's exponents, those of positions before `end`, are all f16's, or zeros' beside those.
-    auto narrow = [&](int tile, int end) {
-        if constexpr (DT == L3M_Q4_0) return true;
-        else {
-            const int left = end - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
-            const uint32_t none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left, w = (keys.four & ~none) | (0x7F7F7F7Fu & none);
-            if (!__ballot(!f16_range(w))) return true;
-            const uint32_t some = (((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | w) & 0x80808080u, zeros = (some ^ 0x80808080u) >> 7;   // bytes that are not 0, that are
-            return !__ballot(!f16_range(w | zeros * 0x7Fu)) && __ballot((keys.four & ~none) != 0) != 0;
-        }
+    // mxfp4: the bytes of a lane's four exponents whose positions lie at `end` or behind; whether all others of the tile are f16's; whether they are f16's
+    // or zeros', and not zeros' alone.
+    auto behind = [&](int tile, int end) {
+        const int left = end - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
+        return left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left;
+    };
+    auto narrow = [&](uint32_t four, uint32_t none) { return !__ballot(!f16_range((four & ~none) | (0x7F7F7F7Fu & none))); };
+    auto narrow_or_zero = [&](uint32_t four, uint32_t none) {
+        const uint32_t w = four & ~none, some = (((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | w) & 0x80808080u;   // bytes that are not 0
+        return narrow(w | ((some ^ 0x80808080u) >> 7) * 0x7Fu, none) && __ballot(w != 0) != 0;
     };
     // A tile (masked: the positions before `end`; each: for the rows that see just those, alone). Then the words of tile `next`.
     auto step = [&](const int tile, const int next, const int end, const bool each, auto masked) {
@@ -825,19 +825,16 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         }
         uint32_t four = 0;
         if constexpr (DT != L3M_Q4_0) four = keys.four;
-        const bool fits = narrow(tile, MASK ? end : INT_MAX);
+        uint32_t none = 0;                                           // exponents of positions that no row sees do not count
+        if constexpr (DT != L3M_Q4_0 && MASK) none = behind(tile, end);
+        const bool fits = DT == L3M_Q4_0 || narrow(four, none);
         keys.load(H, next, lane);
         float to_unit = 1.f;
         uint32_t nan[CT];                                            // blocks whose value is NaN at a position the row sees
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) nan[ct] = 0;
         if constexpr (DT != L3M_Q4_0) {
-            uint32_t none = 0;                                       // exponents of positions that no row sees do not count
-            if constexpr (MASK) {
-                const int left = end - (tile * TILE + 4 * (min(lane, 8 * NB - 1) & 7));
-                none = left >= 4 ? 0u : left <= 0 ? ~0u : ~0u << 8 * left;
-            }
-            if (unit || !fits) {
+            if ((unit || !fits) && (unit || !narrow_or_zero(four, none))) {
                 to_unit = fit_unit(tile, four | none);
                 if constexpr (MASK)                                  // NaN for the rows that see it, and for no other: 0 here, put in below
 #pragma unroll
@@ -964,7 +961,7 @@ template <int DT, int NB, int CT> __global__ void __launch_bounds__(64 * WAVES) 
         const int end = a.pos + last + 1;
         bool each = false;
         if constexpr (DT != L3M_Q4_0) {
-            each = !narrow(tile, end);
+            each = !narrow_or_zero(keys.four, behind(tile, end));
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) each = each || __ballot((range[ct] & 0xFFFF) != 0);
         }
