@@ -163,8 +163,9 @@ int l3m_k_kv4_append(const l3m_kv4 *c, float *q, const float *rows, int stride, 
 int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *stream);
 // Attention of n tokens at positions pos .. pos + n - 1, token t over positions 0 .. pos + t (whose rows, its own among them, are in
 // the cache), scores q.k / sqrt(hd): q and out [n][nq][hd] float32, out may be q; query head h reads kv head h / (nq / nkv). What the
-// cache holds past a token's position does not reach it. Sums are float32's; a weight's share of the output ends at 2^-32 of the token's
-// largest weight times the largest value it sees. work: l3m_kv4_work_bytes(c, n, nq) bytes, 16-byte aligned, of any
+// cache holds past a token's position does not reach it. Sums are float32's. A query's value counts to 2^-24 of the largest of its 32
+// (q4_0: to 2^-22 of itself and 2^-38 of the largest of its head); a weight in 22 bits, and its share of the output ends at 2^-32 of the token's
+// largest weight times the largest value it sees. Scores, times log2(e), up to 3e38 in size. work: l3m_kv4_work_bytes(c, n, nq) bytes, 16-byte aligned, of any
 // contents, used by one call at a time (a captured call uses it at every replay); a larger n's serves a smaller one.
 size_t l3m_kv4_work_bytes(const l3m_kv4 *c, int n, int nq);
 int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq, int pos, void *work, size_t work_bytes, void *stream);

@@ -321,7 +321,7 @@ template <int DT, bool VEC> __global__ void __launch_bounds__(256) k_rows_in(Row
 
 // ---------------------------------------------------------------- read-back
 // A thread a word of K (eight dimensions of a position), then one a dimension of V (its eight positions): stores are contiguous either way.
-// Bound by the bytes it writes: 1000 positions of 8 heads of 128 5.2 us (8.2 MB), one 2.0 us.
+// Bound by the bytes it writes: 1000 positions of 8 heads of 128 (8.2 MB) q4_0 5.0 us, mxfp4 5.7, one 2.0.
 template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, float *k, float *v, int pos, int n, unsigned k_threads) {
     const int nb = (c.hd + 31) >> 5;
     const unsigned id = blockIdx.x * 256 + threadIdx.x, nkv = c.nkv, hd = c.hd;
@@ -367,11 +367,12 @@ template <int DT> __global__ void __launch_bounds__(256) k_kv4_rows(l3m_kv4 c, f
 // All sums in 32 bits. A workgroup's four wavefronts share 16 CT rows and split the tiles; they meet in LDS, and the workgroups of a
 // long cache (splits > 1) in the workspace, added in order by k_kv4_join.
 //
-// A few tokens are bound by latency (one token over 40 positions 3.7 us, 256: 4.3, 480 tokens of 9 heads over 3 of 64 6.2 us: one
+// A few tokens are bound by latency (one token over 40 positions 3.6 us, 256: 4.2, 480 tokens of 9 heads over 3 of 64 6.1 us: one
 // workgroup's tiles one after the other), long caches by the cache's bytes and the conversions together: one token over 131071 positions, 32
-// heads over 8 of 128, q4_0 (151 MB) 37.5 us, 4.0 TB/s with the SIMDs issuing three quarters of the time; mxfp4 over 32768 (36 MB) 10 us.
+// heads over 8 of 128, q4_0 (151 MB) 37 us, 4.1 TB/s with the SIMDs issuing three quarters of the time; mxfp4 over 32768 (36 MB) 10.5 us; with
+// the join, and caches past the Infinity Cache in turn, 44.1 and 14.8.
 // Prompts by instruction issue: 1024 tokens behind 2999, the same heads, mxfp4, 98 us, 600 TFLOP/s: VALU and matrix instructions, some 256 and 52
-// a tile of 32 rows, are issued for 158k of 211k cycles, the matrix unit is busy for 92k. q4_0, with every scale on the weights,
+// a tile of 32 rows, are issued for 157k of 212k cycles, the matrix unit is busy for 92k. q4_0, with every scale on the weights,
 // 177 us. Tried without gain: eight wavefronts a workgroup, a tile requested ahead, values a tile ahead, raised wave priority around the
 // products; a tile's scores beside the products of the one before has no registers.
 typedef float f32x2 __attribute__((ext_vector_type(2)));

@@ -44,3 +44,30 @@ def test_step_from_matrix(dev, dtype):
         q = dev.get(fused, (1, heads, hd), np.float32)[:, :nq]
         assert np.all(np.abs(q - q64) <= np.abs(q64) * 2.0 ** -24 * (1 + 1e-6) + 1e-13) and np.abs(q).max() > 0.1
         near(dev.get(out, (1, nq, hd), np.float32), *attended(dtype, q, k, v, pos))
+
+
+@DTYPES
+@pytest.mark.parametrize("n, pos", [(1, 20), (1, 4000), (37, 100)])
+def test_floats_need_no_more_than_their_alignment(dev, dtype, n, pos):
+    """Rows, queries, outputs, weights and table 4 bytes off: the results of aligned ones, bit for bit."""
+    nq, nkv, hd = 4, 2, 40
+    rng = np.random.default_rng(pos)
+    c, table = dev.kv4(dtype, nkv, hd, pos + n), table_of(pos + n, hd)
+    dev.kv4_append(c, rng.standard_normal((pos + n, 2 * nkv * hd)).astype(np.float32), 0, 0)
+    rows = rng.standard_normal((n, (nq + 2 * nkv) * hd)).astype(np.float32)
+    w = (1 + rng.standard_normal(hd) / 8).astype(np.float32)
+    q = dev.kv4_append(c, rows, nq, pos, w, w, 1e-6, True, dev.put(table))
+    out, (k, v) = dev.kv4_attend(c, q, pos), dev.kv4_rows(c, pos, n)
+
+    def off(x):
+        return dev.put(np.concatenate([np.zeros(1, np.float32), x.ravel()])) + 4
+    drows, dw, dt, dq, do, dk, dv = off(rows), off(w), off(table), *(off(np.zeros(x.size, np.float32)) for x in (q, out, k, v))
+    L, r = dev.lib, C.byref(c)
+    size = L.l3m_kv4_work_bytes(r, n, nq)
+    assert L.l3m_k_kv4_append(r, dq, drows, rows.shape[1], n, nq, dw, dw, 1e-6, 1, pos, dt, None) == 0
+    assert L.l3m_k_kv4_attend(do, dq, r, n, nq, pos, dev.alloc(size), size, None) == 0
+    assert L.l3m_k_kv4_rows(r, dk, dv, pos, n, None) == 0
+    for p, want in ((dq, q), (do, out), (dk, k), (dv, v)):
+        assert np.array_equal(dev.get(p, want.shape, np.float32), want)
+    assert L.l3m_k_qk_norm_rope(dq, dk, drows, rows.shape[1], n, nq, nkv, hd, dw, dw, 1e-6, 1, pos, dt, None) == 0
+    assert np.array_equal(dev.get(dq, q.shape, np.float32), q)
