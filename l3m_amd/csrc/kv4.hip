@@ -386,7 +386,7 @@ typedef float f32x32 __attribute__((ext_vector_type(32)));
 
 constexpr int WAVES = 4;
 constexpr int SPLIT_WGS = 512, SPLITS = 256;                         // workgroups up to which a cache is split; most parts of it
-constexpr int NONE = -1000;
+constexpr int NONE = -1000;                                          // a unit before the first: below every one by more than 60
 constexpr float M0 = -3.40282347e38f;                                // the maximum of no score: float32's lowest, below every one
 
 // A q4_0 K word's eight codes, 0 .. 15, in f16: a nibble alone in a byte is the e4m3 number 2^-9 times it.
