@@ -169,6 +169,104 @@ int l3m_k_kv4_rows(const l3m_kv4 *c, float *k, float *v, int pos, int n, void *s
 // contents, used by one call at a time (a captured call uses it at every replay); a larger n's serves a smaller one.
 size_t l3m_kv4_work_bytes(const l3m_kv4 *c, int n, int nq);
 int l3m_k_kv4_attend(float *out, const float *q, const l3m_kv4 *c, int n, int nq, int pos, void *work, size_t work_bytes, void *stream);
+
+// Many sequences served from one paged 8-bit K/V cache (no counterpart in the reference, which decodes one). A batch is runs of rows one behind the
+// other: run i is rows starts[i] .. starts[i + 1] - 1 of a call's buffers, the last positions of sequence ids[i]. The integers lie in device memory, so a
+// captured call takes whatever they hold when it is replayed; they are used as far as they make sense (starts are brought into 0 .. n and into
+// order, a sequence that is none has length 0). Rows of no run are left as they are. As with the 4-bit cache, every call refuses (-1, l3m_dev_error) what
+// its arguments cannot mean, is asynchronous on `stream` (NULL: the library's) of device 0, allocates nothing and may be captured; nothing to do (no rows)
+// is no error.
+typedef struct {
+    const int32_t *ids;          // [seqs] the runs' sequences; NULL: 0, 1, ..
+    const int32_t *starts;       // [seqs + 1]
+    int seqs, n;                 // runs, up to 65536; rows that the buffers hold
+} l3m_batch;
+
+// Rotary positions: y = mag (u cos(p f) - w sin(p f), u sin(p f) + w cos(p f)) of each pair (u, w) of the first rd values of a head, p the row's position, f
+// the pair's frequency. l3m_rotary_init (host only) makes the frequencies: f = theta^(-2i / rd) of pair i, then by `scaling`
+//   L3M_ROTARY_PLAIN    as they are
+//   L3M_ROTARY_LINEAR   f / factor
+//   L3M_ROTARY_BASE     theta factor^(rd / (rd - 2)) in theta's place
+//   L3M_ROTARY_INDEX    f for pairs up to a, f / factor from b on, in proportion to i between; a and b the pairs that make `high` and `low` turns over
+//                       `trained` positions, rd log(trained / (2 pi turns)) / (2 log theta), rounded outwards; and mag = 0.1 log(factor) + 1
+//   L3M_ROTARY_TURNS    f for pairs of `high` turns or more over `trained` positions, f / factor up to `low`, in proportion to the turns between
+// Angles are exact for any position (whole numbers of 2^-64 of a turn). mag may be set behind the call.
+enum { L3M_ROTARY_PLAIN, L3M_ROTARY_LINEAR, L3M_ROTARY_BASE, L3M_ROTARY_INDEX, L3M_ROTARY_TURNS };
+#define L3M_ROTARY_HD 256        // the largest head
+typedef struct {
+    int      hd, rd, halves;     // head; values of it that turn, an even number; pairs (i, i + rd / 2) instead of (2i, 2i + 1)
+    float    mag;
+    uint64_t turn[L3M_ROTARY_HD / 2];   // frequency of a pair in 2^-64 of a turn
+} l3m_rotary;
+int l3m_rotary_init(l3m_rotary *r, int hd, int rd, int halves, double theta, int scaling, double factor, double low, double high, int trained);
+// The query and key heads of n rows [q heads | k heads | ..], `stride` values apart, turned into q and k, rows of their own strides. dtype, out_dtype:
+// L3M_HIP_F32 or L3M_HIP_BF16 (one rounding). pos: device [n], any int32 (a negative one turns back), or NULL for pos0, pos0 + 1, ... Outputs lie apart
+// from the rows or are the rows' own heads (the same place, type and stride); q and k apart or columns of the same rows. nq or nkv may be 0, and rd:
+// then heads go as they are.
+int l3m_k_rotary(const l3m_rotary *r, void *q, int q_stride, void *k, int k_stride, int out_dtype, const void *rows, int stride, int dtype, int n, int nq, int nkv,
+                 const int32_t *pos, int pos0, void *stream);
+
+// Causal attention over whole prompts, bf16: row t of a run over the run's rows 0 .. t, scores q.k / sqrt(hd), query head h reads kv head h / (nq / nkv). Rows'
+// strides and starts are multiples of 8 values and 16 bytes, hd a multiple of 8 up to 256. out may be q. Sums are float32's; weights are rounded to bf16, as the
+// result is. What lies behind a token, NaN among it, does not reach it.
+int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_stride, const uint16_t *k, const uint16_t *v, int kv_stride, const l3m_batch *b,
+                        int nq, int nkv, int hd, void *stream);
+
+// The cache: pages of 128 positions of all its layers and kv heads, in one allocation of l3m_kv8_bytes (0 for a shape that is refused), 256-byte aligned, which
+// need not be cleared. A page holds for each layer nkv units [K codes 128 x HP][V codes HP x 128], HP hd rounded up to 32, then 8 bytes a head: the
+// exponents of K's and of V's scales for its four blocks of 32 positions; a layer's part is rounded up to 256 bytes. Codes are OCP e4m3; a scale is 2^(byte - 127),
+// the smallest from 2^-126 up by which the block's largest finite value of that head is at most 448; a value that is not finite is stored as NaN.
+#define L3M_PAGE 128
+typedef struct {
+    uint8_t *mem;
+    int pages, layers, nkv, hd;
+} l3m_kv8;
+size_t l3m_kv8_page_bytes(int layers, int nkv, int hd);                        // hd a multiple of 8 up to 256
+size_t l3m_kv8_bytes(int pages, int layers, int nkv, int hd);                  // pages up to 2^20
+int    l3m_kv8_init(l3m_kv8 *c, int pages, int layers, int nkv, int hd, void *mem);   // host only: fills *c
+
+// Who holds which page: device tables in one allocation of l3m_pages_bytes, 16-byte aligned, which l3m_k_pages_reset clears. They may be read (and copied as a
+// whole, as a snapshot) between calls. state[0]: 0, or why a call could not be done (below); state[1]: pages in use.
+typedef struct {
+    int32_t *refs;               // [pages] how many sequences hold a page, 0: free
+    int32_t *table;              // [seqs][width] the page of a sequence's positions 128 i .. 128 i + 127; -1: none
+    int32_t *len;                // [seqs] positions of a sequence
+    int32_t *state, *scratch;
+    int pages, seqs, width;
+} l3m_pages;
+// A call that cannot be done as a whole changes nothing and sets state[0]; until l3m_k_pages_clear (or _reset) every call that changes tables or
+// cache does nothing, and l3m_k_kv8_attend's outputs are NaN.
+enum { L3M_PAGES_OK, L3M_PAGES_FULL /* too few free pages */, L3M_PAGES_LONG /* a sequence of more than width pages */,
+       L3M_PAGES_BAD /* a sequence that is none, is listed twice, should be empty and is not, or would be cut to more than it has */ };
+size_t l3m_pages_bytes(int pages, int seqs, int width);                        // pages up to 2^20, seqs up to 65536, seqs width up to 2^28
+int    l3m_pages_init(l3m_pages *p, int pages, int seqs, int width, void *mem);   // host only: fills *p
+int    l3m_k_pages_reset(const l3m_pages *p, void *stream);                    // no sequence has a position
+int    l3m_k_pages_clear(const l3m_pages *p, void *stream);                    // state[0] = 0
+// Room for a batch: each run's sequence becomes longer by its rows. New pages are the free ones of lowest index, in the runs' order. A page that a run goes on
+// in and that other sequences hold too is replaced by a copy (all layers); where all its holders are in the batch, the first of them keeps it. pos (NULL:
+// not wanted): the rows' positions, [n].
+int    l3m_k_pages_grow(const l3m_pages *p, const l3m_kv8 *c, const l3m_batch *b, int32_t *pos, void *stream);
+// Sequences to[i], which are empty, become copies of from[i]: they hold the same pages. No `to` is listed twice or is a `from`. Device lists of n.
+int    l3m_k_pages_fork(const l3m_pages *p, const int32_t *from, const int32_t *to, int n, void *stream);
+// Sequences ids[i] are cut to their first keep[i] positions (keep NULL: to none); pages that nobody holds any more are free.
+int    l3m_k_pages_cut(const l3m_pages *p, const int32_t *ids, const int32_t *keep, int n, void *stream);
+// The pages in use are moved to the front of the pool: those behind it, by ascending index, into the free ones among the first state[1].
+int    l3m_k_pages_compact(const l3m_pages *p, const l3m_kv8 *c, void *stream);
+
+// K and V rows of a batch, [n] of nkv heads (k and v of one stride, L3M_HIP_F32 or _BF16), into one layer: the last positions of the runs' sequences, whose lengths
+// count them already (l3m_k_pages_grow). The scale of a block that holds earlier positions is the larger of its own and the new rows'; where it rises, the old
+// codes are rounded again. A sequence must not be in the batch twice.
+int l3m_k_kv8_append(const l3m_kv8 *c, const l3m_pages *p, int layer, const void *k, const void *v, int stride, int dtype, const l3m_batch *b, void *stream);
+// The last positions of a batch's sequences as values: k and v float32 [n][nkv][hd] (either may be NULL). Positions whose page is none read as NaN.
+int l3m_k_kv8_rows(const l3m_kv8 *c, const l3m_pages *p, int layer, float *k, float *v, const l3m_batch *b, void *stream);
+// Attention of a batch's rows, the last positions of their sequences, each over its sequence up to itself: q and out [n] of nq heads, dtype L3M_HIP_F32 or _BF16,
+// out may be q; hd and heads as above. A row before its sequence's first position is zeros. Sums are float32's; queries and weights count in
+// 24 bits (f32), or queries exactly and weights in 16 (bf16). longest: no sequence is longer, as far as the
+// caller knows (0: not known); it decides how the work is split and no result's meaning. work: l3m_kv8_work_bytes(c, n, nq), 16-byte aligned, of any contents,
+// used by one call at a time (a captured call uses it at every replay); a larger n's serves a smaller one.
+size_t l3m_kv8_work_bytes(const l3m_kv8 *c, int n, int nq);
+int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int dtype, const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_batch *b, int nq,
+                     int longest, void *work, size_t work_bytes, void *stream);
 // The decode step's own pieces, alone (parity hooks):
 // rows [row0, row0 + n) of m dequantized by the step's embedding lookup (l3m_dequant_row, pack.c:55-62)
 // into out[n][32 * m->nb];

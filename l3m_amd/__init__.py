@@ -38,6 +38,12 @@ PERF_FIELDS = "tokens ns_token ns_compute ns_wait bytes_token l2_bytes l3_miss d
 Perf = _struct("Perf", [(n, C.c_double) for n in PERF_FIELDS])
 DMat = _struct("DMat", [("q", C.c_void_p), ("s", C.c_void_p)] + [(n, C.c_int) for n in "rows tiles nb dtype".split()])
 KV4 = _struct("KV4", [(n, C.c_void_p) for n in "kq ks vq vs".split()] + [(n, C.c_int) for n in "nkv hd cap dtype".split()])
+Batch = _struct("Batch", [(n, C.c_void_p) for n in "ids starts".split()] + [(n, C.c_int) for n in "seqs n".split()])
+Rotary = _struct("Rotary", [(n, C.c_int) for n in "hd rd halves".split()] + [("mag", C.c_float), ("turn", C.c_uint64 * 128)])
+KV8 = _struct("KV8", [("mem", C.c_void_p)] + [(n, C.c_int) for n in "pages layers nkv hd".split()])
+Pages = _struct("Pages", [(n, C.c_void_p) for n in "refs table len state scratch".split()] + [(n, C.c_int) for n in "pages seqs width".split()])
+ROTARY_SCALINGS = {n: i for i, n in enumerate("plain linear base index turns".split())}
+PAGES_STATES = ["ok", "full", "long", "bad"]
 GenSpec = _struct("GenSpec", [("arch", C.c_char_p)] + [(n, C.c_int) for n in "dim n_layers n_heads n_kv_heads ffn_dim vocab ctx".split()]
                   + [("rope_theta", C.c_float), ("norm_eps", C.c_float)] + [(n, C.c_int) for n in "dtype head_dtype tied".split()]
                   + [("seed", C.c_uint64), ("std", C.c_float), ("norm_jitter", C.c_float), ("bos", C.c_int), ("eos", C.c_int)])
@@ -47,7 +53,8 @@ _CODES = {"v": None, "i": C.c_int, "I": C.c_int32, "w": C.c_uint16, "q": C.c_uin
           "d": C.c_double, "p": C.c_void_p, "s": C.c_char_p, "*i": C.POINTER(C.c_int), "*I": _i32, "*f": _f,
           "*d": C.POINTER(C.c_double),
           "**": C.POINTER(C.c_void_p), "O": C.POINTER(Opts), "P": C.POINTER(Perf), "M": C.POINTER(DMat),
-          "G": C.POINTER(GenSpec), "K": C.POINTER(KV4), "cb": TOKEN_CALLBACK}
+          "G": C.POINTER(GenSpec), "K": C.POINTER(KV4), "B": C.POINTER(Batch), "R": C.POINTER(Rotary), "E": C.POINTER(KV8),
+          "A": C.POINTER(Pages), "cb": TOKEN_CALLBACK}
 _SIGNATURES = """
 l3m_load p s O                  | l3m_free v p                   | l3m_logits *f p
 l3m_generate i p *I i i f q cb p | l3m_vocab i p                 | l3m_ctx i p
@@ -80,6 +87,13 @@ l3m_tokenize i s s i *I i | l3m_head_dim i p | l3m_gemv_matrix_cores i i
 l3m_kv4_bytes z i i i i | l3m_kv4_init i K i i i i p | l3m_kv4_work_bytes z K i i
 l3m_k_qk_norm_rope i p p p i i i i i p p f i i p p | l3m_k_kv4_append i K p p i i i p p f i i p p
 l3m_k_kv4_rows i K p p i i p | l3m_k_kv4_attend i p p K i i i p z p
+l3m_rotary_init i R i i i d i d d d i | l3m_k_rotary i R p i p i i p i i i i i p i p
+l3m_k_attend_packed i p i p i p p i B i i i p | l3m_kv8_page_bytes z i i i | l3m_kv8_bytes z i i i i
+l3m_kv8_init i E i i i i p | l3m_pages_bytes z i i i | l3m_pages_init i A i i i p
+l3m_k_pages_reset i A p | l3m_k_pages_clear i A p | l3m_k_pages_grow i A E B p p
+l3m_k_pages_fork i A p p i p | l3m_k_pages_cut i A p p i p | l3m_k_pages_compact i A E p
+l3m_k_kv8_append i E A i p p i i B p | l3m_k_kv8_rows i E A i p p B p | l3m_kv8_work_bytes z E i i
+l3m_k_kv8_attend i p i p i i E A i B i i p z p
 l3m_time_read d ** i z i         | l3m_hip_attend_noalloc i p p p p i i i | l3m_phase_stamps i i i i p
 """
 _SIG = {}
@@ -511,3 +525,121 @@ class Device:
         do = self.alloc(q.nbytes)
         self._check(self.lib.l3m_k_kv4_attend(do, self.put(q), C.byref(c), n, nq, pos, self.alloc(size), size, None), "kv4_attend")
         return self.get(do, q.shape, np.float32)
+
+    # ---- many sequences: rows are float32, or bf16 as uint16
+
+    @staticmethod
+    def _rows(x):
+        """Rows as the kernels take them, their dtype and an empty array's."""
+        x = np.ascontiguousarray(x)
+        if x.dtype == np.uint16:
+            return x, BF16
+        return np.ascontiguousarray(x, np.float32), F32
+
+    def batch(self, starts, ids=None, n=None):
+        """Runs of rows: run i is rows starts[i] .. starts[i + 1] - 1, of sequence ids[i] (None: i)."""
+        starts = np.ascontiguousarray(starts, np.int32)
+        if ids is not None and len(ids) != len(starts) - 1:
+            raise ValueError(f"{len(ids)} sequences for {len(starts) - 1} runs")
+        return Batch(None if ids is None else self.put(np.int32(ids)), self.put(starts), len(starts) - 1, int(starts[-1]) if n is None else n)
+
+    def rotary_plan(self, hd, rd=None, halves=False, theta=10000.0, scaling="plain", factor=1.0, low=1.0, high=4.0, trained=1):
+        """The frequencies of a head of hd values of which the first rd (None: all) turn (l3m_rotary_init; host only)."""
+        r = Rotary()
+        self._check(self.lib.l3m_rotary_init(C.byref(r), hd, hd if rd is None else rd, int(halves), theta, ROTARY_SCALINGS[scaling], factor, low, high, trained), "rotary_plan")
+        return r
+
+    def rotary(self, plan, rows, nq, nkv, pos=None, pos0=0, out=F32):
+        """The query and key heads of rows [n, width] turned: q [n, nq, hd], k [n, nkv, hd] of type `out` (l3m_k_rotary)."""
+        rows, dtype = self._rows(rows)
+        n, width = rows.shape
+        if pos is not None and len(pos) != n:
+            raise ValueError(f"{len(pos)} positions for {n} rows")
+        kind = np.float32 if out == F32 else np.uint16
+        q, k = (np.zeros((n, h, plan.hd), kind) for h in (nq, nkv))
+        dq, dk = (self.alloc(max(x.nbytes, 4)) for x in (q, k))
+        self._check(self.lib.l3m_k_rotary(C.byref(plan), dq, nq * plan.hd, dk, nkv * plan.hd, out, self.put(rows), width, dtype, n, nq, nkv,
+                                          None if pos is None else self.put(np.int32(pos)), pos0, None), "rotary")
+        return self.get(dq, q.shape, kind), self.get(dk, k.shape, kind)
+
+    def attend_packed(self, q, k, v, b):
+        """Causal attention of packed prompts, bf16 as uint16: q [n, nq, hd], k and v [n, nkv, hd] (l3m_k_attend_packed)."""
+        q, k, v = (np.ascontiguousarray(x, np.uint16) for x in (q, k, v))
+        if k.shape != v.shape or len(q) < b.n or len(k) < b.n or q.shape[2] != k.shape[2]:
+            raise ValueError(f"rows {q.shape}, {k.shape} and {v.shape} for a batch of {b.n}")
+        do = self.alloc(max(q.nbytes, 16))
+        self._check(self.lib.l3m_k_attend_packed(do, q.shape[1] * q.shape[2], self.put(q), q.shape[1] * q.shape[2], self.put(k), self.put(v), k.shape[1] * k.shape[2],
+                                                 C.byref(b), q.shape[1], k.shape[1], q.shape[2], None), "attend_packed")
+        return self.get(do, q.shape, np.uint16)
+
+    def kv8(self, pages, layers, nkv, hd):
+        """An empty paged 8-bit K/V cache of `pages` pages of 128 positions."""
+        c = KV8()
+        size = self.lib.l3m_kv8_bytes(pages, layers, nkv, hd)
+        if not size:
+            raise ValueError(f"no 8-bit cache of {pages} pages, {layers} layers, {nkv} heads of {hd}")
+        self._check(self.lib.l3m_kv8_init(C.byref(c), pages, layers, nkv, hd, self.alloc(size)), "kv8")
+        return c
+
+    def pages(self, pages, seqs, width):
+        """Tables of `seqs` empty sequences of up to `width` pages each."""
+        p = Pages()
+        size = self.lib.l3m_pages_bytes(pages, seqs, width)
+        if not size:
+            raise ValueError(f"no tables of {pages} pages, {seqs} sequences of up to {width}")
+        self._check(self.lib.l3m_pages_init(C.byref(p), pages, seqs, width, self.alloc(size)), "pages")
+        self._check(self.lib.l3m_k_pages_reset(C.byref(p), None), "pages")
+        return p
+
+    def pages_state(self, p):
+        """What the tables hold: state ("ok", "full", "long" or "bad"), pages used, refs, table, len."""
+        state = self.get(p.state, 2, np.int32)
+        return {"state": PAGES_STATES[state[0]], "used": int(state[1]), "refs": self.get(p.refs, p.pages, np.int32),
+                "table": self.get(p.table, (p.seqs, p.width), np.int32), "len": self.get(p.len, p.seqs, np.int32)}
+
+    def pages_grow(self, p, c, b):
+        """Room for a batch's rows: their positions (l3m_k_pages_grow)."""
+        pos = self.alloc(max(4 * b.n, 4))
+        self._check(self.lib.l3m_k_pages_grow(C.byref(p), C.byref(c), C.byref(b), pos, None), "pages_grow")
+        return self.get(pos, b.n, np.int32)
+
+    def pages_fork(self, p, sources, to):
+        if len(sources) != len(to):
+            raise ValueError(f"{len(sources)} sequences forked to {len(to)}")
+        self._check(self.lib.l3m_k_pages_fork(C.byref(p), self.put(np.int32(sources)), self.put(np.int32(to)), len(to), None), "pages_fork")
+
+    def pages_cut(self, p, ids, keep=None):
+        if keep is not None and len(keep) != len(ids):
+            raise ValueError(f"{len(keep)} lengths for {len(ids)} sequences")
+        self._check(self.lib.l3m_k_pages_cut(C.byref(p), self.put(np.int32(ids)), None if keep is None else self.put(np.int32(keep)), len(ids), None), "pages_cut")
+
+    def pages_compact(self, p, c):
+        self._check(self.lib.l3m_k_pages_compact(C.byref(p), C.byref(c), None), "pages_compact")
+
+    def pages_clear(self, p):
+        self._check(self.lib.l3m_k_pages_clear(C.byref(p), None), "pages_clear")
+
+    def kv8_append(self, c, p, layer, k, v, b):
+        """Rows k, v [n, nkv, hd] of a batch into a layer of the cache (l3m_k_kv8_append)."""
+        (k, dtype), (v, dv) = self._rows(k), self._rows(v)
+        if dtype != dv or k.shape != v.shape or k.shape[1:] != (c.nkv, c.hd) or len(k) < b.n:
+            raise ValueError(f"rows {k.shape} and {v.shape} for a batch of {b.n}, {c.nkv} heads of {c.hd}")
+        self._check(self.lib.l3m_k_kv8_append(C.byref(c), C.byref(p), layer, self.put(k), self.put(v), c.nkv * c.hd, dtype, C.byref(b), None), "kv8_append")
+
+    def kv8_rows(self, c, p, layer, b):
+        """The last positions of a batch's sequences as values: k, v [n, nkv, hd] (l3m_k_kv8_rows)."""
+        dk, dv = (self.alloc(4 * max(b.n, 1) * c.nkv * c.hd) for _ in range(2))
+        self._check(self.lib.l3m_k_kv8_rows(C.byref(c), C.byref(p), layer, dk, dv, C.byref(b), None), "kv8_rows")
+        return tuple(self.get(x, (b.n, c.nkv, c.hd), np.float32) for x in (dk, dv))
+
+    def kv8_attend(self, c, p, layer, q, b, longest=0):
+        """Attention of a batch's rows q [n, nq, hd], the last positions of their sequences (l3m_k_kv8_attend)."""
+        q, dtype = self._rows(q)
+        n, nq, hd = q.shape
+        if hd != c.hd or n < b.n:
+            raise ValueError(f"rows {q.shape} for a batch of {b.n}, heads of {c.hd}")
+        size = self.lib.l3m_kv8_work_bytes(C.byref(c), max(b.n, 1), nq)
+        do = self.alloc(max(q.nbytes, 16))
+        self._check(self.lib.l3m_k_kv8_attend(do, nq * hd, self.put(q), nq * hd, dtype, C.byref(c), C.byref(p), layer, C.byref(b), nq, longest, self.alloc(max(size, 16)),
+                                              size, None), "kv8_attend")
+        return self.get(do, q.shape, q.dtype)

@@ -1,0 +1,598 @@
+// A paged K/V cache of 8-bit codes for CDNA4 (gfx950): the writer, the read-back, and the attention of a batch's last tokens over it.
+//
+// Layout. A page's unit of a layer and kv head: K codes [128 positions][HP] and V codes [HP][128 positions], HP hd rounded up to 32 (zeros), so that a lane's
+// 16 bytes of either are columns of the matrix cores' operands as they lie. A block of 32 positions has one scale of a kv head's K and one of its V, a power
+// of two, which the conversion of the codes takes.
+#include "serve.h"
+
+namespace {
+
+constexpr int WAVES = 4;
+constexpr int E4M3_NAN = 0x7F;
+constexpr float M0 = -3.40282347e38f;                                // the maximum of no score: float32's lowest
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// ---------------------------------------------------------------- writer
+
+__device__ __forceinline__ float max_wave(float x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+// The exponent byte of a block by its largest finite magnitude: the smallest power of two, 2^-126 at least, by which it is at most 448 = 1.75 2^8.
+__device__ __forceinline__ int exponent_for(float most) {
+    const uint32_t u = __float_as_uint(most);
+    return max((int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u), 1);
+}
+__device__ __forceinline__ float finite_size(float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? a : 0.f;
+}
+// Four values times 2^(127 - exponent) as codes, to the nearest, ties to even; what is not finite is NaN.
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float up) {
+    uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * up, b * up, 0, false);
+    w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * up, d * up, (int)w, true);
+    const float x[4] = {a, b, c, d};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (!(fabsf(x[i]) < INFINITY)) w = (w & ~(255u << 8 * i)) | (uint32_t)E4M3_NAN << 8 * i;
+    return w;
+}
+// Four codes times `by`, as codes.
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float by) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return encode4(a.x, a.y, b.x, b.y, by);
+}
+__device__ __forceinline__ float pow2_byte(int e) { return __uint_as_float((uint32_t)e << 23); }   // 2^(e - 127), e 1 .. 254
+
+template <class T> __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 a = *(const f32x4_a4 *)p, b = *(const f32x4_a4 *)(p + 4);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = i < 4 ? a[i & 3] : b[i & 3];
+    } else {
+        typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+        const u32x4 w = *(const u32x4_a2 *)p;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    }
+}
+
+struct RowsIn {
+    l3m_kv8    c;
+    Runs       b;
+    const void *k, *v;                                               // rows in
+    float      *ok, *ov;                                             // rows out (read-back)
+    long long  stride;
+    const int32_t *table, *len, *state;
+    int        layer, pages, seqs, width;
+};
+// The blocks of 32 positions that a run's rows, the last ones of its sequence, lie in.
+__device__ __forceinline__ int length_of(const RowsIn &a, int id) { return (unsigned)id < (unsigned)a.seqs ? clamp(a.len[id], 0, a.width * PAGE) : 0; }
+__device__ __forceinline__ int blocks_of(const RowsIn &a, int run, int rows) {
+    const int len = length_of(a, a.b.id(run)), first = len - rows;
+    return rows && first >= 0 ? (len - 1) / BLOCK - first / BLOCK + 1 : 0;
+}
+
+// The new rows of a block of 32 positions of one kv head, K or V: a wavefront each. Their largest magnitude and the scale of what the block holds already make the
+// block's scale; where that rises, the old codes are rounded again.
+template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(RowsIn a) {
+    constexpr int HP = 32 * NB, PER = 4 * NB, IT = 2 * NB;           // eight values a lane: chunks of a row, turns for 32 rows
+    __shared__ __align__(16) uint8_t code_s[4][BLOCK * (HP + 4)];
+    if (a.state[0]) return;                                          // a failed call on the tables: nothing is written
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nkv = a.c.nkv;
+    const int w = (int)(blockIdx.x * 4 + wave), per = 2 * nkv, item = w / per, which = w - item * per, h = which >> 1;
+    const bool value = which & 1;
+    const Found f = find_run(a.b, item, [&](int r, int, int rows) { return blocks_of(a, r, rows); });
+    if (f.run < 0) return;
+    const int id = a.b.id(f.run), len = length_of(a, id), first = len - f.rows, block = first / BLOCK + f.at;
+    const int page = a.table[(size_t)id * a.width + block / SCALES];
+    if ((unsigned)page >= (unsigned)a.pages) return;
+    const Unit u = unit_of(a.c, page, a.layer, h);
+    const int sub = block % SCALES, p0 = block * BLOCK, before = max(first - p0, 0), end = min(len - p0, BLOCK);
+    uint8_t *scale = u.s + (value ? SCALES : 0) + sub;
+    const T *rows = (const T *)(value ? a.v : a.k) + (size_t)h * a.c.hd;
+    float x[IT][8], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < IT; i++) {
+        const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[i][j] = 0.f;
+        if (r >= before && r < end && d < a.c.hd) load8(rows + (long long)(f.s0 + p0 + r - first) * a.stride + d, x[i]);
+#pragma unroll
+        for (int j = 0; j < 8; j++) most = fmaxf(most, finite_size(x[i][j]));
+    }
+    const int had = before ? max((int)*scale, 1) : 0, e = max(exponent_for(max_wave(most)), had);
+    const float up = pow2_byte(254 - e), down = had && had < e ? (e - had < 127 ? pow2_byte(127 - (e - had)) : 0.f) : 1.f;
+    if (!value) {
+#pragma unroll
+        for (int i = 0; i < IT; i++) {
+            const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
+            u32x2 *to = (u32x2 *)(u.k + (size_t)(sub * BLOCK + r) * HP + d);
+            if (r >= before && r < end) *to = u32x2{encode4(x[i][0], x[i][1], x[i][2], x[i][3], up), encode4(x[i][4], x[i][5], x[i][6], x[i][7], up)};
+            else if (r < before && down != 1.f) {
+                const u32x2 was = *to;
+                *to = u32x2{recode4(was.x, down), recode4(was.y, down)};
+            }
+        }
+    } else {
+        // codes through LDS to words along positions: lane's dimensions lane, lane + 64 ..
+        uint8_t *row_s = code_s[wave];
+#pragma unroll
+        for (int i = 0; i < IT; i++) {
+            const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
+            uint32_t *to = (uint32_t *)(row_s + r * (HP + 4) + d);
+            to[0] = encode4(x[i][0], x[i][1], x[i][2], x[i][3], up);
+            to[1] = encode4(x[i][4], x[i][5], x[i][6], x[i][7], up);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        for (int d = lane; d < HP; d += 64) {
+            uint32_t *to = (uint32_t *)(u.v + (size_t)d * PAGE + sub * BLOCK);
+#pragma unroll
+            for (int q = 0; q < BLOCK / 4; q++) {
+                if (4 * q >= end || (4 * q + 4 <= before && down == 1.f)) continue;
+                uint32_t word = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) word |= (uint32_t)row_s[(4 * q + j) * (HP + 4) + d] << 8 * j;
+                if (4 * q < before) {                                // some that were there
+                    const uint32_t was = down == 1.f ? to[q] : recode4(to[q], down);
+                    const int n = min(before - 4 * q, 4);
+                    const uint32_t keep = n == 4 ? ~0u : ~(~0u << 8 * n);
+                    word = (was & keep) | (word & ~keep);
+                }
+                to[q] = word;
+            }
+        }
+    }
+    if (lane == 0) *scale = (uint8_t)e;
+}
+
+// ---------------------------------------------------------------- read-back
+// A block of 32 positions of one kv head, K or V, to a wavefront: float32 rows of the run's last positions.
+template <int NB> __global__ void __launch_bounds__(256) k_kv8_rows(RowsIn a) {
+    constexpr int HP = 32 * NB;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nkv = a.c.nkv, hd = a.c.hd;
+    const int w = (int)(blockIdx.x * 4 + wave), per = 2 * nkv, item = w / per, which = w - item * per, h = which >> 1;
+    const bool value = which & 1;
+    float *out = value ? a.ov : a.ok;
+    if (!out) return;
+    const Found f = find_run(a.b, item, [&](int r, int, int rows) { return blocks_of(a, r, rows); });
+    if (f.run < 0) return;
+    const int id = a.b.id(f.run), len = length_of(a, id), first = len - f.rows, block = first / BLOCK + f.at;
+    const int page = a.table[(size_t)id * a.width + block / SCALES];
+    const bool lost = (unsigned)page >= (unsigned)a.pages;
+    const Unit u = unit_of(a.c, lost ? 0 : page, a.layer, h);
+    const int sub = block % SCALES, p0 = block * BLOCK, begin = max(first - p0, 0), end = min(len - p0, BLOCK);
+    const float s = lost ? NAN : pow2_byte(max((int)u.s[(value ? SCALES : 0) + sub], 1));
+    float *to = out + ((size_t)(f.s0 + p0 - first + begin) * nkv + h) * hd;
+    if (!value) {
+        for (int i = lane; i < (end - begin) * (hd / 4); i += 64) {
+            const int r = i / (hd / 4), d = 4 * (i - r * (hd / 4));
+            const uint32_t c = *(const uint32_t *)(u.k + (size_t)(sub * BLOCK + begin + r) * HP + d);
+            const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+            *(f32x4_a4 *)(to + (size_t)r * nkv * hd + d) = f32x4{x.x * s, x.y * s, y.x * s, y.y * s};
+        }
+        return;
+    }
+    for (int d = lane; d < hd; d += 64)
+        for (int r = begin; r < end; r++) {
+            const uint32_t c = u.v[(size_t)d * PAGE + sub * BLOCK + r];
+            to[(size_t)(r - begin) * nkv * hd + d] = __builtin_amdgcn_cvt_f32_fp8((int)c, 0) * s;
+        }
+}
+
+// ---------------------------------------------------------------- attention
+// Rows: a kv head's (token, query head) pairs of a run, a token's heads side by side (g = nq / nkv), 16 to a product. Per tile, a page, and wavefront, codes
+// converted to bf16 as they are used, exactly, their scale with them (v_cvt_scalef32_pk_bf16_fp8):
+//   S = K Q^T        16 positions x 16 rows x 32 dimensions (v_mfma_f32_16x16x32_bf16), q in PARTS of bf16
+//   P = 2^(S - m)    m the running maximum
+//   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions, P in PARTS of bf16
+// A lane of group c reads 16 bytes at once, which are two products' eight columns: the dimensions 64 f + 16 c .. of K and of q, the positions 64 u + 16 c .. of
+// V. K's rows are taken in the order in which a lane then holds the scores of those positions, so no value crosses lanes. All sums in 32 bits; q and P in three
+// parts are float32's 24 bits; for bf16 rows q is one part, exactly, and P two, 2^-16 of a weight at the most.
+// (v_mfma_scale_f32_16x16x128_f8f6f4 takes the codes as they lie, but aligns a product's 128 terms to the largest one: sums were off by 2^-11 of that.)
+template <bool F32> struct Parts {
+    static constexpr int q = F32 ? 3 : 1, p = F32 ? 3 : 2;
+};
+
+template <int M> __device__ __forceinline__ float other(float x, float &y) {                // lane ^ 16, lane ^ 32
+    const uint32_t a = __float_as_uint(x);
+    if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+        y = __uint_as_float(r[1]);
+        return __uint_as_float(r[0]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+        y = __uint_as_float(r[1]);
+        return __uint_as_float(r[0]);
+    }
+}
+__device__ __forceinline__ float max_groups(float x) {               // over the four lane groups
+    float y;
+    x = other<16>(x, y); x = fmaxf(x, y);
+    x = other<32>(x, y); return fmaxf(x, y);
+}
+__device__ __forceinline__ float sum_groups(float x) {
+    float y;
+    x = other<16>(x, y); x += y;
+    x = other<32>(x, y); return x + y;
+}
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// Eight codes times `scale`, a power of two.
+__device__ __forceinline__ bf16x8 widen(u32x2 w, float scale) {
+    u32x4 r;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, scale, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, scale, true));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, scale, false));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, scale, true));
+    return __builtin_bit_cast(bf16x8, r);
+}
+// Eight values as the sum of N bf16 ones each.
+template <int N> __device__ __forceinline__ void in_parts(const float (&v)[8], bf16x8 (&w)[N]) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = v[i];
+#pragma unroll
+    for (int p = 0; p < N; p++) {
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            r[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+            if (p + 1 < N) {
+                x[2 * i] -= __uint_as_float(r[i] << 16);
+                x[2 * i + 1] -= __uint_as_float(r[i] & 0xFFFF0000u);
+            }
+        }
+        w[p] = __builtin_bit_cast(bf16x8, r);
+    }
+}
+
+struct AttendIn {
+    l3m_kv8     c;
+    Runs        b;
+    const void *q;
+    void       *out;
+    long long   q_stride, out_stride;
+    const int32_t *table, *len, *state;
+    float      *work;
+    int         layer, pages, seqs, width, nq, g;
+    uint32_t    g_mul;
+};
+__device__ __forceinline__ int length_of(const AttendIn &a, int id) { return (unsigned)id < (unsigned)a.seqs ? clamp(a.len[id], 0, a.width * PAGE) : 0; }
+
+// Products' columns over a row's dimensions: step s holds a lane's dimensions dim_of(s, c) .. + 7.
+template <int NB> __device__ __forceinline__ int dim_of(int s, int c) { return s / 2 * 2 + 1 < NB ? 64 * (s >> 1) + 16 * c + 8 * (s & 1) : 32 * s + 8 * c; }
+template <bool F32, int NB> struct Queries {
+    static constexpr int QP = Parts<F32>::q;
+    bf16x8 part[NB][QP];
+    __device__ __forceinline__ void load(const void *q, long long at, int hd, int lane) {
+#pragma unroll
+        for (int s = 0; s < NB; s++) {
+            const int d = dim_of<NB>(s, lane >> 4);
+            const bool in = d < hd;
+            float x[8];
+            if constexpr (F32) load8((const float *)q + at + (in ? d : 0), x);
+            else load8((const uint16_t *)q + at + (in ? d : 0), x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = in ? x[i] : 0.f;
+            in_parts<QP>(x, part[s]);
+        }
+    }
+};
+// The scores' products of a tile, t = 4 u + 2 e + f, element i of lane group c: position 64 u + 16 c + 8 e + 4 f + i. So row m of the operand is
+__device__ __forceinline__ int position_of(int t, int m) { return 64 * (t >> 2) + 16 * (m >> 2) + 4 * (t & 3) + (m & 3); }
+template <int NB> struct KeysIn {
+    u32x2 w[NB];
+    __device__ __forceinline__ void load(const uint8_t *k, int t, int lane) {
+        const uint8_t *row = k + position_of(t, lane & 15) * (32 * NB);
+        const int c = lane >> 4;
+#pragma unroll
+        for (int s = 0; s + 1 < NB; s += 2) {
+            const u32x4 x = *(const u32x4 *)(row + 32 * s + 16 * c);
+            w[s] = u32x2{x.x, x.y};
+            w[s + 1] = u32x2{x.z, x.w};
+        }
+        if constexpr (NB % 2) w[NB - 1] = *(const u32x2 *)(row + 32 * (NB - 1) + 8 * c);
+    }
+};
+
+template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_attend(AttendIn a) {
+    constexpr int QP = Parts<F32>::q, PP = Parts<F32>::p, HP = 32 * NB, OS = HP + 4;
+    __shared__ float o_s[2][16][OS], m_s[WAVES][16], l_s[WAVES][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, c = lane >> 4, hd = a.c.hd, g = a.g;
+    const int h = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const Found f = find_run(a.b, (int)(blockIdx.x / (unsigned)a.c.nkv), [&](int, int, int rows) { return (rows * g + 15) >> 4; });
+    if (f.run < 0) return;
+    const int id = a.b.id(f.run), len = length_of(a, id), row0 = 16 * f.at, rows = min(f.rows * g - row0, 16);
+    const bool failed = a.state[0] != 0;
+    // the row of this lane's column: its token, and the positions it sees
+    const int r = row0 + min(r16, rows - 1), token = (int)divide(r, g, a.g_mul), head = h * g + r - token * g, seen = max(len - f.rows + token + 1, 0);
+    const int last = (int)divide(row0 + rows - 1, g, a.g_mul), end = max(len - f.rows + last + 1, 0), tiles = (end + PAGE - 1) / PAGE;
+    const int whole = max(len - f.rows + (int)divide(row0, g, a.g_mul) + 1, 0) / PAGE;     // tiles that every row sees whole
+    Queries<F32, NB> qs;
+    qs.load(a.q, (long long)(f.s0 + token) * a.q_stride + (long long)head * hd, hd, lane);
+    const float scale = 1.44269504f / sqrtf((float)hd);             // of the scores: base 2
+
+    f32x4 acc[2 * NB];
+#pragma unroll
+    for (int t = 0; t < 2 * NB; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = M0, l = 0.f;
+    for (int tile = wave; tile < tiles; tile += WAVES) {
+        const int page = __builtin_amdgcn_readfirstlane(a.table[(size_t)id * a.width + tile]);
+        const bool lost = (unsigned)page >= (unsigned)a.pages;
+        const Unit u = unit_of(a.c, lost ? 0 : page, a.layer, h);
+        const uint32_t ks = *(const uint32_t *)u.s, vs = *(const uint32_t *)(u.s + 4);
+        const int left = end - tile * PAGE;                          // positions that some row sees
+        const bool masked = tile >= whole;
+        float p[32];
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+            KeysIn<NB> k;
+            k.load(u.k, t, lane);
+            if (lost)
+#pragma unroll
+                for (int i = 0; i < NB; i++) k.w[i] = u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
+            const float sk = pow2_byte((int)(ks >> 8 * (2 * (t >> 2) + (r16 >> 3)) & 255u));
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const bf16x8 x = widen(k.w[i], sk);
+#pragma unroll
+                for (int q = QP - 1; q >= 0; q--) s = mfma(x, qs.part[i][q], s);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[4 * t + i] = s[i];
+        }
+        const int p0 = tile * PAGE + 16 * c;                         // of p[i]: p0 + i, behind the first half 48 more
+        if (masked)
+#pragma unroll
+            for (int i = 0; i < 32; i++) p[i] = p0 + i + (i < 16 ? 0 : 48) < seen ? p[i] : -INFINITY;
+        float top = p[0];
+#pragma unroll
+        for (int i = 1; i < 32; i++) top = fmaxf(top, p[i]);
+        top = fmaxf(max_groups(top) * scale, m);
+        if (__ballot(top > m)) {
+            const float by = __builtin_amdgcn_exp2f(m - top);
+            l *= by;
+#pragma unroll
+            for (int t = 0; t < 2 * NB; t++) acc[t] *= by;
+            m = top;
+        }
+        bf16x8 w[4][PP];                                             // by products: 64 u + 16 c + 8 e ..
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[i] = __builtin_amdgcn_exp2f(fmaf(p[8 * t + i], scale, -m));
+                l += x[i];
+            }
+            in_parts<PP>(x, w[t]);
+        }
+        u32x4 v[2 * NB][2];
+#pragma unroll
+        for (int t = 0; t < 2 * NB; t++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) v[t][j] = *(const u32x4 *)(u.v + (16 * t + r16) * PAGE + 64 * j + 16 * c);
+        float sv[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) sv[j] = 64 * j + 32 * (c >> 1) < left ? pow2_byte((int)(vs >> 8 * (2 * j + (c >> 1)) & 255u)) : 1.f;   // or never written
+        uint32_t nan = 0;                                            // codes of NaN among the values that some row sees
+        if (masked || lost)
+#pragma unroll
+            for (int t = 0; t < 2 * NB; t++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int n = left - (64 * j + 16 * c + 4 * i);
+                        const uint32_t x = lost ? 0x7F7F7F7Fu : v[t][j][i];
+                        v[t][j][i] = n >= 4 ? x : n <= 0 ? 0u : x & ~(~0u << 8 * n);
+                        nan |= ((v[t][j][i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    }
+        auto product = [&](const u32x4 (&x)[2 * NB][2], f32x4 (&to)[2 * NB]) {
+#pragma unroll
+            for (int t = 0; t < 2 * NB; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const u32x4 &y = x[t][j >> 1];
+                    const bf16x8 va = widen(j & 1 ? u32x2{y.z, y.w} : u32x2{y.x, y.y}, sv[j >> 1]);
+#pragma unroll
+                    for (int q = PP - 1; q >= 0; q--) to[t] = mfma(va, w[j][q], to[t]);
+                }
+        };
+        if (!masked || !__ballot(nan != 0)) product(v, acc);
+        else                                                         // a NaN is the rows' that see it: a token's rows at a time, over its own positions
+            for (int to = min(seen, end), at = __builtin_amdgcn_readfirstlane(to);;) {
+                u32x4 x[2 * NB][2];
+                f32x4 part[2 * NB];
+#pragma unroll
+                for (int t = 0; t < 2 * NB; t++) {
+                    part[t] = acc[t];
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int n = at - tile * PAGE - (64 * j + 16 * c + 4 * i);
+                            x[t][j][i] = n >= 4 ? v[t][j][i] : n <= 0 ? 0u : v[t][j][i] & ~(~0u << 8 * n);
+                        }
+                }
+                product(x, part);
+#pragma unroll
+                for (int t = 0; t < 2 * NB; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][i] = to == at ? part[t][i] : acc[t][i];
+                int next = INT_MAX;                                  // the next larger number of positions that a row sees
+                for (uint64_t more = __ballot(to > at); more; more &= more - 1) next = min(next, __builtin_amdgcn_readlane(to, __builtin_ctzll(more)));
+                if (next == INT_MAX) break;
+                at = next;
+            }
+    }
+
+    // the wavefronts' parts at their common maximum, two at a time
+    l = sum_groups(l);
+    if (c == 0) {
+        m_s[wave][r16] = m;
+        l_s[wave][r16] = l;
+    }
+    __syncthreads();
+    float most = m_s[0][r16];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) most = fmaxf(most, m_s[w][r16]);
+    const float by = __builtin_amdgcn_exp2f(m - most);
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        if (wave >> 1 == half)
+#pragma unroll
+            for (int t = 0; t < 2 * NB; t++) {
+                f32x4 &to = *(f32x4 *)&o_s[wave & 1][r16][16 * t + 4 * c];
+                to = half ? to + acc[t] * by : acc[t] * by;
+            }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < rows * (hd / 4); i += 64 * WAVES) {
+        const int row = i / (hd / 4), d = 4 * (i - row * (hd / 4));
+        float top = m_s[0][row], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][row]);
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) sum = fmaf(l_s[w][row], __builtin_amdgcn_exp2f(m_s[w][row] - top), sum);
+        f32x4 x = *(const f32x4 *)&o_s[0][row][d] + *(const f32x4 *)&o_s[1][row][d];
+        const int t = (int)divide(row0 + row, g, a.g_mul), hh = h * g + row0 + row - t * g;
+        const bool none = len - f.rows + t < 0;                      // a token before its sequence's first position sees nothing
+        x = failed ? f32x4{NAN, NAN, NAN, NAN} : none ? f32x4{0.f, 0.f, 0.f, 0.f} : x / sum;
+        const long long at = (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d;
+        if constexpr (F32) *(f32x4_a4 *)((float *)a.out + at) = x;
+        else {
+            typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+            *(u32x2_a2 *)((uint16_t *)a.out + at) = u32x2{bf16_pair(x.x, x.y), bf16_pair(x.z, x.w)};
+        }
+    }
+}
+
+Runs runs_of(const l3m_batch *b) { return {b->ids, b->starts, b->seqs, b->n}; }
+// What calls over the cache refuse alike, or NULL.
+const char *call_bad(const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_batch *b) {
+    if (const char *why = paged_bad(c, p)) return why;
+    if (const char *why = batch_bad(b)) return why;
+    if (layer < 0 || layer >= c->layers) return "kv8: no such layer";
+    if (on_batch(b, c->mem, l3m_kv8_bytes(c->pages, c->layers, c->nkv, c->hd))) return "kv8: the batch overlaps the cache";
+    return nullptr;
+}
+#define BY_BLOCKS(CALL)                                                                                                                                        \
+    switch (padded(c->hd) / 32) {                                                                                                                              \
+    case 1: CALL(1); break;                                                                                                                                    \
+    case 2: CALL(2); break;                                                                                                                                    \
+    case 3: CALL(3); break;                                                                                                                                    \
+    case 4: CALL(4); break;                                                                                                                                    \
+    case 5: CALL(5); break;                                                                                                                                    \
+    case 6: CALL(6); break;                                                                                                                                    \
+    case 7: CALL(7); break;                                                                                                                                    \
+    default: CALL(8); break;                                                                                                                                   \
+    }
+// Blocks of 32 positions that a batch's rows can lie in: a run of r rows in (r + 62) / 32 of them.
+long long most_blocks(const l3m_batch *b) { return b->n / BLOCK + 2ll * b->seqs; }
+
+}  // namespace
+
+extern "C" {
+
+size_t l3m_kv8_page_bytes(int layers, int nkv, int hd) {
+    if (layers < 1 || layers > 4096 || nkv < 1 || nkv > 4096 || hd < 8 || hd > 256 || hd % 8) return 0;
+    return layers * layer_bytes(nkv, hd);
+}
+size_t l3m_kv8_bytes(int pages, int layers, int nkv, int hd) { return pages < 1 || pages > 1 << 20 ? 0 : pages * l3m_kv8_page_bytes(layers, nkv, hd); }
+
+int l3m_kv8_init(l3m_kv8 *c, int pages, int layers, int nkv, int hd, void *mem) {
+    if (!c || !mem || (uintptr_t)mem % 256) return l3m_dev_fail("kv8: memory must be 256-byte aligned");
+    if (!l3m_kv8_bytes(pages, layers, nkv, hd)) return l3m_dev_fail("kv8: hd a multiple of 8 up to 256, pages up to 2^20, layers and kv heads up to 4096");
+    *c = l3m_kv8{(uint8_t *)mem, pages, layers, nkv, hd};
+    return 0;
+}
+
+int l3m_k_kv8_append(const l3m_kv8 *c, const l3m_pages *p, int layer, const void *k, const void *v, int stride, int dtype, const l3m_batch *b, void *stream) {
+    if (const char *why = call_bad(c, p, layer, b)) return l3m_dev_fail(why);
+    const size_t size = value_bytes(dtype);
+    if (!size) return l3m_dev_fail("kv8_append: rows are f32 or bf16");
+    const long long width = (long long)c->nkv * c->hd;
+    if (stride < width) return l3m_dev_fail("kv8_append: a row holds fewer values than its heads");
+    if (!b->seqs || !b->n) return 0;
+    if (!k || !v || ((uintptr_t)k | (uintptr_t)v) % size) return l3m_dev_fail("kv8_append: no rows, or not aligned to their values");
+    const size_t bytes = rows_bytes(b->n, stride, width, size);
+    if (on_cache(c, k, bytes) || on_cache(c, v, bytes)) return l3m_dev_fail("kv8_append: the rows overlap the cache");
+    const long long items = most_blocks(b) * 2 * c->nkv;
+    if (items > 1ll << 28) return l3m_dev_fail("kv8_append: too many rows for one call");
+    const RowsIn a = {*c, runs_of(b), k, v, nullptr, nullptr, stride, p->table, p->len, p->state, layer, p->pages, p->seqs, p->width};
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
+    const dim3 grid((unsigned)((items + 3) / 4));
+#define APPEND(NB)                                                                      \
+    if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_append<float, NB>), grid, dim3(256), 0, st, a); \
+    else hipLaunchKernelGGL((k_kv8_append<uint16_t, NB>), grid, dim3(256), 0, st, a)
+    BY_BLOCKS(APPEND)
+    return l3m_dev_launched("k_kv8_append");
+}
+
+int l3m_k_kv8_rows(const l3m_kv8 *c, const l3m_pages *p, int layer, float *k, float *v, const l3m_batch *b, void *stream) {
+    if (const char *why = call_bad(c, p, layer, b)) return l3m_dev_fail(why);
+    if ((!k && !v) || ((uintptr_t)k | (uintptr_t)v) % 4) return l3m_dev_fail("kv8_rows: no output, or one that is not 4-byte aligned");
+    if (!b->seqs || !b->n) return 0;
+    const size_t bytes = 4 * (size_t)b->n * c->nkv * c->hd;
+    if (overlap(k, bytes, v, bytes)) return l3m_dev_fail("kv8_rows: k overlaps v");
+    if (on_cache(c, k, bytes) || on_cache(c, v, bytes) || on_pages(p, k, bytes) || on_pages(p, v, bytes) || on_batch(b, k, bytes) || on_batch(b, v, bytes))
+        return l3m_dev_fail("kv8_rows: k or v overlaps the cache, the tables or the batch");
+    const long long items = most_blocks(b) * 2 * c->nkv;
+    if (items > 1ll << 28) return l3m_dev_fail("kv8_rows: too many rows for one call");
+    const RowsIn a = {*c, runs_of(b), nullptr, nullptr, k, v, 0, p->table, p->len, p->state, layer, p->pages, p->seqs, p->width};
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
+    const dim3 grid((unsigned)((items + 3) / 4));
+#define ROWS(NB) hipLaunchKernelGGL((k_kv8_rows<NB>), grid, dim3(256), 0, st, a)
+    BY_BLOCKS(ROWS)
+    return l3m_dev_launched("k_kv8_rows");
+}
+
+size_t l3m_kv8_work_bytes(const l3m_kv8 *c, int n, int nq) {
+    if (kv8_bad(c) || n < 1 || n > 1 << 28 || nq < 1 || nq > 65536 || nq % c->nkv) return 0;
+    return 16;
+}
+
+int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int dtype, const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_batch *b, int nq,
+                     int longest, void *work, size_t work_bytes, void *stream) {
+    if (const char *why = call_bad(c, p, layer, b)) return l3m_dev_fail(why);
+    const size_t size = value_bytes(dtype);
+    if (!size) return l3m_dev_fail("kv8_attend: queries and outputs are f32 or bf16");
+    if (nq < 1 || nq > 65536 || nq % c->nkv) return l3m_dev_fail("kv8_attend: query heads must be a multiple of the kv heads");
+    const long long width = (long long)nq * c->hd;
+    if (q_stride < width || out_stride < width) return l3m_dev_fail("kv8_attend: a row holds fewer values than its heads");
+    if (longest < 0) return l3m_dev_fail("kv8_attend: a negative length");
+    if (!b->seqs || !b->n) return 0;
+    if (!out || !q || ((uintptr_t)out | (uintptr_t)q) % size) return l3m_dev_fail("kv8_attend: no queries or output, or not aligned to their values");
+    const size_t qb = rows_bytes(b->n, q_stride, width, size), ob = rows_bytes(b->n, out_stride, width, size), need = l3m_kv8_work_bytes(c, b->n, nq);
+    if (!(out == q && out_stride == q_stride) && overlap(out, ob, q, qb)) return l3m_dev_fail("kv8_attend: q and out must be the same or apart");
+    if (!work || (uintptr_t)work % 16 || work_bytes < need) return l3m_dev_fail("kv8_attend: the workspace is too small (l3m_kv8_work_bytes) or not 16-byte aligned");
+    if (overlap(work, need, q, qb) || overlap(work, need, out, ob)) return l3m_dev_fail("kv8_attend: the workspace overlaps q or out");
+    if (on_cache(c, out, ob) || on_cache(c, work, need) || on_pages(p, out, ob) || on_pages(p, work, need) || on_batch(b, out, ob) || on_batch(b, work, need))
+        return l3m_dev_fail("kv8_attend: out or the workspace overlaps the cache, the tables or the batch");
+    const int g = nq / c->nkv;
+    if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
+    const long long groups = ((long long)b->n * g + 15) / 16 + b->seqs;
+    if (groups * c->nkv > 1ll << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
+    const AttendIn a = {*c, runs_of(b), q, out, q_stride, out_stride, p->table, p->len, p->state, (float *)work, layer, p->pages, p->seqs, p->width, nq, g,
+                        multiplier(g, (uint64_t)b->n * g)};
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
+    const dim3 grid((unsigned)(groups * c->nkv));
+#define ATTEND(NB)                                                                      \
+    if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_attend<true, NB>), grid, dim3(64 * WAVES), 0, st, a); \
+    else hipLaunchKernelGGL((k_kv8_attend<false, NB>), grid, dim3(64 * WAVES), 0, st, a)
+    BY_BLOCKS(ATTEND)
+    return l3m_dev_launched("k_kv8_attend");
+}
+
+}

@@ -1,0 +1,273 @@
+// Causal attention over whole prompts for CDNA4 (gfx950): bf16 rows of many sequences packed one behind the other, grouped heads.
+//
+// Rows: a kv head's (token, query head) pairs of a run, a token's heads side by side (g = nq / nkv); 32 to a wavefront. Per tile of 64 positions:
+//   S = K Q^T        32 positions x 32 rows (v_mfma_f32_32x32x16_bf16), twice. The operand's rows are K's positions with bits 2 and 3 exchanged, so that a
+//                    lane holds the scores of its row for eight positions in a row, which is what the next product wants of it: no value crosses lanes
+//   P = 2^(S - m)    m moves only where a score passes it by 8: weights up to 2^8, and the sums are seldom scaled. Rounded to bf16
+//   O^T += V^T P^T   32 dimensions x 32 rows x 16 positions, V read from LDS transposed (ds_read_b64_tr_b16)
+// K's and V's tiles go from memory to LDS directly, 16 bytes a lane, in an order of pieces within a row by which no read meets a bank twice.
+#include "serve.h"
+
+namespace {
+
+constexpr int TILE = 64, ROWS = 32, WAVES = 4;
+constexpr float M0 = -3.40282347e38f;                                // the maximum of no score: float32's lowest
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+#define LOCAL __attribute__((address_space(3)))
+#define GLOBAL __attribute__((address_space(1)))
+
+struct PromptIn {
+    const uint16_t *q, *k, *v;
+    uint16_t       *out;
+    Runs            b;
+    long long       q_stride, kv_stride, out_stride;
+    int             nq, nkv, hd, g;
+    uint32_t        g_mul;
+};
+
+// Values of a row in LDS, a power of two; pieces of 16 bytes.
+__host__ __device__ constexpr int row_values(int nb) { return nb <= 1 ? 32 : nb <= 2 ? 64 : nb <= 4 ? 128 : 256; }
+// Where a row's piece lies in it: K by rows read side by side, V by pairs of pieces, of rows r .. r + 3 and r + 8 .. r + 11.
+template <int PIECES> __device__ __forceinline__ int k_turn(int row) { return PIECES >= 16 ? row & 15 : PIECES == 8 ? row >> 1 & 7 : row >> 2 & 3; }
+template <int PIECES> __device__ __forceinline__ int v_turn(int row) {
+    return PIECES >= 16 ? (row & 3) | (row >> 1 & 4) : PIECES == 8 ? (row >> 1 & 1) | (row >> 2 & 2) : 0;
+}
+__device__ __forceinline__ float other_half(float x, float &y) {     // lane ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    y = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+
+// Positions tile .. of a run's K and V into LDS, by the whole workgroup; positions past the last one are the last one again, pieces past the head its last.
+template <int NB> __device__ __forceinline__ void load_tile(const PromptIn &a, const uint16_t *k, const uint16_t *v, int tile, int len, uint16_t *k_s, uint16_t *v_s) {
+    constexpr int RW = row_values(NB), PIECES = RW / 8, TURNS = TILE * PIECES / (64 * WAVES);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), last = (a.hd >> 3) - 1;
+#pragma unroll
+    for (int i = 0; i < TURNS; i++) {
+        const int at0 = 64 * (i * WAVES + wave), at = at0 + lane, row = at / PIECES, slot = at % PIECES;
+        const long long from = (long long)min(tile + row, len - 1) * a.kv_stride;
+        const int kp = slot ^ k_turn<PIECES>(row), vp = slot ^ v_turn<PIECES>(row) << 1;
+        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(k + from + 8 * min(kp, last)), (LOCAL void *)(k_s + 8 * at0), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(v + from + 8 * min(vp, last)), (LOCAL void *)(v_s + 8 * at0), 16, 0, 0);
+    }
+}
+__device__ __forceinline__ void loads_done() {                       // and the workgroup's
+    __builtin_amdgcn_s_waitcnt(0x0F70);                              // vmcnt(0)
+    __syncthreads();
+}
+
+// One row by the formula, a position at a time: for rows whose products met a value that is not finite behind their token.
+__device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *k, const uint16_t *v, int seen, uint16_t *out) {
+    const int lane = threadIdx.x & 63;
+    float qv[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) qv[i] = lane + 64 * i < a.hd ? bf16_float(q[lane + 64 * i]) : 0.f;
+    const float scale = 1.44269504f / sqrtf((float)a.hd);
+    for (int p = 0; p < seen; p++) {
+        float s = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) s += lane + 64 * i < a.hd ? qv[i] * bf16_float(k[(long long)p * a.kv_stride + lane + 64 * i]) : 0.f;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+        s *= scale;
+        const float top = fmaxf(m, s), by = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top), e = __builtin_amdgcn_exp2f(s - top);
+        l = l * by + e;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = o[i] * by + (lane + 64 * i < a.hd ? e * bf16_float(v[(long long)p * a.kv_stride + lane + 64 * i]) : 0.f);
+        m = top;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (lane + 64 * i < a.hd) out[lane + 64 * i] = (uint16_t)bf16_pair(o[i] / l, 0.f);
+}
+
+template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(PromptIn a) {
+    constexpr int RW = row_values(NB), PIECES = RW / 8;
+    __shared__ __align__(16) uint16_t k_s[TILE * RW], v_s[TILE * RW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, c = lane >> 5, hd = a.hd, g = a.g;
+    const int h = (int)(blockIdx.x % (unsigned)a.nkv), item = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)a.nkv);
+    const Found f = find_run(a.b, item, [&](int, int, int rows) { return (int)(((unsigned)rows * g + ROWS * WAVES - 1) / (ROWS * WAVES)); });
+    if (f.run < 0) return;
+    const uint16_t *q = a.q + (long long)f.s0 * a.q_stride, *k = a.k + (long long)f.s0 * a.kv_stride + h * hd, *v = a.v + (long long)f.s0 * a.kv_stride + h * hd;
+    uint16_t *out = a.out + (long long)f.s0 * a.out_stride;
+    const int R = f.rows * g, first = f.at * ROWS * WAVES, row0 = first + wave * ROWS;
+    const int tiles = (int)divide(min(first + ROWS * WAVES, R) - 1, g, a.g_mul) / TILE + 1;      // of the workgroup
+    const int rows = clamp(R - row0, 0, ROWS), row = row0 + min(r32, max(rows, 1) - 1);
+    const int token = rows ? (int)divide(row, g, a.g_mul) : 0, head = rows ? h * g + row - token * g : 0;
+    const int low = rows ? (int)divide(row0, g, a.g_mul) : 0, high = rows ? (int)divide(row0 + rows - 1, g, a.g_mul) : -1;   // the wavefront's tokens
+    const uint16_t *my_q = q + (long long)token * a.q_stride + (long long)head * hd;
+    bf16x8 qs[2 * NB];
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) {
+        const int d = 16 * i + 8 * c;
+        u32x4 x = *(const u32x4 *)(my_q + (d < hd ? d : 0));
+        if (d >= hd) x = u32x4{0, 0, 0, 0};
+        qs[i] = __builtin_bit_cast(bf16x8, x);
+    }
+    const float scale = 1.44269504f / sqrtf((float)hd);              // of the scores: base 2
+    f32x16 acc[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
+    float m = M0, l = 0.f;
+
+    for (int tile = 0; tile < tiles; tile++) {
+        __syncthreads();
+        load_tile<NB>(a, k, v, tile * TILE, f.rows, k_s, v_s);
+        loads_done();
+        if (tile * TILE > high) continue;
+        f32x16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[b][j] = 0.f;
+            const int at = 32 * b + (r32 & 19) + (r32 & 4) * 2 + (r32 & 8) / 2;       // bits 2 and 3 exchanged
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                const bf16x8 kx = *(const bf16x8 *)(k_s + at * RW + 8 * ((2 * i + c) ^ k_turn<PIECES>(at)));
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kx, qs[i], s[b], 0, 0, 0);
+            }
+        }
+        // s[b][8 j + e]: position 32 b + 16 j + 8 c + e
+        if (tile * TILE + TILE - 1 > low)
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[b][j] = tile * TILE + 32 * b + 16 * (j >> 3) + 8 * c + (j & 7) <= token ? s[b][j] : -INFINITY;
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) top = fmaxf(top, s[b][j]);
+        float y;
+        top = other_half(top, y);
+        top = fmaxf(top, y) * scale;
+        if (__ballot(top > m + 8.f)) {
+            const float to = top > m + 8.f ? top : m, by = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to);
+            l *= by;
+#pragma unroll
+            for (int i = 0; i < NB; i++) acc[i] *= by;
+            m = to;
+        }
+        bf16x8 p[2][2];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x0 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e], scale, -m)), x1 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e + 1], scale, -m));
+                    l += x0 + x1;
+                    w[e] = bf16_pair(x0, x1);
+                }
+                p[b][j] = __builtin_bit_cast(bf16x8, w);
+            }
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    // lane (c, d): positions 8 c .. + 7 of dimension d, four at a time of 16 dimensions by 16 lanes
+                    s16x4 x[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const int at = 32 * b + 16 * j + 8 * c + 4 * u + (lane >> 2 & 3), pair = 2 * i + (lane >> 4 & 1);
+                        x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LOCAL s16x4 *)(v_s + at * RW + 16 * (pair ^ v_turn<PIECES>(at)) + 4 * (lane & 3)));
+                    }
+                    typedef short s16x8 __attribute__((ext_vector_type(8)));
+                    const bf16x8 vx = __builtin_bit_cast(bf16x8, s16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]});
+                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vx, p[b][j], acc[i], 0, 0, 0);
+                }
+    }
+    if (!rows) return;
+    float y;
+    l = other_half(l, y);
+    l += y;
+    float bad = 0.f;                                                 // NaN where a value is not finite
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) bad = fmaf(acc[i][j], 0.f, bad);
+    const uint64_t lanes = __ballot(bad != bad);
+    uint32_t wrong = 0;                                              // rows that a value behind their token may have reached
+    for (uint32_t of = (uint32_t)lanes | (uint32_t)(lanes >> 32); of; of &= of - 1) {
+        const int r = __builtin_ctz(of), t = __builtin_amdgcn_readlane(token, r), upto = min((high / TILE + 1) * TILE, f.rows);
+        if (r >= rows) break;
+        bool some = false;
+        for (int at = lane; at < (upto - t - 1) * (hd >> 3); at += 64) {
+            const u32x4 x = *(const u32x4 *)(v + (long long)(t + 1 + at / (hd >> 3)) * a.kv_stride + 8 * (at % (hd >> 3)));
+#pragma unroll
+            for (int i = 0; i < 4; i++) some |= (x[i] & 0x7F80u) == 0x7F80u || (x[i] & 0x7F800000u) == 0x7F800000u;
+        }
+        if (__ballot(some)) wrong |= 1u << r;
+    }
+    for (uint32_t of = wrong; of; of &= of - 1) {
+        const int r = __builtin_ctz(of), t = __builtin_amdgcn_readlane(token, r), hh = __builtin_amdgcn_readlane(head, r);
+        row_alone(a, q + (long long)t * a.q_stride + (long long)hh * hd, k, v, t + 1, out + (long long)t * a.out_stride + (long long)hh * hd);
+    }
+    if (r32 >= rows || wrong >> r32 & 1u) return;
+    uint16_t *to = out + (long long)token * a.out_stride + (long long)head * hd;
+    const float by = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = 32 * i + 8 * j + 4 * c;
+            if (d < hd) *(u32x2 *)(to + d) = u32x2{bf16_pair(acc[i][4 * j] * by, acc[i][4 * j + 1] * by), bf16_pair(acc[i][4 * j + 2] * by, acc[i][4 * j + 3] * by)};
+        }
+}
+
+}  // namespace
+
+extern "C" {
+
+int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_stride, const uint16_t *k, const uint16_t *v, int kv_stride, const l3m_batch *b,
+                        int nq, int nkv, int hd, void *stream) {
+    if (const char *why = batch_bad(b)) return l3m_dev_fail(why);
+    if (hd < 8 || hd > 256 || hd % 8) return l3m_dev_fail("attend_packed: hd must be a multiple of 8 up to 256");
+    if (nkv < 1 || nkv > 4096 || nq < 1 || nq > 65536 || nq % nkv) return l3m_dev_fail("attend_packed: query heads must be a multiple of the kv heads");
+    const long long qw = (long long)nq * hd, kw = (long long)nkv * hd;
+    if (q_stride < qw || out_stride < qw || kv_stride < kw) return l3m_dev_fail("attend_packed: a row holds fewer values than its heads");
+    if (!b->seqs || !b->n) return 0;
+    if (!out || !q || !k || !v) return l3m_dev_fail("attend_packed: no rows, or no output");
+    if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8 || kv_stride % 8 || out_stride % 8)
+        return l3m_dev_fail("attend_packed: rows must be 16-byte aligned, strides multiples of 8 values");
+    const size_t ob = rows_bytes(b->n, out_stride, qw, 2), kb = rows_bytes(b->n, kv_stride, kw, 2);
+    if (!(out == q && out_stride == q_stride) && overlap(out, ob, q, rows_bytes(b->n, q_stride, qw, 2))) return l3m_dev_fail("attend_packed: q and out must be the same or apart");
+    // in a fused row k and v lie behind q, so out == q lies between them
+    auto apart = [&](const uint16_t *x) {
+        if (!overlap(out, ob, x, kb)) return true;
+        const long long gap = x - out;
+        return out_stride == kv_stride && (gap >= 0 ? gap >= qw && gap + kw <= kv_stride : -gap >= kw && qw - gap <= kv_stride);
+    };
+    if (!apart(k) || !apart(v)) return l3m_dev_fail("attend_packed: out overlaps k or v");
+    if (on_batch(b, out, ob)) return l3m_dev_fail("attend_packed: out overlaps the batch");
+    const int g = nq / nkv;
+    if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("attend_packed: too many rows for one call");
+    const long long items = (long long)b->n * g / (ROWS * WAVES) + b->seqs;
+    if (items * nkv > 1ll << 28) return l3m_dev_fail("attend_packed: too many rows for one call");
+    const PromptIn a = {q, k, v, out, {b->ids, b->starts, b->seqs, b->n}, q_stride, kv_stride, out_stride, nq, nkv, hd, g, multiplier(g, (uint64_t)b->n * g)};
+    hipStream_t st;
+    if (!stream_of(stream, st)) return -1;
+    const dim3 grid((unsigned)(items * nkv)), wg(64 * WAVES);
+#define ATTEND(NB) hipLaunchKernelGGL((k_attend_packed<NB>), grid, wg, 0, st, a)
+    switch ((hd + 31) / 32) {
+    case 1: ATTEND(1); break;
+    case 2: ATTEND(2); break;
+    case 3: ATTEND(3); break;
+    case 4: ATTEND(4); break;
+    case 5: ATTEND(5); break;
+    case 6: ATTEND(6); break;
+    case 7: ATTEND(7); break;
+    default: ATTEND(8); break;
+    }
+#undef ATTEND
+    return l3m_dev_launched("k_attend_packed");
+}
+
+}
