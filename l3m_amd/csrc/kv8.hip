@@ -8,6 +8,7 @@
 namespace {
 
 constexpr int WAVES = 4;
+constexpr int TILE = 64;                                             // positions that a wavefront takes at once
 constexpr int E4M3_NAN = 0x7F;
 constexpr float M0 = -3.40282347e38f;                                // the maximum of no score: float32's lowest
 
@@ -185,13 +186,12 @@ template <int NB> __global__ void __launch_bounds__(256) k_kv8_rows(RowsIn a) {
 }
 
 // ---------------------------------------------------------------- attention
-// Rows: a kv head's (token, query head) pairs of a run, a token's heads side by side (g = nq / nkv), 16 to a product. Per tile, a page, and wavefront, codes
-// converted to bf16 as they are used, exactly, their scale with them (v_cvt_scalef32_pk_bf16_fp8):
+// Rows: a kv head's (token, query head) pairs of a run, a token's heads side by side (g = nq / nkv), 16 to a product. Per tile, half a page, and wavefront,
+// codes converted to bf16 as they are used, exactly, their scale with them (v_cvt_scalef32_pk_bf16_fp8):
 //   S = K Q^T        16 positions x 16 rows x 32 dimensions (v_mfma_f32_16x16x32_bf16), q in PARTS of bf16
 //   P = 2^(S - m)    m the running maximum
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions, P in PARTS of bf16
-// A lane of group c reads 16 bytes at once, which are two products' eight columns: the dimensions 64 f + 16 c .. of K and of q, the positions 64 u + 16 c .. of
-// V. K's rows are taken in the order in which a lane then holds the scores of those positions, so no value crosses lanes. All sums in 32 bits; q and P in three
+// A lane of group c reads 16 bytes at once, which are two products' eight columns: the dimensions 64 f + 16 c .. of K and of q, the positions 16 c .. of V. K's rows are taken in the order in which a lane then holds the scores of those positions, so no value crosses lanes. All sums in 32 bits; q and P in three
 // parts are float32's 24 bits; for bf16 rows q is one part, exactly, and P two, 2^-16 of a weight at the most.
 // (v_mfma_scale_f32_16x16x128_f8f6f4 takes the codes as they lie, but aligns a product's 128 terms to the largest one: sums were off by 2^-11 of that.)
 template <bool F32> struct Parts {
@@ -252,6 +252,11 @@ template <int N> __device__ __forceinline__ void in_parts(const float (&v)[8], b
     }
 }
 
+// Splitting. Per kv head the runs' groups of 16 rows over all their tiles are the work; a group over more than `chunk` tiles is split over as many workgroups as
+// have a chunk each, all nearly equal, and their parts are joined by a second launch. The lengths lie in device memory, so each workgroup counts the work and
+// finds its share of it by itself (share_of), the same in both launches.
+constexpr int SPLIT_ROWS = 1 << 14;
+constexpr int TARGET = 512, CHUNK_MIN = WAVES;                       // workgroups that the work is spread over; tiles that a workgroup takes at the least
 struct AttendIn {
     l3m_kv8     c;
     Runs        b;
@@ -259,11 +264,62 @@ struct AttendIn {
     void       *out;
     long long   q_stride, out_stride;
     const int32_t *table, *len, *state;
-    float      *work;
-    int         layer, pages, seqs, width, nq, g;
+    float      *ml, *parts;                                          // [slot][row] maximum and sum, output; a slot's rows: slot_rows
+    int         layer, pages, seqs, width, nq, g, target, slot_rows; // target: workgroups of a kv head, 0: nothing is split
     uint32_t    g_mul;
 };
 __device__ __forceinline__ int length_of(const AttendIn &a, int id) { return (unsigned)id < (unsigned)a.seqs ? clamp(a.len[id], 0, a.width * PAGE) : 0; }
+__device__ __forceinline__ int groups_of(int rows, int g) { return (int)(((unsigned)rows * (unsigned)g + 15) >> 4); }
+__device__ __forceinline__ int tiles_of(int len) { return (len + TILE - 1) / TILE; }
+
+// A workgroup's share: of run `run`, id its sequence, of len positions, rows s0 ..; row group `group`, part `part` of `parts`, whose first one's slot is `slot`.
+struct Share {
+    int run, id, len, s0, rows, group, part, parts, slot;
+};
+// The item-th share of a kv head's work, or, rows being asked for (ROW), the first share of the group that row `item` of the buffers times g is in. run < 0: none. By a
+// whole wavefront, 64 runs at a time; the first 64 are read once.
+template <bool ROW> __device__ __forceinline__ Share share_of(const AttendIn &a, int item) {
+    const int lane = threadIdx.x & 63;
+    auto read = [&](int r0, int &id, int &len, int &s0, int &rows) {
+        const int r = r0 + lane;
+        id = len = s0 = rows = 0;
+        if (r < a.b.seqs) {
+            id = a.b.id(r);
+            s0 = a.b.from(r);
+            rows = a.b.to(r, s0) - s0;
+            len = length_of(a, id);
+            id = (unsigned)id < (unsigned)a.seqs ? id : 0;           // none: no position of any
+        }
+    };
+    int id, len, s0, rows, chunk = 1 << 30;
+    read(0, id, len, s0, rows);
+    if (a.target) {
+        long long work = 0;
+        for (int r0 = 0;; r0 += 64) {
+            int i = id, n = len, s = s0, m = rows;
+            if (r0) read(r0, i, n, s, m);
+            work += (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)((unsigned)groups_of(m, a.g) * (unsigned)tiles_of(n))), 63);
+            if (r0 + 64 >= a.b.seqs) break;
+        }
+        chunk = max(CHUNK_MIN, (int)((work + a.target - 1) / a.target));
+    }
+    int base = 0, slots = 0;
+    for (int r0 = 0; r0 < a.b.seqs; r0 += 64) {
+        if (r0) read(r0, id, len, s0, rows);
+        const int groups = groups_of(rows, a.g), parts = max((tiles_of(len) + chunk - 1) / chunk, 1), mine = groups * parts;
+        const int upto = scan_wave(mine) + base, slot = scan_wave(parts > 1 ? mine : 0) + slots;
+        const uint64_t here = ROW ? __ballot(item >= s0 && item < s0 + rows) : __ballot(upto > item);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            const int n = of(parts), first = of(upto) - of(mine), at = ROW ? (int)((unsigned)(item - of(s0)) * a.g >> 4) * n : item - first, group = (int)((unsigned)at / (unsigned)n);
+            return {r0 + l, of(id), of(len), of(s0), of(rows), group, at - group * n, n, of(slot) - of(parts > 1 ? mine : 0) + group * n};
+        }
+        base = __builtin_amdgcn_readlane(upto, 63);
+        slots = __builtin_amdgcn_readlane(slot, 63);
+    }
+    return {-1, 0, 0, 0, 0, 0, 0, 1, 0};
+}
 
 // Products' columns over a row's dimensions: step s holds a lane's dimensions dim_of(s, c) .. + 7.
 template <int NB> __device__ __forceinline__ int dim_of(int s, int c) { return s / 2 * 2 + 1 < NB ? 64 * (s >> 1) + 16 * c + 8 * (s & 1) : 32 * s + 8 * c; }
@@ -284,36 +340,76 @@ template <bool F32, int NB> struct Queries {
         }
     }
 };
-// The scores' products of a tile, t = 4 u + 2 e + f, element i of lane group c: position 64 u + 16 c + 8 e + 4 f + i. So row m of the operand is
-__device__ __forceinline__ int position_of(int t, int m) { return 64 * (t >> 2) + 16 * (m >> 2) + 4 * (t & 3) + (m & 3); }
+// The scores' products of a tile, t of them, element i of lane group c: position 16 c + 4 t + i. So row m of the operand is
+__device__ __forceinline__ int position_of(int t, int m) { return 16 * (m >> 2) + 4 * t + (m & 3); }
 template <int NB> struct KeysIn {
-    u32x2 w[NB];
-    __device__ __forceinline__ void load(const uint8_t *k, int t, int lane) {
-        const uint8_t *row = k + position_of(t, lane & 15) * (32 * NB);
+    u32x2 w[4][NB];
+    __device__ __forceinline__ void load(const uint8_t *k, int lane) {
         const int c = lane >> 4;
 #pragma unroll
-        for (int s = 0; s + 1 < NB; s += 2) {
-            const u32x4 x = *(const u32x4 *)(row + 32 * s + 16 * c);
-            w[s] = u32x2{x.x, x.y};
-            w[s + 1] = u32x2{x.z, x.w};
+        for (int t = 0; t < 4; t++) {
+            const uint8_t *row = k + position_of(t, lane & 15) * (32 * NB);
+#pragma unroll
+            for (int s = 0; s + 1 < NB; s += 2) {
+                const u32x4 x = *(const u32x4 *)(row + 32 * s + 16 * c);
+                w[t][s] = u32x2{x.x, x.y};
+                w[t][s + 1] = u32x2{x.z, x.w};
+            }
+            if constexpr (NB % 2) w[t][NB - 1] = *(const u32x2 *)(row + 32 * (NB - 1) + 8 * c);
         }
-        if constexpr (NB % 2) w[NB - 1] = *(const u32x2 *)(row + 32 * (NB - 1) + 8 * c);
     }
 };
+// Four values of a result. NaN behind a failed call on the tables; a token before its sequence's first position sees nothing: zeros.
+template <bool F32> __device__ __forceinline__ void put_row(const AttendIn &a, long long at, f32x4 x, bool none) {
+    if (none) x = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (a.state[0]) x = f32x4{NAN, NAN, NAN, NAN};
+    if constexpr (F32) *(f32x4_a4 *)((float *)a.out + at) = x;
+    else {
+        typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+        *(u32x2_a2 *)((uint16_t *)a.out + at) = u32x2{bf16_pair(x.x, x.y), bf16_pair(x.z, x.w)};
+    }
+}
+// 32-bit words of bytes: those before position `end` of them that begin at `from`.
+__device__ __forceinline__ uint32_t bytes_before(int from, int end) {
+    const int n = end - from;
+    return n >= 4 ? ~0u : n <= 0 ? 0u : ~(~0u << 8 * n);
+}
 
 template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_attend(AttendIn a) {
     constexpr int QP = Parts<F32>::q, PP = Parts<F32>::p, HP = 32 * NB, OS = HP + 4;
     __shared__ float o_s[2][16][OS], m_s[WAVES][16], l_s[WAVES][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, c = lane >> 4, hd = a.c.hd, g = a.g;
+    // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
     const int h = (int)(blockIdx.x % (unsigned)a.c.nkv);
-    const Found f = find_run(a.b, (int)(blockIdx.x / (unsigned)a.c.nkv), [&](int, int, int rows) { return (rows * g + 15) >> 4; });
+    const Share f = share_of<false>(a, (int)(blockIdx.x / (unsigned)a.c.nkv));
     if (f.run < 0) return;
-    const int id = a.b.id(f.run), len = length_of(a, id), row0 = 16 * f.at, rows = min(f.rows * g - row0, 16);
-    const bool failed = a.state[0] != 0;
+    const int len = f.len, row0 = 16 * f.group, rows = min(f.rows * g - row0, 16);
     // the row of this lane's column: its token, and the positions it sees
     const int r = row0 + min(r16, rows - 1), token = (int)divide(r, g, a.g_mul), head = h * g + r - token * g, seen = max(len - f.rows + token + 1, 0);
-    const int last = (int)divide(row0 + rows - 1, g, a.g_mul), end = max(len - f.rows + last + 1, 0), tiles = (end + PAGE - 1) / PAGE;
-    const int whole = max(len - f.rows + (int)divide(row0, g, a.g_mul) + 1, 0) / PAGE;     // tiles that every row sees whole
+    const int last = (int)divide(row0 + rows - 1, g, a.g_mul), end = max(len - f.rows + last + 1, 0);
+    const int whole = max(len - f.rows + (int)divide(row0, g, a.g_mul) + 1, 0) / TILE;     // tiles that every row sees whole
+    // this part's tiles (of all the sequence's; the last ones may lie behind every row)
+    const int all = tiles_of(len), share = all / f.parts, more = all - share * f.parts, t0 = f.part * share + min(f.part, more);
+    const int t1 = min(t0 + share + (f.part < more), tiles_of(end));
+    const int32_t *table = a.table + (size_t)f.id * a.width;
+    int tile = t0 + wave;
+    // the pages of this tile and the next, one turn ahead of their use
+    auto page_of = [&](int t) { return __builtin_amdgcn_readfirstlane(table[min(t, max(t1 - 1, 0)) * TILE / PAGE]); };
+    struct Tile {                                                    // where a tile's K and V begin, its two blocks' exponents
+        const uint8_t *k, *v;
+        uint32_t ks, vs;
+        bool lost;
+    };
+    auto tile_at = [&](int t, int page) {
+        const int half = min(t, max(t1 - 1, 0)) & 1;
+        const bool lost = (unsigned)page >= (unsigned)a.pages;
+        const Unit u = unit_of(a.c, lost ? 0 : page, a.layer, h);
+        return Tile{u.k + half * TILE * HP, u.v + half * TILE, *(const uint16_t *)(u.s + 2 * half), *(const uint16_t *)(u.s + SCALES + 2 * half), lost};
+    };
+    KeysIn<NB> keys;
+    Tile u = tile_at(tile, page_of(tile));
+    int page = page_of(tile + WAVES);
+    keys.load(u.k, lane);
     Queries<F32, NB> qs;
     qs.load(a.q, (long long)(f.s0 + token) * a.q_stride + (long long)head * hd, hd, lane);
     const float scale = 1.44269504f / sqrtf((float)hd);             // of the scores: base 2
@@ -322,39 +418,42 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
 #pragma unroll
     for (int t = 0; t < 2 * NB; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = M0, l = 0.f;
-    for (int tile = wave; tile < tiles; tile += WAVES) {
-        const int page = __builtin_amdgcn_readfirstlane(a.table[(size_t)id * a.width + tile]);
-        const bool lost = (unsigned)page >= (unsigned)a.pages;
-        const Unit u = unit_of(a.c, lost ? 0 : page, a.layer, h);
-        const uint32_t ks = *(const uint32_t *)u.s, vs = *(const uint32_t *)(u.s + 4);
-        const int left = end - tile * PAGE;                          // positions that some row sees
-        const bool masked = tile >= whole;
-        float p[32];
+    for (; tile < t1; tile += WAVES) {
+        const bool lost = u.lost, masked = tile >= whole;
+        const int left = end - tile * TILE;                          // positions that some row sees
+        u32x4 v[2 * NB];
 #pragma unroll
-        for (int t = 0; t < 8; t++) {
-            KeysIn<NB> k;
-            k.load(u.k, t, lane);
-            if (lost)
+        for (int t = 0; t < 2 * NB; t++) v[t] = *(const u32x4 *)(u.v + (16 * t + r16) * PAGE + 16 * c);
+        if (lost)
 #pragma unroll
-                for (int i = 0; i < NB; i++) k.w[i] = u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
-            const float sk = pow2_byte((int)(ks >> 8 * (2 * (t >> 2) + (r16 >> 3)) & 255u));
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < NB; i++) keys.w[t][i] = u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
+        const float sk = pow2_byte((int)(u.ks >> 8 * (r16 >> 3) & 255u));
+        float p[16];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
             f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NB; i++) {
-                const bf16x8 x = widen(k.w[i], sk);
+                const bf16x8 x = widen(keys.w[t][i], sk);
 #pragma unroll
                 for (int q = QP - 1; q >= 0; q--) s = mfma(x, qs.part[i][q], s);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) p[4 * t + i] = s[i];
         }
-        const int p0 = tile * PAGE + 16 * c;                         // of p[i]: p0 + i, behind the first half 48 more
+        const float sv = 32 * (c >> 1) < left ? pow2_byte((int)(u.vs >> 8 * (c >> 1) & 255u)) : 1.f;   // 1: never written
+        u = tile_at(tile + WAVES, page);
+        keys.load(u.k, lane);
+        page = page_of(tile + 2 * WAVES);
+        const int p0 = tile * TILE + 16 * c;                         // of p[i]: p0 + i
         if (masked)
 #pragma unroll
-            for (int i = 0; i < 32; i++) p[i] = p0 + i + (i < 16 ? 0 : 48) < seen ? p[i] : -INFINITY;
+            for (int i = 0; i < 16; i++) p[i] = p0 + i < seen ? p[i] : -INFINITY;
         float top = p[0];
 #pragma unroll
-        for (int i = 1; i < 32; i++) top = fmaxf(top, p[i]);
+        for (int i = 1; i < 16; i++) top = fmaxf(top, p[i]);
         top = fmaxf(max_groups(top) * scale, m);
         if (__ballot(top > m)) {
             const float by = __builtin_amdgcn_exp2f(m - top);
@@ -363,9 +462,9 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
             for (int t = 0; t < 2 * NB; t++) acc[t] *= by;
             m = top;
         }
-        bf16x8 w[4][PP];                                             // by products: 64 u + 16 c + 8 e ..
+        bf16x8 w[2][PP];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+        for (int t = 0; t < 2; t++) {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -374,61 +473,41 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
             }
             in_parts<PP>(x, w[t]);
         }
-        u32x4 v[2 * NB][2];
-#pragma unroll
-        for (int t = 0; t < 2 * NB; t++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) v[t][j] = *(const u32x4 *)(u.v + (16 * t + r16) * PAGE + 64 * j + 16 * c);
-        float sv[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) sv[j] = 64 * j + 32 * (c >> 1) < left ? pow2_byte((int)(vs >> 8 * (2 * j + (c >> 1)) & 255u)) : 1.f;   // or never written
         uint32_t nan = 0;                                            // codes of NaN among the values that some row sees
         if (masked || lost)
 #pragma unroll
             for (int t = 0; t < 2 * NB; t++)
 #pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int n = left - (64 * j + 16 * c + 4 * i);
-                        const uint32_t x = lost ? 0x7F7F7F7Fu : v[t][j][i];
-                        v[t][j][i] = n >= 4 ? x : n <= 0 ? 0u : x & ~(~0u << 8 * n);
-                        nan |= ((v[t][j][i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                    }
-        auto product = [&](const u32x4 (&x)[2 * NB][2], f32x4 (&to)[2 * NB]) {
+                for (int i = 0; i < 4; i++) {
+                    v[t][i] = (lost ? 0x7F7F7F7Fu : v[t][i]) & bytes_before(16 * c + 4 * i, left);
+                    nan |= ((v[t][i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                }
+        if (!masked || !__ballot(nan != 0)) {
 #pragma unroll
             for (int t = 0; t < 2 * NB; t++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const u32x4 &y = x[t][j >> 1];
-                    const bf16x8 va = widen(j & 1 ? u32x2{y.z, y.w} : u32x2{y.x, y.y}, sv[j >> 1]);
+                for (int j = 0; j < 2; j++) {
+                    const bf16x8 x = widen(j ? u32x2{v[t].z, v[t].w} : u32x2{v[t].x, v[t].y}, sv);
 #pragma unroll
-                    for (int q = PP - 1; q >= 0; q--) to[t] = mfma(va, w[j][q], to[t]);
+                    for (int q = PP - 1; q >= 0; q--) acc[t] = mfma(x, w[j][q], acc[t]);
                 }
-        };
-        if (!masked || !__ballot(nan != 0)) product(v, acc);
-        else                                                         // a NaN is the rows' that see it: a token's rows at a time, over its own positions
+        } else                                                       // a NaN is the rows' that see it: a token's rows at a time, over its own positions
             for (int to = min(seen, end), at = __builtin_amdgcn_readfirstlane(to);;) {
-                u32x4 x[2 * NB][2];
-                f32x4 part[2 * NB];
 #pragma unroll
                 for (int t = 0; t < 2 * NB; t++) {
-                    part[t] = acc[t];
+                    f32x4 part = acc[t];
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    for (int j = 0; j < 2; j++) {
+                        const int from = 16 * c + 8 * j, upto = at - tile * TILE;
+                        const bf16x8 x = widen(u32x2{(j ? v[t].z : v[t].x) & bytes_before(from, upto), (j ? v[t].w : v[t].y) & bytes_before(from + 4, upto)}, sv);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int n = at - tile * PAGE - (64 * j + 16 * c + 4 * i);
-                            x[t][j][i] = n >= 4 ? v[t][j][i] : n <= 0 ? 0u : v[t][j][i] & ~(~0u << 8 * n);
-                        }
+                        for (int q = PP - 1; q >= 0; q--) part = mfma(x, w[j][q], part);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][i] = to == at ? part[i] : acc[t][i];
                 }
-                product(x, part);
-#pragma unroll
-                for (int t = 0; t < 2 * NB; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][i] = to == at ? part[t][i] : acc[t][i];
                 int next = INT_MAX;                                  // the next larger number of positions that a row sees
-                for (uint64_t more = __ballot(to > at); more; more &= more - 1) next = min(next, __builtin_amdgcn_readlane(to, __builtin_ctzll(more)));
+                for (uint64_t others = __ballot(to > at); others; others &= others - 1) next = min(next, __builtin_amdgcn_readlane(to, __builtin_ctzll(others)));
                 if (next == INT_MAX) break;
                 at = next;
             }
@@ -462,17 +541,49 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
         for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][row]);
 #pragma unroll
         for (int w = 0; w < WAVES; w++) sum = fmaf(l_s[w][row], __builtin_amdgcn_exp2f(m_s[w][row] - top), sum);
-        f32x4 x = *(const f32x4 *)&o_s[0][row][d] + *(const f32x4 *)&o_s[1][row][d];
-        const int t = (int)divide(row0 + row, g, a.g_mul), hh = h * g + row0 + row - t * g;
-        const bool none = len - f.rows + t < 0;                      // a token before its sequence's first position sees nothing
-        x = failed ? f32x4{NAN, NAN, NAN, NAN} : none ? f32x4{0.f, 0.f, 0.f, 0.f} : x / sum;
-        const long long at = (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d;
-        if constexpr (F32) *(f32x4_a4 *)((float *)a.out + at) = x;
-        else {
-            typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
-            *(u32x2_a2 *)((uint16_t *)a.out + at) = u32x2{bf16_pair(x.x, x.y), bf16_pair(x.z, x.w)};
+        const f32x4 x = *(const f32x4 *)&o_s[0][row][d] + *(const f32x4 *)&o_s[1][row][d];
+        if (f.parts > 1) {
+            const size_t to = ((size_t)(f.slot + f.part) * a.c.nkv + h) * a.slot_rows + row;
+            *(f32x4 *)(a.parts + to * hd + d) = x;
+            if (d == 0) *(f32x2 *)(a.ml + 2 * to) = f32x2{top, sum};
+            continue;
         }
+        const int t = (int)divide(row0 + row, g, a.g_mul), hh = h * g + row0 + row - t * g;
+        put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, x / sum, len - f.rows + t < 0);
     }
+}
+
+// The parts of a row that was split, a workgroup a (row of the buffers, query head): groups of hd / 4 lanes take every so many parts, and meet in LDS in a fixed order.
+template <bool F32> __global__ void __launch_bounds__(256) k_kv8_join(AttendIn a) {
+    __shared__ f32x4 o_s[256];
+    __shared__ float s_s[256];
+    const int row = (int)(blockIdx.x / (unsigned)a.nq), hh = (int)(blockIdx.x - (unsigned)row * a.nq), h = hh / a.g, tid = threadIdx.x, hd = a.c.hd;
+    const Share run = share_of<true>(a, row);
+    if (run.run < 0 || run.parts < 2) return;
+    const int r = (row - run.s0) * a.g + hh - h * a.g, group = r >> 4;                     // of the run's rows of this kv head
+    const int slot = run.slot + (group - run.group) * run.parts, quads = hd >> 2, mine = tid / quads, groups = 256 / quads, d = 4 * (tid - mine * quads);
+    auto at = [&](int part) { return ((size_t)(slot + part) * a.c.nkv + h) * a.slot_rows + (r & 15); };
+    float top = M0;
+    for (int i = tid & 63; i < run.parts; i += 64) top = fmaxf(top, a.ml[2 * at(i)]);
+    top = max_wave(top);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    if (mine < groups)
+        for (int i = mine; i < run.parts; i += groups) {
+            const f32x2 ml = *(const f32x2 *)(a.ml + 2 * at(i));
+            const float by = __builtin_amdgcn_exp2f(ml.x - top);
+            x += *(const f32x4 *)(a.parts + at(i) * hd + d) * by;
+            sum = fmaf(ml.y, by, sum);
+        }
+    o_s[tid] = x;
+    s_s[tid] = sum;
+    __syncthreads();
+    if (tid >= quads) return;
+    for (int i = 1; i < groups; i++) {
+        x += o_s[i * quads + tid];
+        sum += s_s[i * quads + tid];
+    }
+    put_row<F32>(a, (long long)row * a.out_stride + (long long)hh * hd + d, x / sum, run.len - run.rows + row - run.s0 < 0);
 }
 
 Runs runs_of(const l3m_batch *b) { return {b->ids, b->starts, b->seqs, b->n}; }
@@ -495,6 +606,10 @@ const char *call_bad(const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_
     case 7: CALL(7); break;                                                                                                                                    \
     default: CALL(8); break;                                                                                                                                   \
     }
+// A split group has more than one chunk, so all of them have at most twice the chunks of the work.
+int target_of(int nkv) { return nkv < TARGET ? TARGET / nkv : 1; }
+size_t slots(int nkv) { return 2 * (size_t)target_of(nkv) * nkv; }
+int slot_rows(int n, int g) { return (long long)n * g < 16 ? n * g : 16; }
 // Blocks of 32 positions that a batch's rows can lie in: a run of r rows in (r + 62) / 32 of them.
 long long most_blocks(const l3m_batch *b) { return b->n / BLOCK + 2ll * b->seqs; }
 
@@ -559,7 +674,7 @@ int l3m_k_kv8_rows(const l3m_kv8 *c, const l3m_pages *p, int layer, float *k, fl
 
 size_t l3m_kv8_work_bytes(const l3m_kv8 *c, int n, int nq) {
     if (kv8_bad(c) || n < 1 || n > 1 << 28 || nq < 1 || nq > 65536 || nq % c->nkv) return 0;
-    return 16;
+    return 4 * slots(c->nkv) * slot_rows(n, nq / c->nkv) * (c->hd + 2) + 16;
 }
 
 int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int dtype, const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_batch *b, int nq,
@@ -583,15 +698,24 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
     const long long groups = ((long long)b->n * g + 15) / 16 + b->seqs;
     if (groups * c->nkv > 1ll << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
-    const AttendIn a = {*c, runs_of(b), q, out, q_stride, out_stride, p->table, p->len, p->state, (float *)work, layer, p->pages, p->seqs, p->width, nq, g,
-                        multiplier(g, (uint64_t)b->n * g)};
+    // rows of many tokens fill the card by themselves, and a launch to join them would ask about every row
+    const bool split = (long long)b->n * nq <= SPLIT_ROWS && (longest == 0 ? (long long)p->width * PAGE : longest) > CHUNK_MIN * TILE;
+    const int per = slot_rows(b->n, g), target = split ? target_of(c->nkv) : 0;
+    float *ml = (float *)work;
+    const AttendIn a = {*c, runs_of(b), q, out, q_stride, out_stride, p->table, p->len, p->state, ml, ml + (2 * slots(c->nkv) * per + 3) / 4 * 4, layer, p->pages, p->seqs, p->width,
+                        nq, g, target, per, multiplier(g, (uint64_t)b->n * g)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
-    const dim3 grid((unsigned)(groups * c->nkv));
+    const dim3 grid((unsigned)((groups + target) * c->nkv));
 #define ATTEND(NB)                                                                      \
     if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_attend<true, NB>), grid, dim3(64 * WAVES), 0, st, a); \
     else hipLaunchKernelGGL((k_kv8_attend<false, NB>), grid, dim3(64 * WAVES), 0, st, a)
     BY_BLOCKS(ATTEND)
+    if (split) {
+        const dim3 rows((unsigned)(b->n * nq));
+        if (dtype == L3M_HIP_F32) hipLaunchKernelGGL(k_kv8_join<true>, rows, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(k_kv8_join<false>, rows, dim3(256), 0, st, a);
+    }
     return l3m_dev_launched("k_kv8_attend");
 }
 

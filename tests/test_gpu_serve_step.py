@@ -231,7 +231,7 @@ o = torch.zeros(4, 4 * 64, dtype=torch.bfloat16, device="cuda")
 starts = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
 mem = torch.zeros(lib.l3m_kv8_bytes(2, 1, 1, 64), dtype=torch.uint8, device="cuda")
 tab = torch.zeros(lib.l3m_pages_bytes(2, 1, 2), dtype=torch.uint8, device="cuda")
-work = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+work = torch.zeros(lib.l3m_kv8_work_bytes(C.byref(A.KV8(1 << 20, 2, 1, 1, 64)), 4, 4), dtype=torch.uint8, device="cuda")
 f = torch.zeros(4, 64, device="cuda")
 torch.cuda.synchronize()
 r, c, p, b = A.Rotary(), A.KV8(), A.Pages(), A.Batch(None, starts.data_ptr(), 1, 4)
