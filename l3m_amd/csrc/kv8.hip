@@ -3,11 +3,11 @@
 // Layout. A page's unit of a layer and kv head: K codes [128 positions][HP] and V codes [HP][128 positions], HP hd rounded up to 32 (zeros), so that a lane's
 // 16 bytes of either are columns of the matrix cores' operands as they lie. A block of 32 positions has one scale of a kv head's K and one of its V, a power
 // of two, which the conversion of the codes takes.
+#include <type_traits>
 #include "serve.h"
 
 namespace {
 
-constexpr int WAVES = 4;
 constexpr int TILE = 64;                                             // positions that a wavefront takes at once
 constexpr int E4M3_NAN = 0x7F;
 constexpr float M0 = -3.40282347e38f;                                // the maximum of no score: float32's lowest
@@ -255,8 +255,9 @@ template <int N> __device__ __forceinline__ void in_parts(const float (&v)[8], b
 // Splitting. Per kv head the runs' groups of 16 rows over all their tiles are the work; a group over more than `chunk` tiles is split over as many workgroups as
 // have a chunk each, all nearly equal, and their parts are joined by a second launch. The lengths lie in device memory, so each workgroup counts the work and
 // finds its share of it by itself (share_of), the same in both launches.
-constexpr int SPLIT_ROWS = 1 << 14;
-constexpr int TARGET = 512, CHUNK_MIN = WAVES;                       // workgroups that the work is spread over; tiles that a workgroup takes at the least
+constexpr int SPLIT_ROWS = 1 << 14, SPLIT_FROM = 1024;
+constexpr int WAVES = 4;
+constexpr int TARGET = 512;                                          // workgroups that the work is spread over
 struct AttendIn {
     l3m_kv8     c;
     Runs        b;
@@ -265,7 +266,7 @@ struct AttendIn {
     long long   q_stride, out_stride;
     const int32_t *table, *len, *state;
     float      *ml, *parts;                                          // [slot][row] maximum and sum, output; a slot's rows: slot_rows
-    int         layer, pages, seqs, width, nq, g, target, slot_rows; // target: workgroups of a kv head, 0: nothing is split
+    int         layer, pages, seqs, width, nq, g, target, least, slot_rows; // target: workgroups of a kv head, 0: nothing is split; least: tiles of a part
     uint32_t    g_mul;
 };
 __device__ __forceinline__ int length_of(const AttendIn &a, int id) { return (unsigned)id < (unsigned)a.seqs ? clamp(a.len[id], 0, a.width * PAGE) : 0; }
@@ -276,9 +277,9 @@ __device__ __forceinline__ int tiles_of(int len) { return (len + TILE - 1) / TIL
 struct Share {
     int run, id, len, s0, rows, group, part, parts, slot;
 };
-// The item-th share of a kv head's work, or, rows being asked for (ROW), the first share of the group that row `item` of the buffers times g is in. run < 0: none. By a
-// whole wavefront, 64 runs at a time; the first 64 are read once.
-template <bool ROW> __device__ __forceinline__ Share share_of(const AttendIn &a, int item) {
+// The item-th share of a kv head's work, or (GROUP) the first share of the item-th group of rows. run < 0: none. By a whole wavefront, 64 runs at a time; the first 64 are
+// read once.
+template <bool GROUP> __device__ __forceinline__ Share share_of(const AttendIn &a, int item) {
     const int lane = threadIdx.x & 63;
     auto read = [&](int r0, int &id, int &len, int &s0, int &rows) {
         const int r = r0 + lane;
@@ -301,19 +302,19 @@ template <bool ROW> __device__ __forceinline__ Share share_of(const AttendIn &a,
             work += (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)((unsigned)groups_of(m, a.g) * (unsigned)tiles_of(n))), 63);
             if (r0 + 64 >= a.b.seqs) break;
         }
-        chunk = max(CHUNK_MIN, (int)((work + a.target - 1) / a.target));
+        chunk = max(a.least, (int)((work + a.target - 1) / a.target));
     }
     int base = 0, slots = 0;
     for (int r0 = 0; r0 < a.b.seqs; r0 += 64) {
         if (r0) read(r0, id, len, s0, rows);
         const int groups = groups_of(rows, a.g), parts = max((tiles_of(len) + chunk - 1) / chunk, 1), mine = groups * parts;
-        const int upto = scan_wave(mine) + base, slot = scan_wave(parts > 1 ? mine : 0) + slots;
-        const uint64_t here = ROW ? __ballot(item >= s0 && item < s0 + rows) : __ballot(upto > item);
+        const int upto = scan_wave(GROUP ? groups : mine) + base, slot = scan_wave(parts > 1 ? mine : 0) + slots;
+        const uint64_t here = __ballot(upto > item);
         if (here) {
             const int l = __builtin_ctzll(here);
             auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-            const int n = of(parts), first = of(upto) - of(mine), at = ROW ? (int)((unsigned)(item - of(s0)) * a.g >> 4) * n : item - first, group = (int)((unsigned)at / (unsigned)n);
-            return {r0 + l, of(id), of(len), of(s0), of(rows), group, at - group * n, n, of(slot) - of(parts > 1 ? mine : 0) + group * n};
+            const int n = of(parts), at = item - (of(upto) - of(GROUP ? groups : mine)), group = GROUP ? at : (int)((unsigned)at / (unsigned)n);
+            return {r0 + l, of(id), of(len), of(s0), of(rows), group, GROUP ? 0 : at - group * n, n, of(slot) - of(parts > 1 ? mine : 0) + group * n};
         }
         base = __builtin_amdgcn_readlane(upto, 63);
         slots = __builtin_amdgcn_readlane(slot, 63);
@@ -339,26 +340,43 @@ template <bool F32, int NB> struct Queries {
             in_parts<QP>(x, part[s]);
         }
     }
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int s = 0; s < NB; s++)
+#pragma unroll
+            for (int p = 0; p < QP; p++) asm volatile("" : "+v"(part[s][p]));
+    }
 };
 // The scores' products of a tile, t of them, element i of lane group c: position 16 c + 4 t + i. So row m of the operand is
 __device__ __forceinline__ int position_of(int t, int m) { return 16 * (m >> 2) + 4 * t + (m & 3); }
-template <int NB> struct KeysIn {
-    u32x2 w[4][NB];
-    __device__ __forceinline__ void load(const uint8_t *k, int lane) {
-        const int c = lane >> 4;
+#define LOCAL __attribute__((address_space(3)))
+#define GLOBAL __attribute__((address_space(1)))
+#define CONSTANT __attribute__((address_space(4)))
+// A wavefront's tile in LDS, 64 rows of K (positions) of 32 NB bytes and 32 NB rows of V (dimensions) of 64, in pieces of 16 bytes, which memory gives in order: 64
+// lanes a KiB, where rows read as an operand takes them would be 64 lines. A row's pieces lie in an order of its own, by which a read of 16 rows
+// meets no bank more often than it must.
+template <int NB> __device__ __forceinline__ int k_turn(int row) {
+    return NB % 4 == 0 ? (row & 3) | (row >> 2 & 4) : NB % 2 == 0 ? (row >> 1 & 1) | (row >> 3 & 2) : row >> 2 & 1;
+}
+__device__ __forceinline__ int v_turn(int row) { return row >> 1 & 3; }
+template <int NB> __device__ __forceinline__ void request_k(const uint8_t *k, uint8_t *k_s, int lane) {
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const uint8_t *row = k + position_of(t, lane & 15) * (32 * NB);
-#pragma unroll
-            for (int s = 0; s + 1 < NB; s += 2) {
-                const u32x4 x = *(const u32x4 *)(row + 32 * s + 16 * c);
-                w[t][s] = u32x2{x.x, x.y};
-                w[t][s + 1] = u32x2{x.z, x.w};
-            }
-            if constexpr (NB % 2) w[t][NB - 1] = *(const u32x2 *)(row + 32 * (NB - 1) + 8 * c);
-        }
+    for (int i = 0; i < 2 * NB; i++) {
+        const int at = 64 * i + lane, row = at / (2 * NB), piece = (at - row * (2 * NB)) ^ k_turn<NB>(row);
+        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(k + row * (32 * NB) + 16 * piece), (LOCAL void *)(k_s + 1024 * i), 16, 0, 0);
     }
-};
+}
+template <int NB> __device__ __forceinline__ void request_v(const uint8_t *v, uint8_t *v_s, int lane) {
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) {
+        const int row = 16 * i + (lane >> 2), piece = (lane & 3) ^ v_turn(row);
+        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(v + row * PAGE + 16 * piece), (LOCAL void *)(v_s + 1024 * i), 16, 0, 0);
+    }
+}
+// All but the last N requests are done; all reads of LDS are.
+template <int N> __device__ __forceinline__ void requests_but() { __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14); }
+__device__ __forceinline__ void reads_done() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
 // Four values of a result. NaN behind a failed call on the tables; a token before its sequence's first position sees nothing: zeros.
 template <bool F32> __device__ __forceinline__ void put_row(const AttendIn &a, long long at, f32x4 x, bool none) {
     if (none) x = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -376,8 +394,11 @@ __device__ __forceinline__ uint32_t bytes_before(int from, int end) {
 }
 
 template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_attend(AttendIn a) {
-    constexpr int QP = Parts<F32>::q, PP = Parts<F32>::p, HP = 32 * NB, OS = HP + 4;
-    __shared__ float o_s[2][16][OS], m_s[WAVES][16], l_s[WAVES][16];
+    constexpr int QP = Parts<F32>::q, PP = Parts<F32>::p, HP = 32 * NB, OS = HP + 4, REQUESTS = 2 * NB;
+    __shared__ __align__(16) uint8_t k_s[WAVES][TILE * HP], v_s[WAVES][TILE * HP];
+    __shared__ float m_s[WAVES][16], l_s[WAVES][16];
+    static_assert(sizeof(k_s) + sizeof(v_s) >= 2 * 16 * OS * 4, "");
+    float (*o_s)[16][OS] = (float (*)[16][OS])k_s;                   // behind the tiles
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, c = lane >> 4, hd = a.c.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
     const int h = (int)(blockIdx.x % (unsigned)a.c.nkv);
@@ -391,27 +412,31 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     // this part's tiles (of all the sequence's; the last ones may lie behind every row)
     const int all = tiles_of(len), share = all / f.parts, more = all - share * f.parts, t0 = f.part * share + min(f.part, more);
     const int t1 = min(t0 + share + (f.part < more), tiles_of(end));
-    const int32_t *table = a.table + (size_t)f.id * a.width;
-    int tile = t0 + wave;
-    // the pages of this tile and the next, one turn ahead of their use
-    auto page_of = [&](int t) { return __builtin_amdgcn_readfirstlane(table[min(t, max(t1 - 1, 0)) * TILE / PAGE]); };
+    const CONSTANT int32_t *table = (const CONSTANT int32_t *)(a.table + (size_t)f.id * a.width);
+    // the pages' numbers come a turn ahead of their use
+    auto page_of = [&](int t) { return table[min(t, max(t1 - 1, 0)) * TILE / PAGE]; };
     struct Tile {                                                    // where a tile's K and V begin, its two blocks' exponents
         const uint8_t *k, *v;
-        uint32_t ks, vs;
+        const CONSTANT uint32_t *s;
+        int half;
         bool lost;
     };
     auto tile_at = [&](int t, int page) {
         const int half = min(t, max(t1 - 1, 0)) & 1;
         const bool lost = (unsigned)page >= (unsigned)a.pages;
         const Unit u = unit_of(a.c, lost ? 0 : page, a.layer, h);
-        return Tile{u.k + half * TILE * HP, u.v + half * TILE, *(const uint16_t *)(u.s + 2 * half), *(const uint16_t *)(u.s + SCALES + 2 * half), lost};
+        return Tile{u.k + half * TILE * HP, u.v + half * TILE, (const CONSTANT uint32_t *)u.s, half, lost};
     };
-    KeysIn<NB> keys;
-    Tile u = tile_at(tile, page_of(tile));
-    int page = page_of(tile + WAVES);
-    keys.load(u.k, lane);
+    int tile = t0 + wave;
     Queries<F32, NB> qs;
     qs.load(a.q, (long long)(f.s0 + token) * a.q_stride + (long long)head * hd, hd, lane);
+    Tile u = tile_at(tile, page_of(tile));
+    int page = page_of(tile + WAVES);
+    uint32_t ks = u.s[0], vs = u.s[1];
+    uint8_t *my_k = k_s[wave], *my_v = v_s[wave];
+    request_k<NB>(u.k, my_k, lane);
+    request_v<NB>(u.v, my_v, lane);
+    qs.arrived();                                                    // here, or the loop waits for all requests at its top
     const float scale = 1.44269504f / sqrtf((float)hd);             // of the scores: base 2
 
     f32x4 acc[2 * NB];
@@ -421,36 +446,46 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     for (; tile < t1; tile += WAVES) {
         const bool lost = u.lost, masked = tile >= whole;
         const int left = end - tile * TILE;                          // positions that some row sees
-        u32x4 v[2 * NB];
+        const float sk = pow2_byte((int)(ks >> (16 * u.half + 8 * (r16 >> 3)) & 255u));
+        const float sv = 32 * (c >> 1) < left ? pow2_byte((int)(vs >> (16 * u.half + 8 * (c >> 1)) & 255u)) : 1.f;   // 1: never written
+        requests_but<REQUESTS>();                                    // V's, which came behind K's
+        f32x4 s[4];
 #pragma unroll
-        for (int t = 0; t < 2 * NB; t++) v[t] = *(const u32x4 *)(u.v + (16 * t + r16) * PAGE + 16 * c);
-        if (lost)
+        for (int t = 0; t < 4; t++) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+        for (int i = 0; i < NB; i += 2)
 #pragma unroll
-                for (int i = 0; i < NB; i++) keys.w[t][i] = u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
-        const float sk = pow2_byte((int)(u.ks >> 8 * (r16 >> 3) & 255u));
-        float p[16];
+            for (int t = 0; t < 4; t++) {
+                const int row = position_of(t, r16);
+                const uint8_t *at = my_k + row * HP;
+                u32x2 w[2];
+                if (i + 1 < NB) {
+                    const u32x4 x = *(const u32x4 *)(at + 16 * ((2 * i + c) ^ k_turn<NB>(row)));
+                    w[0] = u32x2{x.x, x.y};
+                    w[1] = u32x2{x.z, x.w};
+                } else w[0] = *(const u32x2 *)(at + 16 * ((2 * i + (c >> 1)) ^ k_turn<NB>(row)) + 8 * (c & 1));
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 2; j++)
+                    if (i + j < NB) {
+                        const bf16x8 x = widen(w[j], sk);
 #pragma unroll
-            for (int i = 0; i < NB; i++) {
-                const bf16x8 x = widen(keys.w[t][i], sk);
-#pragma unroll
-                for (int q = QP - 1; q >= 0; q--) s = mfma(x, qs.part[i][q], s);
+                        for (int q = QP - 1; q >= 0; q--) s[t] = mfma(x, qs.part[i + j < NB ? i + j : 0][q], s[t]);
+                    }
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) p[4 * t + i] = s[i];
-        }
-        const float sv = 32 * (c >> 1) < left ? pow2_byte((int)(u.vs >> 8 * (c >> 1) & 255u)) : 1.f;   // 1: never written
         u = tile_at(tile + WAVES, page);
-        keys.load(u.k, lane);
+        reads_done();
+        request_k<NB>(u.k, my_k, lane);
+        __builtin_amdgcn_sched_barrier(0);                           // scalar loads are waited for with LDS's reads: not before them
+        ks = u.s[0];
+        vs = u.s[1];
         page = page_of(tile + 2 * WAVES);
+        float p[16];
         const int p0 = tile * TILE + 16 * c;                         // of p[i]: p0 + i
-        if (masked)
 #pragma unroll
-            for (int i = 0; i < 16; i++) p[i] = p0 + i < seen ? p[i] : -INFINITY;
+        for (int i = 0; i < 16; i++) p[i] = s[i >> 2][i & 3];
+        if (masked || lost)
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = p0 + i >= seen ? -INFINITY : lost ? NAN : p[i];
         float top = p[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) top = fmaxf(top, p[i]);
@@ -473,36 +508,37 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
             }
             in_parts<PP>(x, w[t]);
         }
-        uint32_t nan = 0;                                            // codes of NaN among the values that some row sees
-        if (masked || lost)
+        requests_but<REQUESTS>();                                    // the next K's, which came behind V's
+        auto values = [&](int t) { return *(const u32x4 *)(my_v + (16 * t + r16) * TILE + 16 * (c ^ v_turn(16 * t + r16))); };
+        // 16 dimensions' values of the positions before `upto` of the tile
+        auto product = [&](int t, f32x4 to, auto some, int upto) {
+            const u32x4 v = values(t);
 #pragma unroll
-            for (int t = 0; t < 2 * NB; t++)
+            for (int j = 0; j < 2; j++) {
+                u32x2 z = {v[2 * j], v[2 * j + 1]};
+                if constexpr (decltype(some)::value) z = u32x2{z.x & bytes_before(16 * c + 8 * j, upto), z.y & bytes_before(16 * c + 8 * j + 4, upto)};
+                const bf16x8 x = widen(z, sv);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    v[t][i] = (lost ? 0x7F7F7F7Fu : v[t][i]) & bytes_before(16 * c + 4 * i, left);
-                    nan |= ((v[t][i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                }
-        if (!masked || !__ballot(nan != 0)) {
+                for (int q = PP - 1; q >= 0; q--) to = mfma(x, w[j][q], to);
+            }
+            return to;
+        };
+        if (!masked) {
 #pragma unroll
-            for (int t = 0; t < 2 * NB; t++)
+            for (int t = 0; t < 2 * NB; t++) acc[t] = product(t, acc[t], std::false_type{}, 0);
+        } else {
+            uint32_t nan = 0;                                        // codes of NaN among the values that some row sees
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const bf16x8 x = widen(j ? u32x2{v[t].z, v[t].w} : u32x2{v[t].x, v[t].y}, sv);
+            for (int t = 0; t < 2 * NB; t++) {
+                const u32x4 v = values(t);
 #pragma unroll
-                    for (int q = PP - 1; q >= 0; q--) acc[t] = mfma(x, w[j][q], acc[t]);
-                }
-        } else                                                       // a NaN is the rows' that see it: a token's rows at a time, over its own positions
-            for (int to = min(seen, end), at = __builtin_amdgcn_readfirstlane(to);;) {
+                for (int i = 0; i < 4; i++) nan |= ((v[i] & bytes_before(16 * c + 4 * i, left) & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            }
+            const bool apart = __ballot(nan != 0) != 0;              // a NaN is the rows' that see it: a token's rows at a time, over its own positions
+            for (int to = apart ? min(seen, end) : end, at = __builtin_amdgcn_readfirstlane(to);;) {
 #pragma unroll
                 for (int t = 0; t < 2 * NB; t++) {
-                    f32x4 part = acc[t];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int from = 16 * c + 8 * j, upto = at - tile * TILE;
-                        const bf16x8 x = widen(u32x2{(j ? v[t].z : v[t].x) & bytes_before(from, upto), (j ? v[t].w : v[t].y) & bytes_before(from + 4, upto)}, sv);
-#pragma unroll
-                        for (int q = PP - 1; q >= 0; q--) part = mfma(x, w[j][q], part);
-                    }
+                    const f32x4 part = product(t, acc[t], std::true_type{}, at - tile * TILE);
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[t][i] = to == at ? part[i] : acc[t][i];
                 }
@@ -511,7 +547,11 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
                 if (next == INT_MAX) break;
                 at = next;
             }
+        }
+        reads_done();
+        request_v<NB>(u.v, my_v, lane);
     }
+    requests_but<0>();
 
     // the wavefronts' parts at their common maximum, two at a time
     l = sum_groups(l);
@@ -519,18 +559,18 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
         m_s[wave][r16] = m;
         l_s[wave][r16] = l;
     }
-    __syncthreads();
+    __syncthreads();                                                 // and the tiles are done with
     float most = m_s[0][r16];
 #pragma unroll
     for (int w = 1; w < WAVES; w++) most = fmaxf(most, m_s[w][r16]);
     const float by = __builtin_amdgcn_exp2f(m - most);
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-        if (wave >> 1 == half)
+    for (int turn = 0; turn < WAVES / 2; turn++) {
+        if (wave >> 1 == turn)
 #pragma unroll
             for (int t = 0; t < 2 * NB; t++) {
                 f32x4 &to = *(f32x4 *)&o_s[wave & 1][r16][16 * t + 4 * c];
-                to = half ? to + acc[t] * by : acc[t] * by;
+                to = turn ? to + acc[t] * by : acc[t] * by;
             }
         __syncthreads();
     }
@@ -553,37 +593,51 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     }
 }
 
-// The parts of a row that was split, a workgroup a (row of the buffers, query head): groups of hd / 4 lanes take every so many parts, and meet in LDS in a fixed order.
-template <bool F32> __global__ void __launch_bounds__(256) k_kv8_join(AttendIn a) {
-    __shared__ f32x4 o_s[256];
-    __shared__ float s_s[256];
-    const int row = (int)(blockIdx.x / (unsigned)a.nq), hh = (int)(blockIdx.x - (unsigned)row * a.nq), h = hh / a.g, tid = threadIdx.x, hd = a.c.hd;
-    const Share run = share_of<true>(a, row);
-    if (run.run < 0 || run.parts < 2) return;
-    const int r = (row - run.s0) * a.g + hh - h * a.g, group = r >> 4;                     // of the run's rows of this kv head
-    const int slot = run.slot + (group - run.group) * run.parts, quads = hd >> 2, mine = tid / quads, groups = 256 / quads, d = 4 * (tid - mine * quads);
-    auto at = [&](int part) { return ((size_t)(slot + part) * a.c.nkv + h) * a.slot_rows + (r & 15); };
-    float top = M0;
-    for (int i = tid & 63; i < run.parts; i += 64) top = fmaxf(top, a.ml[2 * at(i)]);
-    top = max_wave(top);
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    if (mine < groups)
-        for (int i = mine; i < run.parts; i += groups) {
-            const f32x2 ml = *(const f32x2 *)(a.ml + 2 * at(i));
+// The parts of a group of rows that was split, of one kv head, to a workgroup: a wavefront a row makes the parts' factors, while the first parts come; threads of one part
+// after the other meet in LDS in a fixed order.
+constexpr int JOIN = 1024, PARTS = 2 * TARGET;                       // most parts of a group: a chunk each, of at most TARGET, and the last
+template <bool F32> __global__ void __launch_bounds__(JOIN) k_kv8_join(AttendIn a) {
+    __shared__ f32x4 o_s[JOIN];
+    __shared__ float f_s[16][PARTS], sum_s[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, quads = hd >> 2, h = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const Share f = share_of<true>(a, (int)(blockIdx.x / (unsigned)a.c.nkv));
+    if (f.run < 0 || f.parts < 2) return;
+    const int rows = min(f.rows * a.g - 16 * f.group, 16), items = rows * quads, groups = JOIN / items, mine = tid / items, item = tid - mine * items, row = item / quads, d = 4 * (item - row * quads);
+    auto at = [&](int part, int r) { return ((size_t)(f.slot + part) * a.c.nkv + h) * a.slot_rows + r; };
+    f32x4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(mine + i * groups, f.parts - 1), row) * hd + d);
+    if (wave < rows) {
+        float top = M0, sum = 0.f;
+        for (int i = lane; i < f.parts; i += 64) top = fmaxf(top, a.ml[2 * at(i, wave)]);
+        top = max_wave(top);
+        for (int i = lane; i < f.parts; i += 64) {
+            const f32x2 ml = *(const f32x2 *)(a.ml + 2 * at(i, wave));
             const float by = __builtin_amdgcn_exp2f(ml.x - top);
-            x += *(const f32x4 *)(a.parts + at(i) * hd + d) * by;
+            f_s[wave][i] = by;
             sum = fmaf(ml.y, by, sum);
         }
-    o_s[tid] = x;
-    s_s[tid] = sum;
-    __syncthreads();
-    if (tid >= quads) return;
-    for (int i = 1; i < groups; i++) {
-        x += o_s[i * quads + tid];
-        sum += s_s[i * quads + tid];
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
+        if (lane == 0) sum_s[wave] = sum;
     }
-    put_row<F32>(a, (long long)row * a.out_stride + (long long)hh * hd + d, x / sum, run.len - run.rows + row - run.s0 < 0);
+    __syncthreads();
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (mine < groups)
+        for (int p = mine; p < f.parts; p += 8 * groups) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (p + i * groups < f.parts) o += x[i] * f_s[row][p + i * groups];
+            if (p + 8 * groups < f.parts)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(p + (8 + i) * groups, f.parts - 1), row) * hd + d);
+        }
+    o_s[tid] = o;
+    __syncthreads();
+    if (tid >= items) return;
+    for (int i = 1; i < groups; i++) o += o_s[i * items + tid];
+    const int r = 16 * f.group + row, t = (int)divide(r, a.g, a.g_mul), hh = h * a.g + r - t * a.g;
+    put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, o / sum_s[row], f.len - f.rows + t < 0);
 }
 
 Runs runs_of(const l3m_batch *b) { return {b->ids, b->starts, b->seqs, b->n}; }
@@ -698,12 +752,12 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
     const long long groups = ((long long)b->n * g + 15) / 16 + b->seqs;
     if (groups * c->nkv > 1ll << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
-    // rows of many tokens fill the card by themselves, and a launch to join them would ask about every row
-    const bool split = (long long)b->n * nq <= SPLIT_ROWS && (longest == 0 ? (long long)p->width * PAGE : longest) > CHUNK_MIN * TILE;
+    // rows of many tokens fill the card by themselves
+    const bool split = (long long)b->n * nq <= SPLIT_ROWS && (longest == 0 ? (long long)p->width * PAGE : longest) > SPLIT_FROM;
     const int per = slot_rows(b->n, g), target = split ? target_of(c->nkv) : 0;
     float *ml = (float *)work;
     const AttendIn a = {*c, runs_of(b), q, out, q_stride, out_stride, p->table, p->len, p->state, ml, ml + (2 * slots(c->nkv) * per + 3) / 4 * 4, layer, p->pages, p->seqs, p->width,
-                        nq, g, target, per, multiplier(g, (uint64_t)b->n * g)};
+                        nq, g, target, WAVES, per, multiplier(g, (uint64_t)b->n * g)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
     const dim3 grid((unsigned)((groups + target) * c->nkv));
@@ -712,9 +766,9 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     else hipLaunchKernelGGL((k_kv8_attend<false, NB>), grid, dim3(64 * WAVES), 0, st, a)
     BY_BLOCKS(ATTEND)
     if (split) {
-        const dim3 rows((unsigned)(b->n * nq));
-        if (dtype == L3M_HIP_F32) hipLaunchKernelGGL(k_kv8_join<true>, rows, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(k_kv8_join<false>, rows, dim3(256), 0, st, a);
+        const dim3 all((unsigned)(groups * c->nkv));
+        if (dtype == L3M_HIP_F32) hipLaunchKernelGGL(k_kv8_join<true>, all, dim3(JOIN), 0, st, a);
+        else hipLaunchKernelGGL(k_kv8_join<false>, all, dim3(JOIN), 0, st, a);
     }
     return l3m_dev_launched("k_kv8_attend");
 }
