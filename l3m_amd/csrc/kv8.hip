@@ -295,19 +295,21 @@ template <bool GROUP> __device__ __forceinline__ Share share_of(const AttendIn &
     int id, len, s0, rows, chunk = 1 << 30;
     read(0, id, len, s0, rows);
     if (a.target) {
-        long long work = 0;
+        uint32_t work = 0;                                           // counted up to 2^31: more is no cache's
         for (int r0 = 0;; r0 += 64) {
             int i = id, n = len, s = s0, m = rows;
             if (r0) read(r0, i, n, s, m);
-            work += (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)((unsigned)groups_of(m, a.g) * (unsigned)tiles_of(n))), 63);
+            // a lane's at most 2^25, so that 64 of them are a sum
+            const uint32_t more = (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)min((unsigned long long)groups_of(m, a.g) * (unsigned)tiles_of(n), 1ull << 25)), 63);
+            work = min(work, 1u << 31) + min(more, (1u << 31) - 1);
             if (r0 + 64 >= a.b.seqs) break;
         }
-        chunk = max(a.least, (int)((work + a.target - 1) / a.target));
+        chunk = max(a.least, (int)((work - 1) / (unsigned)a.target) + 1);
     }
     int base = 0, slots = 0;
     for (int r0 = 0; r0 < a.b.seqs; r0 += 64) {
         if (r0) read(r0, id, len, s0, rows);
-        const int groups = groups_of(rows, a.g), parts = max((tiles_of(len) + chunk - 1) / chunk, 1), mine = groups * parts;
+        const int groups = groups_of(rows, a.g), parts = max((int)((unsigned)(tiles_of(len) + chunk - 1) / (unsigned)chunk), 1), mine = groups * parts;
         const int upto = scan_wave(GROUP ? groups : mine) + base, slot = scan_wave(parts > 1 ? mine : 0) + slots;
         const uint64_t here = __ballot(upto > item);
         if (here) {
@@ -595,49 +597,56 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
 
 // The parts of a group of rows that was split, of one kv head, to a workgroup: a wavefront a row makes the parts' factors, while the first parts come; threads of one part
 // after the other meet in LDS in a fixed order.
-constexpr int JOIN = 1024, PARTS = 2 * TARGET;                       // most parts of a group: a chunk each, of at most TARGET, and the last
-template <bool F32> __global__ void __launch_bounds__(JOIN) k_kv8_join(AttendIn a) {
+constexpr int PARTS = TARGET + 1;                       // most parts of a group: a chunk each, of at most TARGET, and the last
+template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join(AttendIn a) {
     __shared__ f32x4 o_s[JOIN];
     __shared__ float f_s[16][PARTS], sum_s[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, quads = hd >> 2, h = (int)(blockIdx.x % (unsigned)a.c.nkv);
     const Share f = share_of<true>(a, (int)(blockIdx.x / (unsigned)a.c.nkv));
     if (f.run < 0 || f.parts < 2) return;
-    const int rows = min(f.rows * a.g - 16 * f.group, 16), items = rows * quads, groups = JOIN / items, mine = tid / items, item = tid - mine * items, row = item / quads, d = 4 * (item - row * quads);
+    const int rows = min(f.rows * a.g - 16 * f.group, 16);
     auto at = [&](int part, int r) { return ((size_t)(f.slot + part) * a.c.nkv + h) * a.slot_rows + r; };
-    f32x4 x[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(mine + i * groups, f.parts - 1), row) * hd + d);
-    if (wave < rows) {
+    for (int r = wave; r < rows; r += JOIN / 64) {
         float top = M0, sum = 0.f;
-        for (int i = lane; i < f.parts; i += 64) top = fmaxf(top, a.ml[2 * at(i, wave)]);
+        for (int i = lane; i < f.parts; i += 64) top = fmaxf(top, a.ml[2 * at(i, r)]);
         top = max_wave(top);
         for (int i = lane; i < f.parts; i += 64) {
-            const f32x2 ml = *(const f32x2 *)(a.ml + 2 * at(i, wave));
+            const f32x2 ml = *(const f32x2 *)(a.ml + 2 * at(i, r));
             const float by = __builtin_amdgcn_exp2f(ml.x - top);
-            f_s[wave][i] = by;
+            f_s[r][i] = by;
             sum = fmaf(ml.y, by, sum);
         }
 #pragma unroll
         for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
-        if (lane == 0) sum_s[wave] = sum;
+        if (lane == 0) sum_s[r] = sum;
     }
-    __syncthreads();
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (mine < groups)
-        for (int p = mine; p < f.parts; p += 8 * groups) {
+    // threads by part, row and four dimensions; where the rows are more than the threads, in turns
+    const int items = min(rows * quads, JOIN), groups = JOIN / items, mine = tid / items, item = tid - mine * items;
+    for (int i0 = 0; i0 < rows * quads; i0 += items) {
+        const int all = min(i0 + item, rows * quads - 1), row = all / quads, d = 4 * (all - row * quads);
+        f32x4 x[8], o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (p + i * groups < f.parts) o += x[i] * f_s[row][p + i * groups];
-            if (p + 8 * groups < f.parts)
+        for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(mine + i * groups, f.parts - 1), row) * hd + d);
+        __syncthreads();                                             // the factors; the last turn's sums
+        if (mine < groups)
+            for (int p = mine; p < f.parts; p += 8 * groups) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(p + (8 + i) * groups, f.parts - 1), row) * hd + d);
+                for (int i = 0; i < 8; i++)
+                    if (p + i * groups < f.parts) o += x[i] * f_s[row][p + i * groups];
+                if (p + 8 * groups < f.parts)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(p + (8 + i) * groups, f.parts - 1), row) * hd + d);
+            }
+        if (groups > 1) {
+            o_s[tid] = o;
+            __syncthreads();
         }
-    o_s[tid] = o;
-    __syncthreads();
-    if (tid >= items) return;
-    for (int i = 1; i < groups; i++) o += o_s[i * items + tid];
-    const int r = 16 * f.group + row, t = (int)divide(r, a.g, a.g_mul), hh = h * a.g + r - t * a.g;
-    put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, o / sum_s[row], f.len - f.rows + t < 0);
+        if (mine == 0 && i0 + item < rows * quads) {
+            for (int i = 1; i < groups; i++) o += o_s[i * items + item];
+            const int r = 16 * f.group + row, t = (int)divide(r, a.g, a.g_mul), hh = h * a.g + r - t * a.g;
+            put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, o / sum_s[row], f.len - f.rows + t < 0);
+        }
+    }
 }
 
 Runs runs_of(const l3m_batch *b) { return {b->ids, b->starts, b->seqs, b->n}; }
@@ -767,8 +776,14 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     BY_BLOCKS(ATTEND)
     if (split) {
         const dim3 all((unsigned)(groups * c->nkv));
-        if (dtype == L3M_HIP_F32) hipLaunchKernelGGL(k_kv8_join<true>, all, dim3(JOIN), 0, st, a);
-        else hipLaunchKernelGGL(k_kv8_join<false>, all, dim3(JOIN), 0, st, a);
+#define JOINED(N)                                                                       \
+    if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_join<true, N>), all, dim3(N), 0, st, a); \
+    else hipLaunchKernelGGL((k_kv8_join<false, N>), all, dim3(N), 0, st, a)
+        if (groups * c->nkv < 128) {
+            JOINED(1024);
+        } else {
+            JOINED(256);
+        }
     }
     return l3m_dev_launched("k_kv8_attend");
 }

@@ -34,14 +34,16 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// Inclusive sum over the lanes of a wavefront.
+// Inclusive sum over the lanes of a wavefront: within rows of 16, then each row's last lane onto the row behind, and lane 31 onto the upper half. Lanes that
+// nothing comes to add 0.
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_or_0(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false); }
 __device__ __forceinline__ int scan_wave(int x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        x += lane >= d ? y : 0;
-    }
+    x += dpp_or_0<0x111, 0xF>(x);                                    // row_shr 1, 2, 4, 8
+    x += dpp_or_0<0x112, 0xF>(x);
+    x += dpp_or_0<0x114, 0xF>(x);
+    x += dpp_or_0<0x118, 0xF>(x);
+    x += dpp_or_0<0x142, 0xA>(x);                                    // row_bcast 15 into rows 1 and 3
+    x += dpp_or_0<0x143, 0xC>(x);                                    // row_bcast 31 into rows 2 and 3
     return x;
 }
 
