@@ -16,11 +16,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // ---------------------------------------------------------------- writer
 
-__device__ __forceinline__ float max_wave(float x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
-}
 // The exponent byte of a block by its largest finite magnitude: the smallest power of two, 2^-126 at least, by which it is at most 448 = 1.75 2^8.
 __device__ __forceinline__ int exponent_for(float most) {
     const uint32_t u = __float_as_uint(most);
@@ -46,6 +41,16 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float by) {
     return encode4(a.x, a.y, b.x, b.y, by);
 }
 __device__ __forceinline__ float pow2_byte(int e) { return __uint_as_float((uint32_t)e << 23); }   // 2^(e - 127), e 1 .. 254
+
+// Bytes i of four words as word i.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
 
 template <class T> __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
     if constexpr (sizeof(T) == 4) {
@@ -81,7 +86,7 @@ __device__ __forceinline__ int blocks_of(const RowsIn &a, int run, int rows) {
 template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(RowsIn a) {
     constexpr int HP = 32 * NB, PER = 4 * NB, IT = 2 * NB;           // eight values a lane: chunks of a row, turns for 32 rows
     __shared__ __align__(16) uint8_t code_s[4][BLOCK * (HP + 4)];
-    if (a.state[0]) return;                                          // a failed call on the tables: nothing is written
+    const int failed = a.state[0];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nkv = a.c.nkv;
     const int w = (int)(blockIdx.x * 4 + wave), per = 2 * nkv, item = w / per, which = w - item * per, h = which >> 1;
     const bool value = which & 1;
@@ -89,10 +94,7 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
     if (f.run < 0) return;
     const int id = a.b.id(f.run), len = length_of(a, id), first = len - f.rows, block = first / BLOCK + f.at;
     const int page = a.table[(size_t)id * a.width + block / SCALES];
-    if ((unsigned)page >= (unsigned)a.pages) return;
-    const Unit u = unit_of(a.c, page, a.layer, h);
     const int sub = block % SCALES, p0 = block * BLOCK, before = max(first - p0, 0), end = min(len - p0, BLOCK);
-    uint8_t *scale = u.s + (value ? SCALES : 0) + sub;
     const T *rows = (const T *)(value ? a.v : a.k) + (size_t)h * a.c.hd;
     float x[IT][8], most = 0.f;
 #pragma unroll
@@ -101,11 +103,29 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
 #pragma unroll
         for (int j = 0; j < 8; j++) x[i][j] = 0.f;
         if (r >= before && r < end && d < a.c.hd) load8(rows + (long long)(f.s0 + p0 + r - first) * a.stride + d, x[i]);
+    }
+    if (failed || (unsigned)page >= (unsigned)a.pages) return;       // behind a failed call on the tables nothing is written
+    const Unit u = unit_of(a.c, page, a.layer, h);
+    uint8_t *scale = u.s + (value ? SCALES : 0) + sub;
+    // V's words, four positions 4 q .. of a dimension: a lane's are of one q and the dimensions 4 (8 i + lane / 8) .. + 3. Those that hold earlier positions
+    // beside new ones:
+    const int q = lane & 7, dq = lane >> 3;
+    uint32_t *const words = (uint32_t *)(u.v + (size_t)(4 * dq) * PAGE + sub * BLOCK) + q, shared[NB][4] = {};
+    auto read_shared = [&] {
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) shared[i][j] = words[(32 * i + j) * (PAGE / 4)];
+    };
+    if (value && before % 4 && q == before >> 2) read_shared();
+    const int had = before ? max((int)*scale, 1) : 0;
+#pragma unroll
+    for (int i = 0; i < IT; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) most = fmaxf(most, finite_size(x[i][j]));
-    }
-    const int had = before ? max((int)*scale, 1) : 0, e = max(exponent_for(max_wave(most)), had);
+    const int e = max(exponent_for(max_wave(most)), had);
     const float up = pow2_byte(254 - e), down = had && had < e ? (e - had < 127 ? pow2_byte(127 - (e - had)) : 0.f) : 1.f;
+    if (lane == 0) *scale = (uint8_t)e;                              // read by no other lane by now
     if (!value) {
 #pragma unroll
         for (int i = 0; i < IT; i++) {
@@ -118,37 +138,41 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
             }
         }
     } else {
-        // codes through LDS to words along positions: lane's dimensions lane, lane + 64 ..
+        // codes through LDS to words along positions
         uint8_t *row_s = code_s[wave];
 #pragma unroll
         for (int i = 0; i < IT; i++) {
             const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
             uint32_t *to = (uint32_t *)(row_s + r * (HP + 4) + d);
+            if (r < before || r >= end) continue;
             to[0] = encode4(x[i][0], x[i][1], x[i][2], x[i][3], up);
             to[1] = encode4(x[i][4], x[i][5], x[i][6], x[i][7], up);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        for (int d = lane; d < HP; d += 64) {
-            uint32_t *to = (uint32_t *)(u.v + (size_t)d * PAGE + sub * BLOCK);
+        if (4 * q >= end || (4 * q + 4 <= before && down == 1.f)) return;
+        if (down != 1.f && 4 * q < before) {
+            if (4 * q + 4 <= before) read_shared();
 #pragma unroll
-            for (int q = 0; q < BLOCK / 4; q++) {
-                if (4 * q >= end || (4 * q + 4 <= before && down == 1.f)) continue;
-                uint32_t word = 0;
+            for (int i = 0; i < NB; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) word |= (uint32_t)row_s[(4 * q + j) * (HP + 4) + d] << 8 * j;
-                if (4 * q < before) {                                // some that were there
-                    const uint32_t was = down == 1.f ? to[q] : recode4(to[q], down);
-                    const int n = min(before - 4 * q, 4);
-                    const uint32_t keep = n == 4 ? ~0u : ~(~0u << 8 * n);
-                    word = (was & keep) | (word & ~keep);
-                }
-                to[q] = word;
+                for (int j = 0; j < 4; j++) shared[i][j] = recode4(shared[i][j], down);
+        }
+        const uint32_t keep = before <= 4 * q ? 0u : before - 4 * q >= 4 ? ~0u : ~(~0u << 8 * (before - 4 * q));    // positions that were there
+        const uint32_t gone = 4 * q + 4 > end ? ~0u << 8 * (end - 4 * q) : 0u;                                      // behind the sequence: zeros
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = *(const uint32_t *)(row_s + (4 * q + j) * (HP + 4) + 32 * i + 4 * dq);
+            transpose4(w);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                words[(32 * i + j) * (PAGE / 4)] = (shared[i][j] & keep) | (w[j] & ~keep & ~gone);
             }
         }
     }
-    if (lane == 0) *scale = (uint8_t)e;
 }
 
 // ---------------------------------------------------------------- read-back
@@ -168,21 +192,42 @@ template <int NB> __global__ void __launch_bounds__(256) k_kv8_rows(RowsIn a) {
     const Unit u = unit_of(a.c, lost ? 0 : page, a.layer, h);
     const int sub = block % SCALES, p0 = block * BLOCK, begin = max(first - p0, 0), end = min(len - p0, BLOCK);
     const float s = lost ? NAN : pow2_byte(max((int)u.s[(value ? SCALES : 0) + sub], 1));
-    float *to = out + ((size_t)(f.s0 + p0 - first + begin) * nkv + h) * hd;
+    float *to = out + ((size_t)(f.s0 + p0 - first) * nkv + h) * hd;
     if (!value) {
-        for (int i = lane; i < (end - begin) * (hd / 4); i += 64) {
-            const int r = i / (hd / 4), d = 4 * (i - r * (hd / 4));
-            const uint32_t c = *(const uint32_t *)(u.k + (size_t)(sub * BLOCK + begin + r) * HP + d);
-            const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-            *(f32x4_a4 *)(to + (size_t)r * nkv * hd + d) = f32x4{x.x * s, x.y * s, y.x * s, y.y * s};
+        constexpr int PER = 4 * NB, IT = 2 * NB;
+        u32x2 code[IT];
+#pragma unroll
+        for (int i = 0; i < IT; i++) code[i] = *(const u32x2 *)(u.k + (size_t)sub * BLOCK * HP + 8 * (64 * i + lane));
+#pragma unroll
+        for (int i = 0; i < IT; i++) {
+            const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
+            if (r < begin || r >= end || d >= hd) continue;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[i][j], false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[i][j], true);
+                *(f32x4_a4 *)(to + (size_t)r * nkv * hd + d + 4 * j) = f32x4{x.x * s, x.y * s, y.x * s, y.y * s};
+            }
         }
         return;
     }
-    for (int d = lane; d < hd; d += 64)
-        for (int r = begin; r < end; r++) {
-            const uint32_t c = u.v[(size_t)d * PAGE + sub * BLOCK + r];
-            to[(size_t)(r - begin) * nkv * hd + d] = __builtin_amdgcn_cvt_f32_fp8((int)c, 0) * s;
+    const int q = lane & 7, dq = lane >> 3;                          // four positions of four dimensions, as the writer has them
+    uint32_t code[NB][4];
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) code[i][j] = *(const uint32_t *)(u.v + (size_t)(32 * i + 4 * dq + j) * PAGE + sub * BLOCK + 4 * q);
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        transpose4(code[i]);
+        const int d = 32 * i + 4 * dq;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int r = 4 * q + j;
+            if (r < begin || r >= end || d >= hd) continue;
+            const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[i][j], false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[i][j], true);
+            *(f32x4_a4 *)(to + (size_t)r * nkv * hd + d) = f32x4{x.x * s, x.y * s, y.x * s, y.y * s};
         }
+    }
 }
 
 // ---------------------------------------------------------------- attention
@@ -380,9 +425,9 @@ template <int N> __device__ __forceinline__ void requests_but() { __builtin_amdg
 __device__ __forceinline__ void reads_done() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
 // Four values of a result. NaN behind a failed call on the tables; a token before its sequence's first position sees nothing: zeros.
-template <bool F32> __device__ __forceinline__ void put_row(const AttendIn &a, long long at, f32x4 x, bool none) {
+template <bool F32> __device__ __forceinline__ void put_row(const AttendIn &a, long long at, f32x4 x, bool none, bool failed) {
     if (none) x = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (a.state[0]) x = f32x4{NAN, NAN, NAN, NAN};
+    if (failed) x = f32x4{NAN, NAN, NAN, NAN};
     if constexpr (F32) *(f32x4_a4 *)((float *)a.out + at) = x;
     else {
         typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
@@ -404,6 +449,7 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, c = lane >> 4, hd = a.c.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
     const int h = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const bool failed = *(const CONSTANT int32_t *)a.state != 0;
     const Share f = share_of<false>(a, (int)(blockIdx.x / (unsigned)a.c.nkv));
     if (f.run < 0) return;
     const int len = f.len, row0 = 16 * f.group, rows = min(f.rows * g - row0, 16);
@@ -591,7 +637,7 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
             continue;
         }
         const int t = (int)divide(row0 + row, g, a.g_mul), hh = h * g + row0 + row - t * g;
-        put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, x / sum, len - f.rows + t < 0);
+        put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, x / sum, len - f.rows + t < 0, failed);
     }
 }
 
@@ -602,6 +648,7 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
     __shared__ f32x4 o_s[JOIN];
     __shared__ float f_s[16][PARTS], sum_s[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, quads = hd >> 2, h = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const bool failed = *(const CONSTANT int32_t *)a.state != 0;
     const Share f = share_of<true>(a, (int)(blockIdx.x / (unsigned)a.c.nkv));
     if (f.run < 0 || f.parts < 2) return;
     const int rows = min(f.rows * a.g - 16 * f.group, 16);
@@ -644,7 +691,7 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
         if (mine == 0 && i0 + item < rows * quads) {
             for (int i = 1; i < groups; i++) o += o_s[i * items + item];
             const int r = 16 * f.group + row, t = (int)divide(r, a.g, a.g_mul), hh = h * a.g + r - t * a.g;
-            put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, o / sum_s[row], f.len - f.rows + t < 0);
+            put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, o / sum_s[row], f.len - f.rows + t < 0, failed);
         }
     }
 }

@@ -41,38 +41,52 @@ __device__ int scan_all(Scan &s, int x, int &total) {
     }
     return before + upto - x;
 }
-// Numbers of sequences that were listed, a bit each.
+// Numbers of sequences that were listed, a bit each; and the gravest reason against a call, 0: none.
 struct Listed {
     uint32_t bits[MOST_SEQS / 32];
+    int      why;
     __device__ void clear() {
+        if (threadIdx.x == 0) why = 0;
         for (int i = threadIdx.x; i < MOST_SEQS / 32; i += PLAN) bits[i] = 0;
         __syncthreads();
     }
     __device__ bool add(int id) { return !(atomicOr(&bits[id >> 5], 1u << (id & 31)) >> (id & 31) & 1u); }    // false: it was there
     __device__ bool has(int id) const { return bits[id >> 5] >> (id & 31) & 1u; }
+    __device__ int worst(int mine) {
+        if (mine) atomicMax(&why, mine);
+        __syncthreads();
+        return why;
+    }
 };
-__device__ __forceinline__ int worst(int why) {                      // the largest of the workgroup's
-    __shared__ int w;
+// f(v, 0 .. count - 1) of each thread's own count and values, over all threads of the workgroup alike.
+template <int N> struct Spread {
+    int first[PLAN], v[N][PLAN];
+};
+template <int N, class F> __device__ __forceinline__ void spread(Scan &scan, Spread<N> &s, int count, const int (&v)[N], F f) {
+    int total;
+    const int before = scan_all(scan, count, total);
+    s.first[threadIdx.x] = before;
+#pragma unroll
+    for (int i = 0; i < N; i++) s.v[i][threadIdx.x] = v[i];
     __syncthreads();
-    if (threadIdx.x == 0) w = 0;
-    __syncthreads();
-    if (why) atomicMax(&w, why);
-    __syncthreads();
-    return w;
-}
-// f(v, 0 .. count - 1) for each thread's own count and values: the first two by the thread, the rest by its wavefront. Every lane calls it.
-template <int N, class F> __device__ __forceinline__ void spread(int count, const int (&v)[N], F f) {
-    const int lane = threadIdx.x & 63;
-    for (int j = 0; j < min(count, 2); j++) f(v, j);
-    for (uint64_t more = __ballot(count > 2); more; more &= more - 1) {
-        const int l = __builtin_ctzll(more), n = __builtin_amdgcn_readlane(count, l);
+    for (int e = threadIdx.x; e < total; e += PLAN) {
+        int of = 0;                                                  // the last one that begins at e or before it
+#pragma unroll
+        for (int step = PLAN / 2; step; step >>= 1) of += s.first[of + step] <= e ? step : 0;
         int u[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) u[i] = __builtin_amdgcn_readlane(v[i], l);
-        for (int j = 2 + lane; j < n; j += 64) f(u, j);
+        for (int i = 0; i < N; i++) u[i] = s.v[i][of];
+        f(u, e - s.first[of]);
     }
 }
 __device__ __forceinline__ bool in_pool(const Tables &t, int page) { return (unsigned)page < (unsigned)t.pages; }
+// One workgroup's stores and atomics to memory are done, and every thread is here: they meet in one L2, so no fence beyond the workgroup is needed (an
+// agent's writes that L2 back).
+__device__ __forceinline__ void memory_done() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0x0F70);                              // vmcnt(0)
+    __syncthreads();
+}
 // Values that this launch's atomics changed, past the CU's cache.
 __device__ __forceinline__ int32_t now(const int32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
@@ -90,83 +104,92 @@ __global__ void k_pages_clear(Tables t) { t.state[STATE_FAILED] = 0; }
 
 // A run of `add` rows makes its sequence that much longer. The pages that it begins are new; one that it goes on in and that others hold too is replaced by
 // a new one and listed to be copied, but where all of its holders are in the list the first of them keeps it.
+// Bound by latency: each step's loads hang on the last one's. Up to PLAN runs are read once and kept in registers.
+struct Grown {
+    int id, s0, add, old, page, held;                                // page: that it goes on in, -1: none; held: by so many
+    int more, copy, at;                                              // new pages, one of them a copy; where they begin among all
+};
 __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *pos) {
     __shared__ Listed listed;
     __shared__ Scan   scan;
+    __shared__ Spread<5> spread_s;
     __shared__ int    copies_s;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, first_free = tid < t.pages ? t.refs[tid] : 1;
     int32_t *growers = scratch(t, 2), *eldest = scratch(t, 3), *fresh = eldest, *plan = scratch(t, 4);   // of a page: how many grow into it, and the first
-    if (t.state[STATE_FAILED]) {
+    const int failed = t.state[STATE_FAILED];
+    auto read = [&](int i) {
+        Grown r = {b.id(i), b.from(i), 0, 0, -1, 0, 0, 0, 0};
+        r.add = b.to(i, r.s0) - r.s0;
+        if ((unsigned)r.id >= (unsigned)t.seqs) return r;
+        r.old = t.len[r.id];
+        if (r.add && r.old % PAGE && r.old > 0 && r.old <= (long long)t.width * PAGE) {
+            r.page = t.table[(size_t)r.id * t.width + r.old / PAGE];
+            r.held = in_pool(t, r.page) ? t.refs[r.page] : 0;
+        }
+        return r;
+    };
+    const bool one = b.seqs <= PLAN;
+    Grown mine = {};
+    if (tid < b.seqs) mine = read(tid);
+    if (failed) {
         if (tid == 0) t.state[STATE_COPIES] = 0;
         return;
     }
     listed.clear();
     if (tid == 0) copies_s = 0;
-    int why = 0;
+    int why = 0, shared = 0;
     for (int i = tid; i < b.seqs; i += PLAN) {
-        const int id = b.id(i), s0 = b.from(i), add = b.to(i, s0) - s0;
-        if ((unsigned)id >= (unsigned)t.seqs || !listed.add(id)) {
-            why = max(why, (int)L3M_PAGES_BAD);
-            continue;
-        }
-        const int old = t.len[id];
-        if (old < 0 || old > (long long)t.width * PAGE) why = max(why, (int)L3M_PAGES_BAD);
-        else if ((long long)old + add > (long long)t.width * PAGE || (long long)old + add > INT_MAX) why = max(why, (int)L3M_PAGES_LONG);
-        else if (add && old % PAGE) {
-            const int page = t.table[(size_t)id * t.width + old / PAGE];
-            if (!in_pool(t, page)) why = max(why, (int)L3M_PAGES_BAD);
-            else if (t.refs[page] > 1) {
-                growers[page] = 0;
-                eldest[page] = INT_MAX;
-            }
+        const Grown r = one ? mine : read(i);
+        if ((unsigned)r.id >= (unsigned)t.seqs || !listed.add(r.id) || r.old < 0 || r.old > (long long)t.width * PAGE) why = max(why, (int)L3M_PAGES_BAD);
+        else if ((long long)r.old + r.add > (long long)t.width * PAGE) why = max(why, (int)L3M_PAGES_LONG);
+        else if (r.add && r.old % PAGE && !in_pool(t, r.page)) why = max(why, (int)L3M_PAGES_BAD);
+        else if (r.held > 1) {
+            shared = 1;
+            growers[r.page] = 0;
+            eldest[r.page] = INT_MAX;
         }
     }
-    why = worst(why);
-    __threadfence();
-    __syncthreads();
-    if (!why)
+    why = listed.worst(why);
+    if (!why && __syncthreads_or(shared)) {
+        memory_done();
         for (int i = tid; i < b.seqs; i += PLAN) {
-            const int id = b.id(i), s0 = b.from(i), add = b.to(i, s0) - s0, old = t.len[id];
-            if (!add || old % PAGE == 0) continue;
-            const int page = t.table[(size_t)id * t.width + old / PAGE];
-            if (t.refs[page] > 1) {
-                atomicAdd(&growers[page], 1);
-                atomicMin(&eldest[page], i);
+            const Grown r = one ? mine : read(i);
+            if (r.held > 1) {
+                atomicAdd(&growers[r.page], 1);
+                atomicMin(&eldest[r.page], i);
             }
         }
-    __threadfence();
-    __syncthreads();
+        memory_done();
+    }
     int total = 0;
     if (!why)
         for (int i0 = 0; i0 < b.seqs; i0 += PLAN) {
             const int i = i0 + tid;
-            int more = 0, copy = 0;
+            Grown r = {};
             if (i < b.seqs) {
-                const int id = b.id(i), s0 = b.from(i), add = b.to(i, s0) - s0, old = t.len[id];
-                if (add && old % PAGE) {
-                    const int page = t.table[(size_t)id * t.width + old / PAGE], held = t.refs[page];
-                    copy = held > 1 && !(now(&growers[page]) == held && now(&eldest[page]) == i);
-                }
-                more = pages_for(old + add) - pages_for(old) + copy;
+                r = one ? mine : read(i);
+                r.copy = r.held > 1 && !(now(&growers[r.page]) == r.held && now(&eldest[r.page]) == i);
+                r.more = pages_for(r.old + r.add) - pages_for(r.old) + r.copy;
             }
             int sum;
-            const int at = scan_all(scan, more, sum);
-            if (i < b.seqs) {
-                plan[i] = total + at;
-                plan[t.seqs + i] = 2 * more + copy;
+            r.at = scan_all(scan, r.more, sum) + total;
+            if (one) mine = r;
+            else if (i < b.seqs) {
+                plan[i] = r.at;
+                plan[t.seqs + i] = 2 * r.more + r.copy;
             }
             total += sum;
             if (total > t.pages) break;                              // uniform; no pool has so many
         }
-    __syncthreads();
     // the free pages that are needed, in order
     if (!why && total) {
+        __syncthreads();
         int got = 0;
         for (int p0 = 0; p0 < t.pages && got < total; p0 += PLAN) {
-            const int p = p0 + tid, free = p < t.pages && t.refs[p] == 0;
+            const int p = p0 + tid, free = p < t.pages && (p0 ? t.refs[p] : first_free) == 0;
             int sum;
             const int at = scan_all(scan, free, sum);
-            if (free && got + at < total) fresh[got + at] = p;         // who grows where is in the plan by now
+            if (free && got + at < total) fresh[got + at] = p;       // who grows where is in the plan by now
             got += sum;
         }
         if (got < total) why = L3M_PAGES_FULL;
@@ -179,32 +202,36 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
         return;
     }
     __syncthreads();
-    for (int i0 = 0; i0 < b.seqs; i0 += PLAN) {                      // whole wavefronts: spread takes all lanes
+    for (int i0 = 0; i0 < b.seqs; i0 += PLAN) {
         const int i = i0 + tid;
-        int more = 0, add = 0, v[5] = {0, 0, 0, 0, 0};               // its first new page's place among them, sequence, place in the table, first row, length
+        Grown r = {};
+        int v[5] = {0, 0, 0, 0, 0};                                  // its first new page's place among them, sequence, place in the table, first row, length
         if (i < b.seqs) {
-            const int id = b.id(i), s0 = b.from(i), old = t.len[id], copy = plan[t.seqs + i] & 1;
-            add = b.to(i, s0) - s0;
-            more = plan[t.seqs + i] >> 1;
-            v[0] = plan[i];
-            v[1] = id;
-            v[2] = copy ? old / PAGE : pages_for(old);
-            v[3] = s0;
-            v[4] = old;
-            if (copy) {
-                const int page = t.table[(size_t)id * t.width + v[2]], k = atomicAdd(&copies_s, 1);
-                atomicSub(&t.refs[page], 1);
-                scratch(t, 0)[k] = page;
-                scratch(t, 1)[k] = fresh[v[0]];
+            r = one ? mine : read(i);
+            if (!one) {
+                r.at = plan[i];
+                r.copy = plan[t.seqs + i] & 1;
+                r.more = plan[t.seqs + i] >> 1;
             }
-            t.len[id] = old + add;
+            v[0] = r.at;
+            v[1] = r.id;
+            v[2] = r.copy ? r.old / PAGE : pages_for(r.old);
+            v[3] = r.s0;
+            v[4] = r.old;
+            if (r.copy) {
+                const int k = atomicAdd(&copies_s, 1);
+                atomicSub(&t.refs[r.page], 1);
+                scratch(t, 0)[k] = r.page;
+                scratch(t, 1)[k] = fresh[r.at];
+            }
+            t.len[r.id] = r.old + r.add;
         }
-        spread(more, v, [&](const int (&u)[5], int j) {
+        spread<5>(scan, spread_s, r.more, v, [&](const int (&u)[5], int j) {
             const int page = fresh[u[0] + j];
             t.refs[page] = 1;
             t.table[(size_t)u[1] * t.width + u[2] + j] = page;
         });
-        if (pos) spread(add, v, [&](const int (&u)[5], int j) { pos[u[3] + j] = u[4] + j; });
+        if (pos) spread<5>(scan, spread_s, r.add, v, [&](const int (&u)[5], int j) { pos[u[3] + j] = u[4] + j; });
     }
     __syncthreads();
     if (tid == 0) {
@@ -216,32 +243,41 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
 // to[i] becomes a sequence of from[i]'s pages.
 __global__ void __launch_bounds__(PLAN) k_pages_fork(Tables t, const int32_t *from, const int32_t *to, int n) {
     __shared__ Listed listed;
+    __shared__ Scan   scan;
+    __shared__ Spread<2> spread_s;
     const int tid = threadIdx.x;
+    // the first PLAN pairs are read once: number, number, lengths
+    auto read = [&](int i, int (&v)[4]) {
+        v[0] = from[i];
+        v[1] = to[i];
+        v[2] = (unsigned)v[0] < (unsigned)t.seqs ? t.len[v[0]] : -1;
+        v[3] = (unsigned)v[1] < (unsigned)t.seqs ? t.len[v[1]] : -1;
+    };
+    int mine[4] = {0, 0, 0, 0};
+    if (tid < n) read(tid, mine);
     if (t.state[STATE_FAILED]) return;
     listed.clear();
     int why = 0;
-    for (int i = tid; i < n; i += PLAN)
-        if ((unsigned)to[i] >= (unsigned)t.seqs || (unsigned)from[i] >= (unsigned)t.seqs || !listed.add(to[i]) || t.len[to[i]] != 0 || t.len[from[i]] < 0 ||
-            t.len[from[i]] > (long long)t.width * PAGE)
-            why = L3M_PAGES_BAD;
+    for (int i = tid; i < n; i += PLAN) {
+        int v[4] = {mine[0], mine[1], mine[2], mine[3]};
+        if (i >= PLAN) read(i, v);
+        if (v[2] < 0 || v[2] > (long long)t.width * PAGE || v[3] != 0 || !listed.add(v[1])) why = L3M_PAGES_BAD;
+    }
     __syncthreads();
-    for (int i = tid; i < n; i += PLAN)
-        if ((unsigned)from[i] < (unsigned)t.seqs && listed.has(from[i])) why = L3M_PAGES_BAD;
-    if ((why = worst(why))) {
+    for (int i = tid; i < n; i += PLAN) {
+        const int id = i < PLAN ? mine[0] : from[i];
+        if ((unsigned)id < (unsigned)t.seqs && listed.has(id)) why = L3M_PAGES_BAD;
+    }
+    if ((why = listed.worst(why))) {
         if (tid == 0) t.state[STATE_FAILED] = why;
         return;
     }
     for (int i0 = 0; i0 < n; i0 += PLAN) {
         const int i = i0 + tid;
-        int count = 0, v[2] = {0, 0};
-        if (i < n) {
-            v[0] = from[i];
-            v[1] = to[i];
-            const int len = t.len[v[0]];
-            count = pages_for(len);
-            t.len[v[1]] = len;
-        }
-        spread(count, v, [&](const int (&u)[2], int j) {
+        int v[4] = {mine[0], mine[1], mine[2], mine[3]};
+        if (i0 && i < n) read(i, v);
+        if (i < n) t.len[v[1]] = v[2];
+        spread<2>(scan, spread_s, i < n ? pages_for(v[2]) : 0, {v[0], v[1]}, [&](const int (&u)[2], int j) {
             const int page = t.table[(size_t)u[0] * t.width + j];
             t.table[(size_t)u[1] * t.width + j] = page;
             if (in_pool(t, page)) atomicAdd(&t.refs[page], 1);
@@ -252,6 +288,8 @@ __global__ void __launch_bounds__(PLAN) k_pages_fork(Tables t, const int32_t *fr
 // Sequence ids[i] is cut to its first keep[i] positions (keep NULL: none).
 __global__ void __launch_bounds__(PLAN) k_pages_cut(Tables t, const int32_t *ids, const int32_t *keep, int n) {
     __shared__ Listed listed;
+    __shared__ Scan   scan;
+    __shared__ Spread<2> spread_s;
     __shared__ int    freed_s;
     const int tid = threadIdx.x;
     if (t.state[STATE_FAILED]) return;
@@ -262,7 +300,7 @@ __global__ void __launch_bounds__(PLAN) k_pages_cut(Tables t, const int32_t *ids
         const int id = ids[i], to = keep ? keep[i] : 0;
         if ((unsigned)id >= (unsigned)t.seqs || !listed.add(id) || to < 0 || to > t.len[id] || t.len[id] > (long long)t.width * PAGE) why = L3M_PAGES_BAD;
     }
-    if ((why = worst(why))) {
+    if ((why = listed.worst(why))) {
         if (tid == 0) t.state[STATE_FAILED] = why;
         return;
     }
@@ -276,7 +314,7 @@ __global__ void __launch_bounds__(PLAN) k_pages_cut(Tables t, const int32_t *ids
             count = pages_for(t.len[v[0]]) - v[1];
             t.len[v[0]] = to;
         }
-        spread(count, v, [&](const int (&u)[2], int j) {
+        spread<2>(scan, spread_s, count, v, [&](const int (&u)[2], int j) {
             int32_t &entry = t.table[(size_t)u[0] * t.width + u[1] + j];
             if (in_pool(t, entry) && atomicSub(&t.refs[entry], 1) == 1) atomicAdd(&freed_s, 1);
             entry = -1;

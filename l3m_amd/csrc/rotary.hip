@@ -13,7 +13,7 @@ struct RotaryIn {
     const int32_t *pos;
     long long      stride, q_stride, k_stride;
     int            n, nq, nkv, pos0, tokens;                         // tokens: of a workgroup
-    int            turned, per_head, per_token;                      // items: of the turned part of a head, of a head, of a token
+    int            turned, per_head, per_token, rest_gap;            // items: of the turned part of a head, of a head, of a token; rest_gap: below
     uint32_t       token_mul, head_mul, pair_mul;                    // of per_token, per_head and rd / 2 (divide)
 };
 
@@ -30,33 +30,75 @@ __device__ __forceinline__ void sincos_turns(uint64_t turns, double &s, double &
     if ((quarter + 1) & 2) c = -c;
 }
 
-// V values of type T at p as float32, and back.
-template <class T, int V> __device__ __forceinline__ void load_values(const T *p, float (&x)[V]) {
-    if constexpr (V == 1) x[0] = sizeof(T) == 4 ? *(const float *)p : bf16_float(*(const uint16_t *)p);
-    else if constexpr (sizeof(T) == 4) {
+// V values of type T as they lie in memory, and as float32.
+template <class T, int V> struct Raw {
+    static constexpr int words = V * (int)sizeof(T) < 4 ? 1 : V * (int)sizeof(T) / 4;
+    uint32_t w[words];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (V == 1) w[0] = sizeof(T) == 4 ? *(const uint32_t *)p : *(const uint16_t *)p;
+        else
 #pragma unroll
-        for (int i = 0; i < V; i += 4) *(f32x4 *)&x[i] = *(const f32x4 *)(p + i);
-    } else {
-        const u32x4 w = *(const u32x4 *)p;
+            for (int i = 0; i < words; i += 4) {
+                const u32x4 x = *(const u32x4 *)(p + i * V / words);
 #pragma unroll
-        for (int i = 0; i < V; i++) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+                for (int j = 0; j < 4; j++) w[i + j] = x[j];
+            }
     }
-}
+    __device__ __forceinline__ float value(int i) const { return sizeof(T) == 4 ? __uint_as_float(w[i]) : __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16); }
+};
 template <class T, int V> __device__ __forceinline__ void store_values(T *p, const float (&x)[V]) {
     if constexpr (V == 1) {
         if constexpr (sizeof(T) == 4) *(float *)p = x[0];
         else *(uint16_t *)p = (uint16_t)bf16_pair(x[0], 0.f);
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) *(f32x4 *)(p + i) = *(const f32x4 *)&x[i];
+        for (int i = 0; i < V; i += 4) *(f32x4 *)(p + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
     } else *(u32x4 *)p = u32x4{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]), bf16_pair(x[6], x[7])};
 }
 
 // y = mag (u c - w s, u s + w c) of each pair (u, w), c and s of position times frequency; what lies behind the turned part goes as it is. A workgroup makes
-// its tokens' sines once, in LDS, and then turns every head by them.
+// its tokens' sines once, in LDS, while the first rows come, and then turns every head by them. A thread's items, UNROLL at once: V pairs (halves: V values of
+// either half; else V values, pairs side by side; V 1: a pair), or of what lies behind the turned part V values, and V more rest_gap behind them where that is not 0.
+// Bound by the bytes.
+template <class TI, int V> constexpr int unroll() { return V == 1 || sizeof(TI) == 4 ? 2 : 4; }
 template <class TI, class TO, int V> __global__ void __launch_bounds__(THREADS) k_rotary(RotaryIn a) {
+    constexpr int UNROLL = unroll<TI, V>();
     extern __shared__ float cs_s[];                                  // [tokens][rd / 2] (cos, sin)
-    const int pairs = a.r.rd >> 1, t0 = (int)blockIdx.x * a.tokens, tokens = min(a.tokens, a.n - t0);
+    const int pairs = a.r.rd >> 1, t0 = (int)blockIdx.x * a.tokens, tokens = min(a.tokens, a.n - t0), halves = a.r.halves, hd = a.r.hd, rd = a.r.rd;
+    const unsigned items = (unsigned)(tokens * a.per_token);
+    struct Item {
+        const TI *x;
+        TO       *y;
+        const float *cs;
+        int       d, gap;                                            // first value; how far second ones lie behind, 0: beside them, or there are none
+        bool      turn;
+    };
+    auto item_at = [&](unsigned i) {
+        const unsigned t = divide(i, a.per_token, a.token_mul), j = i - t * a.per_token, h = divide(j, a.per_head, a.head_mul);
+        const int e = (int)(j - h * a.per_head);
+        const size_t row = (size_t)t0 + t;
+        Item m;
+        m.turn = e < a.turned;
+        m.gap = !m.turn ? a.rest_gap : halves ? pairs : V == 1 ? 1 : 0;
+        m.d = !m.turn ? rd + (e - a.turned) * V : V == 1 && !halves ? 2 * e : e * V;
+        m.x = (const TI *)a.x + row * a.stride + (size_t)h * hd + m.d;
+        m.y = ((int)h >= a.nq ? (TO *)a.k + row * a.k_stride + (size_t)((int)h - a.nq) * hd : (TO *)a.q + row * a.q_stride + (size_t)h * hd) + m.d;
+        m.cs = cs_s + 2 * (t * pairs) + (halves ? 2 * m.d : m.d);
+        return m;
+    };
+    Item         m[UNROLL];
+    Raw<TI, V>   u[UNROLL], w[UNROLL];
+    auto request = [&](unsigned i0) {
+#pragma unroll
+        for (int k = 0; k < UNROLL; k++) {
+            const unsigned i = i0 + k * THREADS;
+            if (i >= items) continue;
+            m[k] = item_at(i);
+            u[k].load(m[k].x);
+            if (m[k].gap > 0) w[k].load(m[k].x + m[k].gap);
+        }
+    };
+    request(threadIdx.x);
     for (int i = threadIdx.x; i < tokens * pairs; i += THREADS) {
         const int t = (int)divide(i, pairs, a.pair_mul), p = i - t * pairs;
         const long long pos = a.pos ? a.pos[t0 + t] : (long long)a.pos0 + t0 + t;
@@ -66,65 +108,57 @@ template <class TI, class TO, int V> __global__ void __launch_bounds__(THREADS) 
         cs_s[2 * i + 1] = (float)(s * (double)a.r.mag);
     }
     __syncthreads();
-    const int halves = a.r.halves, hd = a.r.hd, rd = a.r.rd;
-    for (unsigned i = threadIdx.x; i < (unsigned)(tokens * a.per_token); i += THREADS) {
-        const unsigned t = divide(i, a.per_token, a.token_mul), j = i - t * a.per_token, h = divide(j, a.per_head, a.head_mul);
-        const int e = (int)(j - h * a.per_head);
-        const size_t row = (size_t)t0 + t;
-        const bool key = (int)h >= a.nq;
-        const TI *x = (const TI *)a.x + row * a.stride + (size_t)h * hd;
-        TO *y = key ? (TO *)a.k + row * a.k_stride + (size_t)((int)h - a.nq) * hd : (TO *)a.q + row * a.q_stride + (size_t)h * hd;
-        const float *cs = cs_s + 2 * t * pairs;
-        if (e >= a.turned) {
-            if ((const void *)x == (const void *)y) continue;        // in place
-            float v[V];
-            const int d = rd + (e - a.turned) * V;
-            load_values<TI, V>(x + d, v);
-            store_values<TO, V>(y + d, v);
-        } else if (halves) {
-            float u[V], w[V];
-            const int d = e * V;
-            load_values<TI, V>(x + d, u);
-            load_values<TI, V>(x + d + pairs, w);
+    for (unsigned i0 = threadIdx.x; i0 < items; i0 += UNROLL * THREADS) {
+        if (i0 != threadIdx.x) request(i0);
 #pragma unroll
-            for (int r = 0; r < V; r++) {
-                const float c = cs[2 * (d + r)], s = cs[2 * (d + r) + 1], z = u[r] * c - w[r] * s;
-                w[r] = u[r] * s + w[r] * c;
-                u[r] = z;
-            }
-            store_values<TO, V>(y + d, u);
-            store_values<TO, V>(y + d + pairs, w);
-        } else if constexpr (V == 1) {
-            float u[1], w[1];
-            load_values<TI, 1>(x + 2 * e, u);
-            load_values<TI, 1>(x + 2 * e + 1, w);
-            const float c = cs[2 * e], s = cs[2 * e + 1], z = u[0] * c - w[0] * s;
-            w[0] = u[0] * s + w[0] * c;
-            u[0] = z;
-            store_values<TO, 1>(y + 2 * e, u);
-            store_values<TO, 1>(y + 2 * e + 1, w);
-        } else {
-            float v[V];
-            const int d = e * V;
-            load_values<TI, V>(x + d, v);
+        for (int k = 0; k < UNROLL; k++) {
+            if (i0 + k * THREADS >= items) continue;
+            float x[V], z[V];
+            const float *cs = m[k].cs;
+            if (!m[k].turn) {
 #pragma unroll
-            for (int r = 0; r < V; r += 2) {
-                const float c = cs[d + r], s = cs[d + r + 1], z = v[r] * c - v[r + 1] * s;
-                v[r + 1] = v[r] * s + v[r + 1] * c;
-                v[r] = z;
+                for (int r = 0; r < V; r++) {
+                    x[r] = u[k].value(r);
+                    z[r] = w[k].value(r);
+                }
+            } else if (m[k].gap > 0) {
+#pragma unroll
+                for (int r = 0; r < V; r++) {
+                    const float c = cs[2 * r], s = cs[2 * r + 1], p = u[k].value(r), o = w[k].value(r);
+                    x[r] = p * c - o * s;
+                    z[r] = p * s + o * c;
+                }
+            } else if constexpr (V > 1) {
+#pragma unroll
+                for (int r = 0; r < V; r += 2) {
+                    const float c = cs[r], s = cs[r + 1], p = u[k].value(r), o = u[k].value(r + 1);
+                    x[r] = p * c - o * s;
+                    x[r + 1] = p * s + o * c;
+                }
             }
-            store_values<TO, V>(y + d, v);
+            if (m[k].gap > 0) store_values<TO, V>(m[k].y + m[k].gap, z);
+            store_values<TO, V>(m[k].y, x);
         }
     }
 }
 
 template <class TI, class TO, int V> int launch(RotaryIn a, hipStream_t st) {
     const int pairs = a.r.rd / 2, heads = a.nq + a.nkv;
+    // what does not turn stays where it is where both outputs are the rows' own heads
+    const bool in_place = (!a.q || a.q == a.x) && (!a.k || a.k == (const TI *)a.x + (size_t)a.nq * a.r.hd), rest = !in_place;
+    const int  behind = rest ? a.r.hd - a.r.rd : 0;
+    a.rest_gap = V > 1 && a.r.halves && behind % (2 * V) == 0 ? behind / 2 : 0;    // as many bytes an item as the halves' items
     a.turned = V == 1 ? pairs : a.r.halves ? pairs / V : a.r.rd / V;
-    a.per_head = a.turned + (a.r.hd - a.r.rd) / V;
+    a.per_head = a.turned + (a.rest_gap ? behind / 2 : behind) / V;
     a.per_token = a.per_head * heads;
-    // a workgroup's tokens: as many as have a sine for each thread, one while there are few
-    a.tokens = a.n < 1024 || !pairs ? 1 : THREADS / pairs < 1 ? 1 : THREADS / pairs > 8 ? 8 : THREADS / pairs;
+    if (!a.per_token) return 0;
+    // a workgroup's tokens: one while there are few; then as many up to 8 as give its threads whole turns, with a sine a thread at the most
+    constexpr int TURN = THREADS * unroll<TI, V>();
+    a.tokens = 1;
+    auto used = [&](int t) { return (double)t * a.per_token / ((t * a.per_token + TURN - 1) / TURN * TURN); };
+    if (a.n >= 1024)
+        for (int t = 2; t <= 8 && t * pairs <= THREADS; t++)
+            if (used(t) >= used(a.tokens)) a.tokens = t;
     a.token_mul = multiplier(a.per_token, (uint64_t)a.tokens * a.per_token);
     a.head_mul = multiplier(a.per_head, a.per_token);
     a.pair_mul = multiplier(pairs, (uint64_t)a.tokens * pairs);
@@ -204,7 +238,7 @@ int l3m_k_rotary(const l3m_rotary *r, void *q, int q_stride, void *k, int k_stri
     const bool columns = q_stride == k_stride && (gap >= 0 ? gap >= qw && gap + kw <= q_stride : -gap >= kw && qw - gap <= q_stride);
     if (!columns && overlap(q, qb, k, kb)) return l3m_dev_fail("rotary: q overlaps k");
     if (overlap(q, qb, pos, 4 * (size_t)n) || overlap(k, kb, pos, 4 * (size_t)n)) return l3m_dev_fail("rotary: an output overlaps the positions");
-    const RotaryIn a = {*r, rows, q, k, pos, stride, q_stride, k_stride, n, nq, nkv, pos0, 0, 0, 0, 0, 0, 0, 0};
+    const RotaryIn a = {*r, rows, q, k, pos, stride, q_stride, k_stride, n, nq, nkv, pos0, 0, 0, 0, 0, 0, 0, 0, 0};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
     const bool wide = r->hd % 8 == 0 && r->rd % (r->halves ? 16 : 8) == 0 && stride % 8 == 0 && (!q || q_stride % 8 == 0) && (!k || k_stride % 8 == 0) &&

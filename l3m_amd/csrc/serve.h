@@ -47,6 +47,19 @@ __device__ __forceinline__ int scan_wave(int x) {
     return x;
 }
 
+// The largest of a wavefront's, in all lanes: within rows of 16 by moves, then over the halves.
+template <int CTRL> __device__ __forceinline__ float dpp_move(float x) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true)); }
+__device__ __forceinline__ float max_wave(float x) {
+    x = fmaxf(x, dpp_move<0xB1>(x));                                 // lane ^ 1, lane ^ 2, the half row and the row mirrored
+    x = fmaxf(x, dpp_move<0x4E>(x));
+    x = fmaxf(x, dpp_move<0x141>(x));
+    x = fmaxf(x, dpp_move<0x140>(x));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // A batch as kernels take it: starts whatever they hold are brought into 0 .. n, in order.
 struct Runs {
     const int32_t *ids, *starts;
