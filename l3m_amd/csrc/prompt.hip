@@ -6,6 +6,7 @@
 //   P = 2^(S - m)    m moves only where a score passes it by 8: weights up to 2^8, and the sums are seldom scaled. Rounded to bf16
 //   O^T += V^T P^T   32 dimensions x 32 rows x 16 positions, V read from LDS transposed (ds_read_b64_tr_b16)
 // K's and V's tiles go from memory to LDS directly, 16 bytes a lane, in an order of pieces within a row by which no read meets a bank twice.
+#include <type_traits>
 #include "serve.h"
 
 namespace {
@@ -40,19 +41,49 @@ __device__ __forceinline__ float other_half(float x, float &y) {     // lane ^ 3
     return __uint_as_float(r[0]);
 }
 
-// Positions tile .. of a run's K and V into LDS, by the whole workgroup; positions past the last one are the last one again, pieces past the head its last.
-template <int NB> __device__ __forceinline__ void load_tile(const PromptIn &a, const uint16_t *k, const uint16_t *v, int tile, int len, uint16_t *k_s, uint16_t *v_s) {
-    constexpr int RW = row_values(NB), PIECES = RW / 8, TURNS = TILE * PIECES / (64 * WAVES);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), last = (a.hd >> 3) - 1;
+// A workgroup's requests for a tile of K and V, 16 bytes a lane: the i-th round of them is rows i ROUND .. of the tile, in the order of LDS.
+template <int NB> struct Loader {
+    static constexpr int RW = row_values(NB), PIECES = RW / 8, TURNS = TILE * PIECES / (64 * WAVES), ROUND = 64 * WAVES / PIECES;
+    static constexpr int KINDS = ROUND % 16 ? 2 : 1;                 // orders of pieces among the rounds
+    uint32_t k_off[KINDS], v_off[KINDS];                             // bytes behind a round's first row
+    const char *k, *v;
+    long long row_bytes;
+    int len, row, wave;
+    __device__ __forceinline__ void init(const PromptIn &a, const uint16_t *k0, const uint16_t *v0, int rows) {
+        const int slot = threadIdx.x % PIECES, last = (a.hd >> 3) - 1;
+        k = (const char *)k0;
+        v = (const char *)v0;
+        len = rows;
+        row_bytes = 2 * a.kv_stride;
+        row = threadIdx.x / PIECES;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int i = 0; i < TURNS; i++) {
-        const int at0 = 64 * (i * WAVES + wave), at = at0 + lane, row = at / PIECES, slot = at % PIECES;
-        const long long from = (long long)min(tile + row, len - 1) * a.kv_stride;
-        const int kp = slot ^ k_turn<PIECES>(row), vp = slot ^ v_turn<PIECES>(row) << 1;
-        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(k + from + 8 * min(kp, last)), (LOCAL void *)(k_s + 8 * at0), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(v + from + 8 * min(vp, last)), (LOCAL void *)(v_s + 8 * at0), 16, 0, 0);
+        for (int i = 0; i < KINDS; i++) {
+            k_off[i] = (uint32_t)(row * (int)row_bytes + 16 * min(slot ^ k_turn<PIECES>(row + i * ROUND), last));
+            v_off[i] = (uint32_t)(row * (int)row_bytes + 16 * min(slot ^ v_turn<PIECES>(row + i * ROUND) << 1, last));
+        }
     }
-}
+    // Positions TILE tile .. into LDS; positions past the last one are the last one again, pieces past the head its last.
+    __device__ __forceinline__ void request(int tile, uint16_t *k_s, uint16_t *v_s) const {
+        const char *kt = k + tile * TILE * row_bytes, *vt = v + tile * TILE * row_bytes;
+        const int over = tile * TILE + TILE - len;                   // rows past the last
+        if (__builtin_expect(over > 0, 0)) {
+            asm volatile("");                                        // no selects for all tiles' sake
+#pragma unroll
+            for (int i = 0; i < TURNS; i++) {
+                const int less = max(row + i * ROUND - (TILE - 1 - over), 0), at = i * ROUND - less;
+                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(kt + (at * row_bytes + k_off[i % KINDS])), (LOCAL void *)(k_s + 512 * (i * WAVES + wave)), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(vt + (at * row_bytes + v_off[i % KINDS])), (LOCAL void *)(v_s + 512 * (i * WAVES + wave)), 16, 0, 0);
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < TURNS; i++) {
+                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(kt + i * ROUND * row_bytes + k_off[i % KINDS]), (LOCAL void *)(k_s + 512 * (i * WAVES + wave)), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(vt + i * ROUND * row_bytes + v_off[i % KINDS]), (LOCAL void *)(v_s + 512 * (i * WAVES + wave)), 16, 0, 0);
+            }
+    }
+};
+
 __device__ __forceinline__ void loads_done() {                       // and the workgroup's
     __builtin_amdgcn_s_waitcnt(0x0F70);                              // vmcnt(0)
     __syncthreads();
@@ -85,7 +116,8 @@ __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *
 
 template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(PromptIn a) {
     constexpr int RW = row_values(NB), PIECES = RW / 8;
-    __shared__ __align__(16) uint16_t k_s[TILE * RW], v_s[TILE * RW];
+    // two tiles: the next one comes while one is used. Arrays of their own, so that the compiler sees that reads of one do not wait for the other's requests
+    __shared__ __align__(16) uint16_t k0_s[TILE * RW], v0_s[TILE * RW], k1_s[TILE * RW], v1_s[TILE * RW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, c = lane >> 5, hd = a.hd, g = a.g;
     const int h = (int)(blockIdx.x % (unsigned)a.nkv), item = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)a.nkv);
     const Found f = find_run(a.b, item, [&](int, int, int rows) { return (int)(((unsigned)rows * g + ROWS * WAVES - 1) / (ROWS * WAVES)); });
@@ -106,6 +138,11 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
         if (d >= hd) x = u32x4{0, 0, 0, 0};
         qs[i] = __builtin_bit_cast(bf16x8, x);
     }
+    Loader<NB> loads;
+    loads.init(a, k, v, f.rows);
+    loads.request(0, k0_s, v0_s);
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) asm volatile("" : "+v"(qs[i]));   // here, or the loop waits for requests at its top
     const float scale = 1.44269504f / sqrtf((float)hd);              // of the scores: base 2
     f32x16 acc[NB];
 #pragma unroll
@@ -114,29 +151,41 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
         for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
     float m = M0, l = 0.f;
 
-    for (int tile = 0; tile < tiles; tile++) {
-        __syncthreads();
-        load_tile<NB>(a, k, v, tile * TILE, f.rows, k_s, v_s);
-        loads_done();
-        if (tile * TILE > high) continue;
+    auto step = [&](int tile, const uint16_t *k_s, const uint16_t *v_s) {
         f32x16 s[2];
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int j = 0; j < 16; j++) s[b][j] = 0.f;
-            const int at = 32 * b + (r32 & 19) + (r32 & 4) * 2 + (r32 & 8) / 2;       // bits 2 and 3 exchanged
+        const int key = (r32 & 19) + (r32 & 4) * 2 + (r32 & 8) / 2;    // bits 2 and 3 exchanged
+        auto keys = [&](int i, int b) { return *(const bf16x8 *)(k_s + (32 * b + key) * RW + 8 * ((2 * i + c) ^ k_turn<PIECES>(key))); };
+        bf16x8 kx[2][2];
+        kx[0][0] = keys(0, 0);
+        kx[0][1] = keys(0, 1);
 #pragma unroll
-            for (int i = 0; i < 2 * NB; i++) {
-                const bf16x8 kx = *(const bf16x8 *)(k_s + at * RW + 8 * ((2 * i + c) ^ k_turn<PIECES>(at)));
-                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kx, qs[i], s[b], 0, 0, 0);
+        for (int i = 0; i < 2 * NB; i++) {
+            if (i + 1 < 2 * NB) {
+                kx[(i + 1) & 1][0] = keys(i + 1, 0);
+                kx[(i + 1) & 1][1] = keys(i + 1, 1);
             }
+#pragma unroll
+            for (int b = 0; b < 2; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kx[i & 1][b], qs[i], s[b], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);           // LDS reads two products ahead
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
         // s[b][8 j + e]: position 32 b + 16 j + 8 c + e
-        if (tile * TILE + TILE - 1 > low)
+        if (__builtin_expect(tile * TILE + TILE - 1 > low, 0)) {
+            asm volatile("");                                        // no selects for all tiles' sake
+            const int seen = token - tile * TILE - 8 * c;
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) s[b][j] = tile * TILE + 32 * b + 16 * (j >> 3) + 8 * c + (j & 7) <= token ? s[b][j] : -INFINITY;
+                for (int j = 0; j < 16; j++) s[b][j] = 32 * b + 16 * (j >> 3) + (j & 7) <= seen ? s[b][j] : -INFINITY;
+        }
         float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -152,7 +201,20 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
             for (int i = 0; i < NB; i++) acc[i] *= by;
             m = to;
         }
-        bf16x8 p[2][2];
+        // lane (c, d): positions 8 c .. + 7 of dimension d, four at a time of 16 dimensions by 16 lanes
+        auto values = [&](int n) {
+            const int i = n % NB, b = n / NB >> 1, j = n / NB & 1;
+            s16x4 x[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int at = 32 * b + 16 * j + 8 * c + 4 * u + (lane >> 2 & 3), pair = 2 * i + (lane >> 4 & 1);
+                x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LOCAL s16x4 *)(v_s + at * RW + 16 * (pair ^ v_turn<PIECES>(8 * c + (lane >> 2 & 3))) + 4 * (lane & 3)));
+            }
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            return __builtin_bit_cast(bf16x8, s16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]});
+        };
+        bf16x8 p[2][2], vx[2];
+        vx[0] = values(0);
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -161,28 +223,25 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float x0 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e], scale, -m)), x1 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e + 1], scale, -m));
-                    l += x0 + x1;
                     w[e] = bf16_pair(x0, x1);
+                    l += x0 + x1;
                 }
                 p[b][j] = __builtin_bit_cast(bf16x8, w);
             }
 #pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    // lane (c, d): positions 8 c .. + 7 of dimension d, four at a time of 16 dimensions by 16 lanes
-                    s16x4 x[2];
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const int at = 32 * b + 16 * j + 8 * c + 4 * u + (lane >> 2 & 3), pair = 2 * i + (lane >> 4 & 1);
-                        x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LOCAL s16x4 *)(v_s + at * RW + 16 * (pair ^ v_turn<PIECES>(at)) + 4 * (lane & 3)));
-                    }
-                    typedef short s16x8 __attribute__((ext_vector_type(8)));
-                    const bf16x8 vx = __builtin_bit_cast(bf16x8, s16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]});
-                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vx, p[b][j], acc[i], 0, 0, 0);
-                }
+        for (int n = 0; n < 4 * NB; n++) {
+            if (n + 1 < 4 * NB) vx[(n + 1) & 1] = values(n + 1);
+            acc[n % NB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vx[n & 1], p[n / NB >> 1][n / NB & 1], acc[n % NB], 0, 0, 0);
+        }
+    };
+    auto turn = [&](int tile, const uint16_t *k_s, const uint16_t *v_s, uint16_t *next_k, uint16_t *next_v) {
+        loads_done();                                                // this tile is here, and nobody reads the last one any more
+        if (tile + 1 < tiles) loads.request(tile + 1, next_k, next_v);
+        if (tile * TILE <= high) step(tile, k_s, v_s);
+    };
+    for (int tile = 0; tile < tiles; tile += 2) {
+        turn(tile, k0_s, v0_s, k1_s, v1_s);
+        if (tile + 1 < tiles) turn(tile + 1, k1_s, v1_s, k0_s, v0_s);
     }
     if (!rows) return;
     float y;
@@ -247,6 +306,7 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
     };
     if (!apart(k) || !apart(v)) return l3m_dev_fail("attend_packed: out overlaps k or v");
     if (on_batch(b, out, ob)) return l3m_dev_fail("attend_packed: out overlaps the batch");
+    if (kv_stride > 1 << 23) return l3m_dev_fail("attend_packed: rows of K and V may be up to 2^23 values apart");   // a tile's offsets in 32 bits
     const int g = nq / nkv;
     if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("attend_packed: too many rows for one call");
     const long long items = (long long)b->n * g / (ROWS * WAVES) + b->seqs;
