@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int TILE = 64, ROWS = 32, WAVES = 4;
+constexpr int TILE = 64, ROWS = 32, WAVES = 4, CUS = 256;
 constexpr float M0 = -3.40282347e38f;                                // the maximum of no score: float32's lowest
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -89,6 +89,37 @@ __device__ __forceinline__ void loads_done() {                       // and the 
     __syncthreads();
 }
 
+// Groups of ROWS WAVES rows, a workgroup's. Those of the last rows have the most tiles, so they come first, over all runs, or the longest run's would be left at the end:
+// the item-th of a kv head's groups by descending number in their run (up to 64 runs; more fill the card without an order). Where all are resident
+// at once, two to a CU, the second ones come shortest first, so that a CU's two are about as long together as any other's.
+__device__ __forceinline__ int groups_of(int rows, int g) { return (int)(((unsigned)rows * (unsigned)g + ROWS * WAVES - 1) / (ROWS * WAVES)); }
+__device__ __forceinline__ Found group_of(const Runs &b, int g, int item, int items, int cus) {
+    if (items <= 2 * cus && item >= cus) item = cus + items - 1 - item;
+    if (b.seqs > 64) return find_run(b, items - 1 - item, [&](int, int, int rows) { return groups_of(rows, g); });
+    const int lane = threadIdx.x & 63;
+    int s0 = 0, rows = 0;
+    if (lane < b.seqs) {
+        s0 = b.from(lane);
+        rows = b.to(lane, s0) - s0;
+    }
+    const int groups = groups_of(rows, g);
+    // the highest level at which more than `item` groups lie at it or above
+    auto above = [&](int level) { return __builtin_amdgcn_readlane(scan_wave(max(groups - level, 0)), 63); };
+    int level = 0, top = (int)max_wave((float)min(groups, 1 << 24));
+    if (above(0) <= item) return {-1, 0, 0, 0};
+    while (top - level > 1) {
+        const int mid = (level + top) >> 1;
+        if (above(mid) > item) level = mid;
+        else top = mid;
+    }
+    const int rank = item - above(level + 1);                        // among the runs that have a group there
+    const bool has = groups > level;
+    const int before = scan_wave(has) - has;
+    const uint64_t at = __ballot(has && before == rank);
+    const int l = __builtin_ctzll(at);
+    return {l, level, __builtin_amdgcn_readlane(s0, l), __builtin_amdgcn_readlane(rows, l)};
+}
+
 // One row by the formula, a position at a time: for rows whose products met a value that is not finite behind their token.
 __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *k, const uint16_t *v, int seen, uint16_t *out) {
     const int lane = threadIdx.x & 63;
@@ -119,8 +150,9 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
     // two tiles: the next one comes while one is used. Arrays of their own, so that the compiler sees that reads of one do not wait for the other's requests
     __shared__ __align__(16) uint16_t k0_s[TILE * RW], v0_s[TILE * RW], k1_s[TILE * RW], v1_s[TILE * RW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, c = lane >> 5, hd = a.hd, g = a.g;
-    const int h = (int)(blockIdx.x % (unsigned)a.nkv), item = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)a.nkv);
-    const Found f = find_run(a.b, item, [&](int, int, int rows) { return (int)(((unsigned)rows * g + ROWS * WAVES - 1) / (ROWS * WAVES)); });
+    // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
+    const int h = (int)(blockIdx.x % (unsigned)a.nkv);
+    const Found f = group_of(a.b, g, (int)(blockIdx.x / (unsigned)a.nkv), (int)(gridDim.x / (unsigned)a.nkv), CUS / a.nkv);
     if (f.run < 0) return;
     const uint16_t *q = a.q + (long long)f.s0 * a.q_stride, *k = a.k + (long long)f.s0 * a.kv_stride + h * hd, *v = a.v + (long long)f.s0 * a.kv_stride + h * hd;
     uint16_t *out = a.out + (long long)f.s0 * a.out_stride;
@@ -243,6 +275,7 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
         turn(tile, k0_s, v0_s, k1_s, v1_s);
         if (tile + 1 < tiles) turn(tile + 1, k1_s, v1_s, k0_s, v0_s);
     }
+    __syncthreads();                                                 // the tiles are done with
     if (!rows) return;
     float y;
     l = other_half(l, y);
@@ -269,16 +302,27 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
         const int r = __builtin_ctz(of), t = __builtin_amdgcn_readlane(token, r), hh = __builtin_amdgcn_readlane(head, r);
         row_alone(a, q + (long long)t * a.q_stride + (long long)hh * hd, k, v, t + 1, out + (long long)t * a.out_stride + (long long)hh * hd);
     }
-    if (r32 >= rows || wrong >> r32 & 1u) return;
-    uint16_t *to = out + (long long)token * a.out_stride + (long long)head * hd;
+    // through LDS, 32 rows a wavefront, so that rows leave in whole lines; a row's pieces of 16 bytes in the order that K's have
+    constexpr int HP = 32 * NB;
+    uint16_t *o_s = wave < 2 ? k0_s + wave * ROWS * HP : v0_s + (wave - 2) * ROWS * HP;
+    static_assert(WAVES == 4 && 2 * ROWS * HP <= TILE * RW, "");
     const float by = 1.f / l;
 #pragma unroll
     for (int i = 0; i < NB; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int d = 32 * i + 8 * j + 4 * c;
-            if (d < hd) *(u32x2 *)(to + d) = u32x2{bf16_pair(acc[i][4 * j] * by, acc[i][4 * j + 1] * by), bf16_pair(acc[i][4 * j + 2] * by, acc[i][4 * j + 3] * by)};
-        }
+        for (int j = 0; j < 4; j++)
+            *(u32x2 *)(o_s + r32 * HP + 8 * ((4 * i + j) ^ (r32 & 3)) + 4 * c) = u32x2{bf16_pair(acc[i][4 * j] * by, acc[i][4 * j + 1] * by), bf16_pair(acc[i][4 * j + 2] * by, acc[i][4 * j + 3] * by)};
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) {
+        const int at = 64 * i + lane, r = at / (4 * NB), piece = at - r * (4 * NB);
+        const u32x4 x = *(const u32x4 *)(o_s + r * HP + 8 * (piece ^ (r & 3)));
+        if (r >= rows || 8 * piece >= hd || wrong >> r & 1u) continue;
+        const int rr = row0 + r, t = (int)divide(rr, g, a.g_mul), hh = h * g + rr - t * g;
+        *(u32x4 *)(out + (long long)t * a.out_stride + (long long)hh * hd + 8 * piece) = x;
+    }
 }
 
 }  // namespace
