@@ -301,7 +301,6 @@ template <int N> __device__ __forceinline__ void in_parts(const float (&v)[8], b
 // have a chunk each, all nearly equal, and their parts are joined by a second launch. The lengths lie in device memory, so each workgroup counts the work and
 // finds its share of it by itself (share_of), the same in both launches.
 constexpr int SPLIT_ROWS = 1 << 14, SPLIT_FROM = 1024;
-constexpr int WAVES = 4;
 constexpr int TARGET = 512;                                          // workgroups that the work is spread over
 struct AttendIn {
     l3m_kv8     c;
@@ -311,8 +310,11 @@ struct AttendIn {
     long long   q_stride, out_stride;
     const int32_t *table, *len, *state;
     float      *ml, *parts;                                          // [slot][row] maximum and sum, output; a slot's rows: slot_rows
-    int         layer, pages, seqs, width, nq, g, target, least, slot_rows; // target: workgroups of a kv head, 0: nothing is split; least: tiles of a part
-    uint32_t    g_mul;
+    int         pages, seqs, width, nq, g, target, least, slot_rows; // target: workgroups of a kv head, 0: nothing is split; least: tiles of a part
+    uint32_t    g_mul, nkv_mul;                                      // of g and of nkv (divide)
+    uint8_t    *mem;                                                 // the layer's part of page 0
+    size_t      page_bytes;
+    float       scale;                                               // of the scores: base 2
 };
 __device__ __forceinline__ int length_of(const AttendIn &a, int id) { return (unsigned)id < (unsigned)a.seqs ? clamp(a.len[id], 0, a.width * PAGE) : 0; }
 __device__ __forceinline__ int groups_of(int rows, int g) { return (int)(((unsigned)rows * (unsigned)g + 15) >> 4); }
@@ -354,13 +356,13 @@ template <bool GROUP> __device__ __forceinline__ Share share_of(const AttendIn &
     int base = 0, slots = 0;
     for (int r0 = 0; r0 < a.b.seqs; r0 += 64) {
         if (r0) read(r0, id, len, s0, rows);
-        const int groups = groups_of(rows, a.g), parts = max((int)((unsigned)(tiles_of(len) + chunk - 1) / (unsigned)chunk), 1), mine = groups * parts;
+        const int groups = groups_of(rows, a.g), parts = a.target ? max((int)((unsigned)(tiles_of(len) + chunk - 1) / (unsigned)chunk), 1) : 1, mine = groups * parts;
         const int upto = scan_wave(GROUP ? groups : mine) + base, slot = scan_wave(parts > 1 ? mine : 0) + slots;
         const uint64_t here = __ballot(upto > item);
         if (here) {
             const int l = __builtin_ctzll(here);
             auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-            const int n = of(parts), at = item - (of(upto) - of(GROUP ? groups : mine)), group = GROUP ? at : (int)((unsigned)at / (unsigned)n);
+            const int n = of(parts), at = item - (of(upto) - of(GROUP ? groups : mine)), group = GROUP || n == 1 ? at : (int)((unsigned)at / (unsigned)n);
             return {r0 + l, of(id), of(len), of(s0), of(rows), group, GROUP ? 0 : at - group * n, n, of(slot) - of(parts > 1 ? mine : 0) + group * n};
         }
         base = __builtin_amdgcn_readlane(upto, 63);
@@ -440,7 +442,7 @@ __device__ __forceinline__ uint32_t bytes_before(int from, int end) {
     return n >= 4 ? ~0u : n <= 0 ? 0u : ~(~0u << 8 * n);
 }
 
-template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_attend(AttendIn a) {
+template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WAVES) k_kv8_attend(AttendIn a) {
     constexpr int QP = Parts<F32>::q, PP = Parts<F32>::p, HP = 32 * NB, OS = HP + 4, REQUESTS = 2 * NB;
     __shared__ __align__(16) uint8_t k_s[WAVES][TILE * HP], v_s[WAVES][TILE * HP];
     __shared__ float m_s[WAVES][16], l_s[WAVES][16];
@@ -448,9 +450,9 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     float (*o_s)[16][OS] = (float (*)[16][OS])k_s;                   // behind the tiles
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, c = lane >> 4, hd = a.c.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
-    const int h = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const int item = (int)divide(blockIdx.x, a.c.nkv, a.nkv_mul), h = (int)blockIdx.x - item * a.c.nkv;
     const bool failed = *(const CONSTANT int32_t *)a.state != 0;
-    const Share f = share_of<false>(a, (int)(blockIdx.x / (unsigned)a.c.nkv));
+    const Share f = share_of<false>(a, item);
     if (f.run < 0) return;
     const int len = f.len, row0 = 16 * f.group, rows = min(f.rows * g - row0, 16);
     // the row of this lane's column: its token, and the positions it sees
@@ -458,8 +460,12 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     const int last = (int)divide(row0 + rows - 1, g, a.g_mul), end = max(len - f.rows + last + 1, 0);
     const int whole = max(len - f.rows + (int)divide(row0, g, a.g_mul) + 1, 0) / TILE;     // tiles that every row sees whole
     // this part's tiles (of all the sequence's; the last ones may lie behind every row)
-    const int all = tiles_of(len), share = all / f.parts, more = all - share * f.parts, t0 = f.part * share + min(f.part, more);
-    const int t1 = min(t0 + share + (f.part < more), tiles_of(end));
+    int t0 = 0, t1 = tiles_of(end);
+    if (f.parts > 1) {
+        const int all = tiles_of(len), share = all / f.parts, more = all - share * f.parts;
+        t0 = f.part * share + min(f.part, more);
+        t1 = min(t0 + share + (f.part < more), t1);
+    }
     const CONSTANT int32_t *table = (const CONSTANT int32_t *)(a.table + (size_t)f.id * a.width);
     // the pages' numbers come a turn ahead of their use
     auto page_of = [&](int t) { return table[min(t, max(t1 - 1, 0)) * TILE / PAGE]; };
@@ -472,8 +478,8 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     auto tile_at = [&](int t, int page) {
         const int half = min(t, max(t1 - 1, 0)) & 1;
         const bool lost = (unsigned)page >= (unsigned)a.pages;
-        const Unit u = unit_of(a.c, lost ? 0 : page, a.layer, h);
-        return Tile{u.k + half * TILE * HP, u.v + half * TILE, (const CONSTANT uint32_t *)u.s, half, lost};
+        const uint8_t *at = a.mem + (lost ? 0 : page) * a.page_bytes, *k = at + h * (2 * PAGE * HP);
+        return Tile{k + half * TILE * HP, k + PAGE * HP + half * TILE, (const CONSTANT uint32_t *)(at + a.c.nkv * (2 * PAGE * HP) + 2 * SCALES * h), half, lost};
     };
     int tile = t0 + wave;
     Queries<F32, NB> qs;
@@ -485,7 +491,7 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
     request_k<NB>(u.k, my_k, lane);
     request_v<NB>(u.v, my_v, lane);
     qs.arrived();                                                    // here, or the loop waits for all requests at its top
-    const float scale = 1.44269504f / sqrtf((float)hd);             // of the scores: base 2
+    const float scale = a.scale;
 
     f32x4 acc[2 * NB];
 #pragma unroll
@@ -500,26 +506,32 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
         f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // products onto different sums side by side: one waits for the last onto its own
 #pragma unroll
-        for (int i = 0; i < NB; i += 2)
+        for (int i = 0; i < NB; i += 2) {
+            u32x2 w[2][4];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 const int row = position_of(t, r16);
                 const uint8_t *at = my_k + row * HP;
-                u32x2 w[2];
                 if (i + 1 < NB) {
                     const u32x4 x = *(const u32x4 *)(at + 16 * ((2 * i + c) ^ k_turn<NB>(row)));
-                    w[0] = u32x2{x.x, x.y};
-                    w[1] = u32x2{x.z, x.w};
-                } else w[0] = *(const u32x2 *)(at + 16 * ((2 * i + (c >> 1)) ^ k_turn<NB>(row)) + 8 * (c & 1));
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                    if (i + j < NB) {
-                        const bf16x8 x = widen(w[j], sk);
-#pragma unroll
-                        for (int q = QP - 1; q >= 0; q--) s[t] = mfma(x, qs.part[i + j < NB ? i + j : 0][q], s[t]);
-                    }
+                    w[0][t] = u32x2{x.x, x.y};
+                    w[1][t] = u32x2{x.z, x.w};
+                } else w[0][t] = *(const u32x2 *)(at + 16 * ((2 * i + (c >> 1)) ^ k_turn<NB>(row)) + 8 * (c & 1));
             }
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (i + j < NB) {
+                    bf16x8 x[4];
+#pragma unroll
+                    for (int t = 0; t < 4; t++) x[t] = widen(w[j][t], sk);
+#pragma unroll
+                    for (int q = QP - 1; q >= 0; q--)
+#pragma unroll
+                        for (int t = 0; t < 4; t++) s[t] = mfma(x[t], qs.part[i + j < NB ? i + j : 0][q], s[t]);
+                }
+        }
         u = tile_at(tile + WAVES, page);
         reads_done();
         request_k<NB>(u.k, my_k, lane);
@@ -531,9 +543,11 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
         const int p0 = tile * TILE + 16 * c;                         // of p[i]: p0 + i
 #pragma unroll
         for (int i = 0; i < 16; i++) p[i] = s[i >> 2][i & 3];
-        if (masked || lost)
+        if (__builtin_expect(masked || lost, 0)) {
+            asm volatile("");                                        // no selects for all tiles' sake
 #pragma unroll
             for (int i = 0; i < 16; i++) p[i] = p0 + i >= seen ? -INFINITY : lost ? NAN : p[i];
+        }
         float top = p[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) top = fmaxf(top, p[i]);
@@ -558,22 +572,28 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
         }
         requests_but<REQUESTS>();                                    // the next K's, which came behind V's
         auto values = [&](int t) { return *(const u32x4 *)(my_v + (16 * t + r16) * TILE + 16 * (c ^ v_turn(16 * t + r16))); };
-        // 16 dimensions' values of the positions before `upto` of the tile
-        auto product = [&](int t, f32x4 to, auto some, int upto) {
-            const u32x4 v = values(t);
+        // 32 dimensions' sums with their values at the positions before `upto` of the tile
+        auto product = [&](int t, f32x4 &to0, f32x4 &to1, auto some, int upto) {
+            const u32x4 v[2] = {values(t), values(t + 1)};
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                u32x2 z = {v[2 * j], v[2 * j + 1]};
-                if constexpr (decltype(some)::value) z = u32x2{z.x & bytes_before(16 * c + 8 * j, upto), z.y & bytes_before(16 * c + 8 * j + 4, upto)};
-                const bf16x8 x = widen(z, sv);
+                bf16x8 x[2];
 #pragma unroll
-                for (int q = PP - 1; q >= 0; q--) to = mfma(x, w[j][q], to);
+                for (int i = 0; i < 2; i++) {
+                    u32x2 z = {v[i][2 * j], v[i][2 * j + 1]};
+                    if constexpr (decltype(some)::value) z = u32x2{z.x & bytes_before(16 * c + 8 * j, upto), z.y & bytes_before(16 * c + 8 * j + 4, upto)};
+                    x[i] = widen(z, sv);
+                }
+#pragma unroll
+                for (int q = PP - 1; q >= 0; q--) {
+                    to0 = mfma(x[0], w[j][q], to0);
+                    to1 = mfma(x[1], w[j][q], to1);
+                }
             }
-            return to;
         };
         if (!masked) {
 #pragma unroll
-            for (int t = 0; t < 2 * NB; t++) acc[t] = product(t, acc[t], std::false_type{}, 0);
+            for (int t = 0; t < 2 * NB; t += 2) product(t, acc[t], acc[t + 1], std::false_type{}, 0);
         } else {
             uint32_t nan = 0;                                        // codes of NaN among the values that some row sees
 #pragma unroll
@@ -585,10 +605,14 @@ template <bool F32, int NB> __global__ void __launch_bounds__(64 * WAVES) k_kv8_
             const bool apart = __ballot(nan != 0) != 0;              // a NaN is the rows' that see it: a token's rows at a time, over its own positions
             for (int to = apart ? min(seen, end) : end, at = __builtin_amdgcn_readfirstlane(to);;) {
 #pragma unroll
-                for (int t = 0; t < 2 * NB; t++) {
-                    const f32x4 part = product(t, acc[t], std::true_type{}, at - tile * TILE);
+                for (int t = 0; t < 2 * NB; t += 2) {
+                    f32x4 part[2] = {acc[t], acc[t + 1]};
+                    product(t, part[0], part[1], std::true_type{}, at - tile * TILE);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][i] = to == at ? part[i] : acc[t][i];
+                    for (int i = 0; i < 4; i++) {
+                        acc[t][i] = to == at ? part[0][i] : acc[t][i];
+                        acc[t + 1][i] = to == at ? part[1][i] : acc[t + 1][i];
+                    }
                 }
                 int next = INT_MAX;                                  // the next larger number of positions that a row sees
                 for (uint64_t others = __ballot(to > at); others; others &= others - 1) next = min(next, __builtin_amdgcn_readlane(to, __builtin_ctzll(others)));
@@ -647,9 +671,9 @@ constexpr int PARTS = TARGET + 1;                       // most parts of a group
 template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join(AttendIn a) {
     __shared__ f32x4 o_s[JOIN];
     __shared__ float f_s[16][PARTS], sum_s[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, quads = hd >> 2, h = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, quads = hd >> 2, block = (int)divide(blockIdx.x, a.c.nkv, a.nkv_mul), h = (int)blockIdx.x - block * a.c.nkv;
     const bool failed = *(const CONSTANT int32_t *)a.state != 0;
-    const Share f = share_of<true>(a, (int)(blockIdx.x / (unsigned)a.c.nkv));
+    const Share f = share_of<true>(a, block);
     if (f.run < 0 || f.parts < 2) return;
     const int rows = min(f.rows * a.g - 16 * f.group, 16);
     auto at = [&](int part, int r) { return ((size_t)(f.slot + part) * a.c.nkv + h) * a.slot_rows + r; };
@@ -808,18 +832,23 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
     const long long groups = ((long long)b->n * g + 15) / 16 + b->seqs;
     if (groups * c->nkv > 1ll << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
-    // rows of many tokens fill the card by themselves
+    // rows of many tokens fill the card by themselves; and a join takes as long as some four turns of a workgroup's wavefronts
+    const int nb = padded(c->hd) / 32, waves = nb <= 4 && groups * c->nkv <= 256 ? 8 : 4;
     const bool split = (long long)b->n * nq <= SPLIT_ROWS && (longest == 0 ? (long long)p->width * PAGE : longest) > SPLIT_FROM;
     const int per = slot_rows(b->n, g), target = split ? target_of(c->nkv) : 0;
     float *ml = (float *)work;
-    const AttendIn a = {*c, runs_of(b), q, out, q_stride, out_stride, p->table, p->len, p->state, ml, ml + (2 * slots(c->nkv) * per + 3) / 4 * 4, layer, p->pages, p->seqs, p->width,
-                        nq, g, target, WAVES, per, multiplier(g, (uint64_t)b->n * g)};
+    const AttendIn a = {*c, runs_of(b), q, out, q_stride, out_stride, p->table, p->len, p->state, ml, ml + (2 * slots(c->nkv) * per + 3) / 4 * 4, p->pages, p->seqs, p->width,
+                        nq, g, target, 4, per, multiplier(g, (uint64_t)b->n * g), multiplier(c->nkv, (groups + target) * c->nkv), c->mem + layer * layer_bytes(c->nkv, c->hd),
+                        c->layers * layer_bytes(c->nkv, c->hd), 1.44269504f / sqrtf((float)c->hd)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
     const dim3 grid((unsigned)((groups + target) * c->nkv));
-#define ATTEND(NB)                                                                      \
-    if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_attend<true, NB>), grid, dim3(64 * WAVES), 0, st, a); \
-    else hipLaunchKernelGGL((k_kv8_attend<false, NB>), grid, dim3(64 * WAVES), 0, st, a)
+#define ATTEND(NB)                                                                                                                            \
+    if (NB <= 4 && waves == 8 && !split) {                                                                                                    \
+        if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_attend<true, NB <= 4 ? NB : 4, 8>), grid, dim3(512), 0, st, a);                    \
+        else hipLaunchKernelGGL((k_kv8_attend<false, NB <= 4 ? NB : 4, 8>), grid, dim3(512), 0, st, a);                                        \
+    } else if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_attend<true, NB, 4>), grid, dim3(256), 0, st, a);                               \
+    else hipLaunchKernelGGL((k_kv8_attend<false, NB, 4>), grid, dim3(256), 0, st, a)
     BY_BLOCKS(ATTEND)
     if (split) {
         const dim3 all((unsigned)(groups * c->nkv));

@@ -25,7 +25,9 @@ struct PromptIn {
     Runs            b;
     long long       q_stride, kv_stride, out_stride;
     int             nq, nkv, hd, g;
-    uint32_t        g_mul;
+    uint32_t        g_mul, nkv_mul;                                  // of g and of nkv (divide)
+    int             items, cus;                                      // groups of a kv head, at the most; CUs' share of it
+    float           scale;                                           // of the scores: base 2
 };
 
 // Values of a row in LDS, a power of two; pieces of 16 bytes.
@@ -126,14 +128,13 @@ __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *
     float qv[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) qv[i] = lane + 64 * i < a.hd ? bf16_float(q[lane + 64 * i]) : 0.f;
-    const float scale = 1.44269504f / sqrtf((float)a.hd);
     for (int p = 0; p < seen; p++) {
         float s = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) s += lane + 64 * i < a.hd ? qv[i] * bf16_float(k[(long long)p * a.kv_stride + lane + 64 * i]) : 0.f;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-        s *= scale;
+        s *= a.scale;
         const float top = fmaxf(m, s), by = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top), e = __builtin_amdgcn_exp2f(s - top);
         l = l * by + e;
 #pragma unroll
@@ -151,8 +152,8 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
     __shared__ __align__(16) uint16_t k0_s[TILE * RW], v0_s[TILE * RW], k1_s[TILE * RW], v1_s[TILE * RW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, c = lane >> 5, hd = a.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
-    const int h = (int)(blockIdx.x % (unsigned)a.nkv);
-    const Found f = group_of(a.b, g, (int)(blockIdx.x / (unsigned)a.nkv), (int)(gridDim.x / (unsigned)a.nkv), CUS / a.nkv);
+    const int item = (int)divide(blockIdx.x, a.nkv, a.nkv_mul), h = (int)blockIdx.x - item * a.nkv;
+    const Found f = group_of(a.b, g, item, a.items, a.cus);
     if (f.run < 0) return;
     const uint16_t *q = a.q + (long long)f.s0 * a.q_stride, *k = a.k + (long long)f.s0 * a.kv_stride + h * hd, *v = a.v + (long long)f.s0 * a.kv_stride + h * hd;
     uint16_t *out = a.out + (long long)f.s0 * a.out_stride;
@@ -175,7 +176,7 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
     loads.request(0, k0_s, v0_s);
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) asm volatile("" : "+v"(qs[i]));   // here, or the loop waits for requests at its top
-    const float scale = 1.44269504f / sqrtf((float)hd);              // of the scores: base 2
+    const float scale = a.scale;
     f32x16 acc[NB];
 #pragma unroll
     for (int i = 0; i < NB; i++)
@@ -355,7 +356,8 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
     if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("attend_packed: too many rows for one call");
     const long long items = (long long)b->n * g / (ROWS * WAVES) + b->seqs;
     if (items * nkv > 1ll << 28) return l3m_dev_fail("attend_packed: too many rows for one call");
-    const PromptIn a = {q, k, v, out, {b->ids, b->starts, b->seqs, b->n}, q_stride, kv_stride, out_stride, nq, nkv, hd, g, multiplier(g, (uint64_t)b->n * g)};
+    const PromptIn a = {q, k, v, out, {b->ids, b->starts, b->seqs, b->n}, q_stride, kv_stride, out_stride, nq, nkv, hd, g, multiplier(g, (uint64_t)b->n * g), multiplier(nkv, items * nkv),
+                        (int)items, CUS / nkv, 1.44269504f / sqrtf((float)hd)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
     const dim3 grid((unsigned)(items * nkv)), wg(64 * WAVES);
