@@ -302,6 +302,7 @@ template <int N> __device__ __forceinline__ void in_parts(const float (&v)[8], b
 // finds its share of it by itself (share_of), the same in both launches.
 constexpr int SPLIT_ROWS = 1 << 14, SPLIT_FROM = 1024;
 constexpr int TARGET = 512;                                          // workgroups that the work is spread over
+constexpr int WORK = 25;                                             // a batch's work is up to 2^WORK units, of 2^unit tiles each; 64 lanes' are a sum in 32 bits
 struct AttendIn {
     l3m_kv8     c;
     Runs        b;
@@ -310,7 +311,7 @@ struct AttendIn {
     long long   q_stride, out_stride;
     const int32_t *table, *len, *state;
     float      *ml, *parts;                                          // [slot][row] maximum and sum, output; a slot's rows: slot_rows
-    int         pages, seqs, width, nq, g, target, least, slot_rows; // target: workgroups of a kv head, 0: nothing is split; least: tiles of a part
+    int         pages, seqs, width, nq, g, target, least, unit, slot_rows; // target: workgroups of a kv head, 0: nothing is split; least: units of a part
     uint32_t    g_mul, nkv_mul;                                      // of g and of nkv (divide)
     uint8_t    *mem;                                                 // the layer's part of page 0
     size_t      page_bytes;
@@ -342,16 +343,17 @@ template <bool GROUP> __device__ __forceinline__ Share share_of(const AttendIn &
     int id, len, s0, rows, chunk = 1 << 30;
     read(0, id, len, s0, rows);
     if (a.target) {
-        uint32_t work = 0;                                           // counted up to 2^31: more is no cache's
+        uint32_t work = 0;
         for (int r0 = 0;; r0 += 64) {
             int i = id, n = len, s = s0, m = rows;
             if (r0) read(r0, i, n, s, m);
-            // a lane's at most 2^25, so that 64 of them are a sum
-            const uint32_t more = (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)min((unsigned long long)groups_of(m, a.g) * (unsigned)tiles_of(n), 1ull << 25)), 63);
-            work = min(work, 1u << 31) + min(more, (1u << 31) - 1);
+            const unsigned units = (unsigned)(tiles_of(n) + (1 << a.unit) - 1) >> a.unit;
+            work += (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)min((unsigned long long)groups_of(m, a.g) * units, (1ull << WORK) + 1)), 63);
+            work = min(work, 2u << WORK);
             if (r0 + 64 >= a.b.seqs) break;
         }
-        chunk = max(a.least, (int)((work - 1) / (unsigned)a.target) + 1);
+        // more than that have only runs that overlap: nothing is split, or the parts would be more than the workspace's
+        if (work && work <= 1u << WORK) chunk = (int)min((unsigned long long)max((unsigned)a.least, (work - 1) / (unsigned)a.target + 1) << a.unit, 1ull << 30);
     }
     int base = 0, slots = 0;
     for (int r0 = 0; r0 < a.b.seqs; r0 += 64) {
@@ -836,9 +838,11 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     const int nb = padded(c->hd) / 32, waves = nb <= 4 && groups * c->nkv <= 256 ? 8 : 4;
     const bool split = (long long)b->n * nq <= SPLIT_ROWS && (longest == 0 ? (long long)p->width * PAGE : longest) > SPLIT_FROM;
     const int per = slot_rows(b->n, g), target = split ? target_of(c->nkv) : 0;
+    int unit = 0;
+    while (groups * ((2ll * p->width + (1 << unit) - 1) >> unit) > 1 << WORK) unit++;
     float *ml = (float *)work;
     const AttendIn a = {*c, runs_of(b), q, out, q_stride, out_stride, p->table, p->len, p->state, ml, ml + (2 * slots(c->nkv) * per + 3) / 4 * 4, p->pages, p->seqs, p->width,
-                        nq, g, target, 4, per, multiplier(g, (uint64_t)b->n * g), multiplier(c->nkv, (groups + target) * c->nkv), c->mem + layer * layer_bytes(c->nkv, c->hd),
+                        nq, g, target, 4, unit, per, multiplier(g, (uint64_t)b->n * g), multiplier(c->nkv, (groups + target) * c->nkv), c->mem + layer * layer_bytes(c->nkv, c->hd),
                         c->layers * layer_bytes(c->nkv, c->hd), 1.44269504f / sqrtf((float)c->hd)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;

@@ -323,3 +323,65 @@ def test_far_page(dev):
     out = dev.kv8_attend(c, p, layers - 1, q, dev.batch([0, 1], [1]))
     want, tol = attended(q, got[1][0], got[1][1], [130], 2.0 ** -24, 2.0 ** -126, 2.0 ** -24)
     assert np.all(np.abs(out - want) <= tol)
+
+
+def test_attend_much_work(dev):
+    """Groups of rows times tiles past 2^25: a table that names the same page 2^19 times. Nothing is written behind the workspace."""
+    nkv, hd, g, n, width = 1, 8, 16, 128, 1 << 19
+    c, p = dev.kv8(2, 1, nkv, hd), dev.pages(2, 2, width)
+    rng = np.random.default_rng(8)
+    x = [rng.standard_normal((PAGE, nkv, hd)).astype(np.float32) for _ in range(2)]
+    b = dev.batch([0, PAGE], [0])
+    dev.pages_grow(p, c, b)
+    dev.kv8_append(c, p, 0, *x, b)
+    k, v = dev.kv8_rows(c, p, 0, b)
+    table, lens = np.zeros((2, width), np.int32), np.int32([PAGE, PAGE * width])
+    for at, y in ((p.table, table), (p.len, lens)):
+        assert dev.lib.l3m_dev_upload(at, C.c_void_p(y.ctypes.data), y.nbytes) == 0
+    q = rng.standard_normal((n, g, hd)).astype(np.float32)
+    size = dev.lib.l3m_kv8_work_bytes(C.byref(c), n, g)
+    marks = np.full(size // 4 + 4096, 7.0, np.float32)
+    work, out, b = dev.put(marks), dev.alloc(q.nbytes), dev.batch([0, n], [1])
+    assert dev.lib.l3m_k_kv8_attend(out, g * hd, dev.put(q), g * hd, A.F32, C.byref(c), C.byref(p), 0, C.byref(b), g, 0, work, size, None) == 0
+    assert np.all(dev.get(work, marks.shape, np.float32)[size // 4:] == 7)
+    # position i of the page counts `width` times, those behind the token once less. Four parts a group, four wavefronts a part, 16 positions a lane and tile:
+    # sums of 2^20 terms, of the weights and of the values
+    got, want, size = dev.get(out, q.shape, np.float32), np.zeros(q.shape), np.zeros(q.shape)
+    z = np.einsum("tgd,id->tgi", q.astype(np.float64), k[:, 0].astype(np.float64)) / np.sqrt(hd)
+    for t in range(n):
+        w = np.exp(z[t] - z[t].max(1, keepdims=True)) * (width - (np.arange(PAGE) > t))
+        w /= w.sum(1, keepdims=True)
+        want[t], size[t] = w @ v[:, 0].astype(np.float64), w @ np.abs(v[:, 0].astype(np.float64))
+    assert np.all(np.abs(got - want) <= 2.0 ** -3 * size)
+
+
+def test_attend_runs_that_overlap(dev):
+    """Starts that go up and down give runs over the same rows, more of them than rows: nothing is written behind the workspace or the rows."""
+    o = Cache(dev, 70, 1, 32, pages=300, width=64, seed=9)
+    o.add([0, 1], [8000, 3000])
+    n, seqs, g = 64, 70, 4
+    q = o.rng.standard_normal((n, g, 32)).astype(np.float32)
+    b = dev.batch([0, n] * (seqs // 2) + [0], [i % 2 for i in range(seqs)], n=n)
+    size = dev.lib.l3m_kv8_work_bytes(C.byref(o.c), n, g)
+    work, out = dev.put(np.full(size // 4 + 4096, 7.0, np.float32)), dev.put(np.full(q.size + 4096, 7.0, np.float32))
+    assert dev.lib.l3m_k_kv8_attend(out, g * 32, dev.put(q), g * 32, A.F32, C.byref(o.c), C.byref(o.p), 1, C.byref(b), g, 0, work, size, None) == 0
+    assert np.all(dev.get(work, (size // 4 + 4096,), np.float32)[size // 4:] == 7) and np.all(dev.get(out, (q.size + 4096,), np.float32)[q.size:] == 7)
+
+
+@DTYPES
+def test_attend_split_of_many_runs(dev, dtype):
+    """More runs than a wavefront has lanes, some of them split, some without rows; heads of 128 and 256; a length that is said to be less than it is."""
+    o = Cache(dev, 150, 1, 128, pages=400, width=100, seed=10)
+    counts = [int(x) for x in o.rng.choice([0, 1, 2, 40], 150)]
+    counts[3], counts[77], counts[149] = 9001, 4000, 12000
+    o.add(list(range(150)), counts, dtype)
+    ids = [int(i) for i in o.rng.permutation(150)]
+    rows = [min(counts[i], int(o.rng.choice([0, 1, 3]))) for i in ids]
+    got = attend(o, ids, rows, 4, dtype, longest=12000)
+    dev.free_all()
+    o = Cache(dev, 2, 2, 256, pages=60, width=50, seed=11)
+    o.add([0, 1], [6000, 70], dtype)
+    q = typed(o.rng.standard_normal((2, 6, 256)), dtype)
+    far = attend(o, [0, 1], [1, 1], 6, dtype, q=q)
+    near = attend(o, [0, 1], [1, 1], 6, dtype, longest=1, q=q)
+    assert got.size and far.shape == near.shape
