@@ -207,8 +207,9 @@ int l3m_k_rotary(const l3m_rotary *r, void *q, int q_stride, void *k, int k_stri
                  const int32_t *pos, int pos0, void *stream);
 
 // Causal attention over whole prompts, bf16: row t of a run over the run's rows 0 .. t, scores q.k / sqrt(hd), query head h reads kv head h / (nq / nkv). Rows'
-// strides and starts are multiples of 8 values and 16 bytes, hd a multiple of 8 up to 256. out may be q. Sums are float32's; weights are rounded to bf16, as the
-// result is. What lies behind a token, NaN among it, does not reach it.
+// strides and starts are multiples of 8 values and 16 bytes, hd a multiple of 8 up to 256, rows of k and v up to 2^23 values apart. out may be q. Sums are
+// float32's, of values times weights of up to 2^8, and divided at the end; weights are rounded to bf16, as the result is, and those below 2^-126 of the largest
+// may count as none. What lies behind a token, NaN among it, does not reach it.
 int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_stride, const uint16_t *k, const uint16_t *v, int kv_stride, const l3m_batch *b,
                         int nq, int nkv, int hd, void *stream);
 
@@ -216,6 +217,7 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
 // need not be cleared. A page holds for each layer nkv units [K codes 128 x HP][V codes HP x 128], HP hd rounded up to 32, then 8 bytes a head: the
 // exponents of K's and of V's scales for its four blocks of 32 positions; a layer's part is rounded up to 256 bytes. Codes are OCP e4m3; a scale is 2^(byte - 127),
 // the smallest from 2^-126 up by which the block's largest finite value of that head is at most 448; a value that is not finite is stored as NaN.
+// (Values from 248 2^120 up, float32's largest, are stored as 256 2^120, which reads as infinity.)
 #define L3M_PAGE 128
 typedef struct {
     uint8_t *mem;
@@ -261,8 +263,9 @@ int l3m_k_kv8_append(const l3m_kv8 *c, const l3m_pages *p, int layer, const void
 int l3m_k_kv8_rows(const l3m_kv8 *c, const l3m_pages *p, int layer, float *k, float *v, const l3m_batch *b, void *stream);
 // Attention of a batch's rows, the last positions of their sequences, each over its sequence up to itself: q and out [n] of nq heads, dtype L3M_HIP_F32 or _BF16,
 // out may be q; hd and heads as above. A row before its sequence's first position is zeros. Sums are float32's; queries and weights count in
-// 24 bits (f32), or queries exactly and weights in 16 (bf16). longest: no sequence is longer, as far as the
-// caller knows (0: not known); it decides how the work is split and no result's meaning. work: l3m_kv8_work_bytes(c, n, nq), 16-byte aligned, of any contents,
+// 24 bits (f32), or queries exactly and weights in 16 (bf16), weights below 2^-126 of the largest perhaps not at all; held values count exactly from 2^-126 up, in
+// steps of 2^-133 below. longest: no sequence is longer, as far as the caller knows (0: not known); it decides how the work is split and no result's
+// meaning. work: l3m_kv8_work_bytes(c, n, nq), 16-byte aligned, of any contents,
 // used by one call at a time (a captured call uses it at every replay); a larger n's serves a smaller one.
 size_t l3m_kv8_work_bytes(const l3m_kv8 *c, int n, int nq);
 int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int dtype, const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_batch *b, int nq,

@@ -277,8 +277,8 @@ __device__ __forceinline__ bf16x8 widen(u32x2 w, float scale) {
     r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, scale, true));
     return __builtin_bit_cast(bf16x8, r);
 }
-// Eight values as the sum of N bf16 ones each.
-template <int N> __device__ __forceinline__ void in_parts(const float (&v)[8], bf16x8 (&w)[N]) {
+// Eight values as the sum of N bf16 ones each, the weights' nearest ones. TOWARDS_0: three of them are exactly float32's 24 bits, and the largest values stay finite.
+template <int N, bool TOWARDS_0 = false> __device__ __forceinline__ void in_parts(const float (&v)[8], bf16x8 (&w)[N]) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = v[i];
@@ -287,7 +287,7 @@ template <int N> __device__ __forceinline__ void in_parts(const float (&v)[8], b
         u32x4 r;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            r[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+            r[i] = TOWARDS_0 ? __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u) : bf16_pair(x[2 * i], x[2 * i + 1]);
             if (p + 1 < N) {
                 x[2 * i] -= __uint_as_float(r[i] << 16);
                 x[2 * i + 1] -= __uint_as_float(r[i] & 0xFFFF0000u);
@@ -388,7 +388,7 @@ template <bool F32, int NB> struct Queries {
             else load8((const uint16_t *)q + at + (in ? d : 0), x);
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = in ? x[i] : 0.f;
-            in_parts<QP>(x, part[s]);
+            in_parts<QP, true>(x, part[s]);
         }
     }
     __device__ __forceinline__ void arrived() {
@@ -499,11 +499,12 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
 #pragma unroll
     for (int t = 0; t < 2 * NB; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = M0, l = 0.f;
+    bool large = false;                                              // some row's m is (LARGE_SCORE)
     for (; tile < t1; tile += WAVES) {
         const bool lost = u.lost, masked = tile >= whole;
         const int left = end - tile * TILE;                          // positions that some row sees
         const float sk = pow2_byte((int)(ks >> (16 * u.half + 8 * (r16 >> 3)) & 255u));
-        const float sv = 32 * (c >> 1) < left ? pow2_byte((int)(vs >> (16 * u.half + 8 * (c >> 1)) & 255u)) : 1.f;   // 1: never written
+        const float sv = !lost && 32 * (c >> 1) < left ? pow2_byte((int)(vs >> (16 * u.half + 8 * (c >> 1)) & 255u)) : 1.f;   // 1: never written
         requests_but<REQUESTS>();                                    // V's, which came behind K's
         f32x4 s[4];
 #pragma unroll
@@ -560,6 +561,15 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
 #pragma unroll
             for (int t = 0; t < 2 * NB; t++) acc[t] *= by;
             m = top;
+            large = __ballot(fabsf(m) > LARGE_SCORE && m != M0) != 0;
+        }
+        float by = scale, less = m;
+        if (__builtin_expect(large, 0)) {
+            asm volatile("");
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = scaled_less(p[i], scale, m);
+            by = 1.f;
+            less = 0.f;
         }
         bf16x8 w[2][PP];
 #pragma unroll
@@ -567,7 +577,7 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[i] = __builtin_amdgcn_exp2f(fmaf(p[8 * t + i], scale, -m));
+                x[i] = __builtin_amdgcn_exp2f(fmaf(p[8 * t + i], by, -less));
                 l += x[i];
             }
             in_parts<PP>(x, w[t]);

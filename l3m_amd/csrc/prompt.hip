@@ -183,6 +183,7 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
     float m = M0, l = 0.f;
+    bool large = false;                                              // some row's m is (LARGE_SCORE)
 
     auto step = [&](int tile, const uint16_t *k_s, const uint16_t *v_s) {
         f32x16 s[2];
@@ -233,6 +234,17 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
 #pragma unroll
             for (int i = 0; i < NB; i++) acc[i] *= by;
             m = to;
+            large = __ballot(fabsf(m) > LARGE_SCORE && m != M0) != 0;
+        }
+        float by = scale, less = m;
+        if (__builtin_expect(large, 0)) {
+            asm volatile("");
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[b][j] = scaled_less(s[b][j], scale, m);
+            by = 1.f;
+            less = 0.f;
         }
         // lane (c, d): positions 8 c .. + 7 of dimension d, four at a time of 16 dimensions by 16 lanes
         auto values = [&](int n) {
@@ -255,7 +267,7 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
                 u32x4 w;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float x0 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e], scale, -m)), x1 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e + 1], scale, -m));
+                    const float x0 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e], by, -less)), x1 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e + 1], by, -less));
                     w[e] = bf16_pair(x0, x1);
                     l += x0 + x1;
                 }

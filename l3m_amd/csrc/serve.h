@@ -60,6 +60,15 @@ __device__ __forceinline__ float max_wave(float x) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// The exponents of a softmax are fma(s, scale, -m), m the rounded product of the largest score: off by half a unit of m, alike for all of a row and so for no
+// result's sake, while that is small. From here on it isn't, and both are rounded alike (x scale - m).
+constexpr float LARGE_SCORE = 16777216.f;
+__device__ __forceinline__ float scaled_less(float x, float scale, float m) {
+#pragma clang fp contract(off)
+    const float y = x * scale;
+    return y - m;
+}
+
 // A batch as kernels take it: starts whatever they hold are brought into 0 .. n, in order.
 struct Runs {
     const int32_t *ids, *starts;

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import l3m_amd as A
-from serve import BLOCK, PAGE, Blocks, attended, from_bf16, typed, values
+from serve import BLOCK, PAGE, Blocks, attended, bf16, from_bf16, typed, values
 
 pytestmark = pytest.mark.gpu
 DTYPES = pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -157,7 +157,7 @@ def test_bad_pages_and_sequences(dev):
 
 # ---------------------------------------------------------------- attention
 
-def attend(o, ids, counts, nq, dtype, longest=0, size=1.0, q=None):
+def attend(o, ids, counts, nq, dtype, longest=0, size=1.0, q=None, held=lambda x: x):
     """The cache's attention and its error's bound."""
     n = sum(counts)
     q, qx = q or typed(o.rng.standard_normal((n, nq, o.hd)) * size, dtype)
@@ -165,7 +165,7 @@ def attend(o, ids, counts, nq, dtype, longest=0, size=1.0, q=None):
     got = values(o.dev.kv8_attend(o.c, o.p, o.layer, q, o.dev.batch(starts, ids), longest))
     f32 = dtype == "f32"
     for i, s in enumerate(ids):
-        k, v = (o.want(s, kv) for kv in (0, 1))
+        k, v = (held(o.want(s, kv)) for kv in (0, 1))
         rows = slice(starts[i], starts[i + 1])
         seen = [len(k) - counts[i] + t + 1 for t in range(counts[i])]
         # weights in three parts of bf16 are off by 2^-24 of themselves, in two by 2^-16; one below 2^-126 of the largest may be zero
@@ -385,3 +385,55 @@ def test_attend_split_of_many_runs(dev, dtype):
     far = attend(o, [0, 1], [1, 1], 6, dtype, q=q)
     near = attend(o, [0, 1], [1, 1], 6, dtype, longest=1, q=q)
     assert got.size and far.shape == near.shape
+
+
+@DTYPES
+def test_attend_very_large_scores(dev, dtype):
+    """Scores of 10^4 to 10^34, positive and negative, the largest ones apart by far or the same: one position takes all the weight, or several take equal parts."""
+    hd, n = 64, 700
+    rng = np.random.default_rng(12)
+    for sign in (1, -1):
+        o = Cache(dev, 1, 1, hd, seed=13)
+        k = np.zeros((n, 1, hd), np.float32)
+        k[:, 0, 5] = 2.0 ** -rng.integers(0, 8, n)                    # exactly held
+        k[:, 0, 5][k[:, 0, 5] == (1 if sign > 0 else 2.0 ** -7)] = 2.0 ** -3
+        best = [7, 133, 300, 690]
+        k[best, 0, 5] = 1 if sign > 0 else 2.0 ** -7
+        v = rng.standard_normal((n, 1, hd)).astype(np.float32)
+        o.add([0], [n], rows=[(k, k), (v, v)])
+        held = o.want(0, 1)[:, 0]
+        for e in (20, 40, 70, 100, 113):
+            q = np.zeros((20, 3, hd), np.float32)
+            q[..., 5] = sign * 2.0 ** e * (1 + np.arange(3) / 4)
+            got = values(o.dev.kv8_attend(o.c, o.p, o.layer, typed(q, dtype)[0], dev.batch([0, 20], [0])))
+            for t in range(20):
+                rows = held[[b for b in best if b <= n - 20 + t]]
+                # weights are 1 or 0; sums of four, a quotient, and the rounding to bf16
+                tol = 6 * 2.0 ** -24 * np.abs(rows).mean(0) + (2.0 ** -8 if dtype == "bf16" else 0) * (np.abs(rows.mean(0)) + 1e-6)
+                assert np.all(np.abs(got[t] - rows.mean(0)) <= tol), (sign, e, t)
+        dev.free_all()
+
+
+def test_attend_largest_queries(dev):
+    """float32's largest values as queries of keys so small that the scores are ordinary: bf16 has no value that near them."""
+    o = Cache(dev, 1, 1, 32, seed=14)
+    o.add([0], [90], size=2.0 ** -126)
+    q = np.float32(o.rng.choice([-1, 1], (2, 4, 32)) * 3.4028e38)
+    # what is held of them is taken as bf16, which is the same from 2^-126 up and in steps of 2^-133 below
+    attend(o, [0], [2], 4, "f32", q=(q, q), held=lambda x: from_bf16(bf16(x)))
+
+
+@DTYPES
+def test_attend_lost_pages_are_their_rows(dev, dtype):
+    """A page that is none takes the rows that see it and no others, whatever the cache's unwritten pages hold."""
+    o = Cache(dev, 2, 1, 32, pages=6, width=3, seed=15)
+    dev.pages_grow(o.p, o.c, dev.batch([0, 1], [1]))                 # page 0: never written
+    o.add([0], [130], dtype)
+    q, qx = typed(o.rng.standard_normal((4, 2, 32)), dtype)
+    b = dev.batch([0, 4], [0])
+    whole = values(dev.kv8_attend(o.c, o.p, 1, q, b))
+    table = dev.get(o.p.table, (2, 3), np.int32)
+    table[0, 1] = -1
+    assert dev.lib.l3m_dev_upload(o.p.table, C.c_void_p(table.ctypes.data), table.nbytes) == 0
+    got = values(dev.kv8_attend(o.c, o.p, 1, q, b))
+    assert np.array_equal(got[:2], whole[:2]) and np.isnan(got[2:]).all()

@@ -120,3 +120,28 @@ def test_strides(dev):
     assert np.array_equal(got[:, qw:], x[:, qw:]) and np.array_equal(got[:10], x[:10]) and np.array_equal(got[140:], x[140:])
     assert np.array_equal(got[10:140, :qw], want[10:140])
     check(want[10:140].reshape(130, nq, hd), q[10:140], k[10:140], v[10:140], [50, 80])
+
+
+def test_very_large_scores(dev):
+    """Scores of 10^4 to 10^34, positive and negative, the largest ones apart by far or the same: one position takes all the weight, or several take equal parts."""
+    rng = np.random.default_rng(5)
+    n, hd = 300, 64
+    for sign in (1, -1):
+        top = 1.0 if sign > 0 else 2.0 ** -7
+        k = np.zeros((n, 1, hd), np.float32)
+        k[:, 0, 5] = 2.0 ** -rng.integers(1, 7, n)
+        best = [0, 7, 133, 280]
+        k[best, 0, 5] = top
+        v = rows(rng, n, 1, hd)
+        for e in (20, 40, 70, 100, 113):
+            q = np.zeros((n, 3, hd), np.float32)
+            q[..., 5] = sign * 2.0 ** e * (1 + np.arange(3) / 4)
+            got = from_bf16(dev.attend_packed(bf16(q), bf16(k), v, dev.batch([0, n])))
+            for t in range(n):
+                want = from_bf16(v)[[b for b in best if b <= t], 0]
+                # weights are alike or 0; sums of four, a quotient, and the rounding to bf16. And each weight's rounding to bf16, 2^-8, which its part of the
+                # sum of weights does not have: the largest weight is 2^(s c - m), m the rounded s c, which is off by up to 1/2 for m below 2^24, so no power of two
+                tol = (2.0 ** -8 + 6 * 2.0 ** -24) * np.abs(want).mean(0)
+                tol = tol + 2.0 ** -8 * (np.abs(want.mean(0)) + tol)
+                assert np.all(np.abs(got[t] - want.mean(0)) <= tol), (sign, e, t)
+        dev.free_all()
