@@ -72,7 +72,8 @@ struct RowsIn {
     float      *ok, *ov;                                             // rows out (read-back)
     long long  stride;
     const int32_t *table, *len, *state;
-    int        layer, pages, seqs, width;
+    int        layer, pages, seqs, width, per;                       // per: workgroups of a block of positions
+    uint32_t   per_mul;
 };
 // The blocks of 32 positions that a run's rows, the last ones of its sequence, lie in.
 __device__ __forceinline__ int length_of(const RowsIn &a, int id) { return (unsigned)id < (unsigned)a.seqs ? clamp(a.len[id], 0, a.width * PAGE) : 0; }
@@ -88,10 +89,10 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
     __shared__ __align__(16) uint8_t code_s[4][BLOCK * (HP + 4)];
     const int failed = a.state[0];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nkv = a.c.nkv;
-    const int w = (int)(blockIdx.x * 4 + wave), per = 2 * nkv, item = w / per, which = w - item * per, h = which >> 1;
+    const int item = (int)divide(blockIdx.x, a.per, a.per_mul), which = 4 * ((int)blockIdx.x - item * a.per) + wave, h = which >> 1;
     const bool value = which & 1;
-    const Found f = find_run(a.b, item, [&](int r, int, int rows) { return blocks_of(a, r, rows); });
-    if (f.run < 0) return;
+    const Found f = find_run<4>(a.b, item, [&](int r, int, int rows) { return blocks_of(a, r, rows); });
+    if (f.run < 0 || h >= nkv) return;
     const int id = a.b.id(f.run), len = length_of(a, id), first = len - f.rows, block = first / BLOCK + f.at;
     const int page = a.table[(size_t)id * a.width + block / SCALES];
     const int sub = block % SCALES, p0 = block * BLOCK, before = max(first - p0, 0), end = min(len - p0, BLOCK);
@@ -180,12 +181,11 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
 template <int NB> __global__ void __launch_bounds__(256) k_kv8_rows(RowsIn a) {
     constexpr int HP = 32 * NB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nkv = a.c.nkv, hd = a.c.hd;
-    const int w = (int)(blockIdx.x * 4 + wave), per = 2 * nkv, item = w / per, which = w - item * per, h = which >> 1;
+    const int item = (int)divide(blockIdx.x, a.per, a.per_mul), which = 4 * ((int)blockIdx.x - item * a.per) + wave, h = which >> 1;
     const bool value = which & 1;
     float *out = value ? a.ov : a.ok;
-    if (!out) return;
-    const Found f = find_run(a.b, item, [&](int r, int, int rows) { return blocks_of(a, r, rows); });
-    if (f.run < 0) return;
+    const Found f = find_run<4>(a.b, item, [&](int r, int, int rows) { return blocks_of(a, r, rows); });
+    if (f.run < 0 || h >= nkv || !out) return;
     const int id = a.b.id(f.run), len = length_of(a, id), first = len - f.rows, block = first / BLOCK + f.at;
     const int page = a.table[(size_t)id * a.width + block / SCALES];
     const bool lost = (unsigned)page >= (unsigned)a.pages;
@@ -325,12 +325,17 @@ __device__ __forceinline__ int tiles_of(int len) { return (len + TILE - 1) / TIL
 struct Share {
     int run, id, len, s0, rows, group, part, parts, slot;
 };
-// The item-th share of a kv head's work, or (GROUP) the first share of the item-th group of rows. run < 0: none. By a whole wavefront, 64 runs at a time; the first 64 are
-// read once.
-template <bool GROUP> __device__ __forceinline__ Share share_of(const AttendIn &a, int item) {
-    const int lane = threadIdx.x & 63;
-    auto read = [&](int r0, int &id, int &len, int &s0, int &rows) {
-        const int r = r0 + lane;
+// The item-th share of a kv head's work, or (GROUP) the first share of the item-th group of rows. run < 0: none. Up to 64 runs are counted by each wavefront for
+// itself, a lane a run; more by the workgroup's W wavefronts, 64 each, which meet in LDS.
+template <bool GROUP, int W> __device__ __forceinline__ Share share_of(const AttendIn &a, int item) {
+    __shared__ uint32_t work_s[W];
+    __shared__ int      sums_s[2][2][W];
+    __shared__ Share    found_s;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool alone = a.b.seqs <= 64, once = a.b.seqs <= 64 * W;
+    const int mine0 = alone ? 0 : 64 * wave;
+    int id, len, s0, rows, chunk = 1 << 30;
+    auto read = [&](int r) {
         id = len = s0 = rows = 0;
         if (r < a.b.seqs) {
             id = a.b.id(r);
@@ -340,35 +345,68 @@ template <bool GROUP> __device__ __forceinline__ Share share_of(const AttendIn &
             id = (unsigned)id < (unsigned)a.seqs ? id : 0;           // none: no position of any
         }
     };
-    int id, len, s0, rows, chunk = 1 << 30;
-    read(0, id, len, s0, rows);
+    read(mine0 + lane);
     if (a.target) {
         uint32_t work = 0;
-        for (int r0 = 0;; r0 += 64) {
-            int i = id, n = len, s = s0, m = rows;
-            if (r0) read(r0, i, n, s, m);
-            const unsigned units = (unsigned)(tiles_of(n) + (1 << a.unit) - 1) >> a.unit;
-            work += (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)min((unsigned long long)groups_of(m, a.g) * units, (1ull << WORK) + 1)), 63);
+        for (int r0 = 0;; r0 += 64 * W) {
+            if (r0) read(r0 + mine0 + lane);
+            const unsigned units = (unsigned)(tiles_of(len) + (1 << a.unit) - 1) >> a.unit;
+            work += (uint32_t)__builtin_amdgcn_readlane(scan_wave((int)min((unsigned long long)groups_of(rows, a.g) * units, (1ull << WORK) + 1)), 63);
             work = min(work, 2u << WORK);
-            if (r0 + 64 >= a.b.seqs) break;
+            if (r0 + 64 * W >= a.b.seqs) break;
+        }
+        if (!alone) {
+            if (lane == 0) work_s[wave] = work;
+            __syncthreads();
+            work = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++) work = min(work + work_s[w], 2u << WORK);
         }
         // more than that have only runs that overlap: nothing is split, or the parts would be more than the workspace's
         if (work && work <= 1u << WORK) chunk = (int)min((unsigned long long)max((unsigned)a.least, (work - 1) / (unsigned)a.target + 1) << a.unit, 1ull << 30);
     }
     int base = 0, slots = 0;
-    for (int r0 = 0; r0 < a.b.seqs; r0 += 64) {
-        if (r0) read(r0, id, len, s0, rows);
-        const int groups = groups_of(rows, a.g), parts = a.target ? max((int)((unsigned)(tiles_of(len) + chunk - 1) / (unsigned)chunk), 1) : 1, mine = groups * parts;
-        const int upto = scan_wave(GROUP ? groups : mine) + base, slot = scan_wave(parts > 1 ? mine : 0) + slots;
-        const uint64_t here = __ballot(upto > item);
-        if (here) {
-            const int l = __builtin_ctzll(here);
-            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-            const int n = of(parts), at = item - (of(upto) - of(GROUP ? groups : mine)), group = GROUP || n == 1 ? at : (int)((unsigned)at / (unsigned)n);
-            return {r0 + l, of(id), of(len), of(s0), of(rows), group, GROUP ? 0 : at - group * n, n, of(slot) - of(parts > 1 ? mine : 0) + group * n};
+    for (int r0 = 0, turn = 0; r0 < a.b.seqs; r0 += 64 * W, turn ^= 1) {
+        if (!once && (r0 || a.target)) read(r0 + mine0 + lane);
+        const int groups = groups_of(rows, a.g), parts = a.target ? max((int)((unsigned)(tiles_of(len) + chunk - 1) / (unsigned)chunk), 1) : 1, split = parts > 1 ? groups * parts : 0;
+        const int c = GROUP ? groups : groups * parts;
+        int upto = scan_wave(c), slot = scan_wave(split), all = __builtin_amdgcn_readlane(upto, 63), all_slots = __builtin_amdgcn_readlane(slot, 63);
+        if (!alone) {
+            if (lane == 0) {
+                sums_s[turn][0][wave] = min(all, MOST_ITEMS);
+                sums_s[turn][1][wave] = all_slots;
+            }
+            __syncthreads();
+            upto += base;
+            slot += slots;
+            all = base;
+            all_slots = slots;
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const int x = sums_s[turn][0][w], y = sums_s[turn][1][w];
+                upto += w < wave ? x : 0;
+                slot += w < wave ? y : 0;
+                all += x;
+                all_slots += y;
+            }
         }
-        base = __builtin_amdgcn_readlane(upto, 63);
-        slots = __builtin_amdgcn_readlane(slot, 63);
+        if (all > item) {
+            const uint64_t here = __ballot(upto > item && upto - c <= item);
+            Share f = {r0, 0, 0, 0, 0, 0, 0, 1, 0};
+            if (here) {
+                const int l = __builtin_ctzll(here);
+                auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+                const int n = of(parts), at = item - of(upto - c), group = GROUP || n == 1 ? at : (int)((unsigned)at / (unsigned)n);
+                f = {r0 + mine0 + l, of(id), of(len), of(s0), of(rows), group, GROUP ? 0 : at - group * n, n, of(slot - split) + group * n};
+            }
+            if (alone) return f;
+            if (here && lane == 0) found_s = f;
+            __syncthreads();
+            auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+            return {same(found_s.run), same(found_s.id), same(found_s.len), same(found_s.s0), same(found_s.rows), same(found_s.group), same(found_s.part), same(found_s.parts), same(found_s.slot)};
+        }
+        base = all;
+        slots = all_slots;
     }
     return {-1, 0, 0, 0, 0, 0, 0, 1, 0};
 }
@@ -454,7 +492,7 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
     const int item = (int)divide(blockIdx.x, a.c.nkv, a.nkv_mul), h = (int)blockIdx.x - item * a.c.nkv;
     const bool failed = *(const CONSTANT int32_t *)a.state != 0;
-    const Share f = share_of<false>(a, item);
+    const Share f = share_of<false, WAVES>(a, item);
     if (f.run < 0) return;
     const int len = f.len, row0 = 16 * f.group, rows = min(f.rows * g - row0, 16);
     // the row of this lane's column: its token, and the positions it sees
@@ -685,7 +723,7 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
     __shared__ float f_s[16][PARTS], sum_s[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.c.hd, quads = hd >> 2, block = (int)divide(blockIdx.x, a.c.nkv, a.nkv_mul), h = (int)blockIdx.x - block * a.c.nkv;
     const bool failed = *(const CONSTANT int32_t *)a.state != 0;
-    const Share f = share_of<true>(a, block);
+    const Share f = share_of<true, JOIN / 64>(a, block);
     if (f.run < 0 || f.parts < 2) return;
     const int rows = min(f.rows * a.g - 16 * f.group, 16);
     auto at = [&](int part, int r) { return ((size_t)(f.slot + part) * a.c.nkv + h) * a.slot_rows + r; };
@@ -786,12 +824,13 @@ int l3m_k_kv8_append(const l3m_kv8 *c, const l3m_pages *p, int layer, const void
     if (!k || !v || ((uintptr_t)k | (uintptr_t)v) % size) return l3m_dev_fail("kv8_append: no rows, or not aligned to their values");
     const size_t bytes = rows_bytes(b->n, stride, width, size);
     if (on_cache(c, k, bytes) || on_cache(c, v, bytes)) return l3m_dev_fail("kv8_append: the rows overlap the cache");
-    const long long items = most_blocks(b) * 2 * c->nkv;
+    const int per = (c->nkv + 1) / 2;
+    const long long items = most_blocks(b) * per;
     if (items > 1ll << 28) return l3m_dev_fail("kv8_append: too many rows for one call");
-    const RowsIn a = {*c, runs_of(b), k, v, nullptr, nullptr, stride, p->table, p->len, p->state, layer, p->pages, p->seqs, p->width};
+    const RowsIn a = {*c, runs_of(b), k, v, nullptr, nullptr, stride, p->table, p->len, p->state, layer, p->pages, p->seqs, p->width, per, multiplier(per, items)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
-    const dim3 grid((unsigned)((items + 3) / 4));
+    const dim3 grid((unsigned)items);
 #define APPEND(NB)                                                                      \
     if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_append<float, NB>), grid, dim3(256), 0, st, a); \
     else hipLaunchKernelGGL((k_kv8_append<uint16_t, NB>), grid, dim3(256), 0, st, a)
@@ -807,12 +846,13 @@ int l3m_k_kv8_rows(const l3m_kv8 *c, const l3m_pages *p, int layer, float *k, fl
     if (overlap(k, bytes, v, bytes)) return l3m_dev_fail("kv8_rows: k overlaps v");
     if (on_cache(c, k, bytes) || on_cache(c, v, bytes) || on_pages(p, k, bytes) || on_pages(p, v, bytes) || on_batch(b, k, bytes) || on_batch(b, v, bytes))
         return l3m_dev_fail("kv8_rows: k or v overlaps the cache, the tables or the batch");
-    const long long items = most_blocks(b) * 2 * c->nkv;
+    const int per = (c->nkv + 1) / 2;
+    const long long items = most_blocks(b) * per;
     if (items > 1ll << 28) return l3m_dev_fail("kv8_rows: too many rows for one call");
-    const RowsIn a = {*c, runs_of(b), nullptr, nullptr, k, v, 0, p->table, p->len, p->state, layer, p->pages, p->seqs, p->width};
+    const RowsIn a = {*c, runs_of(b), nullptr, nullptr, k, v, 0, p->table, p->len, p->state, layer, p->pages, p->seqs, p->width, per, multiplier(per, items)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
-    const dim3 grid((unsigned)((items + 3) / 4));
+    const dim3 grid((unsigned)items);
 #define ROWS(NB) hipLaunchKernelGGL((k_kv8_rows<NB>), grid, dim3(256), 0, st, a)
     BY_BLOCKS(ROWS)
     return l3m_dev_launched("k_kv8_rows");

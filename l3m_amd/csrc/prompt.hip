@@ -97,7 +97,7 @@ __device__ __forceinline__ void loads_done() {                       // and the 
 __device__ __forceinline__ int groups_of(int rows, int g) { return (int)(((unsigned)rows * (unsigned)g + ROWS * WAVES - 1) / (ROWS * WAVES)); }
 __device__ __forceinline__ Found group_of(const Runs &b, int g, int item, int items, int cus) {
     if (items <= 2 * cus && item >= cus) item = cus + items - 1 - item;
-    if (b.seqs > 64) return find_run(b, items - 1 - item, [&](int, int, int rows) { return groups_of(rows, g); });
+    if (b.seqs > 64) return find_run<WAVES>(b, items - 1 - item, [&](int, int, int rows) { return groups_of(rows, g); });
     const int lane = threadIdx.x & 63;
     int s0 = 0, rows = 0;
     if (lane < b.seqs) {

@@ -77,30 +77,55 @@ struct Runs {
     __device__ __forceinline__ int from(int i) const { return clamp(starts[i], 0, n); }
     __device__ __forceinline__ int to(int i, int first) const { return clamp(starts[i + 1], first, n); }
 };
-// The run that holds item `item` of the runs' items one behind the other, count(run, first row, rows) each, and the item's place in it; by a
-// whole wavefront. run < 0: there are fewer items.
+// The run that holds item `item` of the runs' items one behind the other, count(run, first row, rows) each, and the item's place in it. run < 0: there are
+// fewer items. Up to 64 runs are counted by each wavefront for itself, a lane a run; of more the W wavefronts of a workgroup, which then all look for the same
+// item, count 64 each and meet in LDS.
 struct Found {
     int run, at, s0, rows;
 };
-template <class Count> __device__ __forceinline__ Found find_run(const Runs &b, int item, Count count) {
-    const int lane = threadIdx.x & 63;
+constexpr int MOST_ITEMS = 1 << 26;                                  // of a wavefront's 64 runs; a call has fewer, unless its runs overlap
+template <int W, class Count> __device__ __forceinline__ Found find_run(const Runs &b, int item, Count count) {
+    __shared__ int   sums_s[2][W];
+    __shared__ Found found_s;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool alone = b.seqs <= 64;
     int base = 0;
-    for (int r0 = 0; r0 < b.seqs; r0 += 64) {
-        const int r = r0 + lane;
+    for (int r0 = 0, turn = 0; r0 < b.seqs; r0 += 64 * W, turn ^= 1) {
+        const int r = r0 + (alone ? 0 : 64 * wave) + lane;
         int s0 = 0, rows = 0, c = 0;
         if (r < b.seqs) {
             s0 = b.from(r);
             rows = b.to(r, s0) - s0;
             c = count(r, s0, rows);
         }
-        const int upto = scan_wave(c) + base;
-        const uint64_t past = __ballot(upto > item);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            return {r0 + l, item - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(c, l)), __builtin_amdgcn_readlane(s0, l),
-                    __builtin_amdgcn_readlane(rows, l)};
+        const int sum = scan_wave(c);
+        int upto = sum, all = __builtin_amdgcn_readlane(sum, 63);
+        if (!alone) {
+            if (lane == 0) sums_s[turn][wave] = min(all, MOST_ITEMS);
+            __syncthreads();
+            upto += base;
+            all = base;
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const int x = sums_s[turn][w];
+                upto += w < wave ? x : 0;
+                all += x;
+            }
         }
-        base = __builtin_amdgcn_readlane(upto, 63);
+        if (all > item) {
+            const uint64_t past = __ballot(upto > item && upto - c <= item);
+            Found f = {r - lane, 0, 0, 0};
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                f = {f.run + l, item - __builtin_amdgcn_readlane(upto - c, l), __builtin_amdgcn_readlane(s0, l), __builtin_amdgcn_readlane(rows, l)};
+            }
+            if (alone) return f;
+            if (past && lane == 0) found_s = f;
+            __syncthreads();
+            return {__builtin_amdgcn_readfirstlane(found_s.run), __builtin_amdgcn_readfirstlane(found_s.at), __builtin_amdgcn_readfirstlane(found_s.s0),
+                    __builtin_amdgcn_readfirstlane(found_s.rows)};
+        }
+        base = all;
     }
     return {-1, 0, 0, 0};
 }
