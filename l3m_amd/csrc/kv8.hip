@@ -323,7 +323,7 @@ __device__ __forceinline__ int tiles_of(int len) { return (len + TILE - 1) / TIL
 
 // A workgroup's share: of run `run`, id its sequence, of len positions, rows s0 ..; row group `group`, part `part` of `parts`, whose first one's slot is `slot`.
 struct Share {
-    int run, id, len, s0, rows, group, part, parts, slot;
+    int run, id, len, s0, rows, group, part, parts, slot, page;     // page: of the wavefront's first tile, where nothing is split; else to be read
 };
 // The item-th share of a kv head's work, or (GROUP) the first share of the item-th group of rows. run < 0: none. Up to 64 runs are counted by each wavefront for
 // itself, a lane a run; more by the workgroup's W wavefronts, 64 each, which meet in LDS.
@@ -334,7 +334,9 @@ template <bool GROUP, int W> __device__ __forceinline__ Share share_of(const Att
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool alone = a.b.seqs <= 64, once = a.b.seqs <= 64 * W;
     const int mine0 = alone ? 0 : 64 * wave;
-    int id, len, s0, rows, chunk = 1 << 30;
+    int id, len, s0, rows, page = 0, chunk = 1 << 30;
+    const int column = min(wave * TILE / PAGE, a.width - 1);
+    const bool early = !GROUP && alone && !a.target;                // the first pages' numbers come with the lengths
     auto read = [&](int r) {
         id = len = s0 = rows = 0;
         if (r < a.b.seqs) {
@@ -343,6 +345,7 @@ template <bool GROUP, int W> __device__ __forceinline__ Share share_of(const Att
             rows = a.b.to(r, s0) - s0;
             len = length_of(a, id);
             id = (unsigned)id < (unsigned)a.seqs ? id : 0;           // none: no position of any
+            if (early) page = a.table[(size_t)id * a.width + column];
         }
     };
     read(mine0 + lane);
@@ -392,23 +395,23 @@ template <bool GROUP, int W> __device__ __forceinline__ Share share_of(const Att
         }
         if (all > item) {
             const uint64_t here = __ballot(upto > item && upto - c <= item);
-            Share f = {r0, 0, 0, 0, 0, 0, 0, 1, 0};
+            Share f = {r0, 0, 0, 0, 0, 0, 0, 1, 0, 0};
             if (here) {
                 const int l = __builtin_ctzll(here);
                 auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
                 const int n = of(parts), at = item - of(upto - c), group = GROUP || n == 1 ? at : (int)((unsigned)at / (unsigned)n);
-                f = {r0 + mine0 + l, of(id), of(len), of(s0), of(rows), group, GROUP ? 0 : at - group * n, n, of(slot - split) + group * n};
+                f = {r0 + mine0 + l, of(id), of(len), of(s0), of(rows), group, GROUP ? 0 : at - group * n, n, of(slot - split) + group * n, of(page)};
             }
             if (alone) return f;
             if (here && lane == 0) found_s = f;
             __syncthreads();
             auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-            return {same(found_s.run), same(found_s.id), same(found_s.len), same(found_s.s0), same(found_s.rows), same(found_s.group), same(found_s.part), same(found_s.parts), same(found_s.slot)};
+            return {same(found_s.run), same(found_s.id), same(found_s.len), same(found_s.s0), same(found_s.rows), same(found_s.group), same(found_s.part), same(found_s.parts), same(found_s.slot), 0};
         }
         base = all;
         slots = all_slots;
     }
-    return {-1, 0, 0, 0, 0, 0, 0, 1, 0};
+    return {-1, 0, 0, 0, 0, 0, 0, 1, 0, 0};
 }
 
 // Products' columns over a row's dimensions: step s holds a lane's dimensions dim_of(s, c) .. + 7.
@@ -421,12 +424,18 @@ template <bool F32, int NB> struct Queries {
         for (int s = 0; s < NB; s++) {
             const int d = dim_of<NB>(s, lane >> 4);
             const bool in = d < hd;
-            float x[8];
-            if constexpr (F32) load8((const float *)q + at + (in ? d : 0), x);
-            else load8((const uint16_t *)q + at + (in ? d : 0), x);
+            if constexpr (F32) {
+                float x[8];
+                load8((const float *)q + at + (in ? d : 0), x);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = in ? x[i] : 0.f;
-            in_parts<QP, true>(x, part[s]);
+                for (int i = 0; i < 8; i++) x[i] = in ? x[i] : 0.f;
+                in_parts<QP, true>(x, part[s]);
+            } else {
+                typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+                u32x4 x = *(const u32x4_a2 *)((const uint16_t *)q + at + (in ? d : 0));
+                if (!in) x = u32x4{0, 0, 0, 0};
+                part[s][0] = __builtin_bit_cast(bf16x8, x);
+            }
         }
     }
     __device__ __forceinline__ void arrived() {
@@ -484,10 +493,10 @@ __device__ __forceinline__ uint32_t bytes_before(int from, int end) {
 
 template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WAVES) k_kv8_attend(AttendIn a) {
     constexpr int QP = Parts<F32>::q, PP = Parts<F32>::p, HP = 32 * NB, OS = HP + 4, REQUESTS = 2 * NB;
-    __shared__ __align__(16) uint8_t k_s[WAVES][TILE * HP], v_s[WAVES][TILE * HP];
+    __shared__ __align__(16) uint8_t tile_s[WAVES][2][TILE * HP];    // K's and V's
     __shared__ float m_s[WAVES][16], l_s[WAVES][16];
-    static_assert(sizeof(k_s) + sizeof(v_s) >= 2 * 16 * OS * 4, "");
-    float (*o_s)[16][OS] = (float (*)[16][OS])k_s;                   // behind the tiles
+    static_assert(sizeof(tile_s) >= WAVES * 16 * OS * 4, "");
+    float (*o_s)[16][OS] = (float (*)[16][OS])tile_s;                // behind the tiles
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, c = lane >> 4, hd = a.c.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
     const int item = (int)divide(blockIdx.x, a.c.nkv, a.nkv_mul), h = (int)blockIdx.x - item * a.c.nkv;
@@ -498,6 +507,7 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
     // the row of this lane's column: its token, and the positions it sees
     const int r = row0 + min(r16, rows - 1), token = (int)divide(r, g, a.g_mul), head = h * g + r - token * g, seen = max(len - f.rows + token + 1, 0);
     const int last = (int)divide(row0 + rows - 1, g, a.g_mul), end = max(len - f.rows + last + 1, 0);
+    const bool several = last != (int)divide(row0, g, a.g_mul);      // tokens: rows that see different numbers of positions
     const int whole = max(len - f.rows + (int)divide(row0, g, a.g_mul) + 1, 0) / TILE;     // tiles that every row sees whole
     // this part's tiles (of all the sequence's; the last ones may lie behind every row)
     int t0 = 0, t1 = tiles_of(end);
@@ -524,10 +534,10 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
     int tile = t0 + wave;
     Queries<F32, NB> qs;
     qs.load(a.q, (long long)(f.s0 + token) * a.q_stride + (long long)head * hd, hd, lane);
-    Tile u = tile_at(tile, page_of(tile));
+    Tile u = tile_at(tile, !a.target && a.b.seqs <= 64 && tile < t1 ? f.page : page_of(tile));
     int page = page_of(tile + WAVES);
     uint32_t ks = u.s[0], vs = u.s[1];
-    uint8_t *my_k = k_s[wave], *my_v = v_s[wave];
+    uint8_t *my_k = tile_s[wave][0], *my_v = tile_s[wave][1];
     request_k<NB>(u.k, my_k, lane);
     request_v<NB>(u.v, my_v, lane);
     qs.arrived();                                                    // here, or the loop waits for all requests at its top
@@ -645,14 +655,17 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
 #pragma unroll
             for (int t = 0; t < 2 * NB; t += 2) product(t, acc[t], acc[t + 1], std::false_type{}, 0);
         } else {
-            uint32_t nan = 0;                                        // codes of NaN among the values that some row sees
+            bool apart = false;                                      // a NaN is the rows' that see it: a token's rows at a time, over its own positions
+            if (several) {
+                uint32_t nan = 0;                                    // codes of NaN among the values that some row sees
 #pragma unroll
-            for (int t = 0; t < 2 * NB; t++) {
-                const u32x4 v = values(t);
+                for (int t = 0; t < 2 * NB; t++) {
+                    const u32x4 v = values(t);
 #pragma unroll
-                for (int i = 0; i < 4; i++) nan |= ((v[i] & bytes_before(16 * c + 4 * i, left) & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    for (int i = 0; i < 4; i++) nan |= ((v[i] & bytes_before(16 * c + 4 * i, left) & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                }
+                apart = __ballot(nan != 0) != 0;
             }
-            const bool apart = __ballot(nan != 0) != 0;              // a NaN is the rows' that see it: a token's rows at a time, over its own positions
             for (int to = apart ? min(seen, end) : end, at = __builtin_amdgcn_readfirstlane(to);;) {
 #pragma unroll
                 for (int t = 0; t < 2 * NB; t += 2) {
@@ -675,35 +688,28 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
     }
     requests_but<0>();
 
-    // the wavefronts' parts at their common maximum, two at a time
+    // the wavefronts' parts meet in LDS
     l = sum_groups(l);
     if (c == 0) {
         m_s[wave][r16] = m;
         l_s[wave][r16] = l;
     }
-    __syncthreads();                                                 // and the tiles are done with
-    float most = m_s[0][r16];
+    __syncthreads();                                                 // the tiles are done with
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) most = fmaxf(most, m_s[w][r16]);
-    const float by = __builtin_amdgcn_exp2f(m - most);
-#pragma unroll
-    for (int turn = 0; turn < WAVES / 2; turn++) {
-        if (wave >> 1 == turn)
-#pragma unroll
-            for (int t = 0; t < 2 * NB; t++) {
-                f32x4 &to = *(f32x4 *)&o_s[wave & 1][r16][16 * t + 4 * c];
-                to = turn ? to + acc[t] * by : acc[t] * by;
-            }
-        __syncthreads();
-    }
+    for (int t = 0; t < 2 * NB; t++) *(f32x4 *)&o_s[wave][r16][16 * t + 4 * c] = acc[t];
+    __syncthreads();
     for (int i = threadIdx.x; i < rows * (hd / 4); i += 64 * WAVES) {
         const int row = i / (hd / 4), d = 4 * (i - row * (hd / 4));
         float top = m_s[0][row], sum = 0.f;
 #pragma unroll
         for (int w = 1; w < WAVES; w++) top = fmaxf(top, m_s[w][row]);
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) sum = fmaf(l_s[w][row], __builtin_amdgcn_exp2f(m_s[w][row] - top), sum);
-        const f32x4 x = *(const f32x4 *)&o_s[0][row][d] + *(const f32x4 *)&o_s[1][row][d];
+        for (int w = 0; w < WAVES; w++) {
+            const float by = __builtin_amdgcn_exp2f(m_s[w][row] - top);
+            sum = fmaf(l_s[w][row], by, sum);
+            x += *(const f32x4 *)&o_s[w][row][d] * by;
+        }
         if (f.parts > 1) {
             const size_t to = ((size_t)(f.slot + f.part) * a.c.nkv + h) * a.slot_rows + row;
             *(f32x4 *)(a.parts + to * hd + d) = x;
@@ -711,7 +717,7 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
             continue;
         }
         const int t = (int)divide(row0 + row, g, a.g_mul), hh = h * g + row0 + row - t * g;
-        put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, x / sum, len - f.rows + t < 0, failed);
+        put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, x * (1.f / sum), len - f.rows + t < 0, failed);
     }
 }
 
