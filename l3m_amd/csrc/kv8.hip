@@ -21,14 +21,15 @@ __device__ __forceinline__ int exponent_for(float most) {
     const uint32_t u = __float_as_uint(most);
     return max((int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u), 1);
 }
-__device__ __forceinline__ float finite_size(float x) {
-    const float a = fabsf(x);
-    return a < INFINITY ? a : 0.f;
-}
-// Four values times 2^(127 - exponent) as codes, to the nearest, ties to even; what is not finite is NaN.
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float up) {
+// Sizes as whole numbers: of finite values in order, from FINITE up; of others, as the sum wraps, less.
+constexpr uint32_t FINITE = 0x01000000u;
+__device__ __forceinline__ uint32_t size_of(float x) { return (__float_as_uint(x) << 1) + FINITE; }
+__device__ __forceinline__ float value_of(uint32_t size) { return size < FINITE ? 0.f : __uint_as_float((size - FINITE) >> 1); }
+// Four values times 2^(127 - exponent) as codes, to the nearest, ties to even; what is not finite (FINITE_ONLY: there is none) is NaN.
+template <bool FINITE_ONLY> __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float up) {
     uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * up, b * up, 0, false);
     w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * up, d * up, (int)w, true);
+    if constexpr (FINITE_ONLY) return w;
     const float x[4] = {a, b, c, d};
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -38,7 +39,7 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, 
 // Four codes times `by`, as codes.
 __device__ __forceinline__ uint32_t recode4(uint32_t w, float by) {
     const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-    return encode4(a.x, a.y, b.x, b.y, by);
+    return encode4<false>(a.x, a.y, b.x, b.y, by);
 }
 __device__ __forceinline__ float pow2_byte(int e) { return __uint_as_float((uint32_t)e << 23); }   // 2^(e - 127), e 1 .. 254
 
@@ -64,6 +65,26 @@ template <class T> __device__ __forceinline__ void load8(const T *p, float (&x)[
         for (int i = 0; i < 8; i++) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
     }
 }
+
+// Eight values as they lie in memory.
+template <class T> struct Raw8 {
+    u32x4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
+        typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+        typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+        typedef std::conditional_t<sizeof(T) == 4, u32x4_a4, u32x4_a2> u32x4_at;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = *(const u32x4_at *)(p + 16 / sizeof(T) * i);
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = u32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i >> 2][i & 3]);
+        else return __uint_as_float(i & 1 ? w[0][i >> 1] & 0xFFFF0000u : w[0][i >> 1] << 16);
+    }
+};
 
 struct RowsIn {
     l3m_kv8    c;
@@ -97,13 +118,13 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
     const int page = a.table[(size_t)id * a.width + block / SCALES];
     const int sub = block % SCALES, p0 = block * BLOCK, before = max(first - p0, 0), end = min(len - p0, BLOCK);
     const T *rows = (const T *)(value ? a.v : a.k) + (size_t)h * a.c.hd;
-    float x[IT][8], most = 0.f;
+    // turn i: rows 64 i / PER .. (64 i + 63) / PER of the block; a row to a turn is the rule of steps, so turns without new rows are left out as a whole
+    auto has = [&](int i) { return 64 * i / PER < end && (64 * i + 63) / PER >= before; };
+    Raw8<T> x[IT];
 #pragma unroll
     for (int i = 0; i < IT; i++) {
         const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[i][j] = 0.f;
-        if (r >= before && r < end && d < a.c.hd) load8(rows + (long long)(f.s0 + p0 + r - first) * a.stride + d, x[i]);
+        if (has(i)) x[i].load(rows + (long long)(f.s0 + p0 + clamp(r, before, end - 1) - first) * a.stride + (d < a.c.hd ? d : 0));
     }
     if (failed || (unsigned)page >= (unsigned)a.pages) return;       // behind a failed call on the tables nothing is written
     const Unit u = unit_of(a.c, page, a.layer, h);
@@ -120,19 +141,33 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
     };
     if (value && before % 4 && q == before >> 2) read_shared();
     const int had = before ? max((int)*scale, 1) : 0;
+    uint32_t most = 0, least = ~0u;
 #pragma unroll
-    for (int i = 0; i < IT; i++)
+    for (int i = 0; i < IT; i++) {
+        const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
+        if (!has(i)) continue;
+        if (d >= a.c.hd) x[i].clear();                               // the head's end; rows beside the new ones are the first or last again
 #pragma unroll
-        for (int j = 0; j < 8; j++) most = fmaxf(most, finite_size(x[i][j]));
-    const int e = max(exponent_for(max_wave(most)), had);
+        for (int j = 0; j < 8; j++) {
+            const uint32_t size = size_of(x[i].value(j));
+            most = max(most, size);
+            least = min(least, size);
+        }
+    }
+    const bool finite = !__ballot(least < FINITE);
+    const int e = max(exponent_for(max_wave(value_of(most))), had);
     const float up = pow2_byte(254 - e), down = had && had < e ? (e - had < 127 ? pow2_byte(127 - (e - had)) : 0.f) : 1.f;
     if (lane == 0) *scale = (uint8_t)e;                              // read by no other lane by now
+    auto encode = [&](const Raw8<T> &x) {
+        auto four = [&](int i) { return finite ? encode4<true>(x.value(i), x.value(i + 1), x.value(i + 2), x.value(i + 3), up) : encode4<false>(x.value(i), x.value(i + 1), x.value(i + 2), x.value(i + 3), up); };
+        return u32x2{four(0), four(4)};
+    };
     if (!value) {
 #pragma unroll
         for (int i = 0; i < IT; i++) {
             const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
             u32x2 *to = (u32x2 *)(u.k + (size_t)(sub * BLOCK + r) * HP + d);
-            if (r >= before && r < end) *to = u32x2{encode4(x[i][0], x[i][1], x[i][2], x[i][3], up), encode4(x[i][4], x[i][5], x[i][6], x[i][7], up)};
+            if (has(i) && r >= before && r < end) *to = encode(x[i]);
             else if (r < before && down != 1.f) {
                 const u32x2 was = *to;
                 *to = u32x2{recode4(was.x, down), recode4(was.y, down)};
@@ -145,9 +180,10 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
         for (int i = 0; i < IT; i++) {
             const int at = 64 * i + lane, r = at / PER, d = 8 * (at - r * PER);
             uint32_t *to = (uint32_t *)(row_s + r * (HP + 4) + d);
-            if (r < before || r >= end) continue;
-            to[0] = encode4(x[i][0], x[i][1], x[i][2], x[i][3], up);
-            to[1] = encode4(x[i][4], x[i][5], x[i][6], x[i][7], up);
+            if (!has(i) || r < before || r >= end) continue;
+            const u32x2 w = encode(x[i]);
+            to[0] = w.x;
+            to[1] = w.y;
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
