@@ -768,16 +768,18 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
     const Share f = share_of<true, JOIN / 64>(a, block);
     if (f.run < 0 || f.parts < 2) return;
     const int rows = min(f.rows * a.g - 16 * f.group, 16);
-    auto at = [&](int part, int r) { return ((size_t)(f.slot + part) * a.c.nkv + h) * a.slot_rows + r; };
+    const size_t slot = ((size_t)f.slot * a.c.nkv + h) * a.slot_rows;                        // of the first part's first row
+    const unsigned step = (unsigned)(a.c.nkv * a.slot_rows);                                 // to the next part's
     for (int r = wave; r < rows; r += JOIN / 64) {
+        const f32x2 *ml = (const f32x2 *)a.ml + slot + r;
         float top = M0, sum = 0.f;
-        for (int i = lane; i < f.parts; i += 64) top = fmaxf(top, a.ml[2 * at(i, r)]);
+        for (int i = lane; i < f.parts; i += 64) top = fmaxf(top, ml[i * step].x);
         top = max_wave(top);
         for (int i = lane; i < f.parts; i += 64) {
-            const f32x2 ml = *(const f32x2 *)(a.ml + 2 * at(i, r));
-            const float by = __builtin_amdgcn_exp2f(ml.x - top);
+            const f32x2 x = ml[i * step];
+            const float by = __builtin_amdgcn_exp2f(x.x - top);
             f_s[r][i] = by;
-            sum = fmaf(ml.y, by, sum);
+            sum = fmaf(x.y, by, sum);
         }
 #pragma unroll
         for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
@@ -787,9 +789,11 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
     const int items = min(rows * quads, JOIN), groups = JOIN / items, mine = tid / items, item = tid - mine * items;
     for (int i0 = 0; i0 < rows * quads; i0 += items) {
         const int all = min(i0 + item, rows * quads - 1), row = all / quads, d = 4 * (all - row * quads);
+        const float *from = a.parts + (slot + row) * hd + d;
+        const unsigned apart = step * hd;
         f32x4 x[8], o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(mine + i * groups, f.parts - 1), row) * hd + d);
+        for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(from + min(mine + i * groups, f.parts - 1) * apart);
         __syncthreads();                                             // the factors; the last turn's sums
         if (mine < groups)
             for (int p = mine; p < f.parts; p += 8 * groups) {
@@ -798,7 +802,7 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
                     if (p + i * groups < f.parts) o += x[i] * f_s[row][p + i * groups];
                 if (p + 8 * groups < f.parts)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(a.parts + at(min(p + (8 + i) * groups, f.parts - 1), row) * hd + d);
+                    for (int i = 0; i < 8; i++) x[i] = *(const f32x4 *)(from + min(p + (8 + i) * groups, f.parts - 1) * apart);
             }
         if (groups > 1) {
             o_s[tid] = o;
@@ -807,7 +811,7 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
         if (mine == 0 && i0 + item < rows * quads) {
             for (int i = 1; i < groups; i++) o += o_s[i * items + item];
             const int r = 16 * f.group + row, t = (int)divide(r, a.g, a.g_mul), hh = h * a.g + r - t * a.g;
-            put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, o / sum_s[row], f.len - f.rows + t < 0, failed);
+            put_row<F32>(a, (long long)(f.s0 + t) * a.out_stride + (long long)hh * hd + d, o * (1.f / sum_s[row]), f.len - f.rows + t < 0, failed);
         }
     }
 }
