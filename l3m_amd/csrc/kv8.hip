@@ -104,7 +104,8 @@ __device__ __forceinline__ int blocks_of(const RowsIn &a, int run, int rows) {
 }
 
 // The new rows of a block of 32 positions of one kv head, K or V: a wavefront each. Their largest magnitude and the scale of what the block holds already make the
-// block's scale; where that rises, the old codes are rounded again.
+// block's scale; where that rises, the old codes are rounded again. Bound by latency for single rows (48 sequences, 8 heads of 128: 5.0 us, of which a launch is 1.6:
+// lengths, page, scale, codes, each behind the last), by bytes for prompts.
 template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(RowsIn a) {
     constexpr int HP = 32 * NB, PER = 4 * NB, IT = 2 * NB;           // eight values a lane: chunks of a row, turns for 32 rows
     __shared__ __align__(16) uint8_t code_s[4][BLOCK * (HP + 4)];
@@ -159,7 +160,10 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
     const float up = pow2_byte(254 - e), down = had && had < e ? (e - had < 127 ? pow2_byte(127 - (e - had)) : 0.f) : 1.f;
     if (lane == 0) *scale = (uint8_t)e;                              // read by no other lane by now
     auto encode = [&](const Raw8<T> &x) {
-        auto four = [&](int i) { return finite ? encode4<true>(x.value(i), x.value(i + 1), x.value(i + 2), x.value(i + 3), up) : encode4<false>(x.value(i), x.value(i + 1), x.value(i + 2), x.value(i + 3), up); };
+        auto four = [&](int i) {
+            return finite ? encode4<true>(x.value(i), x.value(i + 1), x.value(i + 2), x.value(i + 3), up)
+                          : encode4<false>(x.value(i), x.value(i + 1), x.value(i + 2), x.value(i + 3), up);
+        };
         return u32x2{four(0), four(4)};
     };
     if (!value) {
@@ -213,7 +217,8 @@ template <class T, int NB> __global__ void __launch_bounds__(256) k_kv8_append(R
 }
 
 // ---------------------------------------------------------------- read-back
-// A block of 32 positions of one kv head, K or V, to a wavefront: float32 rows of the run's last positions.
+// A block of 32 positions of one kv head, K or V, to a wavefront: float32 rows of the run's last positions. Bound by what it writes; 4 x 2000 rows of 8 heads of
+// 128 stored and read back, 131 MB: 36.3 us, 3.6 TB/s for the two.
 template <int NB> __global__ void __launch_bounds__(256) k_kv8_rows(RowsIn a) {
     constexpr int HP = 32 * NB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nkv = a.c.nkv, hd = a.c.hd;
@@ -272,9 +277,17 @@ template <int NB> __global__ void __launch_bounds__(256) k_kv8_rows(RowsIn a) {
 //   S = K Q^T        16 positions x 16 rows x 32 dimensions (v_mfma_f32_16x16x32_bf16), q in PARTS of bf16
 //   P = 2^(S - m)    m the running maximum
 //   O^T += V^T P^T   16 dimensions x 16 rows x 32 positions, P in PARTS of bf16
-// A lane of group c reads 16 bytes at once, which are two products' eight columns: the dimensions 64 f + 16 c .. of K and of q, the positions 16 c .. of V. K's rows are taken in the order in which a lane then holds the scores of those positions, so no value crosses lanes. All sums in 32 bits; q and P in three
-// parts are float32's 24 bits; for bf16 rows q is one part, exactly, and P two, 2^-16 of a weight at the most.
+// A lane of group c reads 16 bytes at once, which are two products' eight columns: the dimensions 64 f + 16 c .. of K and of q, the positions 16 c .. of V.
+// K's rows are taken in the order in which a lane then holds the scores of those positions, so no value crosses lanes. All sums in 32 bits; q and P in
+// three parts are float32's 24 bits; for bf16 rows q is one part, exactly, and P two, 2^-16 of a weight at the most.
 // (v_mfma_scale_f32_16x16x128_f8f6f4 takes the codes as they lie, but aligns a product's 128 terms to the largest one: sums were off by 2^-11 of that.)
+//
+// Long caches are bound by their bytes: a wavefront has a tile of K and one of V under way, 16 KiB at hd 128, while it uses the last ones; two workgroups
+// of four fill LDS. One token over 131071 positions of 8 kv heads of 128 (269 MB), 32 heads: 58.4 us, of which the products' launch is 50 (5.3 TB/s; a copy
+// reaches 5.2) and the join 5; float32 queries, three products for one: 59.6. 64 sequences of 2243: 60.4 us; of 100 to 8000: 75 (3.9 TB/s), as the last
+// workgroups don't fill the card. Short ones are bound by their instructions one after the other, some 900 a wavefront: 100 positions 6.2 us, 600 8.4.
+// Measured and not built: shares by descending size (the listing costs what it saves); a wavefront to a kv head, without the meeting in LDS (512 sequences
+// of 281 85 us against 104, but 128 of 100 to 8000 220 against 123); rows' tiles read from memory as operands (64 lines a load: 1346 us for the 131071).
 template <bool F32> struct Parts {
     static constexpr int q = F32 ? 3 : 1, p = F32 ? 3 : 2;
 };
@@ -336,8 +349,10 @@ template <int N, bool TOWARDS_0 = false> __device__ __forceinline__ void in_part
 // Splitting. Per kv head the runs' groups of 16 rows over all their tiles are the work; a group over more than `chunk` tiles is split over as many workgroups as
 // have a chunk each, all nearly equal, and their parts are joined by a second launch. The lengths lie in device memory, so each workgroup counts the work and
 // finds its share of it by itself (share_of), the same in both launches.
-constexpr int SPLIT_ROWS = 1 << 14, SPLIT_FROM = 1024;
-constexpr int TARGET = 512;                                          // workgroups that the work is spread over
+constexpr int SPLIT_ROWS = 1 << 14;
+// Workgroups that the work is spread over. One token over 131071: 58.6 us (256: 57.1, 1024: 62.0), over 32768 22.2 (21.9, 28.2); 64 sequences of 100 to 8000 75.8
+// (81.5, 72.6), 16 of 8000 57.4 (1024: 60.2).
+constexpr int TARGET = 512;
 constexpr int WORK = 25;                                             // a batch's work is up to 2^WORK units, of 2^unit tiles each; 64 lanes' are a sum in 32 bits
 struct AttendIn {
     l3m_kv8     c;
@@ -758,7 +773,7 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
 }
 
 // The parts of a group of rows that was split, of one kv head, to a workgroup: a wavefront a row makes the parts' factors, while the first parts come; threads of one part
-// after the other meet in LDS in a fixed order.
+// after the other meet in LDS in a fixed order. Bound by latency: 5 us for 66 parts of 4 rows of each of 8 kv heads.
 constexpr int PARTS = TARGET + 1;                       // most parts of a group: a chunk each, of at most TARGET, and the last
 template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join(AttendIn a) {
     __shared__ f32x4 o_s[JOIN];
@@ -930,9 +945,14 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
     const long long groups = ((long long)b->n * g + 15) / 16 + b->seqs;
     if (groups * c->nkv > 1ll << 28) return l3m_dev_fail("kv8_attend: too many rows for one call");
-    // rows of many tokens fill the card by themselves; and a join takes as long as some four turns of a workgroup's wavefronts
-    const int nb = padded(c->hd) / 32, waves = nb <= 4 && groups * c->nkv <= 256 ? 8 : 4;
-    const bool split = (long long)b->n * nq <= SPLIT_ROWS && (longest == 0 ? (long long)p->width * PAGE : longest) > SPLIT_FROM;
+    const long long most = longest ? longest : (long long)p->width * PAGE, shares = groups * c->nkv;
+    // Eight wavefronts where there is work for them and a CU for each workgroup; two of four have the same tiles under way and the shorter meeting. 600 positions
+    // of 8 kv heads: 8.4 us against 9.1, 100: 6.8 against 6.2, 32 times 300: 11.4 against 10.6.
+    const int nb = padded(c->hd) / 32, waves = nb <= 4 && shares <= 256 && most > 4 * TILE ? 8 : 4;
+    // Split where a workgroup's turns, 4 positions a ns, outlast the join, 4 to 5 us. 8 kv heads of 1024 positions: 11.5 us split, 9.8 not; 2048: 11.6 and 13.9;
+    // 4001: 12.2 and 22.6. Where there are many shares, the join has more to read, and the turns' loads share the memory: 128 shares of 2000: 21.8 and
+    // 18.0, of 4000: 31.9 and 36.0; 1024 of up to 1500: 47.9 and 41.3, 512 of up to 8000: 75.5 and 80.8. Rows of many tokens fill the card by themselves.
+    const bool split = (long long)b->n * nq <= SPLIT_ROWS && most > (shares < 64 ? 1024 : 2560);
     const int per = slot_rows(b->n, g), target = split ? target_of(c->nkv) : 0;
     int unit = 0;
     while (groups * ((2ll * p->width + (1 << unit) - 1) >> unit) > 1 << WORK) unit++;
@@ -955,7 +975,9 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
 #define JOINED(N)                                                                       \
     if (dtype == L3M_HIP_F32) hipLaunchKernelGGL((k_kv8_join<true, N>), all, dim3(N), 0, st, a); \
     else hipLaunchKernelGGL((k_kv8_join<false, N>), all, dim3(N), 0, st, a)
-        if (groups * c->nkv < 128) {
+        // more threads where few workgroups have many parts: one token over 131071 58.6 us, by 256 threads 60.4; over 4001 12.3 and 11.7; 64 sequences of 100
+        // to 8000 78.1 and 75.6
+        if (shares < 128 && most > 8192) {
             JOINED(1024);
         } else {
             JOINED(256);

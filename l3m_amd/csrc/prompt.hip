@@ -6,6 +6,13 @@
 //   P = 2^(S - m)    m moves only where a score passes it by 8: weights up to 2^8, and the sums are seldom scaled. Rounded to bf16
 //   O^T += V^T P^T   32 dimensions x 32 rows x 16 positions, V read from LDS transposed (ds_read_b64_tr_b16)
 // K's and V's tiles go from memory to LDS directly, 16 bytes a lane, in an order of pieces within a row by which no read meets a bank twice.
+//
+// Bound by instruction issue: beside a tile's products of a wavefront (32, hd 128) stand its softmax's some 130 vector instructions and 32 exponentials. Two
+// workgroups of four wavefronts a CU fill each other's gaps. 8191 rows of 32/8 heads of 128: 520 to 540 us, 1.02 to 1.06 PFLOP/s (a bf16 product of 8192^3:
+// 1.34); heads of 64 0.87 to 0.90, of 80 0.77 (80 of 96 columns are work), of 256 0.82 (one wavefront a SIMD). 24 prompts of 16 to 2048: 93 to 95 us, 0.52: many of
+// their tiles lie on the diagonal, and workgroups are too short to hide their first loads. Five of 1 to 64 rows: 5.5 us, of which a launch is 1.6.
+// Measured and not built: one tile in LDS and three workgroups a CU (8191 547 us, 24 prompts 97; hd 256 630 against 671); a tile's scores beside the last
+// one's softmax (256 registers: 622 us); eight wavefronts a workgroup; wavefront priorities.
 #include <type_traits>
 #include "serve.h"
 
@@ -93,7 +100,8 @@ __device__ __forceinline__ void loads_done() {                       // and the 
 
 // Groups of ROWS WAVES rows, a workgroup's. Those of the last rows have the most tiles, so they come first, over all runs, or the longest run's would be left at the end:
 // the item-th of a kv head's groups by descending number in their run (up to 64 runs; more fill the card without an order). Where all are resident
-// at once, two to a CU, the second ones come shortest first, so that a CU's two are about as long together as any other's.
+// at once, two to a CU, the second ones come shortest first, so that a CU's two are about as long together as any other's. 24 prompts: 94.7 us, run by run 103.3;
+// 8191 rows: 535, by ascending number 582; 2048: 54.3, without the second half's order 55.8.
 __device__ __forceinline__ int groups_of(int rows, int g) { return (int)(((unsigned)rows * (unsigned)g + ROWS * WAVES - 1) / (ROWS * WAVES)); }
 __device__ __forceinline__ Found group_of(const Runs &b, int g, int item, int items, int cus) {
     if (items <= 2 * cus && item >= cus) item = cus + items - 1 - item;
