@@ -6,14 +6,14 @@
 // sums of whole numbers. A call that cannot be done as a whole changes nothing and sets state[0], and until that is cleared every call that changes
 // something does nothing.
 //
-// Measured: 8 sequences forked by 4 and all grown by a row, shared pages of 4 layers of 8 heads of 64 copied (34 MB), 22 us: three launches, the plans of 2 and
-// 6.5 us (a chain of loads, scans and barriers), the copies 6.2. 700 pages half in use compacted (163 MB): 43 us, of which the plan 4 and the copies 33
+// Measured: 8 sequences forked by 4 and all grown by a row, shared pages of 4 layers of 8 heads of 64 copied (34 MB), 20.5 us: three launches, the plans of 2 and
+// 5 us (a chain of loads, scans and barriers), the copies 6.2. 700 pages half in use compacted (163 MB): 43 us, of which the plan 4 and the copies 33
 // (4.9 TB/s).
 #include "serve.h"
 
 namespace {
 
-constexpr int PLAN = 1024;                                           // threads of the planning workgroup
+constexpr int PLAN = 1024;                                           // threads of the planning workgroup, at the most
 constexpr int MOST_SEQS = 65536;
 enum { STATE_FAILED, STATE_USED, STATE_COPIES };
 
@@ -27,11 +27,11 @@ __device__ __forceinline__ int32_t *scratch(const Tables &t, int plane) { return
 
 __device__ __forceinline__ int pages_for(int n) { return (int)(((unsigned)n + PAGE - 1) / PAGE); }
 
-// The sums of x over the threads before this one; total: over all. Every thread of the planning workgroup calls it.
+// The sums of x over the threads before this one; total: over all. Every thread of the planning workgroup, T of them, calls it.
 struct Scan {
     int sums[PLAN / 64];
 };
-__device__ int scan_all(Scan &s, int x, int &total) {
+template <int T = PLAN> __device__ int scan_all(Scan &s, int x, int &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, upto = scan_wave(x);
     __syncthreads();
     if (lane == 63) s.sums[wave] = upto;
@@ -39,7 +39,7 @@ __device__ int scan_all(Scan &s, int x, int &total) {
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < PLAN / 64; w++) {
+    for (int w = 0; w < T / 64; w++) {
         before += w < wave ? s.sums[w] : 0;
         total += s.sums[w];
     }
@@ -49,9 +49,9 @@ __device__ int scan_all(Scan &s, int x, int &total) {
 struct Listed {
     uint32_t bits[MOST_SEQS / 32];
     int      why;
-    __device__ void clear() {
+    template <int T = PLAN> __device__ void clear() {
         if (threadIdx.x == 0) why = 0;
-        for (int i = threadIdx.x; i < MOST_SEQS / 32; i += PLAN) bits[i] = 0;
+        for (int i = threadIdx.x; i < MOST_SEQS / 32; i += T) bits[i] = 0;
         __syncthreads();
     }
     __device__ bool add(int id) { return !(atomicOr(&bits[id >> 5], 1u << (id & 31)) >> (id & 31) & 1u); }    // false: it was there
@@ -66,17 +66,17 @@ struct Listed {
 template <int N> struct Spread {
     int first[PLAN], v[N][PLAN];
 };
-template <int N, class F> __device__ __forceinline__ void spread(Scan &scan, Spread<N> &s, int count, const int (&v)[N], F f) {
+template <int N, int T = PLAN, class F> __device__ __forceinline__ void spread(Scan &scan, Spread<N> &s, int count, const int (&v)[N], F f) {
     int total;
-    const int before = scan_all(scan, count, total);
+    const int before = scan_all<T>(scan, count, total);
     s.first[threadIdx.x] = before;
 #pragma unroll
     for (int i = 0; i < N; i++) s.v[i][threadIdx.x] = v[i];
     __syncthreads();
-    for (int e = threadIdx.x; e < total; e += PLAN) {
+    for (int e = threadIdx.x; e < total; e += T) {
         int of = 0;                                                  // the last one that begins at e or before it
 #pragma unroll
-        for (int step = PLAN / 2; step; step >>= 1) of += s.first[of + step] <= e ? step : 0;
+        for (int step = T / 2; step; step >>= 1) of += s.first[of + step] <= e ? step : 0;
         int u[N];
 #pragma unroll
         for (int i = 0; i < N; i++) u[i] = s.v[i][of];
@@ -108,12 +108,13 @@ __global__ void k_pages_clear(Tables t) { t.state[STATE_FAILED] = 0; }
 
 // A run of `add` rows makes its sequence that much longer. The pages that it begins are new; one that it goes on in and that others hold too is replaced by
 // a new one and listed to be copied, but where all of its holders are in the list the first of them keeps it.
-// Bound by latency: each step's loads hang on the last one's. Up to PLAN runs are read once and kept in registers.
+// Bound by latency: each step's loads hang on the last one's. Up to T runs are read once and kept in registers. Steps of few rows meet sooner with
+// fewer threads: 40 sequences a row each, forks and copies among them, 20.5 us by 256 threads, 22.5 by 1024; 80 of 200 rows each 45.5 and 32.9.
 struct Grown {
     int id, s0, add, old, page, held;                                // page: that it goes on in, -1: none; held: by so many
     int more, copy, at;                                              // new pages, one of them a copy; where they begin among all
 };
-__global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *pos) {
+template <int T> __global__ void __launch_bounds__(T) k_pages_grow(Tables t, Runs b, int32_t *pos) {
     __shared__ Listed listed;
     __shared__ Scan   scan;
     __shared__ Spread<5> spread_s;
@@ -132,17 +133,17 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
         }
         return r;
     };
-    const bool one = b.seqs <= PLAN;
+    const bool one = b.seqs <= T;
     Grown mine = {};
     if (tid < b.seqs) mine = read(tid);
     if (failed) {
         if (tid == 0) t.state[STATE_COPIES] = 0;
         return;
     }
-    listed.clear();
+    listed.clear<T>();
     if (tid == 0) copies_s = 0;
     int why = 0, shared = 0;
-    for (int i = tid; i < b.seqs; i += PLAN) {
+    for (int i = tid; i < b.seqs; i += T) {
         const Grown r = one ? mine : read(i);
         if ((unsigned)r.id >= (unsigned)t.seqs || !listed.add(r.id) || r.old < 0 || r.old > (long long)t.width * PAGE) why = max(why, (int)L3M_PAGES_BAD);
         else if ((long long)r.old + r.add > (long long)t.width * PAGE) why = max(why, (int)L3M_PAGES_LONG);
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
     why = listed.worst(why);
     if (!why && __syncthreads_or(shared)) {
         memory_done();
-        for (int i = tid; i < b.seqs; i += PLAN) {
+        for (int i = tid; i < b.seqs; i += T) {
             const Grown r = one ? mine : read(i);
             if (r.held > 1) {
                 atomicAdd(&growers[r.page], 1);
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
     }
     int total = 0;
     if (!why)
-        for (int i0 = 0; i0 < b.seqs; i0 += PLAN) {
+        for (int i0 = 0; i0 < b.seqs; i0 += T) {
             const int i = i0 + tid;
             Grown r = {};
             if (i < b.seqs) {
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
                 r.more = pages_for(r.old + r.add) - pages_for(r.old) + r.copy;
             }
             int sum;
-            r.at = scan_all(scan, r.more, sum) + total;
+            r.at = scan_all<T>(scan, r.more, sum) + total;
             if (one) mine = r;
             else if (i < b.seqs) {
                 plan[i] = r.at;
@@ -189,10 +190,10 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
     if (!why && total) {
         __syncthreads();
         int got = 0;
-        for (int p0 = 0; p0 < t.pages && got < total; p0 += PLAN) {
+        for (int p0 = 0; p0 < t.pages && got < total; p0 += T) {
             const int p = p0 + tid, free = p < t.pages && (p0 ? t.refs[p] : first_free) == 0;
             int sum;
-            const int at = scan_all(scan, free, sum);
+            const int at = scan_all<T>(scan, free, sum);
             if (free && got + at < total) fresh[got + at] = p;       // who grows where is in the plan by now
             got += sum;
         }
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
         return;
     }
     __syncthreads();
-    for (int i0 = 0; i0 < b.seqs; i0 += PLAN) {
+    for (int i0 = 0; i0 < b.seqs; i0 += T) {
         const int i = i0 + tid;
         Grown r = {};
         int v[5] = {0, 0, 0, 0, 0};                                  // its first new page's place among them, sequence, place in the table, first row, length
@@ -230,12 +231,12 @@ __global__ void __launch_bounds__(PLAN) k_pages_grow(Tables t, Runs b, int32_t *
             }
             t.len[r.id] = r.old + r.add;
         }
-        spread<5>(scan, spread_s, r.more, v, [&](const int (&u)[5], int j) {
+        spread<5, T>(scan, spread_s, r.more, v, [&](const int (&u)[5], int j) {
             const int page = fresh[u[0] + j];
             t.refs[page] = 1;
             t.table[(size_t)u[1] * t.width + u[2] + j] = page;
         });
-        if (pos) spread<5>(scan, spread_s, r.add, v, [&](const int (&u)[5], int j) { pos[u[3] + j] = u[4] + j; });
+        if (pos) spread<5, T>(scan, spread_s, r.add, v, [&](const int (&u)[5], int j) { pos[u[3] + j] = u[4] + j; });
     }
     __syncthreads();
     if (tid == 0) {
@@ -465,7 +466,8 @@ int l3m_k_pages_grow(const l3m_pages *p, const l3m_kv8 *c, const l3m_batch *b, i
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
     const Tables t = tables_of(p);
-    hipLaunchKernelGGL(k_pages_grow, dim3(1), dim3(PLAN), 0, st, t, runs_of(b), pos);
+    if (b->seqs <= 256 && b->n <= 1024 && p->pages <= 4096) hipLaunchKernelGGL((k_pages_grow<256>), dim3(1), dim3(256), 0, st, t, runs_of(b), pos);
+    else hipLaunchKernelGGL((k_pages_grow<PLAN>), dim3(1), dim3(PLAN), 0, st, t, runs_of(b), pos);
     launch_copy(t, c, 0, st);
     return l3m_dev_launched("k_pages_grow");
 }

@@ -245,3 +245,8 @@ def test_oracle_of_lists():
     for name, wrong in (("state", "bad"), ("used", 3), ("refs", np.int32([1, 1, 1, 0])), ("len", np.int32([131, 0])), ("table", np.int32([[1, 0, -1], [-1, -1, -1]]))):
         with pytest.raises(AssertionError):
             o.check({**good, name: wrong})
+
+
+def test_attend_packed_far_rows():
+    """Rows of K and V so far apart that a tile's offsets pass 32 bits."""
+    refused(prompt(kvs=(1 << 23) + 8, b=batch(n=1)), "2^23")

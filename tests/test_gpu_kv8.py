@@ -437,3 +437,32 @@ def test_attend_lost_pages_are_their_rows(dev, dtype):
     assert dev.lib.l3m_dev_upload(o.p.table, C.c_void_p(table.ctypes.data), table.nbytes) == 0
     got = values(dev.kv8_attend(o.c, o.p, 1, q, b))
     assert np.array_equal(got[:2], whole[:2]) and np.isnan(got[2:]).all()
+
+
+@DTYPES
+@pytest.mark.parametrize("nkv", [1, 3, 4])
+def test_append_many_runs(dev, dtype, nkv):
+    """More runs than lanes, some without rows, heads that are no multiple of a workgroup's wavefronts; then read back, some of K or V alone."""
+    o = Cache(dev, 300, nkv, 24, pages=700, width=4, seed=16)
+    counts = [int(x) for x in o.rng.choice([0, 1, 5, 33, 130], 300)]
+    o.add([int(i) for i in o.rng.permutation(300)], counts, dtype)
+    ids = [int(i) for i in o.rng.permutation(300)]
+    o.add(ids, [1] * 300, dtype, 2.0)
+    o.check(ids)
+    n = len(o.held[ids[0], 0, 0].x)
+    b = dev.batch([0, n], [ids[0]])
+    for kv in (0, 1):
+        out = dev.alloc(4 * n * nkv * 24)
+        assert dev.lib.l3m_k_kv8_rows(C.byref(o.c), C.byref(o.p), 1, None if kv else out, out if kv else None, C.byref(b), None) == 0
+        assert np.array_equal(dev.get(out, (n, nkv, 24), np.float32), np.float32(o.want(ids[0], kv)))
+
+
+@DTYPES
+def test_append_not_finite_beside_finite(dev, dtype):
+    """A block of which one row holds NaN and infinities: the others' codes are what they are without it."""
+    o = Cache(dev, 1, 2, 40, seed=17)
+    (k, kx), (v, vx) = o.rows(70, dtype)
+    bad = [x.copy() for x in (kx, vx)]
+    bad[0][5, 0, 3], bad[0][40, 1, 39], bad[1][33, 1, 0], bad[1][69, 0, 8] = np.nan, -np.inf, np.inf, np.nan
+    o.add([0], [70], rows=[(typed(x, dtype)[0], x) for x in bad])
+    o.check([0])
