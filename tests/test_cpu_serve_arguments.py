@@ -229,7 +229,7 @@ def test_oracle_of_blocks():
     two.add(x[1:2])
     assert np.array_equal(one.x, two.x) and np.array_equal(one.x[1], [1.0, 2.0 ** -9])
     two.add(x[2:])
-    assert two.u == [8.0] and np.array_equal(two.x, [[448, 104], [1, 0], [3072, 0.40625]])
+    assert two.u == [8.0] and np.array_equal(two.x, [[448, 104], [1, 0], [3 * 2.0 ** 10, 0.40625]])
     low.add(x[1:2] * 0)
     assert low.u == [2.0 ** -126]
     low.cut(0)
