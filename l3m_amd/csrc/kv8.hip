@@ -351,7 +351,8 @@ template <int N, bool TOWARDS_0 = false> __device__ __forceinline__ void in_part
 // finds its share of it by itself (share_of), the same in both launches.
 constexpr int SPLIT_ROWS = 1 << 14;
 // Workgroups that the work is spread over. One token over 131071: 58.6 us (256: 57.1, 1024: 62.0), over 32768 22.2 (21.9, 28.2); 64 sequences of 100 to 8000 75.8
-// (81.5, 72.6), 16 of 8000 57.4 (1024: 60.2).
+// (81.5, 72.6), 16 of 8000 57.4 (1024: 60.2). Of heads past 128 one workgroup fills a CU, so half as many where the shares themselves are few: 4 heads of 256,
+// one token over 131071 59.4 us by 256 and 68.4 by 512, over 20000 22.8 and 28.5, 16 sequences of 4000 33.9 and 40.5; but 64 of 100 to 8000 82.3 and 77.9.
 constexpr int TARGET = 512;
 constexpr int WORK = 25;                                             // a batch's work is up to 2^WORK units, of 2^unit tiles each; 64 lanes' are a sum in 32 bits
 struct AttendIn {
@@ -852,8 +853,8 @@ const char *call_bad(const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_
     default: CALL(8); break;                                                                                                                                   \
     }
 // A split group has more than one chunk, so all of them have at most twice the chunks of the work.
-int target_of(int nkv) { return nkv < TARGET ? TARGET / nkv : 1; }
-size_t slots(int nkv) { return 2 * (size_t)target_of(nkv) * nkv; }
+int target_of(int nkv, int all) { return nkv < all ? all / nkv : 1; }
+size_t slots(int nkv) { return 2 * (size_t)target_of(nkv, TARGET) * nkv; }
 int slot_rows(int n, int g) { return (long long)n * g < 16 ? n * g : 16; }
 // Blocks of 32 positions that a batch's rows can lie in: a run of r rows in (r + 62) / 32 of them.
 long long most_blocks(const l3m_batch *b) { return b->n / BLOCK + 2ll * b->seqs; }
@@ -951,9 +952,13 @@ int l3m_k_kv8_attend(void *out, int out_stride, const void *q, int q_stride, int
     const int nb = padded(c->hd) / 32, waves = nb <= 4 && shares <= 256 && most > 4 * TILE ? 8 : 4;
     // Split where a workgroup's turns, 4 positions a ns, outlast the join, 4 to 5 us. 8 kv heads of 1024 positions: 11.5 us split, 9.8 not; 2048: 11.6 and 13.9;
     // 4001: 12.2 and 22.6. Where there are many shares, the join has more to read, and the turns' loads share the memory: 128 shares of 2000: 21.8 and
-    // 18.0, of 4000: 31.9 and 36.0; 1024 of up to 1500: 47.9 and 41.3, 512 of up to 8000: 75.5 and 80.8. Rows of many tokens fill the card by themselves.
-    const bool split = (long long)b->n * nq <= SPLIT_ROWS && most > (shares < 64 ? 1024 : 2560);
-    const int per = slot_rows(b->n, g), target = split ? target_of(c->nkv) : 0;
+    // 18.0, of 4000: 31.9 and 36.0; 1024 of up to 1500: 47.9 and 41.3, 512 of up to 8000: 75.5 and 80.8. Heads past 128 have longer turns and
+    // fill a CU by one workgroup: 4 of 256, one token over 500 12.9 and 10.8, over 1000 12.9 and 15.8; 64 shares of 2500 25.8 and 40.5; 256 of up to 2000 44.1 and
+    // 36.0. Rows of many tokens fill the card by themselves.
+    const bool wide = nb > 4;
+    const int few = wide ? 256 : 64;
+    const bool split = (long long)b->n * nq <= SPLIT_ROWS && most > (shares >= few ? 2560 : wide ? 768 : 1024);
+    const int per = slot_rows(b->n, g), target = split ? target_of(c->nkv, wide && shares < few ? TARGET / 2 : TARGET) : 0;
     int unit = 0;
     while (groups * ((2ll * p->width + (1 << unit) - 1) >> unit) > 1 << WORK) unit++;
     float *ml = (float *)work;
