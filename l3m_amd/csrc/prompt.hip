@@ -51,68 +51,74 @@ __device__ __forceinline__ float other_half(float x, float &y) {     // lane ^ 3
 }
 
 // A workgroup's requests for a tile of K and V, 16 bytes a lane: the i-th round of them is rows i ROUND .. of the tile, in the order of LDS.
-template <int NB> struct Loader {
-    static constexpr int RW = row_values(NB), PIECES = RW / 8, TURNS = TILE * PIECES / (64 * WAVES), ROUND = 64 * WAVES / PIECES;
-    static constexpr int KINDS = ROUND % 16 ? 2 : 1;                 // orders of pieces among the rounds
+// (W 1: a wavefront's requests for a tile of its own.)
+template <int NB, int W> struct Loader {
+    static constexpr int RW = row_values(NB), PIECES = RW / 8, TURNS = TILE * PIECES / (64 * W), ROUND = 64 * W / PIECES;
+    static constexpr int KINDS = ROUND < 16 ? 16 / ROUND : 1;        // orders of pieces among the rounds
     uint32_t k_off[KINDS], v_off[KINDS];                             // bytes behind a round's first row
     const char *k, *v;
     long long row_bytes;
     int len, row, wave;
     __device__ __forceinline__ void init(const PromptIn &a, const uint16_t *k0, const uint16_t *v0, int rows) {
-        const int slot = threadIdx.x % PIECES, last = (a.hd >> 3) - 1;
+        const int thread = threadIdx.x % (64 * W), slot = thread % PIECES, last = (a.hd >> 3) - 1;
         k = (const char *)k0;
         v = (const char *)v0;
         len = rows;
         row_bytes = 2 * a.kv_stride;
-        row = threadIdx.x / PIECES;
-        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        row = thread / PIECES;
+        wave = __builtin_amdgcn_readfirstlane(thread >> 6);
 #pragma unroll
         for (int i = 0; i < KINDS; i++) {
             k_off[i] = (uint32_t)(row * (int)row_bytes + 16 * min(slot ^ k_turn<PIECES>(row + i * ROUND), last));
             v_off[i] = (uint32_t)(row * (int)row_bytes + 16 * min(slot ^ v_turn<PIECES>(row + i * ROUND) << 1, last));
         }
     }
-    // Positions TILE tile .. into LDS; positions past the last one are the last one again, pieces past the head its last.
-    __device__ __forceinline__ void request(int tile, uint16_t *k_s, uint16_t *v_s) const {
-        const char *kt = k + tile * TILE * row_bytes, *vt = v + tile * TILE * row_bytes;
+    // Positions TILE tile .. of K or V into LDS; positions past the last one are the last one again, pieces past the head its last.
+    __device__ __forceinline__ void request_one(int tile, const char *from, const uint32_t (&off)[KINDS], uint16_t *to) const {
+        const char *at = from + tile * TILE * row_bytes;
         const int over = tile * TILE + TILE - len;                   // rows past the last
         if (__builtin_expect(over > 0, 0)) {
             asm volatile("");                                        // no selects for all tiles' sake
 #pragma unroll
             for (int i = 0; i < TURNS; i++) {
-                const int less = max(row + i * ROUND - (TILE - 1 - over), 0), at = i * ROUND - less;
-                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(kt + (at * row_bytes + k_off[i % KINDS])), (LOCAL void *)(k_s + 512 * (i * WAVES + wave)), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(vt + (at * row_bytes + v_off[i % KINDS])), (LOCAL void *)(v_s + 512 * (i * WAVES + wave)), 16, 0, 0);
+                const int less = max(row + i * ROUND - (TILE - 1 - over), 0);
+                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(at + ((i * ROUND - less) * row_bytes + off[i % KINDS])), (LOCAL void *)(to + 512 * (i * W + wave)), 16, 0, 0);
             }
         } else
 #pragma unroll
-            for (int i = 0; i < TURNS; i++) {
-                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(kt + i * ROUND * row_bytes + k_off[i % KINDS]), (LOCAL void *)(k_s + 512 * (i * WAVES + wave)), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(vt + i * ROUND * row_bytes + v_off[i % KINDS]), (LOCAL void *)(v_s + 512 * (i * WAVES + wave)), 16, 0, 0);
-            }
+            for (int i = 0; i < TURNS; i++)
+                __builtin_amdgcn_global_load_lds((const GLOBAL void *)(at + i * ROUND * row_bytes + off[i % KINDS]), (LOCAL void *)(to + 512 * (i * W + wave)), 16, 0, 0);
+    }
+    __device__ __forceinline__ void request_k(int tile, uint16_t *k_s) const { request_one(tile, k, k_off, k_s); }
+    __device__ __forceinline__ void request_v(int tile, uint16_t *v_s) const { request_one(tile, v, v_off, v_s); }
+    __device__ __forceinline__ void request(int tile, uint16_t *k_s, uint16_t *v_s) const {
+        request_k(tile, k_s);
+        request_v(tile, v_s);
     }
 };
+// All but the last N requests are done.
+template <int N> __device__ __forceinline__ void requests_but() { __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14); }
 
 __device__ __forceinline__ void loads_done() {                       // and the workgroup's
     __builtin_amdgcn_s_waitcnt(0x0F70);                              // vmcnt(0)
     __syncthreads();
 }
 
-// Groups of ROWS WAVES rows, a workgroup's. Those of the last rows have the most tiles, so they come first, over all runs, or the longest run's would be left at the end:
+// Groups of rows, a workgroup's. Those of the last rows have the most tiles, so they come first, over all runs, or the longest run's would be left at the end:
 // the item-th of a kv head's groups by descending number in their run (up to 64 runs; more fill the card without an order). Where all are resident
 // at once, two to a CU, the second ones come shortest first, so that a CU's two are about as long together as any other's. 24 prompts: 94.7 us, run by run 103.3;
 // 8191 rows: 535, by ascending number 582; 2048: 54.3, without the second half's order 55.8.
-__device__ __forceinline__ int groups_of(int rows, int g) { return (int)(((unsigned)rows * (unsigned)g + ROWS * WAVES - 1) / (ROWS * WAVES)); }
-__device__ __forceinline__ Found group_of(const Runs &b, int g, int item, int items, int cus) {
+template <int GROUP> __device__ __forceinline__ int groups_of(int rows, int g) { return (int)(((unsigned)rows * (unsigned)g + GROUP - 1) / GROUP); }
+template <int GROUP> __device__ __forceinline__ Found group_of(const Runs &b, int g, int item, int items, int cus) {
     if (items <= 2 * cus && item >= cus) item = cus + items - 1 - item;
-    if (b.seqs > 64) return find_run<WAVES>(b, items - 1 - item, [&](int, int, int rows) { return groups_of(rows, g); });
+    if (b.seqs > 64) return find_run<WAVES>(b, items - 1 - item, [&](int, int, int rows) { return groups_of<GROUP>(rows, g); });
     const int lane = threadIdx.x & 63;
     int s0 = 0, rows = 0;
     if (lane < b.seqs) {
         s0 = b.from(lane);
         rows = b.to(lane, s0) - s0;
     }
-    const int groups = groups_of(rows, g);
+    const int groups = groups_of<GROUP>(rows, g);
     // the highest level at which more than `item` groups lie at it or above
     auto above = [&](int level) { return __builtin_amdgcn_readlane(scan_wave(max(groups - level, 0)), 63); };
     int level = 0, top = (int)max_wave((float)min(groups, 1 << 24));
@@ -154,19 +160,22 @@ __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *
         if (lane + 64 * i < a.hd) out[lane + 64 * i] = (uint16_t)bf16_pair(o[i] / l, 0.f);
 }
 
-template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(PromptIn a) {
-    constexpr int RW = row_values(NB), PIECES = RW / 8;
+// SPLIT, for few groups: the four wavefronts take a group of 32 rows together, a tile each in turn, by themselves (the next K comes from a tile's scores on, the next V
+// from its values on), and their parts meet in LDS, in a fixed order.
+template <int NB, bool SPLIT> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(PromptIn a) {
+    constexpr int RW = row_values(NB), PIECES = RW / 8, GROUP = SPLIT ? ROWS : ROWS * WAVES;
+    constexpr int TILES = SPLIT ? WAVES * TILE * RW : TILE * RW, OTHER = SPLIT ? 8 : TILE * RW;
     // two tiles: the next one comes while one is used. Arrays of their own, so that the compiler sees that reads of one do not wait for the other's requests
-    __shared__ __align__(16) uint16_t k0_s[TILE * RW], v0_s[TILE * RW], k1_s[TILE * RW], v1_s[TILE * RW];
+    __shared__ __align__(16) uint16_t k0_s[TILES], v0_s[TILES], k1_s[OTHER], v1_s[OTHER];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, c = lane >> 5, hd = a.hd, g = a.g;
     // kv heads fastest: consecutive workgroups go to different XCDs, so 8 heads keep to an L2 each
     const int item = (int)divide(blockIdx.x, a.nkv, a.nkv_mul), h = (int)blockIdx.x - item * a.nkv;
-    const Found f = group_of(a.b, g, item, a.items, a.cus);
+    const Found f = group_of<GROUP>(a.b, g, item, a.items, a.cus);
     if (f.run < 0) return;
     const uint16_t *q = a.q + (long long)f.s0 * a.q_stride, *k = a.k + (long long)f.s0 * a.kv_stride + h * hd, *v = a.v + (long long)f.s0 * a.kv_stride + h * hd;
     uint16_t *out = a.out + (long long)f.s0 * a.out_stride;
-    const int R = f.rows * g, first = f.at * ROWS * WAVES, row0 = first + wave * ROWS;
-    const int tiles = (int)divide(min(first + ROWS * WAVES, R) - 1, g, a.g_mul) / TILE + 1;      // of the workgroup
+    const int R = f.rows * g, first = f.at * GROUP, row0 = SPLIT ? first : first + wave * ROWS;
+    const int tiles = (int)divide(min(first + GROUP, R) - 1, g, a.g_mul) / TILE + 1;      // of the workgroup
     const int rows = clamp(R - row0, 0, ROWS), row = row0 + min(r32, max(rows, 1) - 1);
     const int token = rows ? (int)divide(row, g, a.g_mul) : 0, head = rows ? h * g + row - token * g : 0;
     const int low = rows ? (int)divide(row0, g, a.g_mul) : 0, high = rows ? (int)divide(row0 + rows - 1, g, a.g_mul) : -1;   // the wavefront's tokens
@@ -179,9 +188,10 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
         if (d >= hd) x = u32x4{0, 0, 0, 0};
         qs[i] = __builtin_bit_cast(bf16x8, x);
     }
-    Loader<NB> loads;
+    Loader<NB, SPLIT ? 1 : WAVES> loads;
     loads.init(a, k, v, f.rows);
-    loads.request(0, k0_s, v0_s);
+    uint16_t *my_k = SPLIT ? k0_s + wave * TILE * RW : k0_s, *my_v = SPLIT ? v0_s + wave * TILE * RW : v0_s;
+    loads.request(SPLIT ? min(wave, tiles - 1) : 0, my_k, my_v);
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) asm volatile("" : "+v"(qs[i]));   // here, or the loop waits for requests at its top
     const float scale = a.scale;
@@ -194,6 +204,9 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
     bool large = false;                                              // some row's m is (LARGE_SCORE)
 
     auto step = [&](int tile, const uint16_t *k_s, const uint16_t *v_s) {
+        constexpr int REQUESTS = decltype(loads)::TURNS;
+        const int next = min(tile + WAVES, tiles - 1);
+        if constexpr (SPLIT) requests_but<REQUESTS>();               // V's, which came behind K's
         f32x16 s[2];
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -218,6 +231,10 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
         for (int i = 0; i < 2 * NB; i++) {
             __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        if constexpr (SPLIT) {
+            __builtin_amdgcn_s_waitcnt(0xC07F);                      // LDS is read
+            loads.request_k(next, my_k);
         }
         // s[b][8 j + e]: position 32 b + 16 j + 8 c + e
         if (__builtin_expect(tile * TILE + TILE - 1 > low, 0)) {
@@ -267,6 +284,7 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
             return __builtin_bit_cast(bf16x8, s16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]});
         };
         bf16x8 p[2][2], vx[2];
+        if constexpr (SPLIT) requests_but<REQUESTS>();               // the next K's, which came behind V's
         vx[0] = values(0);
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -286,18 +304,26 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
             if (n + 1 < 4 * NB) vx[(n + 1) & 1] = values(n + 1);
             acc[n % NB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vx[n & 1], p[n / NB >> 1][n / NB & 1], acc[n % NB], 0, 0, 0);
         }
+        if constexpr (SPLIT) {
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+            loads.request_v(next, my_v);
+        }
     };
     auto turn = [&](int tile, const uint16_t *k_s, const uint16_t *v_s, uint16_t *next_k, uint16_t *next_v) {
         loads_done();                                                // this tile is here, and nobody reads the last one any more
         if (tile + 1 < tiles) loads.request(tile + 1, next_k, next_v);
         if (tile * TILE <= high) step(tile, k_s, v_s);
     };
-    for (int tile = 0; tile < tiles; tile += 2) {
-        turn(tile, k0_s, v0_s, k1_s, v1_s);
-        if (tile + 1 < tiles) turn(tile + 1, k1_s, v1_s, k0_s, v0_s);
-    }
+    if constexpr (SPLIT) {
+        for (int tile = wave; tile < tiles; tile += WAVES) step(tile, my_k, my_v);
+        requests_but<0>();
+    } else
+        for (int tile = 0; tile < tiles; tile += 2) {
+            turn(tile, k0_s, v0_s, k1_s, v1_s);
+            if (tile + 1 < tiles) turn(tile + 1, k1_s, v1_s, k0_s, v0_s);
+        }
     __syncthreads();                                                 // the tiles are done with
-    if (!rows) return;
+    if (!rows) return;                                               // (a group has rows, so not where all meet)
     float y;
     l = other_half(l, y);
     l += y;
@@ -319,12 +345,56 @@ template <int NB> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(
         }
         if (__ballot(some)) wrong |= 1u << r;
     }
+    constexpr int HP = 32 * NB;
+    if constexpr (SPLIT) {
+        constexpr int OS = HP + 4;
+        static_assert(2 * ROWS * OS * 4 <= (int)sizeof(k0_s), "");
+        __shared__ float m_s[WAVES][ROWS], l_s[WAVES][ROWS];
+        __shared__ uint32_t wrong_s[WAVES];
+        float (*o_s)[ROWS][OS] = (float (*)[ROWS][OS])k0_s, (*p_s)[ROWS][OS] = (float (*)[ROWS][OS])v0_s;   // of two wavefronts each
+        float (*mine)[OS] = wave < 2 ? o_s[wave] : p_s[wave - 2];
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mine[r32][32 * i + 8 * j + 4 * c + e] = acc[i][4 * j + e];
+        if (c == 0) {
+            m_s[wave][r32] = m;
+            l_s[wave][r32] = l;
+        }
+        if (lane == 0) wrong_s[wave] = wrong;
+        __syncthreads();
+        wrong = wrong_s[0] | wrong_s[1] | wrong_s[2] | wrong_s[3];
+        static_assert(WAVES == 4, "");
+        for (int at = threadIdx.x; at < rows * (hd >> 3); at += 64 * WAVES) {
+            const int r = at / (hd >> 3), d = 8 * (at - r * (hd >> 3));
+            if (wrong >> r & 1u) continue;
+            const float top = fmaxf(fmaxf(m_s[0][r], m_s[1][r]), fmaxf(m_s[2][r], m_s[3][r]));
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float part = __builtin_amdgcn_exp2f(m_s[w][r] - top), *from = w < 2 ? &o_s[w][r][d] : &p_s[w - 2][r][d];
+                sum = fmaf(l_s[w][r], part, sum);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = fmaf(from[e], part, x[e]);
+            }
+            const float one = 1.f / sum;
+            const int rr = row0 + r, t = (int)divide(rr, g, a.g_mul), hh = h * g + rr - t * g;
+            *(u32x4 *)(out + (long long)t * a.out_stride + (long long)hh * hd + d) =
+                u32x4{bf16_pair(x[0] * one, x[1] * one), bf16_pair(x[2] * one, x[3] * one), bf16_pair(x[4] * one, x[5] * one), bf16_pair(x[6] * one, x[7] * one)};
+        }
+        for (uint32_t of = wrong; of; of &= of - 1) {
+            const int r = __builtin_ctz(of), t = __builtin_amdgcn_readlane(token, r), hh = __builtin_amdgcn_readlane(head, r);
+            if (r % WAVES == wave) row_alone(a, q + (long long)t * a.q_stride + (long long)hh * hd, k, v, t + 1, out + (long long)t * a.out_stride + (long long)hh * hd);
+        }
+        return;
+    }
     for (uint32_t of = wrong; of; of &= of - 1) {
         const int r = __builtin_ctz(of), t = __builtin_amdgcn_readlane(token, r), hh = __builtin_amdgcn_readlane(head, r);
         row_alone(a, q + (long long)t * a.q_stride + (long long)hh * hd, k, v, t + 1, out + (long long)t * a.out_stride + (long long)hh * hd);
     }
     // through LDS, 32 rows a wavefront, so that rows leave in whole lines; a row's pieces of 16 bytes in the order that K's have
-    constexpr int HP = 32 * NB;
     uint16_t *o_s = wave < 2 ? k0_s + wave * ROWS * HP : v0_s + (wave - 2) * ROWS * HP;
     static_assert(WAVES == 4 && 2 * ROWS * HP <= TILE * RW, "");
     const float by = 1.f / l;
@@ -374,14 +444,21 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
     if (kv_stride > 1 << 23) return l3m_dev_fail("attend_packed: rows of K and V may be up to 2^23 values apart");   // a tile's offsets in 32 bits
     const int g = nq / nkv;
     if ((long long)b->n * g > 1 << 28) return l3m_dev_fail("attend_packed: too many rows for one call");
-    const long long items = (long long)b->n * g / (ROWS * WAVES) + b->seqs;
+    long long items = (long long)b->n * g / (ROWS * WAVES) + b->seqs;
     if (items * nkv > 1ll << 28) return l3m_dev_fail("attend_packed: too many rows for one call");
+    // Wavefronts share groups of 32 rows where groups of 128 are too few for the card, in one tile's time for four, and not where a run has a tile or so: 2000
+    // rows of 9/3 heads of 64 (141 groups of 128) 19.3 us against 34.5, 3000 (213) 31 and 48, 1500 of 32/4 (376) 31.4 and 28.1; of 64 rows 6.1 and 5.6. Past 64
+    // a CU holds one such workgroup: 1705 of 3/1 heads of 80 (40) 18.2 and 33.8, 700 of 16/2 of 128 (88) 17.6 and 19.2, 400 of 32/8 (104) 17.2 and 14.5. Past 128 none.
+    const bool split = hd <= 128 && items * nkv < (hd <= 64 ? 256 : 96) && b->n > TILE * b->seqs;
+    if (split) items = (long long)b->n * g / ROWS + b->seqs;
     const PromptIn a = {q, k, v, out, {b->ids, b->starts, b->seqs, b->n}, q_stride, kv_stride, out_stride, nq, nkv, hd, g, multiplier(g, (uint64_t)b->n * g), multiplier(nkv, items * nkv),
                         (int)items, CUS / nkv, 1.44269504f / sqrtf((float)hd)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
     const dim3 grid((unsigned)(items * nkv)), wg(64 * WAVES);
-#define ATTEND(NB) hipLaunchKernelGGL((k_attend_packed<NB>), grid, wg, 0, st, a)
+#define ATTEND(NB)                                                                                              \
+    if (split) hipLaunchKernelGGL((k_attend_packed<NB <= 4 ? NB : 4, NB <= 4>), grid, wg, 0, st, a);              \
+    else hipLaunchKernelGGL((k_attend_packed<NB, false>), grid, wg, 0, st, a)
     switch ((hd + 31) / 32) {
     case 1: ATTEND(1); break;
     case 2: ATTEND(2); break;

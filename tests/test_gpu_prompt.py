@@ -145,3 +145,34 @@ def test_very_large_scores(dev):
                 tol = tol + 2.0 ** -8 * (np.abs(want.mean(0)) + tol)
                 assert np.all(np.abs(got[t] - want.mean(0)) <= tol), (sign, e, t)
         dev.free_all()
+
+
+@pytest.mark.parametrize("hd", [8, 32, 40, 64, 80, 96, 128])
+def test_many_groups(dev, hd):
+    """Enough rows that workgroups take groups of their own tiles, and few enough that wavefronts share them: lengths around the borders."""
+    rng = np.random.default_rng(hd + 1)
+    for nkv, g, lens in ((4, 4, [1100, 300, 65]), (2, 2, [900, 1, 31]), (1, 3, [1705]), (1, 1, [257, 0, 256, 255])):
+        n = sum(lens)
+        q, k, v = rows(rng, n, nkv * g, hd), rows(rng, n, nkv, hd), rows(rng, n, nkv, hd)
+        check(dev.attend_packed(q, k, v, dev.batch(np.cumsum([0] + lens))), q, k, v, lens, pick=60)
+        dev.free_all()
+
+
+def test_not_finite_long(dev):
+    """A NaN and infinities among the values of a prompt whose tiles several wavefronts share: they reach the rows from them on and no others."""
+    rng = np.random.default_rng(9)
+    n, hd = 700, 64
+    q, k, v = rows(rng, n, 2, hd), rows(rng, n, 1, hd), rows(rng, n, 1, hd)
+    b = dev.batch([0, n])
+    none = from_bf16(dev.attend_packed(q, k, v, b))
+    vv = v.copy()
+    vv[300, 0, 3], vv[613, 0, 5] = 0x7F80, 0x7FC0
+    got = from_bf16(dev.attend_packed(q, k, vv, b))
+    assert not np.isfinite(got[300:, :, 3]).any() and not np.isfinite(got[613:, :, 5]).any()
+    got[300:, :, 3], got[613:, :, 5] = none[300:, :, 3], none[613:, :, 5]
+    for lo, hi in ((256, 300), (576, 613)):                           # computed another way in those tiles
+        want, tol = attended(from_bf16(q[lo:hi]), from_bf16(k), from_bf16(v), range(lo + 1, hi + 1), 2.0 ** -8, 0.0)
+        same = np.arange(hd) != 3 if lo == 576 else np.ones(hd, bool)
+        assert np.all((np.abs(got[lo:hi] - want) <= tol + 2.0 ** -8 * (np.abs(want) + tol))[..., same])
+        got[lo:hi] = none[lo:hi]
+    assert np.array_equal(got, none)
