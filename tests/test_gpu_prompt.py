@@ -176,3 +176,21 @@ def test_not_finite_long(dev):
         assert np.all((np.abs(got[lo:hi] - want) <= tol + 2.0 ** -8 * (np.abs(want) + tol))[..., same])
         got[lo:hi] = none[lo:hi]
     assert np.array_equal(got, none)
+
+
+@pytest.mark.parametrize("nkv, g, hd", [(2, 3, 48), (3, 2, 128), (8, 4, 64)])
+def test_strides_long(dev, nkv, g, hd):
+    """As above for a prompt of several tiles: fused rows, out in q's place, what no prompt names left as it was; and the same result apart."""
+    rng = np.random.default_rng(10)
+    n, nq = 420, nkv * g
+    width, qw, kw = (nq + 2 * nkv) * hd + 24, nq * hd, nkv * hd
+    x = bf16(rng.standard_normal((n, width)))
+    b = dev.batch([10, 10, 390, 399], n=n)
+    p = dev.put(x)
+    assert dev.lib.l3m_k_attend_packed(p, width, p, width, p + 2 * qw, p + 2 * (qw + kw), width, C.byref(b), nq, nkv, hd, None) == 0
+    got = dev.get(p, x.shape, np.uint16)
+    q, k, v = x[:, :qw].reshape(n, nq, hd), x[:, qw:qw + kw].reshape(n, nkv, hd), x[:, qw + kw:qw + 2 * kw].reshape(n, nkv, hd)
+    want = dev.attend_packed(q, k, v, b).reshape(n, qw)
+    assert np.array_equal(got[:, qw:], x[:, qw:]) and np.array_equal(got[:10], x[:10]) and np.array_equal(got[399:], x[399:])
+    assert np.array_equal(got[10:399, :qw], want[10:399])
+    check(want[10:399].reshape(389, nq, hd), q[10:399], k[10:399], v[10:399], [380, 9])
