@@ -208,8 +208,8 @@ int l3m_k_rotary(const l3m_rotary *r, void *q, int q_stride, void *k, int k_stri
 
 // Causal attention over whole prompts, bf16: row t of a run over the run's rows 0 .. t, scores q.k / sqrt(hd), query head h reads kv head h / (nq / nkv). Rows'
 // strides and starts are multiples of 8 values and 16 bytes, hd a multiple of 8 up to 256, rows of k and v up to 2^23 values apart. out may be q. Sums are
-// float32's, of values times weights of up to 2^8, and divided at the end; weights are rounded to bf16, as the result is, and those below 2^-126 of the largest
-// may count as none. What lies behind a token, NaN among it, does not reach it.
+// float32's, of values times weights of up to 2^8, and divided at the end; weights are rounded to bf16 and summed as rounded, the result is rounded to bf16, and
+// weights below 2^-126 of the largest may count as none. What lies behind a token, NaN among it, does not reach it.
 int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_stride, const uint16_t *k, const uint16_t *v, int kv_stride, const l3m_batch *b,
                         int nq, int nkv, int hd, void *stream);
 

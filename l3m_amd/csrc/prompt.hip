@@ -3,7 +3,8 @@
 // Rows: a kv head's (token, query head) pairs of a run, a token's heads side by side (g = nq / nkv); 32 to a wavefront. Per tile of 64 positions:
 //   S = K Q^T        32 positions x 32 rows (v_mfma_f32_32x32x16_bf16), twice. The operand's rows are K's positions with bits 2 and 3 exchanged, so that a
 //                    lane holds the scores of its row for eight positions in a row, which is what the next product wants of it: no value crosses lanes
-//   P = 2^(S - m)    m moves only where a score passes it by 8: weights up to 2^8, and the sums are seldom scaled. Rounded to bf16
+//   P = 2^(S - m)    m moves only where a score passes it by 8: weights up to 2^8, and the sums are seldom scaled. Rounded to bf16, as the
+//                    matrix cores take them beside V (a second part of what is left would be half as many products again), and summed as rounded
 //   O^T += V^T P^T   32 dimensions x 32 rows x 16 positions, V read from LDS transposed (ds_read_b64_tr_b16)
 // K's and V's tiles go from memory to LDS directly, 16 bytes a lane, in an order of pieces within a row by which no read meets a bank twice.
 //
@@ -37,6 +38,13 @@ struct PromptIn {
     float           scale;                                           // of the scores: base 2
 };
 
+// x plus the two bf16 values of a word, in float32: the weights that the product takes are the ones that are summed, so their rounding cancels where a few
+// positions have all the weight. 8191 rows 547 us, as with the sum of the weights before their rounding; four chains of sums instead of one 555, the two halves
+// made floats and added 561.
+__device__ __forceinline__ float add_pair(uint32_t w, float x) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), x, false);
+}
 // Values of a row in LDS, a power of two; pieces of 16 bytes.
 __host__ __device__ constexpr int row_values(int nb) { return nb <= 1 ? 32 : nb <= 2 ? 64 : nb <= 4 ? 128 : 256; }
 // Where a row's piece lies in it: K by rows read side by side, V by pairs of pieces, of rows r .. r + 3 and r + 8 .. r + 11.
@@ -295,7 +303,7 @@ template <int NB, bool SPLIT> __global__ void __launch_bounds__(64 * WAVES) k_at
                 for (int e = 0; e < 4; e++) {
                     const float x0 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e], by, -less)), x1 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e + 1], by, -less));
                     w[e] = bf16_pair(x0, x1);
-                    l += x0 + x1;
+                    l = add_pair(w[e], l);
                 }
                 p[b][j] = __builtin_bit_cast(bf16x8, w);
             }

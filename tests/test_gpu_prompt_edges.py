@@ -1,0 +1,45 @@
+"""Attention over packed prompts (l3m_k_attend_packed) where it can go wrong: sums of rounded weights, infinities among keys, values behind a token."""
+import numpy as np
+import pytest
+
+from serve import bf16, from_bf16
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean(dev):
+    yield
+    dev.free_all()
+
+
+def rows(rng, n, h, hd, size=1.0):
+    return bf16(rng.standard_normal((n, h, hd)) * size)
+
+
+def equal_parts(rng, n, hd, sign, e):
+    """Queries and keys of one dimension, so that the positions `best` share all of a row's weight in equal parts; scores of some 2^e."""
+    k = np.zeros((n, 1, hd), np.float32)
+    k[:, 0, 5] = 2.0 ** -rng.integers(1, 7, n)
+    best = [b for b in (0, 7, 133, 280) if b < n]
+    k[best, 0, 5] = 1.0 if sign > 0 else 2.0 ** -7
+    q = np.zeros((n, 3, hd), np.float32)
+    q[..., 5] = sign * 2.0 ** e * (1 + np.arange(3) / 4)
+    return bf16(q), bf16(k), best
+
+
+@pytest.mark.parametrize("hd, n", [(64, 300), (64, 60), (160, 300)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_equal_weights(dev, sign, hd, n):
+    """Positions that share all weight in equal parts: a weight's rounding to bf16 stands in the sum that the result is divided by as well, so it cancels, and what is
+    left is float32's steps (four terms, the sum, a quotient) and the result's rounding, 2^-8."""
+    rng = np.random.default_rng(hd + n)
+    v = rows(rng, n, 1, hd)
+    for e in (17, 20, 40, 70, 113):
+        q, k, best = equal_parts(rng, n, hd, sign, e)
+        got = from_bf16(dev.attend_packed(q, k, v, dev.batch([0, n])))
+        for t in range(n):
+            want = from_bf16(v)[[b for b in best if b <= t], 0]
+            tol = 6 * 2.0 ** -24 * np.abs(want).mean(0)
+            tol = tol + 2.0 ** -8 * (np.abs(want.mean(0)) + tol)
+            assert np.all(np.abs(got[t] - want.mean(0)) <= tol), (sign, e, t)
