@@ -144,7 +144,8 @@ template <int GROUP> __device__ __forceinline__ Found group_of(const Runs &b, in
     return {l, level, __builtin_amdgcn_readlane(s0, l), __builtin_amdgcn_readlane(rows, l)};
 }
 
-// One row by the formula, a position at a time: for rows whose products met a value that is not finite behind their token.
+// One row by the formula, a position at a time: for rows whose products met a value that is not finite behind their token. Exponents as where rows are computed
+// together: their rounding cancels for small maxima and is alike for large ones.
 __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *k, const uint16_t *v, int seen, uint16_t *out) {
     const int lane = threadIdx.x & 63;
     float qv[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
@@ -156,8 +157,8 @@ __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *
         for (int i = 0; i < 4; i++) s += lane + 64 * i < a.hd ? qv[i] * bf16_float(k[(long long)p * a.kv_stride + lane + 64 * i]) : 0.f;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-        s *= a.scale;
-        const float top = fmaxf(m, s), by = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top), e = __builtin_amdgcn_exp2f(s - top);
+        const float top = fmaxf(m, s * a.scale), by = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        const float e = __builtin_amdgcn_exp2f(fabsf(top) > LARGE_SCORE ? scaled_less(s, a.scale, top) : fmaf(s, a.scale, -top));
         l = l * by + e;
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = o[i] * by + (lane + 64 * i < a.hd ? e * bf16_float(v[(long long)p * a.kv_stride + lane + 64 * i]) : 0.f);

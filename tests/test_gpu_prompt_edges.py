@@ -43,3 +43,24 @@ def test_equal_weights(dev, sign, hd, n):
             tol = 6 * 2.0 ** -24 * np.abs(want).mean(0)
             tol = tol + 2.0 ** -8 * (np.abs(want.mean(0)) + tol)
             assert np.all(np.abs(got[t] - want.mean(0)) <= tol), (sign, e, t)
+
+
+@pytest.mark.parametrize("hd, n", [(64, 300), (64, 60), (160, 300)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_large_scores_before_values_not_finite(dev, sign, hd, n):
+    """The same with a NaN and an infinity among the values: rows before them in their tile, computed by themselves, are what they are without."""
+    rng = np.random.default_rng(hd + n + 1)
+    v = rows(rng, n, 1, hd)
+    vv, bad = v.copy(), [(50, 3, 0x7FC0), (n - 2, 9, 0xFF80)]
+    for t, d, u in bad:
+        vv[t, 0, d] = u
+    for e in (17, 20, 40, 70, 113):
+        q, k, best = equal_parts(rng, n, hd, sign, e)
+        got = from_bf16(dev.attend_packed(q, k, vv, dev.batch([0, n])))
+        for t in range(n):
+            want = from_bf16(v)[[b for b in best if b <= t], 0]
+            tol = 6 * 2.0 ** -24 * np.abs(want).mean(0)
+            tol = tol + 2.0 ** -8 * (np.abs(want.mean(0)) + tol)
+            keep = np.ones(hd, bool)
+            keep[[d for at, d, _ in bad if at <= t]] = False
+            assert np.all((np.abs(got[t] - want.mean(0)) <= tol)[:, keep]) and not np.isfinite(got[t][:, ~keep]).any(), (sign, e, t)
