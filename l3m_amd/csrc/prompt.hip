@@ -145,10 +145,10 @@ template <int GROUP> __device__ __forceinline__ Found group_of(const Runs &b, in
 }
 
 // One row by the formula, a position at a time: for rows whose products met a value that is not finite behind their token. Exponents as where rows are computed
-// together: their rounding cancels for small maxima and is alike for large ones.
+// together: their rounding cancels for small maxima and is alike for large ones, and a score of -inf has no weight, be it the first.
 __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *k, const uint16_t *v, int seen, uint16_t *out) {
     const int lane = threadIdx.x & 63;
-    float qv[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
+    float qv[4], o[4] = {0, 0, 0, 0}, m = M0, l = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) qv[i] = lane + 64 * i < a.hd ? bf16_float(q[lane + 64 * i]) : 0.f;
     for (int p = 0; p < seen; p++) {
@@ -157,7 +157,7 @@ __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *
         for (int i = 0; i < 4; i++) s += lane + 64 * i < a.hd ? qv[i] * bf16_float(k[(long long)p * a.kv_stride + lane + 64 * i]) : 0.f;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-        const float top = fmaxf(m, s * a.scale), by = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        const float top = fmaxf(m, s * a.scale), by = __builtin_amdgcn_exp2f(m - top);
         const float e = __builtin_amdgcn_exp2f(fabsf(top) > LARGE_SCORE ? scaled_less(s, a.scale, top) : fmaf(s, a.scale, -top));
         l = l * by + e;
 #pragma unroll

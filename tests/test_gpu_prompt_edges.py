@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from serve import bf16, from_bf16
+from serve import attended, bf16, from_bf16
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,30 @@ def test_large_scores_before_values_not_finite(dev, sign, hd, n):
             keep = np.ones(hd, bool)
             keep[[d for at, d, _ in bad if at <= t]] = False
             assert np.all((np.abs(got[t] - want.mean(0)) <= tol)[:, keep]) and not np.isfinite(got[t][:, ~keep]).any(), (sign, e, t)
+
+
+def without(q, k, v, gone):
+    """The attention where the keys of positions `gone` score -inf, so that they have no weight, and its bound. Rows that see no other are NaN."""
+    n = len(q)
+    keep = np.ones(n, bool)
+    keep[gone] = False
+    want, tol = attended(from_bf16(q), from_bf16(k)[keep], from_bf16(v)[keep], np.cumsum(keep), 2.0 ** -8, 2.0 ** -126)
+    want[np.cumsum(keep) == 0] = np.nan
+    return want, tol + 2.0 ** -8 * (np.abs(want) + tol)
+
+
+@pytest.mark.parametrize("hd, n", [(64, 300), (128, 60), (160, 200)])
+def test_first_score_of_minus_infinity(dev, hd, n):
+    """A first position whose score is -inf has no weight, in rows that are computed by themselves too."""
+    rng = np.random.default_rng(hd)
+    q, k, v = rows(rng, n, 2, hd), rows(rng, n, 1, hd), rows(rng, n, 1, hd)
+    q[..., 2] &= 0x7FFF
+    k[0, 0, 2] = 0xFF80
+    want, tol = without(q, k, v, [0])
+    for at in (None, 40):
+        if at:
+            v[at, 0, 7] = 0x7FC0
+        got = from_bf16(dev.attend_packed(q, k, v, dev.batch([0, n])))
+        assert np.isnan(got[0]).all()
+        end = at or n
+        assert np.all(np.abs(got[1:end] - want[1:end]) <= tol[1:end])
