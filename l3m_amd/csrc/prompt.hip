@@ -59,11 +59,14 @@ __device__ __forceinline__ float other_half(float x, float &y) {     // lane ^ 3
 }
 
 // A workgroup's requests for a tile of K and V, 16 bytes a lane: the i-th round of them is rows i ROUND .. of the tile, in the order of LDS.
-// (W 1: a wavefront's requests for a tile of its own.)
-template <int NB, int W> struct Loader {
+// (W 1: a wavefront's requests for a tile of its own.) PAD, for heads that are no multiple of 32: K's pieces past the head, which the products read, are zeros that
+// stay; whatever else stood there would meet the queries' zeros, and an infinity times zero is NaN. (V's make dimensions that nobody reads.) Each of a wavefront's
+// requests has lanes within the head, so the number under way is the same.
+template <int NB, int W, bool PAD> struct Loader {
     static constexpr int RW = row_values(NB), PIECES = RW / 8, TURNS = TILE * PIECES / (64 * W), ROUND = 64 * W / PIECES;
     static constexpr int KINDS = ROUND < 16 ? 16 / ROUND : 1;        // orders of pieces among the rounds
     uint32_t k_off[KINDS], v_off[KINDS];                             // bytes behind a round's first row
+    bool k_in[KINDS];                                                // PAD: the lane's piece of K is one of the head's
     const char *k, *v;
     long long row_bytes;
     int len, row, wave;
@@ -77,9 +80,17 @@ template <int NB, int W> struct Loader {
         wave = __builtin_amdgcn_readfirstlane(thread >> 6);
 #pragma unroll
         for (int i = 0; i < KINDS; i++) {
+            if constexpr (PAD) k_in[i] = (slot ^ k_turn<PIECES>(row + i * ROUND)) <= last;
             k_off[i] = (uint32_t)(row * (int)row_bytes + 16 * min(slot ^ k_turn<PIECES>(row + i * ROUND), last));
             v_off[i] = (uint32_t)(row * (int)row_bytes + 16 * min(slot ^ v_turn<PIECES>(row + i * ROUND) << 1, last));
         }
+    }
+    // The pieces of K's tile that no request brings. Of a wavefront's own rounds; others read them behind a barrier.
+    __device__ __forceinline__ void clear_k(uint16_t *k_s) const {
+        if constexpr (PAD)
+#pragma unroll
+            for (int i = 0; i < TURNS; i++)
+                if (!k_in[i % KINDS]) *(u32x4 *)(k_s + 512 * (i * W + wave) + 8 * (threadIdx.x & 63)) = u32x4{0, 0, 0, 0};
     }
     // Positions TILE tile .. of K or V into LDS; positions past the last one are the last one again, pieces past the head its last.
     __device__ __forceinline__ void request_one(int tile, const char *from, const uint32_t (&off)[KINDS], uint16_t *to) const {
@@ -97,7 +108,30 @@ template <int NB, int W> struct Loader {
             for (int i = 0; i < TURNS; i++)
                 __builtin_amdgcn_global_load_lds((const GLOBAL void *)(at + i * ROUND * row_bytes + off[i % KINDS]), (LOCAL void *)(to + 512 * (i * W + wave)), 16, 0, 0);
     }
-    __device__ __forceinline__ void request_k(int tile, uint16_t *k_s) const { request_one(tile, k, k_off, k_s); }
+    // The same of K's pieces within the head alone; a kind's rounds together, so that lanes are left out once for each.
+    __device__ __forceinline__ void request_in_head(int tile, uint16_t *to) const {
+        const char *at = k + tile * TILE * row_bytes;
+        const int over = tile * TILE + TILE - len;
+#pragma unroll
+        for (int j = 0; j < KINDS; j++)
+            if (k_in[j]) {
+                if (__builtin_expect(over > 0, 0)) {
+                    asm volatile("");
+#pragma unroll
+                    for (int i = j; i < TURNS; i += KINDS) {
+                        const int less = max(row + i * ROUND - (TILE - 1 - over), 0);
+                        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(at + ((i * ROUND - less) * row_bytes + k_off[j])), (LOCAL void *)(to + 512 * (i * W + wave)), 16, 0, 0);
+                    }
+                } else
+#pragma unroll
+                    for (int i = j; i < TURNS; i += KINDS)
+                        __builtin_amdgcn_global_load_lds((const GLOBAL void *)(at + i * ROUND * row_bytes + k_off[j]), (LOCAL void *)(to + 512 * (i * W + wave)), 16, 0, 0);
+            }
+    }
+    __device__ __forceinline__ void request_k(int tile, uint16_t *k_s) const {
+        if constexpr (PAD) request_in_head(tile, k_s);
+        else request_one(tile, k, k_off, k_s);
+    }
     __device__ __forceinline__ void request_v(int tile, uint16_t *v_s) const { request_one(tile, v, v_off, v_s); }
     __device__ __forceinline__ void request(int tile, uint16_t *k_s, uint16_t *v_s) const {
         request_k(tile, k_s);
@@ -171,7 +205,7 @@ __device__ void row_alone(const PromptIn &a, const uint16_t *q, const uint16_t *
 
 // SPLIT, for few groups: the four wavefronts take a group of 32 rows together, a tile each in turn, by themselves (the next K comes from a tile's scores on, the next V
 // from its values on), and their parts meet in LDS, in a fixed order.
-template <int NB, bool SPLIT> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(PromptIn a) {
+template <int NB, bool SPLIT, bool PAD> __global__ void __launch_bounds__(64 * WAVES) k_attend_packed(PromptIn a) {
     constexpr int RW = row_values(NB), PIECES = RW / 8, GROUP = SPLIT ? ROWS : ROWS * WAVES;
     constexpr int TILES = SPLIT ? WAVES * TILE * RW : TILE * RW, OTHER = SPLIT ? 8 : TILE * RW;
     // two tiles: the next one comes while one is used. Arrays of their own, so that the compiler sees that reads of one do not wait for the other's requests
@@ -197,9 +231,11 @@ template <int NB, bool SPLIT> __global__ void __launch_bounds__(64 * WAVES) k_at
         if (d >= hd) x = u32x4{0, 0, 0, 0};
         qs[i] = __builtin_bit_cast(bf16x8, x);
     }
-    Loader<NB, SPLIT ? 1 : WAVES> loads;
+    Loader<NB, SPLIT ? 1 : WAVES, PAD> loads;
     loads.init(a, k, v, f.rows);
     uint16_t *my_k = SPLIT ? k0_s + wave * TILE * RW : k0_s, *my_v = SPLIT ? v0_s + wave * TILE * RW : v0_s;
+    loads.clear_k(my_k);
+    if constexpr (!SPLIT) loads.clear_k(k1_s);
     loads.request(SPLIT ? min(wave, tiles - 1) : 0, my_k, my_v);
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) asm volatile("" : "+v"(qs[i]));   // here, or the loop waits for requests at its top
@@ -465,9 +501,15 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;
     const dim3 grid((unsigned)(items * nkv)), wg(64 * WAVES);
+#define KERNEL(NB, SPLIT)                                                                                       \
+    if (hd % 32) hipLaunchKernelGGL((k_attend_packed<NB, SPLIT, true>), grid, wg, 0, st, a);                      \
+    else hipLaunchKernelGGL((k_attend_packed<NB, SPLIT, false>), grid, wg, 0, st, a)
 #define ATTEND(NB)                                                                                              \
-    if (split) hipLaunchKernelGGL((k_attend_packed<NB <= 4 ? NB : 4, NB <= 4>), grid, wg, 0, st, a);              \
-    else hipLaunchKernelGGL((k_attend_packed<NB, false>), grid, wg, 0, st, a)
+    if (split) {                                                                                                \
+        KERNEL((NB <= 4 ? NB : 4), (NB <= 4));                                                                  \
+    } else {                                                                                                    \
+        KERNEL(NB, false);                                                                                      \
+    }
     switch ((hd + 31) / 32) {
     case 1: ATTEND(1); break;
     case 2: ATTEND(2); break;
@@ -479,6 +521,7 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
     default: ATTEND(8); break;
     }
 #undef ATTEND
+#undef KERNEL
     return l3m_dev_launched("k_attend_packed");
 }
 

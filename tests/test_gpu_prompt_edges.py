@@ -91,3 +91,27 @@ def test_first_score_of_minus_infinity(dev, hd, n):
         assert np.isnan(got[0]).all()
         end = at or n
         assert np.all(np.abs(got[1:end] - want[1:end]) <= tol[1:end])
+
+
+@pytest.mark.parametrize("hd", [8, 16, 24, 40, 48, 72, 80, 104, 120, 128, 136, 176, 200, 256])
+@pytest.mark.parametrize("lens", [[300], [60, 1, 33]])
+def test_infinite_keys(dev, hd, lens):
+    """Infinities among a key's last eight values and its first ones: -inf as a score has no weight, +inf is NaN in the rows that see it and in no others."""
+    rng = np.random.default_rng(hd)
+    n = sum(lens)
+    q, k, v = rows(rng, n, 4, hd), rows(rng, n, 2, hd), rows(rng, n, 2, hd)
+    for d in (hd - 1, hd - 6, 0):
+        q[..., d] &= 0x7FFF
+    for head in (0, 1):
+        k[[5, 30, 59], head, [hd - 1, hd - 6, 0]] = 0xFF80
+    k[41, 1, hd - 6] = 0x7F80
+    got, at = from_bf16(dev.attend_packed(q, k, v, dev.batch(np.cumsum([0] + lens)))), 0
+    for m in lens:
+        part = slice(at, at + m)
+        gone = [t - at for t in (5, 30, 59) if at <= t < at + m]
+        want, tol = without(q[part], np.where(k[part] == 0x7F80, 0, k[part]), v[part], gone)
+        nan = np.zeros(want.shape, bool)
+        if at <= 41 < at + m:
+            nan[41 - at:, 2:] = True
+        assert np.isnan(got[part][nan]).all() and np.all(np.abs(got[part] - want)[~nan] <= tol[~nan])
+        at += m
