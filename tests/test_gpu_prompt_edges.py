@@ -1,4 +1,7 @@
 """Attention over packed prompts (l3m_k_attend_packed) where it can go wrong: sums of rounded weights, infinities among keys, values behind a token."""
+import ctypes as C
+import time
+
 import numpy as np
 import pytest
 
@@ -115,3 +118,31 @@ def test_infinite_keys(dev, hd, lens):
             nan[41 - at:, 2:] = True
         assert np.isnan(got[part][nan]).all() and np.all(np.abs(got[part] - want)[~nan] <= tol[~nan])
         at += m
+
+
+@pytest.mark.parametrize("every", [1, 50])
+def test_time_of_poisoned_values(dev, every):
+    """Values of which a dimension is NaN at every position, or every 50th: rows that are NaN there for their own values' sake are not made anew for those behind
+    them, which at this size takes some hundred times as long."""
+    rng = np.random.default_rng(11)
+    n, nq, nkv, hd = 4096, 16, 4, 128
+    q, k, v = rows(rng, n, nq, hd), rows(rng, n, nkv, hd), rows(rng, n, nkv, hd)
+    poisoned = v.copy()
+    poisoned[::every, :, 77] = 0x7FC0
+    b, out = dev.batch([0, n]), dev.alloc(q.nbytes)
+    dq, dk = dev.put(q), dev.put(k)
+    results, times = [], []
+    for x in (v, poisoned):
+        dv, least = dev.put(x), []
+        for _ in range(5):
+            assert dev.lib.l3m_dev_sync() == 0
+            start = time.perf_counter()
+            assert dev.lib.l3m_k_attend_packed(out, nq * hd, dq, nq * hd, dk, dv, nkv * hd, C.byref(b), nq, nkv, hd, None) == 0 and dev.lib.l3m_dev_sync() == 0
+            least.append(time.perf_counter() - start)
+        times.append(min(least))
+        results.append(from_bf16(dev.get(out, q.shape, np.uint16)))
+    assert times[1] < 10 * times[0], times
+    clean, got = results
+    assert np.isnan(got[..., 77]).all()
+    got[..., 77] = clean[..., 77]
+    assert np.array_equal(got, clean)
