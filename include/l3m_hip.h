@@ -217,7 +217,7 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
 // need not be cleared. A page holds for each layer nkv units [K codes 128 x HP][V codes HP x 128], HP hd rounded up to 32, then 8 bytes a head: the
 // exponents of K's and of V's scales for its four blocks of 32 positions; a layer's part is rounded up to 256 bytes. Codes are OCP e4m3; a scale is 2^(byte - 127),
 // the smallest from 2^-126 up by which the block's largest finite value of that head is at most 448; a value that is not finite is stored as NaN.
-// (Values from 248 2^120 up, float32's largest, are stored as 256 2^120, which reads as infinity.)
+// (Values from 248 2^120 up, float32's largest, are stored as 256 2^120, which reads as infinity: as a key it makes the scores that it meets infinite or NaN.)
 #define L3M_PAGE 128
 typedef struct {
     uint8_t *mem;

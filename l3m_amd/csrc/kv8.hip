@@ -709,12 +709,14 @@ template <bool F32, int NB, int WAVES> __global__ void __launch_bounds__(64 * WA
         } else {
             bool apart = false;                                      // a NaN is the rows' that see it: a token's rows at a time, over its own positions
             if (several) {
-                uint32_t nan = 0;                                    // codes of NaN among the values that some row sees
+                // codes of NaN among the values that some row sees, and where the scale is 2^120 or more those from 256 on, which read as infinities
+                const uint32_t up = sv >= 0x1p120f ? 0x08080808u : 0x01010101u;
+                uint32_t nan = 0;
 #pragma unroll
                 for (int t = 0; t < 2 * NB; t++) {
                     const u32x4 v = values(t);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) nan |= ((v[i] & bytes_before(16 * c + 4 * i, left) & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    for (int i = 0; i < 4; i++) nan |= ((v[i] & bytes_before(16 * c + 4 * i, left) & 0x7F7F7F7Fu) + up) & 0x80808080u;
                 }
                 apart = __ballot(nan != 0) != 0;
             }
