@@ -1,9 +1,12 @@
 """The paged 8-bit K/V cache (l3m_k_kv8_attend) where it can go wrong: values that read as infinities, and the forms of a call by its runs, rows and heads."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
-from serve import attended
-from test_gpu_kv8 import DTYPES, Cache, typed, values
+import l3m_amd as A
+from serve import PAGE, attended
+from test_gpu_kv8 import DTYPES, Cache, attend, typed, values
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +46,70 @@ def test_attend_values_read_as_infinities(dev, dtype, longest):
             for h, d in bad:
                 keep[2 * h:2 * h + 2, d] = False
             assert np.all((np.abs(got[t] - want[0]) <= tol[0])[keep]) and not np.isfinite(got[t][~keep]).any(), (first, t)
+
+
+@DTYPES
+@pytest.mark.parametrize("runs, nkv, g, hd, longest", [(65, 1, 4, 64, 1000), (100, 1, 4, 128, 600), (300, 1, 3, 64, 1000), (90, 4, 2, 128, 1000), (130, 4, 1, 64, 250), (70, 2, 3, 160, 700)])
+def test_attend_many_short_runs(dev, dtype, runs, nkv, g, hd, longest):
+    """More runs than a wavefront has lanes, none of them split: few enough heads that eight wavefronts take a group together, and so many that four do; tokens of
+    several, one or none a run, rows that no run names between them."""
+    o = Cache(dev, runs, nkv, hd, pages=1200, width=9, seed=runs + hd)
+    counts = [int(x) for x in o.rng.choice([1, 5, 31, 64, 65, 200], runs)]
+    counts[0], counts[runs - 1] = longest, longest - 1
+    o.add(list(range(runs)), counts, dtype)
+    ids = [int(i) for i in o.rng.permutation(runs)]
+    rows = [min(counts[i], int(o.rng.choice([0, 1, 1, 1, 2, 7]))) for i in ids]
+    attend(o, ids, rows, nkv * g, dtype, longest=longest)
+
+
+@DTYPES
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_attend_short(dev, dtype, hd):
+    """Sequences of up to four tiles, which four wavefronts take; one group of rows and several."""
+    o = Cache(dev, 4, 2, hd, seed=hd + 50)
+    o.add([0, 1, 2, 3], [256, 1, 130, 64], dtype)
+    attend(o, [1, 0, 3, 2], [1, 1, 1, 1], 8, dtype, longest=256)
+    attend(o, [0, 2, 3], [40, 9, 3], 6, dtype, longest=256)
+
+
+@DTYPES
+def test_attend_many_rows(dev, dtype):
+    """A run of so many rows that nothing is split, over positions before them; the length is not said."""
+    o = Cache(dev, 1, 8, 64, seed=60)
+    o.add([0], [300], dtype)
+    o.add([0], [520], dtype)
+    attend(o, [0], [520], 32, dtype)
+
+
+@pytest.mark.parametrize("order", ["parts", "wavefronts"])
+def test_attend_much_work_of_two_pages(dev, order):
+    """Groups of rows times tiles past 2^25, of a page of values around 1 and one of values around -1: the first quarter of a sequence is one page and the rest the
+    other, or they take turns. A part of a group, a quarter of its tiles, or a wavefront, every fourth tile, that is lost or counted twice moves the result by a
+    sixth or more."""
+    nkv, hd, g, n, width = 1, 8, 16, 128, 1 << 19
+    c, p = dev.kv8(2, 1, nkv, hd), dev.pages(2, 2, width)
+    rng = np.random.default_rng(61)
+    k = rng.standard_normal((2 * PAGE, nkv, hd)).astype(np.float32) / 8
+    v = rng.standard_normal((2 * PAGE, nkv, hd)).astype(np.float32) / 64 + np.float32(np.repeat([1, -1], PAGE))[:, None, None]
+    b = dev.batch([0, 2 * PAGE], [0])
+    dev.pages_grow(p, c, b)
+    dev.kv8_append(c, p, 0, k, v, b)
+    k, v = (x[:, 0].astype(np.float64) for x in dev.kv8_rows(c, p, 0, b))
+    table, lens = np.zeros((2, width), np.int32), np.int32([2 * PAGE, PAGE * width])
+    table[:, 1] = 1
+    table[1] = np.arange(width) >= width // 4 if order == "parts" else np.arange(width) % 2
+    for at, y in ((p.table, table), (p.len, lens)):
+        assert dev.lib.l3m_dev_upload(at, C.c_void_p(y.ctypes.data), y.nbytes) == 0
+    q = rng.standard_normal((n, g, hd)).astype(np.float32)
+    size = dev.lib.l3m_kv8_work_bytes(C.byref(c), n, g)
+    out, b = dev.alloc(q.nbytes), dev.batch([0, n], [1])
+    assert dev.lib.l3m_k_kv8_attend(out, g * hd, dev.put(q), g * hd, A.F32, C.byref(c), C.byref(p), 0, C.byref(b), g, 0, dev.alloc(size), size, None) == 0
+    got = dev.get(out, q.shape, np.float32)
+    # the pages' positions count as often as the table names them, those behind the token in the last page once less; sums of 2^20 terms for a lane, of the weights
+    # (which all have one sign) and of the values, 2^-24 of the sum of their magnitudes each
+    times = np.repeat([np.sum(table[1] == 0), np.sum(table[1] == 1)], PAGE).astype(np.float64)
+    z = q.reshape(-1, hd).astype(np.float64) @ k.T / np.sqrt(hd)
+    for t in range(n):
+        w = np.exp(z[t * g:(t + 1) * g]) * (times - ((np.arange(2 * PAGE) % PAGE > t) & (np.arange(2 * PAGE) // PAGE == table[1, -1])))
+        w /= w.sum(1, keepdims=True)
+        assert np.all(np.abs(got[t] - w @ v) <= 2.0 ** -3 * (w @ np.abs(v)))

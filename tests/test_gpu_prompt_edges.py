@@ -146,3 +146,20 @@ def test_time_of_poisoned_values(dev, every):
     assert np.isnan(got[..., 77]).all()
     got[..., 77] = clean[..., 77]
     assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("hd, nkv, g", [(64, 1, 1), (40, 1, 3), (32, 2, 1)])
+def test_many_longer_prompts(dev, hd, nkv, g):
+    """More prompts than a wavefront has lanes, of one tile or several, whose groups are few enough that wavefronts share them."""
+    rng = np.random.default_rng(hd + 70)
+    lens = [int(x) for x in rng.choice([0, 1, 63, 64, 65, 130, 190], 75)]
+    lens[7] = 700
+    n = sum(lens)
+    assert n > 64 * len(lens) and (n * g // 128 + len(lens)) * nkv < 256
+    q, k, v = rows(rng, n, nkv * g, hd), rows(rng, n, nkv, hd), rows(rng, n, nkv, hd)
+    got, at = from_bf16(dev.attend_packed(q, k, v, dev.batch(np.cumsum([0] + lens)))), 0
+    for m in lens:
+        part = slice(at, at + m)
+        want, tol = without(q[part], k[part], v[part], [])
+        assert np.all(np.abs(got[part] - want) <= tol)
+        at += m
