@@ -53,19 +53,6 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
     w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-template <class T> __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const f32x4 a = *(const f32x4_a4 *)p, b = *(const f32x4_a4 *)(p + 4);
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = i < 4 ? a[i & 3] : b[i & 3];
-    } else {
-        typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
-        const u32x4 w = *(const u32x4_a2 *)p;
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
-    }
-}
-
 // Eight values as they lie in memory.
 template <class T> struct Raw8 {
     u32x4 w[sizeof(T) / 2];
@@ -314,7 +301,6 @@ __device__ __forceinline__ float sum_groups(float x) {
     x = other<16>(x, y); x += y;
     x = other<32>(x, y); return x + y;
 }
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 // Eight codes times `scale`, a power of two.
@@ -477,10 +463,11 @@ template <bool F32, int NB> struct Queries {
             const int d = dim_of<NB>(s, lane >> 4);
             const bool in = d < hd;
             if constexpr (F32) {
+                Raw8<float> raw;
+                raw.load((const float *)q + at + (in ? d : 0));
                 float x[8];
-                load8((const float *)q + at + (in ? d : 0), x);
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = in ? x[i] : 0.f;
+                for (int i = 0; i < 8; i++) x[i] = in ? raw.value(i) : 0.f;
                 in_parts<QP, true>(x, part[s]);
             } else {
                 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
