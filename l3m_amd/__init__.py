@@ -526,11 +526,15 @@ class Device:
         self._check(self.lib.l3m_k_kv4_attend(do, self.put(q), C.byref(c), n, nq, pos, self.alloc(size), size, None), "kv4_attend")
         return self.get(do, q.shape, np.float32)
 
-    # ---- many sequences: rows are float32, or bf16 as uint16
+    # ---- many sequences: rows are float32, or bf16 as uint16; results of rows that no run names are zeros
+
+    def _zeros(self, shape, dtype):
+        """Device memory of so many zeros, at least one."""
+        return self.put(np.zeros(shape if np.prod(shape) else 1, dtype))
 
     @staticmethod
     def _rows(x):
-        """Rows as the kernels take them, their dtype and an empty array's."""
+        """Rows as the kernels take them, and their dtype."""
         x = np.ascontiguousarray(x)
         if x.dtype == np.uint16:
             return x, BF16
@@ -567,7 +571,7 @@ class Device:
         q, k, v = (np.ascontiguousarray(x, np.uint16) for x in (q, k, v))
         if k.shape != v.shape or len(q) < b.n or len(k) < b.n or q.shape[2] != k.shape[2]:
             raise ValueError(f"rows {q.shape}, {k.shape} and {v.shape} for a batch of {b.n}")
-        do = self.alloc(max(q.nbytes, 16))
+        do = self._zeros(q.shape, q.dtype)
         self._check(self.lib.l3m_k_attend_packed(do, q.shape[1] * q.shape[2], self.put(q), q.shape[1] * q.shape[2], self.put(k), self.put(v), k.shape[1] * k.shape[2],
                                                  C.byref(b), q.shape[1], k.shape[1], q.shape[2], None), "attend_packed")
         return self.get(do, q.shape, np.uint16)
@@ -599,7 +603,7 @@ class Device:
 
     def pages_grow(self, p, c, b):
         """Room for a batch's rows: their positions (l3m_k_pages_grow)."""
-        pos = self.alloc(max(4 * b.n, 4))
+        pos = self._zeros(b.n, np.int32)
         self._check(self.lib.l3m_k_pages_grow(C.byref(p), C.byref(c), C.byref(b), pos, None), "pages_grow")
         return self.get(pos, b.n, np.int32)
 
@@ -628,7 +632,7 @@ class Device:
 
     def kv8_rows(self, c, p, layer, b):
         """The last positions of a batch's sequences as values: k, v [n, nkv, hd] (l3m_k_kv8_rows)."""
-        dk, dv = (self.alloc(4 * max(b.n, 1) * c.nkv * c.hd) for _ in range(2))
+        dk, dv = (self._zeros((b.n, c.nkv, c.hd), np.float32) for _ in range(2))
         self._check(self.lib.l3m_k_kv8_rows(C.byref(c), C.byref(p), layer, dk, dv, C.byref(b), None), "kv8_rows")
         return tuple(self.get(x, (b.n, c.nkv, c.hd), np.float32) for x in (dk, dv))
 
@@ -639,7 +643,7 @@ class Device:
         if hd != c.hd or n < b.n:
             raise ValueError(f"rows {q.shape} for a batch of {b.n}, heads of {c.hd}")
         size = self.lib.l3m_kv8_work_bytes(C.byref(c), max(b.n, 1), nq)
-        do = self.alloc(max(q.nbytes, 16))
+        do = self._zeros(q.shape, q.dtype)
         self._check(self.lib.l3m_k_kv8_attend(do, nq * hd, self.put(q), nq * hd, dtype, C.byref(c), C.byref(p), layer, C.byref(b), nq, longest, self.alloc(max(size, 16)),
                                               size, None), "kv8_attend")
         return self.get(do, q.shape, q.dtype)

@@ -113,3 +113,23 @@ def test_attend_much_work_of_two_pages(dev, order):
         w = np.exp(z[t * g:(t + 1) * g]) * (times - ((np.arange(2 * PAGE) % PAGE > t) & (np.arange(2 * PAGE) // PAGE == table[1, -1])))
         w /= w.sum(1, keepdims=True)
         assert np.all(np.abs(got[t] - w @ v) <= 2.0 ** -3 * (w @ np.abs(v)))
+
+
+def test_python_rows_of_no_run(dev, monkeypatch):
+    """Results of the Python calls for rows that no run names, or that a sequence doesn't have, are zeros, whatever their memory held before."""
+    alloc = dev.alloc
+
+    def used(nbytes):
+        p, marks = alloc(nbytes), np.full(nbytes, 0x41, np.uint8)
+        assert dev.lib.l3m_dev_upload(p, C.c_void_p(marks.ctypes.data), nbytes) == 0
+        return p
+
+    monkeypatch.setattr(dev, "alloc", used)
+    o = Cache(dev, 2, 1, 32, seed=62)
+    o.add([0], [9])
+    q, k = np.ones((8, 2, 32), np.uint16), np.ones((8, 1, 32), np.uint16)
+    b = dev.batch([2, 5], [0], n=8)
+    for got in (dev.attend_packed(q, k, k, b), dev.kv8_attend(o.c, o.p, o.layer, q, b), *dev.kv8_rows(o.c, o.p, o.layer, b), dev.pages_grow(o.p, o.c, b)):
+        assert not got[:2].any() and not got[5:].any() and got[2:5].any()
+    k, v = dev.kv8_rows(o.c, o.p, o.layer, dev.batch([0, 20], [0]))
+    assert not k.any() and not v.any()
