@@ -133,3 +133,32 @@ def test_python_rows_of_no_run(dev, monkeypatch):
         assert not got[:2].any() and not got[5:].any() and got[2:5].any()
     k, v = dev.kv8_rows(o.c, o.p, o.layer, dev.batch([0, 20], [0]))
     assert not k.any() and not v.any()
+
+
+@DTYPES
+@pytest.mark.parametrize("hd", [8, 40, 128])
+def test_rows_aligned_to_their_values(dev, dtype, hd):
+    """Rows of odd strides that begin one value behind a round address, in and out: the same bits as dense ones, and nothing beside them."""
+    nkv, nq, n = 3, 6, 75
+    x, y = Cache(dev, 1, nkv, hd, seed=63), Cache(dev, 1, nkv, hd, seed=63)
+    (k, kx), (v, vx) = x.rows(n, dtype)
+    x.add([0], [n], rows=[(k, kx), (v, vx)])
+    kind, size = (A.F32, 4) if dtype == "f32" else (A.BF16, 2)
+    b, width = dev.batch([0, n], [0]), 2 * nkv * hd + 5
+    fused = np.zeros((n, width), k.dtype)
+    fused[:, 1:1 + nkv * hd], fused[:, 2 + nkv * hd:2 + 2 * nkv * hd] = k.reshape(n, -1), v.reshape(n, -1)
+    p = dev.put(fused)
+    dev.pages_grow(y.p, y.c, b)
+    assert dev.lib.l3m_k_kv8_append(C.byref(y.c), C.byref(y.p), y.layer, p + size, p + size * (2 + nkv * hd), width, kind, C.byref(b), None) == 0
+    for one, two in zip(dev.kv8_rows(x.c, x.p, x.layer, b), dev.kv8_rows(y.c, y.p, y.layer, b)):
+        assert np.array_equal(one, two) and one.any()
+    q = typed(x.rng.standard_normal((n, nq, hd)), dtype)[0]
+    wide, marks = np.zeros((n, nq * hd + 3), q.dtype), np.full((n, nq * hd + 7), 3, q.dtype)
+    wide[:, 1:1 + nq * hd] = q.reshape(n, -1)
+    need = dev.lib.l3m_kv8_work_bytes(C.byref(y.c), n, nq)
+    out = dev.put(marks)
+    assert dev.lib.l3m_k_kv8_attend(out + size, nq * hd + 7, dev.put(wide) + size, nq * hd + 3, kind, C.byref(y.c), C.byref(y.p), y.layer, C.byref(b), nq, 0, dev.alloc(need), need, None) == 0
+    got = dev.get(out, marks.shape, q.dtype)
+    assert np.array_equal(got[:, 1:1 + nq * hd], dev.kv8_attend(x.c, x.p, x.layer, q, b).reshape(n, -1))
+    marks[:, 1:1 + nq * hd] = got[:, 1:1 + nq * hd]
+    assert np.array_equal(got, marks)
