@@ -39,8 +39,8 @@ struct PromptIn {
 };
 
 // x plus the two bf16 values of a word, in float32: the weights that the product takes are the ones that are summed, so their rounding cancels where a few
-// positions have all the weight. 8191 rows 547 us, as with the sum of the weights before their rounding; four chains of sums instead of one 555, the two halves
-// made floats and added 561.
+// positions have all the weight. A sum waits for the last, so two take turns: 8191 rows of 32/8 heads of 128 544 us, 548 by one, 541 with the weights before their
+// rounding (and 561 with the halves made floats, 571 by the matrix cores); of 64 307, 309, 309; 24 prompts 89.1, 89.9, 88.5.
 __device__ __forceinline__ float add_pair(uint32_t w, float x) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), x, false);
@@ -271,7 +271,7 @@ template <int NB, bool SPLIT, bool PAD> __global__ void __launch_bounds__(64 * W
     for (int i = 0; i < NB; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
-    float m = M0, l = 0.f;
+    float m = M0, l = 0.f, sums[2] = {};                             // of the weights, in turn (add_pair)
     bool large = false;                                              // some row's m is (LARGE_SCORE)
 
     auto step = [&](int tile, const uint16_t *k_s, const uint16_t *v_s) {
@@ -326,7 +326,8 @@ template <int NB, bool SPLIT, bool PAD> __global__ void __launch_bounds__(64 * W
         top = fmaxf(top, y) * scale;
         if (__ballot(top > m + 8.f)) {
             const float to = top > m + 8.f ? top : m, by = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to);
-            l *= by;
+#pragma unroll
+            for (int i = 0; i < 2; i++) sums[i] *= by;
 #pragma unroll
             for (int i = 0; i < NB; i++) acc[i] *= by;
             m = to;
@@ -366,7 +367,7 @@ template <int NB, bool SPLIT, bool PAD> __global__ void __launch_bounds__(64 * W
                 for (int e = 0; e < 4; e++) {
                     const float x0 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e], by, -less)), x1 = __builtin_amdgcn_exp2f(fmaf(s[b][8 * j + 2 * e + 1], by, -less));
                     w[e] = bf16_pair(x0, x1);
-                    l = add_pair(w[e], l);
+                    sums[e & 1] = add_pair(w[e], sums[e & 1]);
                 }
                 p[b][j] = __builtin_bit_cast(bf16x8, w);
             }
@@ -396,6 +397,8 @@ template <int NB, bool SPLIT, bool PAD> __global__ void __launch_bounds__(64 * W
     __syncthreads();                                                 // the tiles are done with
     if (!rows) return;                                               // (a group has rows, so not where all meet)
     float y;
+#pragma unroll
+    for (int i = 0; i < 2; i++) l += sums[i];
     l = other_half(l, y);
     l += y;
     float bad = 0.f;                                                 // NaN where a value is not finite
