@@ -821,7 +821,6 @@ template <bool F32, int JOIN> __global__ void __launch_bounds__(JOIN) k_kv8_join
     }
 }
 
-Runs runs_of(const l3m_batch *b) { return {b->ids, b->starts, b->seqs, b->n}; }
 // What calls over the cache refuse alike, or NULL.
 const char *call_bad(const l3m_kv8 *c, const l3m_pages *p, int layer, const l3m_batch *b) {
     if (const char *why = paged_bad(c, p)) return why;

@@ -395,7 +395,6 @@ __global__ void __launch_bounds__(256) k_pages_copy(Tables t, uint8_t *mem, size
         }
 }
 
-Runs runs_of(const l3m_batch *b) { return {b->ids, b->starts, b->seqs, b->n}; }
 const char *list_bad(const l3m_pages *p, const int32_t *a, const int32_t *b, int n, bool need_b) {
     if (const char *why = pages_bad(p)) return why;
     if (n < 0 || n > p->seqs) return "pages: more sequences listed than there are";

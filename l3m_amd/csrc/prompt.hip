@@ -520,7 +520,7 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
     // a CU holds one such workgroup: 1705 of 3/1 heads of 80 (40) 18.2 and 33.8, 700 of 16/2 of 128 (88) 17.6 and 19.2, 400 of 32/8 (104) 17.2 and 14.5. Past 128 none.
     const bool split = hd <= 128 && items * nkv < (hd <= 64 ? 256 : 96) && b->n > TILE * b->seqs;
     if (split) items = (long long)b->n * g / ROWS + b->seqs;
-    const PromptIn a = {q, k, v, out, {b->ids, b->starts, b->seqs, b->n}, q_stride, kv_stride, out_stride, nq, nkv, hd, g, multiplier(g, (uint64_t)b->n * g), multiplier(nkv, items * nkv),
+    const PromptIn a = {q, k, v, out, runs_of(b), q_stride, kv_stride, out_stride, nq, nkv, hd, g, multiplier(g, (uint64_t)b->n * g), multiplier(nkv, items * nkv),
                         (int)items, CUS / nkv, 1.44269504f / sqrtf((float)hd)};
     hipStream_t st;
     if (!stream_of(stream, st)) return -1;

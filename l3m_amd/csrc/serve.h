@@ -77,6 +77,7 @@ struct Runs {
     __device__ __forceinline__ int from(int i) const { return clamp(starts[i], 0, n); }
     __device__ __forceinline__ int to(int i, int first) const { return clamp(starts[i + 1], first, n); }
 };
+inline Runs runs_of(const l3m_batch *b) { return {b->ids, b->starts, b->seqs, b->n}; }
 // The run that holds item `item` of the runs' items one behind the other, count(run, first row, rows) each, and the item's place in it. run < 0: there are
 // fewer items. Up to 64 runs are counted by each wavefront for itself, a lane a run; of more the W wavefronts of a workgroup, which then all look for the same
 // item, count 64 each and meet in LDS.
