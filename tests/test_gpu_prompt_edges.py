@@ -5,6 +5,7 @@ import time
 import numpy as np
 import pytest
 
+import l3m_amd as A
 from serve import attended, bf16, from_bf16
 
 pytestmark = pytest.mark.gpu
@@ -163,3 +164,27 @@ def test_many_longer_prompts(dev, hd, nkv, g):
         want, tol = without(q[part], k[part], v[part], [])
         assert np.all(np.abs(got[part] - want) <= tol)
         at += m
+
+
+@pytest.mark.parametrize("hd, runs", [(64, 4), (80, 70)])
+def test_captured(dev, hd, runs):
+    """A call recorded once and replayed: each replay takes the prompts' ends and the rows that it finds, between eager calls, and gives their bits."""
+    rng, hip, n, nq, nkv = np.random.default_rng(hd + 2), C.CDLL("libamdhip64.so"), 600, 4, 2
+    q, k, v = rows(rng, n, nq, hd), rows(rng, n, nkv, hd), rows(rng, n, nkv, hd)
+    dq, dk, dv, out, starts = dev.put(q), dev.put(k), dev.put(v), dev.alloc(q.nbytes), dev.alloc(4 * (runs + 1))
+    b, st, graph, ex = A.Batch(None, starts, runs, n), C.c_void_p(), C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamCreateWithFlags(C.byref(st), 1) == 0 and hip.hipStreamBeginCapture(st, 1) == 0
+    assert dev.lib.l3m_k_attend_packed(out, nq * hd, dq, nq * hd, dk, dv, nkv * hd, C.byref(b), nq, nkv, hd, st) == 0
+    assert hip.hipStreamEndCapture(st, C.byref(graph)) == 0 and hip.hipGraphInstantiate(C.byref(ex), graph, None, None, C.c_size_t(0)) == 0
+    for i in range(4):
+        ends = np.int32(np.sort(rng.integers(0, n + 1, runs + 1)))
+        if i == 2:
+            ends[1:] = n                                             # one prompt and empty ones
+        q = rows(rng, n, nq, hd)
+        for at, x in ((starts, ends), (dq, q), (out, np.full(q.shape, 0x41, np.uint16))):
+            assert dev.lib.l3m_dev_upload(at, C.c_void_p(x.ctypes.data), x.nbytes) == 0
+        assert dev.lib.l3m_dev_sync() == 0 and hip.hipGraphLaunch(ex, st) == 0 and hip.hipStreamSynchronize(st) == 0
+        got, want = dev.get(out, q.shape, np.uint16), dev.attend_packed(q, k, v, dev.batch(ends, n=n))
+        named = slice(ends[0], ends[-1])
+        assert np.array_equal(got[named], want[named]) and np.all(got[:ends[0]] == 0x41) and np.all(got[ends[-1]:] == 0x41)
+    assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0 and hip.hipStreamDestroy(st) == 0
