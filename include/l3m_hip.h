@@ -216,7 +216,8 @@ int l3m_k_attend_packed(uint16_t *out, int out_stride, const uint16_t *q, int q_
 // The cache: pages of 128 positions of all its layers and kv heads, in one allocation of l3m_kv8_bytes (0 for a shape that is refused), 256-byte aligned, which
 // need not be cleared. A page holds for each layer nkv units [K codes 128 x HP][V codes HP x 128], HP hd rounded up to 32, then 8 bytes a head: the
 // exponents of K's and of V's scales for its four blocks of 32 positions; a layer's part is rounded up to 256 bytes. Codes are OCP e4m3; a scale is 2^(byte - 127),
-// the smallest from 2^-126 up by which the block's largest finite value of that head is at most 448; a value that is not finite is stored as NaN.
+// the smallest from 2^-126 up by which the largest finite value that was stored into the block, of that head, is at most 448; a value that is not finite is stored
+// as NaN.
 // (Values from 248 2^120 up, float32's largest, are stored as 256 2^120, which reads as infinity: as a key it makes the scores that it meets infinite or NaN.)
 #define L3M_PAGE 128
 typedef struct {
@@ -246,7 +247,7 @@ int    l3m_k_pages_reset(const l3m_pages *p, void *stream);                    /
 int    l3m_k_pages_clear(const l3m_pages *p, void *stream);                    // state[0] = 0
 // Room for a batch: each run's sequence becomes longer by its rows. New pages are the free ones of lowest index, in the runs' order. A page that a run goes on
 // in and that other sequences hold too is replaced by a copy (all layers); where all its holders are in the batch, the first of them keeps it. pos (NULL:
-// not wanted): the rows' positions, [n].
+// not wanted): the rows' positions, [n]. A run without rows changes nothing, but names a sequence of its own like any other.
 int    l3m_k_pages_grow(const l3m_pages *p, const l3m_kv8 *c, const l3m_batch *b, int32_t *pos, void *stream);
 // Sequences to[i], which are empty, become copies of from[i]: they hold the same pages. No `to` is listed twice or is a `from`. Device lists of n.
 int    l3m_k_pages_fork(const l3m_pages *p, const int32_t *from, const int32_t *to, int n, void *stream);
@@ -257,7 +258,8 @@ int    l3m_k_pages_compact(const l3m_pages *p, const l3m_kv8 *c, void *stream);
 
 // K and V rows of a batch, [n] of nkv heads (k and v of one stride, L3M_HIP_F32 or _BF16), into one layer: the last positions of the runs' sequences, whose lengths
 // count them already (l3m_k_pages_grow). The scale of a block that holds earlier positions is the larger of its own and the new rows'; where it rises, the old
-// codes are rounded again. A sequence must not be in the batch twice.
+// codes are rounded again. So positions are held in steps that later ones of their block may make coarser, in the same call or another one, and which stay as they
+// are where those are cut (l3m_k_pages_cut) and others take their places; a block that is begun anew has a scale of its own. A sequence must not be in the batch twice.
 int l3m_k_kv8_append(const l3m_kv8 *c, const l3m_pages *p, int layer, const void *k, const void *v, int stride, int dtype, const l3m_batch *b, void *stream);
 // The last positions of a batch's sequences as values: k and v float32 [n][nkv][hd] (either may be NULL). Positions whose page is none read as NaN.
 int l3m_k_kv8_rows(const l3m_kv8 *c, const l3m_pages *p, int layer, float *k, float *v, const l3m_batch *b, void *stream);
