@@ -9,7 +9,7 @@
 // K's and V's tiles go from memory to LDS directly, 16 bytes a lane, in an order of pieces within a row by which no read meets a bank twice.
 //
 // Bound by instruction issue: beside a tile's products of a wavefront (32, hd 128) stand its softmax's some 130 vector instructions and 32 exponentials. Two
-// workgroups of four wavefronts a CU fill each other's gaps. 8191 rows of 32/8 heads of 128: 540 to 575 us, 0.96 to 1.02 PFLOP/s, by the box (a bf16 product of 8192^3:
+// workgroups of four wavefronts a CU fill each other's gaps. 8191 rows of 32/8 heads of 128: 540 to 575 us, 0.96 to 1.02 PFLOP/s, by the card (a bf16 product of 8192^3:
 // 1.34); heads of 64 0.83 to 0.90, of 80 0.73 to 0.77 (80 of 96 columns are work), of 256 0.82 to 0.84 (one wavefront a SIMD). 24 prompts of 16 to 2048: 89 to 100 us,
 // 0.49 to 0.55: many of their tiles lie on the diagonal, and workgroups are too short to hide their first loads. Five of 1 to 64 rows: 5.6 us, of which a launch is 1.6.
 // Measured and not built: one tile in LDS and three workgroups a CU (8191 547 us, 24 prompts 97; hd 256 630 against 671); a tile's scores beside the last
